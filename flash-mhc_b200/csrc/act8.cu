@@ -1,0 +1,178 @@
+// 8-bit activation checkpoints on their own: quantise and restore (rows, C)
+// tensors of bf16, f16 or f32 (format: act8.cuh).
+#include "act8.cuh"
+#include "fmhc_launch.h"
+#include "grid.cuh"
+
+namespace fmhc {
+
+using namespace act8;
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;  // chunks of eight values in flight per thread
+
+// Rows of C values (C % 8 == 0, 16-byte aligned rows) are seen as 4 * nb
+// chunks of eight, nb = ceil(C / 32) blocks; chunks past C are empty.  Chunk i
+// belongs to block i / 4 of the whole tensor, so four neighbouring lanes find
+// their block's maximum with two shuffles.  FLAT (C % 32 == 0): no empty
+// chunks, and the chunk's place is 8 i without a division.
+template <class E, int FMT, bool FLAT>
+__global__ void __launch_bounds__(kThreads)
+quantize_kernel(const E *__restrict__ x, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
+                int64_t chunks, int C, int nb4) {
+  pdl_wait();
+  const int64_t step = int64_t(gridDim.x) * kThreads * kUnroll;
+  for (int64_t i0 = int64_t(blockIdx.x) * kThreads * kUnroll; i0 < chunks; i0 += step) {
+    typename Elem<E>::Raw raw[kUnroll];
+    int64_t at[kUnroll];
+    bool in[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = i0 + u * kThreads + threadIdx.x;
+      in[u] = i < chunks;
+      at[u] = i * 8;
+      if constexpr (!FLAT) {
+        const int64_t row = i / nb4;
+        const int c = int(i - row * nb4) * 8;
+        in[u] = in[u] && c < C;
+        at[u] = row * C + c;
+      }
+      raw[u] = {};
+      if (in[u]) raw[u] = ld8(x + at[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = i0 + u * kThreads + threadIdx.x;
+      float f[8];
+      Elem<E>::widen(raw[u], f);
+      const uint32_t e = scale_byte<FMT>(amax_block(amax8(f)));
+      if (in[u]) __stcs(reinterpret_cast<uint2 *>(codes + at[u]), encode8<FMT>(f, e));
+      if ((threadIdx.x & 3) == 0 && i < chunks) __stcs(scales + (i >> 2), uint8_t(e));
+    }
+  }
+}
+
+template <class E, int FMT, bool FLAT>
+__global__ void __launch_bounds__(kThreads)
+dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
+                  E *__restrict__ x, int64_t chunks, int C, int nb4) {
+  pdl_wait();
+  const int64_t step = int64_t(gridDim.x) * kThreads * kUnroll;
+  for (int64_t i0 = int64_t(blockIdx.x) * kThreads * kUnroll; i0 < chunks; i0 += step) {
+    Codes<8> raw[kUnroll];
+    uint32_t e[kUnroll];
+    int64_t at[kUnroll];
+    bool in[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = i0 + u * kThreads + threadIdx.x;
+      in[u] = i < chunks;
+      at[u] = i * 8;
+      if constexpr (!FLAT) {
+        const int64_t row = i / nb4;
+        const int c = int(i - row * nb4) * 8;
+        in[u] = in[u] && c < C;
+        at[u] = row * C + c;
+      }
+      if (in[u]) {
+        raw[u] = ld_codes<8>(codes + at[u]);
+        e[u] = __ldg(scales + (i >> 2));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (in[u]) {
+        float f[8];
+        restore<FMT, 8>(raw[u], scale_value(e[u]), f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = Elem<E>::fit(f[k]);
+        st8(x + at[u], f);
+      }
+    }
+  }
+}
+
+// Any C and any alignment: one warp per block, one value per lane.
+template <class E, int FMT>
+__global__ void __launch_bounds__(kThreads)
+quantize_any_kernel(const E *__restrict__ x, uint8_t *__restrict__ codes,
+                    uint8_t *__restrict__ scales, int64_t blocks, int C, int nb) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
+  const int64_t nwarps = (int64_t(gridDim.x) * kThreads) >> 5;
+  for (int64_t b = warp; b < blocks; b += nwarps) {
+    const int64_t row = b / nb;
+    const int c = int(b - row * nb) * kBlock + lane;
+    const float v = c < C ? Elem<E>::widen1(x[row * C + c]) : 0.f;
+    const uint32_t e = scale_byte<FMT>(
+        __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
+    if (c < C) codes[row * C + c] = uint8_t(encode4<FMT>(v, 0.f, 0.f, 0.f, e));
+    if (lane == 0) scales[b] = uint8_t(e);
+  }
+}
+
+template <class E, int FMT>
+__global__ void __launch_bounds__(kThreads)
+dequantize_any_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
+                      E *__restrict__ x, int64_t blocks, int C, int nb) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
+  const int64_t nwarps = (int64_t(gridDim.x) * kThreads) >> 5;
+  for (int64_t b = warp; b < blocks; b += nwarps) {
+    const int64_t row = b / nb;
+    const int c = int(b - row * nb) * kBlock + lane;
+    if (c < C)
+      x[row * C + c] = Elem<E>::narrow1(
+          Elem<E>::fit(decode1<FMT>(codes[row * C + c]) * scale_value(scales[b])));
+  }
+}
+
+template <class E, int FMT>
+void quantize(const void *x, void *codes, void *scales, int64_t rows, int C, bool vec,
+              cudaStream_t s) {
+  const int nb = (C + kBlock - 1) / kBlock;
+  if (vec) {
+    const int64_t chunks = rows * nb * 4, warps = (chunks + 32 * kUnroll - 1) / (32 * kUnroll);
+    auto k = C % kBlock ? quantize_kernel<E, FMT, false> : quantize_kernel<E, FMT, true>;
+    launch(k, dim3(grid_for(k, warps, kThreads)), dim3(kThreads), 0, s, (const E *)x,
+           (uint8_t *)codes, (uint8_t *)scales, chunks, C, 4 * nb);
+  } else {
+    auto k = quantize_any_kernel<E, FMT>;
+    launch(k, dim3(grid_for(k, rows * nb, kThreads)), dim3(kThreads), 0, s, (const E *)x,
+           (uint8_t *)codes, (uint8_t *)scales, rows * nb, C, nb);
+  }
+}
+
+template <class E, int FMT>
+void dequantize(const void *codes, const void *scales, void *x, int64_t rows, int C, bool vec,
+                cudaStream_t s) {
+  const int nb = (C + kBlock - 1) / kBlock;
+  if (vec) {
+    const int64_t chunks = rows * nb * 4, warps = (chunks + 32 * kUnroll - 1) / (32 * kUnroll);
+    auto k = C % kBlock ? dequantize_kernel<E, FMT, false> : dequantize_kernel<E, FMT, true>;
+    launch(k, dim3(grid_for(k, warps, kThreads)), dim3(kThreads), 0, s, (const uint8_t *)codes,
+           (const uint8_t *)scales, (E *)x, chunks, C, 4 * nb);
+  } else {
+    auto k = dequantize_any_kernel<E, FMT>;
+    launch(k, dim3(grid_for(k, rows * nb, kThreads)), dim3(kThreads), 0, s, (const uint8_t *)codes,
+           (const uint8_t *)scales, (E *)x, rows * nb, C, nb);
+  }
+}
+
+}  // namespace
+
+void launch_act_quantize(const void *x, int dtype, void *codes, int fmt, void *scales, int64_t rows,
+                         int C, bool vec, cudaStream_t s) {
+  FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT(fmt, quantize<E, FMT>(x, codes, scales, rows, C, vec, s)));
+}
+
+void launch_act_dequantize(const void *codes, int fmt, const void *scales, void *x, int dtype,
+                           int64_t rows, int C, bool vec, cudaStream_t s) {
+  FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT(fmt, dequantize<E, FMT>(codes, scales, x, rows, C, vec, s)));
+}
+
+}  // namespace fmhc

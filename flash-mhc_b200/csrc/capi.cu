@@ -489,4 +489,244 @@ int fmhc_k2_bwd_typed(const void *proj, const void *alpha_pre, const void *alpha
   return check_launch(w);
 }
 
+// ------------------------------------------------- 8-bit activation checkpoints
+static bool fmt_ok(int f) { return f == FMHC_ACT8_INT8 || f == FMHC_ACT8_E4M3; }
+static bool dtype_ok(int d) {
+  return d == FMHC_DTYPE_F32 || d == FMHC_DTYPE_BF16 || d == FMHC_DTYPE_F16;
+}
+static uintptr_t dtype_size(int d) { return d == FMHC_DTYPE_F32 ? 4 : 2; }
+
+static int check_rows(const char *w, int64_t rows, int64_t C) {
+  if (rows < 0) return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: rows must be >= 0 (got %lld)", w, (long long)rows);
+  if (C < 1 || C > (int64_t(1) << 28))
+    return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: C must be in [1, 2^28] (got %lld)", w, (long long)C);
+  return FMHC_OK;
+}
+
+#define FMHC_REQUIRE_FMT(w, f)                                                              \
+  if (!fmt_ok(f))                                                                           \
+  return fail(FMHC_ERR_UNSUPPORTED, "%s: the code format must be FMHC_ACT8_INT8 or "        \
+              "FMHC_ACT8_E4M3", w)
+#define FMHC_REQUIRE_DTYPE(w, d)                                                            \
+  if (!dtype_ok(d))                                                                         \
+  return fail(FMHC_ERR_UNSUPPORTED, "%s: the element type must be FMHC_DTYPE_F32, "         \
+              "FMHC_DTYPE_BF16 or FMHC_DTYPE_F16", w)
+#define FMHC_REQUIRE_ALIGN_TO(w, p, a)                                                      \
+  if (!aligned((p), (a)))                                                                   \
+  return fail(FMHC_ERR_ALIGNMENT, "%s: %s must be aligned to its element size", w, #p)
+
+int fmhc_act_quantize(const void *x, int x_dtype, void *codes, int format, void *scales,
+                      int64_t rows, int64_t C, void *stream) {
+  const char *w = "fmhc_act_quantize";
+  if (int e = check_rows(w, rows, C)) return e;
+  FMHC_REQUIRE_DTYPE(w, x_dtype);
+  FMHC_REQUIRE_FMT(w, format);
+  if (rows == 0) return ok();
+  FMHC_REQUIRE_PTR(w, x); FMHC_REQUIRE_PTR(w, codes); FMHC_REQUIRE_PTR(w, scales);
+  FMHC_REQUIRE_ALIGN_TO(w, x, dtype_size(x_dtype));
+  const bool vec = C % 8 == 0 && aligned(x, 16) && aligned(codes, 8);
+  fmhc::launch_act_quantize(x, x_dtype, codes, format, scales, rows, int(C), vec, (cudaStream_t)stream);
+  return check_launch(w);
+}
+
+int fmhc_act_dequantize(const void *codes, int format, const void *scales, void *x, int x_dtype,
+                        int64_t rows, int64_t C, void *stream) {
+  const char *w = "fmhc_act_dequantize";
+  if (int e = check_rows(w, rows, C)) return e;
+  FMHC_REQUIRE_DTYPE(w, x_dtype);
+  FMHC_REQUIRE_FMT(w, format);
+  if (rows == 0) return ok();
+  FMHC_REQUIRE_PTR(w, codes); FMHC_REQUIRE_PTR(w, scales); FMHC_REQUIRE_PTR(w, x);
+  FMHC_REQUIRE_ALIGN_TO(w, x, dtype_size(x_dtype));
+  const bool vec = C % 8 == 0 && aligned(x, 16) && aligned(codes, 8);
+  fmhc::launch_act_dequantize(codes, format, scales, x, x_dtype, rows, int(C), vec, (cudaStream_t)stream);
+  return check_launch(w);
+}
+
+int fmhc_k3_fwd_q8(const void *x, const float *h_pre, void *out, void *x_codes, void *x_scales,
+                   int format, int64_t T, int64_t n, int64_t C, void *stream) {
+  const char *w = "fmhc_k3_fwd_q8";
+  if (int e = check_streams(w, T, n, C)) return e;
+  FMHC_REQUIRE_FMT(w, format);
+  if (T == 0) return ok();
+  FMHC_REQUIRE_PTR(w, x); FMHC_REQUIRE_PTR(w, h_pre); FMHC_REQUIRE_PTR(w, out);
+  FMHC_REQUIRE_PTR(w, x_codes); FMHC_REQUIRE_PTR(w, x_scales);
+  FMHC_REQUIRE_ALIGN16(w, h_pre);
+  FMHC_REQUIRE_ALIGN2(w, x); FMHC_REQUIRE_ALIGN2(w, out);
+  cudaStream_t s = (cudaStream_t)stream;
+  const int vec = pick_vec(C, {x, out});
+  if (vec == 8 && aligned(x_codes, 8)) {
+    fmhc::launch_k3_fwd_q8(x, h_pre, out, x_codes, x_scales, format, T, int(C), s);
+  } else {
+    fmhc::launch_k3_fwd(x, h_pre, out, T, int(C), vec, s);
+    fmhc::launch_act_quantize(x, FMHC_DTYPE_BF16, x_codes, format, x_scales, 4 * T, int(C),
+                              C % 8 == 0 && aligned(x, 16) && aligned(x_codes, 8), s);
+  }
+  return check_launch(w);
+}
+
+int fmhc_k4_fwd_q8(const void *x, const void *lo, const float *H, const float *h_post, void *out,
+                   void *lo_codes, void *lo_scales, int format, int64_t T, int64_t n, int64_t C,
+                   void *stream) {
+  const char *w = "fmhc_k4_fwd_q8";
+  if (int e = check_streams(w, T, n, C)) return e;
+  FMHC_REQUIRE_FMT(w, format);
+  if (T == 0) return ok();
+  FMHC_REQUIRE_PTR(w, x); FMHC_REQUIRE_PTR(w, lo); FMHC_REQUIRE_PTR(w, H);
+  FMHC_REQUIRE_PTR(w, h_post); FMHC_REQUIRE_PTR(w, out); FMHC_REQUIRE_PTR(w, lo_codes);
+  FMHC_REQUIRE_PTR(w, lo_scales);
+  FMHC_REQUIRE_ALIGN16(w, H); FMHC_REQUIRE_ALIGN16(w, h_post);
+  FMHC_REQUIRE_ALIGN2(w, x); FMHC_REQUIRE_ALIGN2(w, lo); FMHC_REQUIRE_ALIGN2(w, out);
+  cudaStream_t s = (cudaStream_t)stream;
+  const int vec = pick_vec(C, {x, lo, out});
+  if (vec == 8 && aligned(lo_codes, 8)) {
+    fmhc::launch_k4_fwd_q8(x, lo, H, h_post, out, lo_codes, lo_scales, format, T, int(C), s);
+  } else {
+    fmhc::launch_k4_fwd(x, lo, H, h_post, out, T, int(C), vec, s);
+    fmhc::launch_act_quantize(lo, FMHC_DTYPE_BF16, lo_codes, format, lo_scales, T, int(C),
+                              C % 8 == 0 && aligned(lo, 16) && aligned(lo_codes, 8), s);
+  }
+  return check_launch(w);
+}
+
+int fmhc_k3_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scales, int format,
+                   float *grad_h, int64_t T, int64_t n, int64_t C, void *stream) {
+  const char *w = "fmhc_k3_bwd_q8";
+  if (int e = check_streams(w, T, n, C)) return e;
+  FMHC_REQUIRE_FMT(w, format);
+  if (T == 0) return ok();
+  FMHC_REQUIRE_PTR(w, grad_out); FMHC_REQUIRE_PTR(w, x_codes); FMHC_REQUIRE_PTR(w, x_scales);
+  FMHC_REQUIRE_PTR(w, grad_h);
+  FMHC_REQUIRE_ALIGN16(w, grad_h); FMHC_REQUIRE_ALIGN2(w, grad_out);
+  const int vec = pick_vec(C, {grad_out}) == 8 && aligned(x_codes, 8) ? 8 : 1;
+  fmhc::launch_k3_bwd_q8(grad_out, x_codes, x_scales, format, grad_h, T, int(C), vec, (cudaStream_t)stream);
+  return check_launch(w);
+}
+
+int fmhc_k4_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scales,
+                   const void *lo_codes, const void *lo_scales, int format, const float *h_post,
+                   void *grad_lo, float *grad_H, float *grad_hp, int64_t T, int64_t n, int64_t C,
+                   void *stream) {
+  const char *w = "fmhc_k4_bwd_q8";
+  if (int e = check_streams(w, T, n, C)) return e;
+  FMHC_REQUIRE_FMT(w, format);
+  if (T == 0) return ok();
+  FMHC_REQUIRE_PTR(w, grad_out); FMHC_REQUIRE_PTR(w, x_codes); FMHC_REQUIRE_PTR(w, x_scales);
+  FMHC_REQUIRE_PTR(w, lo_codes); FMHC_REQUIRE_PTR(w, lo_scales); FMHC_REQUIRE_PTR(w, h_post);
+  FMHC_REQUIRE_PTR(w, grad_lo); FMHC_REQUIRE_PTR(w, grad_H); FMHC_REQUIRE_PTR(w, grad_hp);
+  FMHC_REQUIRE_ALIGN16(w, h_post); FMHC_REQUIRE_ALIGN16(w, grad_H); FMHC_REQUIRE_ALIGN16(w, grad_hp);
+  FMHC_REQUIRE_ALIGN2(w, grad_out); FMHC_REQUIRE_ALIGN2(w, grad_lo);
+  const int vec = pick_vec(C, {grad_out, grad_lo}) == 8 && aligned(x_codes, 8) && aligned(lo_codes, 8) ? 8 : 1;
+  fmhc::launch_k4_bwd_q8(grad_out, x_codes, x_scales, lo_codes, lo_scales, format, h_post, grad_lo,
+                         grad_H, grad_hp, T, int(C), vec, (cudaStream_t)stream);
+  return check_launch(w);
+}
+
+int64_t fmhc_k1_bwd_q8_workspace_size(int64_t T, int64_t C) {
+  if (T <= 0 || C <= 0 || C > (int64_t(1) << 26)) return 0;
+  return ((T * 4 * C * 2 + 255) & ~int64_t(255)) + fmhc_k1_bwd_workspace_size(T, 4 * C, 32);
+}
+
+int fmhc_k1_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scales, int format,
+                   const void *W, const void *proj, const float *inv_rms, void *grad_x,
+                   void *grad_W, void *workspace, int64_t workspace_bytes, int64_t T, int64_t n,
+                   int64_t C, void *stream) {
+  const char *w = "fmhc_k1_bwd_q8";
+  if (int e = check_streams(w, T, n, C)) return e;
+  if (int e = check_k1(w, T, n * C, 32)) return e;
+  FMHC_REQUIRE_FMT(w, format);
+  FMHC_REQUIRE_PTR(w, grad_W);
+  cudaStream_t s = (cudaStream_t)stream;
+  if (T == 0) return fmhc_k1_bwd(nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, grad_W, nullptr,
+                                 0, 0, n * C, 32, stream);
+  FMHC_REQUIRE_PTR(w, x_codes); FMHC_REQUIRE_PTR(w, x_scales); FMHC_REQUIRE_PTR(w, workspace);
+  if (!aligned(workspace, 256)) return fail(FMHC_ERR_ALIGNMENT, "%s: workspace must be 256-byte aligned", w);
+  const int64_t need = fmhc_k1_bwd_q8_workspace_size(T, C);
+  if (workspace_bytes < need)
+    return fail(FMHC_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", w,
+                (long long)workspace_bytes, (long long)need);
+  const int64_t x_bytes = (T * 4 * C * 2 + 255) & ~int64_t(255);
+  fmhc::launch_act_dequantize(x_codes, format, x_scales, workspace, FMHC_DTYPE_BF16, 4 * T, int(C),
+                              C % 8 == 0 && aligned(x_codes, 8), s);
+  return fmhc_k1_bwd(grad_out, workspace, W, proj, inv_rms, grad_x, grad_W,
+                     (char *)workspace + x_bytes, workspace_bytes - x_bytes, T, n * C, 32, stream);
+}
+
+// ------------------------------------------------------------------ layer norm
+int fmhc_layer_norm_fwd(const void *x, int x_dtype, const void *weight, const void *bias,
+                        int param_dtype, float eps, void *y, float *mean, float *rstd,
+                        void *x_codes, int format, void *x_scales, int64_t rows, int64_t C,
+                        void *stream) {
+  const char *w = "fmhc_layer_norm_fwd";
+  if (int e = check_rows(w, rows, C)) return e;
+  FMHC_REQUIRE_DTYPE(w, x_dtype);
+  FMHC_REQUIRE_DTYPE(w, param_dtype);
+  if (!(eps >= 0.f)) return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: eps must be >= 0", w);
+  if (x_codes != nullptr) FMHC_REQUIRE_FMT(w, format);
+  if ((x_codes == nullptr) != (x_scales == nullptr))
+    return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: x_codes and x_scales go together", w);
+  if (rows == 0) return ok();
+  FMHC_REQUIRE_PTR(w, x); FMHC_REQUIRE_PTR(w, y); FMHC_REQUIRE_PTR(w, mean); FMHC_REQUIRE_PTR(w, rstd);
+  FMHC_REQUIRE_ALIGN_TO(w, x, dtype_size(x_dtype)); FMHC_REQUIRE_ALIGN_TO(w, y, dtype_size(x_dtype));
+  FMHC_REQUIRE_ALIGN_TO(w, weight, dtype_size(param_dtype));
+  FMHC_REQUIRE_ALIGN_TO(w, bias, dtype_size(param_dtype));
+  FMHC_REQUIRE_ALIGN_TO(w, mean, 4); FMHC_REQUIRE_ALIGN_TO(w, rstd, 4);
+  const bool vec = aligned(x, 16) && aligned(y, 16) && aligned(weight, 16) && aligned(bias, 16) &&
+                   aligned(x_codes, 8);
+  fmhc::launch_ln_fwd(x, x_dtype, weight, bias, param_dtype, eps, y, mean, rstd, x_codes,
+                      x_codes ? format : -1, x_scales, rows, int(C), vec, (cudaStream_t)stream);
+  return check_launch(w);
+}
+
+int64_t fmhc_layer_norm_bwd_workspace_size(int64_t rows, int64_t C) {
+  if (rows <= 0 || C <= 0 || C > (int64_t(1) << 28)) return 0;
+  return fmhc::ln_bwd_workspace_bytes(rows, int(C));
+}
+
+int fmhc_layer_norm_bwd(const void *grad_y, int x_dtype, const void *x, const void *x_codes,
+                        int format, const void *x_scales, const float *mean, const float *rstd,
+                        const void *weight, int param_dtype, void *grad_x, void *grad_weight,
+                        void *grad_bias, void *workspace, int64_t workspace_bytes, int64_t rows,
+                        int64_t C, void *stream) {
+  const char *w = "fmhc_layer_norm_bwd";
+  if (int e = check_rows(w, rows, C)) return e;
+  FMHC_REQUIRE_DTYPE(w, x_dtype);
+  FMHC_REQUIRE_DTYPE(w, param_dtype);
+  if (x_codes != nullptr) FMHC_REQUIRE_FMT(w, format);
+  if ((x_codes == nullptr) != (x_scales == nullptr))
+    return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: x_codes and x_scales go together", w);
+  FMHC_REQUIRE_ALIGN_TO(w, grad_weight, dtype_size(param_dtype));
+  FMHC_REQUIRE_ALIGN_TO(w, grad_bias, dtype_size(param_dtype));
+  cudaStream_t s = (cudaStream_t)stream;
+  if (rows == 0) {
+    // No rows: the parameters' gradients are exactly zero.
+    for (void *p : {grad_weight, grad_bias})
+      if (p != nullptr && cudaMemsetAsync(p, 0, size_t(C) * dtype_size(param_dtype), s) != cudaSuccess)
+        return fail(FMHC_ERR_CUDA, "%s: cudaMemsetAsync failed", w);
+    return ok();
+  }
+  if ((x == nullptr) == (x_codes == nullptr))
+    return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: exactly one of x and x_codes is wanted", w);
+  FMHC_REQUIRE_PTR(w, grad_y); FMHC_REQUIRE_PTR(w, mean); FMHC_REQUIRE_PTR(w, rstd);
+  FMHC_REQUIRE_PTR(w, grad_x);
+  FMHC_REQUIRE_ALIGN_TO(w, grad_y, dtype_size(x_dtype)); FMHC_REQUIRE_ALIGN_TO(w, x, dtype_size(x_dtype));
+  FMHC_REQUIRE_ALIGN_TO(w, grad_x, dtype_size(x_dtype));
+  FMHC_REQUIRE_ALIGN_TO(w, weight, dtype_size(param_dtype));
+  FMHC_REQUIRE_ALIGN_TO(w, mean, 4); FMHC_REQUIRE_ALIGN_TO(w, rstd, 4);
+  if (grad_weight != nullptr || grad_bias != nullptr) {
+    FMHC_REQUIRE_PTR(w, workspace);
+    if (!aligned(workspace, 256)) return fail(FMHC_ERR_ALIGNMENT, "%s: workspace must be 256-byte aligned", w);
+    const int64_t need = fmhc_layer_norm_bwd_workspace_size(rows, C);
+    if (workspace_bytes < need)
+      return fail(FMHC_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", w,
+                  (long long)workspace_bytes, (long long)need);
+  }
+  const bool vec = aligned(grad_y, 16) && aligned(x, 16) && aligned(x_codes, 8) && aligned(weight, 16) &&
+                   aligned(grad_x, 16);
+  fmhc::launch_ln_bwd(grad_y, x_dtype, x_codes ? x_codes : x, x_codes ? format : -1, x_scales, mean,
+                      rstd, weight, param_dtype, grad_x, grad_weight, grad_bias, (float *)workspace,
+                      rows, int(C), vec, s);
+  return check_launch(w);
+}
+
 }  // extern "C"

@@ -77,4 +77,38 @@ void launch_k2_bwd(const void *proj, const K2Params &P, const float *g_hpre, con
                    const float *g_H, void *g_proj, const K2ParamGrads &Gp, float *ws, int64_t T,
                    cudaStream_t s);
 
+// act8.cu -- 8-bit activation checkpoints (format: act8.cuh).  dtype: enum
+// fmhc_dtype, fmt: enum fmhc_act8_format.  `vec`: C % 8 == 0, 16-byte aligned x
+// and 8-byte aligned codes.
+void launch_act_quantize(const void *x, int dtype, void *codes, int fmt, void *scales, int64_t rows,
+                         int C, bool vec, cudaStream_t s);
+void launch_act_dequantize(const void *codes, int fmt, const void *scales, void *x, int dtype,
+                           int64_t rows, int C, bool vec, cudaStream_t s);
+
+// act8_streams.cu -- K3 and K4 that write or read 8-bit checkpoints.  The
+// forwards need C % 8 == 0, 16-byte aligned bf16 rows and 8-byte aligned codes
+// (else: launch_k3_fwd / launch_k4_fwd and launch_act_quantize); the backwards
+// take vec 8 under the same conditions, or 1.
+void launch_k3_fwd_q8(const void *x, const float *hp, void *out, void *codes, void *scales, int fmt,
+                      int64_t T, int C, cudaStream_t s);
+void launch_k4_fwd_q8(const void *x, const void *lo, const float *H, const float *hp, void *out,
+                      void *codes, void *scales, int fmt, int64_t T, int C, cudaStream_t s);
+void launch_k3_bwd_q8(const void *go, const void *codes, const void *scales, int fmt, float *gh,
+                      int64_t T, int C, int vec, cudaStream_t s);
+void launch_k4_bwd_q8(const void *go, const void *xc, const void *xs, const void *lc,
+                      const void *ls, int fmt, const float *hp, void *glo, float *gH, float *ghp,
+                      int64_t T, int C, int vec, cudaStream_t s);
+
+// layer_norm.cu -- rows of C values of type dtype; w and b (either may be null)
+// of type pdt.  fmt -1: x as it is (codes, scales null); else the forward also
+// writes x in 8 bits and the backward reads codes as its x.  `vec`: every row
+// pointer and w, b 16-byte aligned (codes 8-byte); the width is checked here.
+void launch_ln_fwd(const void *x, int dtype, const void *w, const void *b, int pdt, float eps,
+                   void *y, float *mean, float *rstd, void *codes, int fmt, void *scales,
+                   int64_t rows, int C, bool vec, cudaStream_t s);
+int64_t ln_bwd_workspace_bytes(int64_t rows, int C);
+void launch_ln_bwd(const void *g, int dtype, const void *x, int fmt, const void *scales,
+                   const float *mean, const float *rstd, const void *w, int pdt, void *gx, void *gw,
+                   void *gb, float *ws, int64_t rows, int C, bool vec, cudaStream_t s);
+
 }  // namespace fmhc

@@ -1,0 +1,46 @@
+// Grid size of the persistent streaming kernels.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <mutex>
+
+namespace fmhc {
+
+// Resident blocks per SM of `kernel` and the SM count, cached for the process
+// (occupancy queries and attribute reads stay out of CUDA-graph captures and
+// out of the per-launch cost).  T units of work, one per warp.
+template <class K>
+int grid_for(K kernel, int64_t T, int threads) {
+  struct Entry {
+    const void *k;
+    int dev, per_sm, sms;
+  };
+  static std::mutex mu;
+  static Entry cache[64];
+  static int used = 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int per_sm = 0, sms = 0;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    for (int i = 0; i < used; ++i)
+      if (cache[i].k == reinterpret_cast<const void *>(kernel) && cache[i].dev == dev) {
+        per_sm = cache[i].per_sm;
+        sms = cache[i].sms;
+      }
+    if (sms == 0) {
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0);
+      if (per_sm < 1) per_sm = 1;
+      if (used < 64) cache[used++] = Entry{reinterpret_cast<const void *>(kernel), dev, per_sm, sms};
+    }
+  }
+  const int64_t warps_per_block = threads / 32;
+  const int64_t need = (T + warps_per_block - 1) / warps_per_block;
+  const int64_t cap = int64_t(sms) * per_sm;
+  return int(need < cap ? need : cap);
+}
+
+}  // namespace fmhc

@@ -21,6 +21,7 @@ _lib = None
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
+_int = ctypes.c_int
 
 # name -> argtypes (restype int unless listed in _RESTYPES)
 _SIGNATURES = {
@@ -47,12 +48,28 @@ _SIGNATURES = {
     "fmhc_mhc_grad_x_combine_post": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp],
     "fmhc_k4_fwd": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp],
     "fmhc_k4_bwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp],
+    "fmhc_act_quantize": [_vp, _int, _vp, _int, _vp, _i64, _i64, _vp],
+    "fmhc_act_dequantize": [_vp, _int, _vp, _vp, _int, _i64, _i64, _vp],
+    "fmhc_k3_fwd_q8": [_vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp],
+    "fmhc_k4_fwd_q8": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp],
+    "fmhc_k3_bwd_q8": [_vp, _vp, _vp, _int, _vp, _i64, _i64, _i64, _vp],
+    "fmhc_k4_bwd_q8": [_vp, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp],
+    "fmhc_k1_bwd_q8_workspace_size": [_i64, _i64],
+    "fmhc_k1_bwd_q8": [_vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                       _vp],
+    "fmhc_layer_norm_fwd": [_vp, _int, _vp, _vp, _int, ctypes.c_float, _vp, _vp, _vp, _vp, _int,
+                            _vp, _i64, _i64, _vp],
+    "fmhc_layer_norm_bwd_workspace_size": [_i64, _i64],
+    "fmhc_layer_norm_bwd": [_vp, _int, _vp, _vp, _int, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp,
+                            _i64, _i64, _i64, _vp],
 }
 _RESTYPES = {
     "fmhc_last_error": ctypes.c_char_p,
     "fmhc_version": ctypes.c_char_p,
     "fmhc_k1_bwd_workspace_size": _i64,
     "fmhc_k2_bwd_workspace_size": _i64,
+    "fmhc_k1_bwd_q8_workspace_size": _i64,
+    "fmhc_layer_norm_bwd_workspace_size": _i64,
 }
 
 STATUS = {

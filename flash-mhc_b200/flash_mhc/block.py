@@ -21,7 +21,13 @@ the backward to avoid storing layer_input and the block output; the fused path
 never stores those either, so the flag leaves its memory and results unchanged
 and skips the recomputation.  Every other input takes the pure-PyTorch path
 (which is also what runs on CPU), with the flag honoured through torch
-checkpointing exactly as in the reference.  The constructor argument keeps its
+checkpointing exactly as in the reference.
+
+``checkpoint_format="int8"`` or ``"e4m3"`` (not in the reference) makes the fused
+path keep x and the layer output in 8 bits (``flash_mhc.act8``) from the forward
+to the backward: ~5.2 C bytes per token instead of 10 C.  The block's output is
+unchanged to the bit; gradients are those of the rounded activations.  It has no
+effect without a graph or on the pure-PyTorch path.  The constructor argument keeps its
 reference name ``triton_fused``; here it selects the CUDA kernels.
 """
 
@@ -36,6 +42,7 @@ import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint as _checkpoint
 
 from . import ops as _ops  # noqa: F401  (registers torch.ops.flash_mhc.*)
+from .act8 import FORMATS as _ACT8_FORMATS
 
 
 class _StreamGrad:
@@ -122,6 +129,64 @@ class _FusedPostRes(torch.autograd.Function):
         return None, glo, gH, ghp, None
 
 
+class _FusedPreMapQ8(torch.autograd.Function):
+    """_FusedPreMap that keeps x in 8 bits: K3's forward writes the codes of the
+    x it reads, and K3's grad_h and K1's backward read them in x's place.  The
+    codes are handed on to K4's function, so a layer keeps them once.
+    """
+
+    @staticmethod
+    def forward(ctx, x, W, a_pre, a_post, a_res, bias, perm, slot, fmt):
+        layer_input, proj, inv, h_pre, h_post, H, xc, xs = torch.ops.flash_mhc.mhc_pre_forward_q8(
+            x, W, a_pre, a_post, a_res, bias, perm, fmt)
+        ctx.save_for_backward(xc, xs, W, proj, inv, h_pre, a_pre, a_post, a_res, bias, perm)
+        ctx.mark_non_differentiable(xc, xs)
+        ctx.set_materialize_grads(False)  # no zeros in the size of the codes
+        ctx.slot = slot
+        return layer_input, H, h_post, xc, xs
+
+    @staticmethod
+    def backward(ctx, g_li, g_H, g_hpost, _g_xc, _g_xs):
+        ops = torch.ops.flash_mhc
+        xc, xs, W, proj, inv, h_pre, a_pre, a_post, a_res, bias, perm = ctx.saved_tensors
+        T, _, C = xc.shape
+        z = lambda *s: torch.zeros(*s, device=xc.device, dtype=torch.float32)  # noqa: E731
+        if g_li is None:
+            g_li = torch.zeros((T, C), device=xc.device, dtype=proj.dtype)
+        g_hpre = ops.pre_map_grad_h_q8(g_li, xc, xs)
+        g_proj, ga_pre, ga_post, ga_res, g_bias = ops.mhc_coeffs_backward_split(
+            g_hpre, z(T, 4) if g_hpost is None else g_hpost, z(T, 4, 4) if g_H is None else g_H, proj,
+            a_pre, a_post, a_res, bias, perm)
+        gx1, gW = ops.fused_rmsnorm_project_backward_q8(g_proj, xc, xs, W, proj, inv)
+        g_out, H = ctx.slot.g_out, ctx.slot.H
+        ctx.slot.g_out = ctx.slot.H = None
+        if g_out is None:
+            gx = ops.mhc_grad_x_combine(gx1, g_li, h_pre, None)
+        else:
+            gx = ops.mhc_grad_x_combine_post(gx1, g_li, h_pre, g_out, H)
+        return gx, gW, ga_pre, ga_post, ga_res, g_bias, None, None, None
+
+
+class _FusedPostResQ8(torch.autograd.Function):
+    """_FusedPostRes that keeps the layer output in 8 bits (written by K4's
+    forward) and takes x's codes from the pre-map."""
+
+    @staticmethod
+    def forward(ctx, x, layer_output, H_merged, h_post, xc, xs, slot, fmt):
+        out, lc, ls = torch.ops.flash_mhc.fused_post_res_q8(x, layer_output, H_merged, h_post, fmt)
+        ctx.save_for_backward(xc, xs, lc, ls, H_merged, h_post)
+        ctx.slot = slot
+        return out
+
+    @staticmethod
+    def backward(ctx, g_out):
+        xc, xs, lc, ls, H, hp = ctx.saved_tensors
+        g_out = g_out.contiguous()
+        glo, gH, ghp = torch.ops.flash_mhc.post_res_grad_params_q8(g_out, xc, xs, lc, ls, hp)
+        ctx.slot.g_out, ctx.slot.H = g_out, H
+        return None, glo, gH, ghp, None, None, None, None
+
+
 def build_permutation_matrices(n: int) -> tuple[torch.Tensor, int]:
     """All n! permutation matrices, flattened row-major to (n!, n*n), in
     itertools.permutations order; index 0 is the identity."""
@@ -146,14 +211,19 @@ class MHCLiteBlock(nn.Module):
         layer: nn.Module,
         triton_fused: bool = True,
         activation_checkpointing: bool = False,
+        checkpoint_format: str | None = None,
     ) -> None:
         super().__init__()
+        if checkpoint_format is not None and checkpoint_format not in _ACT8_FORMATS:
+            raise ValueError(f"MHCLiteBlock: checkpoint_format must be None or one of "
+                             f"{sorted(_ACT8_FORMATS)} (got {checkpoint_format!r})")
         self.n = n_streams
         self.C = hidden_size
         self.nC = n_streams * hidden_size
         self.layer = layer
         self.triton_fused = triton_fused
         self.activation_checkpointing = activation_checkpointing
+        self.checkpoint_format = checkpoint_format
         self.n_fact = math.factorial(n_streams)
 
         self.alpha_pre = nn.Parameter(torch.tensor([0.01]))
@@ -270,9 +340,19 @@ class MHCLiteBlock(nn.Module):
         # No torch checkpointing here: the fused autograd functions already keep
         # only the small per-token tensors their backward kernels read.
         slot = _StreamGrad()
+        if self.checkpoint_format is not None:
+            return self._forward_fused_q8(x_streams, slot, **kwargs)
         layer_input, H_merged, h_post = self._mhc_pre_map_triton(x_streams, slot)
         layer_output = self.layer(layer_input, **kwargs)
         return self._mhc_post_res_triton(x_streams, layer_output, H_merged, h_post, slot)
+
+    def _forward_fused_q8(self, x_streams: torch.Tensor, slot, **kwargs) -> torch.Tensor:
+        fmt = self.checkpoint_format
+        layer_input, H_merged, h_post, xc, xs = _FusedPreMapQ8.apply(
+            x_streams, self.W_all.weight.to(x_streams.dtype), self.alpha_pre, self.alpha_post,
+            self.alpha_res, self.W_all.bias, self.perm_mat, slot, fmt)
+        layer_output = self.layer(layer_input, **kwargs)
+        return _FusedPostResQ8.apply(x_streams, layer_output, H_merged, h_post, xc, xs, slot, fmt)
 
     # The reference name is kept above; this alias says what runs.
     _forward_fused = _forward_triton

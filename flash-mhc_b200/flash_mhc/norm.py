@@ -1,0 +1,253 @@
+"""Layer norm for the layers that an mHC-lite block wraps: forward, backward, and an 8-bit input checkpoint.
+
+* ops ``layer_norm`` / ``layer_norm_backward``: y, mean and rstd; the gradients
+  of x, weight and bias in one pass over x and the output's gradient.
+* ops ``layer_norm_q8`` / ``layer_norm_backward_q8``: the same with the input
+  kept in 8 bits (``flash_mhc.act8``) in x's place.  The forward's y is that of
+  ``layer_norm``; only what the backward reads as x is rounded.
+* :func:`layer_norm` and :class:`LayerNorm`: the differentiable function and the
+  module (parameters and state_dict of ``torch.nn.LayerNorm``).
+
+The rows are the last dimension; x is float32, bfloat16 or float16, weight and
+bias (either may be missing) any of these, of one type.  ``mean`` and ``rstd``
+are not differentiable outputs.
+"""
+
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from . import _native
+from .act8 import _DTYPES, _act, _checkpoint, _format, _new_checkpoint, _rows, _same_device, _shape
+from .ops import _lib, _on_device, _stream
+
+_lib.define(
+    "layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor y, Tensor mean, Tensor rstd)"
+)
+_lib.define(
+    "layer_norm_q8(Tensor x, Tensor? weight, Tensor? bias, float eps, str format) -> (Tensor y, Tensor mean, Tensor rstd, Tensor codes, Tensor scales)"
+)
+# grad_weight and grad_bias are empty where the parameter is missing.
+_lib.define(
+    "layer_norm_backward(Tensor grad_out, Tensor x, Tensor mean, Tensor rstd, Tensor? weight, Tensor? bias) -> (Tensor grad_x, Tensor grad_weight, Tensor grad_bias)"
+)
+_lib.define(
+    "layer_norm_backward_q8(Tensor grad_out, Tensor codes, Tensor scales, Tensor mean, Tensor rstd, Tensor? weight, Tensor? bias) -> (Tensor grad_x, Tensor grad_weight, Tensor grad_bias)"
+)
+
+
+def _params(op: str, C: int, weight, bias):
+    """weight and bias as contiguous (C,) tensors of one type, and that type's FMHC_DTYPE_*."""
+    dt = 0
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None:
+            _shape(op, name, p, (C,))
+            if p.dtype not in _DTYPES:
+                raise ValueError(f"flash_mhc::{op}: {name} must be float32, bfloat16 or float16 (got {p.dtype})")
+            dt = _DTYPES[p.dtype]
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError(f"flash_mhc::{op}: weight and bias must have one type (got {weight.dtype} and {bias.dtype})")
+    return (None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), dt)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stats(op: str, mean, rstd, rows_shape):
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        _shape(op, name, t, rows_shape)
+        if t.dtype != torch.float32:
+            raise ValueError(f"flash_mhc::{op}: {name} must be float32 (got {t.dtype})")
+    return mean.contiguous(), rstd.contiguous()
+
+
+def _forward(op: str, x, weight, bias, eps: float, format=None):
+    x = _act(op, "x", x)
+    _same_device(op, x, weight=weight, bias=bias)
+    weight, bias, pdt = _params(op, x.shape[-1], weight, bias)
+    y = torch.empty_like(x)
+    mean = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    fmt, codes, scales = -1, None, None
+    if format is not None:
+        fmt, code_dtype = _format(op, format)
+        codes, scales = _new_checkpoint(x, code_dtype)
+    with _on_device(x):
+        _native.call("fmhc_layer_norm_fwd", x.data_ptr(), _DTYPES[x.dtype], _ptr(weight), _ptr(bias),
+                     pdt, eps, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(codes), fmt,
+                     _ptr(scales), _rows(x), x.shape[-1], _stream(x))
+    return (y, mean, rstd) if format is None else (y, mean, rstd, codes, scales)
+
+
+def _backward(op: str, grad_out, x, codes, scales, mean, rstd, weight, bias):
+    grad_out = _act(op, "grad_out", grad_out)
+    _same_device(op, grad_out, x=x, codes=codes, scales=scales, mean=mean, rstd=rstd, weight=weight,
+                 bias=bias)
+    fmt = -1
+    if codes is None:
+        _shape(op, "x", x, grad_out.shape)
+        if x.dtype != grad_out.dtype:
+            raise ValueError(f"flash_mhc::{op}: grad_out and x must have one type (got {grad_out.dtype} and {x.dtype})")
+        x = x.contiguous()
+    else:
+        _shape(op, "codes", codes, grad_out.shape)
+        codes, scales, fmt = _checkpoint(op, "the", codes, scales)
+    mean, rstd = _stats(op, mean, rstd, grad_out.shape[:-1])
+    C, rows = grad_out.shape[-1], _rows(grad_out)
+    weight, bias, pdt = _params(op, C, weight, bias)
+    grad_x = torch.empty_like(grad_out)
+    none = lambda: torch.empty(0, device=grad_out.device, dtype=torch.float32)  # noqa: E731
+    grad_w = none() if weight is None else torch.empty_like(weight)
+    grad_b = none() if bias is None else torch.empty_like(bias)
+    with _on_device(grad_out):
+        ws, ws_bytes = None, 0
+        if weight is not None or bias is not None:
+            ws_bytes = int(_native.lib().fmhc_layer_norm_bwd_workspace_size(rows, C))
+            ws = torch.empty(max(ws_bytes, 1), device=grad_out.device, dtype=torch.uint8)
+        _native.call("fmhc_layer_norm_bwd", grad_out.data_ptr(), _DTYPES[grad_out.dtype], _ptr(x),
+                     _ptr(codes), fmt, _ptr(scales), mean.data_ptr(), rstd.data_ptr(), _ptr(weight),
+                     pdt, grad_x.data_ptr(), None if weight is None else grad_w.data_ptr(),
+                     None if bias is None else grad_b.data_ptr(), _ptr(ws), ws_bytes, rows, C,
+                     _stream(grad_out))
+    return grad_x, grad_w, grad_b
+
+
+# -------------------------------------------------------------------- fakes
+
+
+@torch.library.register_fake("flash_mhc::layer_norm")
+def _layer_norm_fake(x, weight, bias, eps):
+    stats = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    return torch.empty(x.shape, device=x.device, dtype=x.dtype), stats, torch.empty_like(stats)
+
+
+@torch.library.register_fake("flash_mhc::layer_norm_q8")
+def _layer_norm_q8_fake(x, weight, bias, eps, format):
+    return (*_layer_norm_fake(x, weight, bias, eps),
+            *_new_checkpoint(x, _format("layer_norm_q8", format)[1]))
+
+
+@torch.library.register_fake("flash_mhc::layer_norm_backward")
+def _layer_norm_backward_fake(grad_out, x, mean, rstd, weight, bias):
+    none = lambda: torch.empty(0, device=grad_out.device, dtype=torch.float32)  # noqa: E731
+    return (torch.empty(grad_out.shape, device=grad_out.device, dtype=grad_out.dtype),
+            none() if weight is None else torch.empty_like(weight),
+            none() if bias is None else torch.empty_like(bias))
+
+
+@torch.library.register_fake("flash_mhc::layer_norm_backward_q8")
+def _layer_norm_backward_q8_fake(grad_out, codes, scales, mean, rstd, weight, bias):
+    return _layer_norm_backward_fake(grad_out, codes, mean, rstd, weight, bias)
+
+
+# --------------------------------------------------------------------- CUDA
+
+
+@torch.library.impl(_lib, "layer_norm", "CUDA")
+def _layer_norm_cuda(x, weight, bias, eps):
+    return _forward("layer_norm", x, weight, bias, eps)
+
+
+@torch.library.impl(_lib, "layer_norm_q8", "CUDA")
+def _layer_norm_q8_cuda(x, weight, bias, eps, format):
+    return _forward("layer_norm_q8", x, weight, bias, eps, format)
+
+
+@torch.library.impl(_lib, "layer_norm_backward", "CUDA")
+def _layer_norm_backward_cuda(grad_out, x, mean, rstd, weight, bias):
+    return _backward("layer_norm_backward", grad_out, x, None, None, mean, rstd, weight, bias)
+
+
+@torch.library.impl(_lib, "layer_norm_backward_q8", "CUDA")
+def _layer_norm_backward_q8_cuda(grad_out, codes, scales, mean, rstd, weight, bias):
+    return _backward("layer_norm_backward_q8", grad_out, None, codes, scales, mean, rstd, weight, bias)
+
+
+# ------------------------------------------------------------------ autograd
+
+
+def _setup(ctx, inputs, output):
+    x, weight, bias = inputs[:3]
+    ctx.save_for_backward(x, output[1], output[2], weight, bias)
+    ctx.mark_non_differentiable(*output[1:])
+    ctx.set_materialize_grads(False)
+
+
+def _setup_q8(ctx, inputs, output):
+    _, weight, bias = inputs[:3]
+    ctx.save_for_backward(output[3], output[4], output[1], output[2], weight, bias)
+    ctx.mark_non_differentiable(*output[1:])
+    ctx.set_materialize_grads(False)  # no zeros in the size of the codes
+
+
+def _grads(ctx, gy, op):
+    if gy is None:
+        return None, None, None
+    gx, gw, gb = op(gy, *ctx.saved_tensors)
+    need = ctx.needs_input_grad
+    return gx if need[0] else None, gw if need[1] else None, gb if need[2] else None
+
+
+def _autograd(ctx, gy, *_):
+    return (*_grads(ctx, gy, torch.ops.flash_mhc.layer_norm_backward), None)
+
+
+def _autograd_q8(ctx, gy, *_):
+    return (*_grads(ctx, gy, torch.ops.flash_mhc.layer_norm_backward_q8), None, None)
+
+
+torch.library.register_autograd("flash_mhc::layer_norm", _autograd, setup_context=_setup)
+torch.library.register_autograd("flash_mhc::layer_norm_q8", _autograd_q8, setup_context=_setup_q8)
+
+
+# ---------------------------------------------------------------- public names
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-5, checkpoint_format: str | None = None) -> torch.Tensor:
+    """Layer norm over the last dimension of a CUDA tensor, differentiable in x, weight and bias.
+
+    With ``checkpoint_format`` ("int8" or "e4m3") a call that records a graph
+    keeps x in 8 bits for the backward pass instead of x itself.
+    """
+    if checkpoint_format is not None:
+        _format("layer_norm", checkpoint_format)
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+            return torch.ops.flash_mhc.layer_norm_q8(x, weight, bias, eps, checkpoint_format)[0]
+    return torch.ops.flash_mhc.layer_norm(x, weight, bias, eps)[0]
+
+
+class LayerNorm(nn.Module):
+    """``torch.nn.LayerNorm`` over the last dimension, with the same parameters and state_dict.
+
+    CUDA inputs of float32, bfloat16 or float16 take the fused kernels (and keep
+    their input in ``checkpoint_format``, if given); every other input takes
+    ``torch.nn.functional.layer_norm``, which keeps it as it is.
+    """
+
+    def __init__(self, hidden_size: int, eps: float = 1e-5, elementwise_affine: bool = True,
+                 bias: bool = True, checkpoint_format: str | None = None, device=None,
+                 dtype=None) -> None:
+        super().__init__()
+        if checkpoint_format is not None:
+            _format("layer_norm", checkpoint_format)
+        self.hidden_size = hidden_size
+        self.eps = eps
+        self.checkpoint_format = checkpoint_format
+        f = dict(device=device, dtype=dtype)
+        affine = elementwise_affine
+        self.weight = nn.Parameter(torch.ones(hidden_size, **f)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(hidden_size, **f)) if affine and bias else None
+
+    def extra_repr(self) -> str:
+        return f"{self.hidden_size}, eps={self.eps}, checkpoint_format={self.checkpoint_format}"
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1:] != (self.hidden_size,):
+            raise ValueError(f"LayerNorm: expected a last dimension of {self.hidden_size} (got {tuple(x.shape)})")
+        if x.is_cuda and x.dtype in _DTYPES:
+            return layer_norm(x, self.weight, self.bias, self.eps, self.checkpoint_format)
+        return F.layer_norm(x, (self.hidden_size,), self.weight, self.bias, self.eps)

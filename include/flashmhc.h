@@ -252,8 +252,8 @@ FMHC_API int fmhc_k2_fwd(const void *proj, const float *params, const float *per
                          float *h_pre, float *h_post, float *H_merged, int64_t T,
                          void *stream);
 
-/* Element types of fmhc_k2_fwd_typed's parameter pointers. */
-enum fmhc_dtype { FMHC_DTYPE_F32 = 0, FMHC_DTYPE_BF16 = 1 };
+/* Element types (fmhc_k2_fwd_typed and fmhc_k2_bwd_typed take the first two). */
+enum fmhc_dtype { FMHC_DTYPE_F32 = 0, FMHC_DTYPE_BF16 = 1, FMHC_DTYPE_F16 = 2 };
 
 /* ------------------------------------------------------------------------
  * The same K2 forward reading the parameters where they live, in their own
@@ -320,6 +320,89 @@ FMHC_API int fmhc_k2_bwd_typed(const void *proj, const void *alpha_pre, const vo
                                void *grad_proj, void *grad_alpha_pre, void *grad_alpha_post,
                                void *grad_alpha_res, void *grad_bias, void *workspace,
                                int64_t workspace_bytes, int64_t T, void *stream);
+
+/* ------------------------------------------------------------------------
+ * 8-bit activation checkpoints.  A (rows, C) tensor is kept as codes
+ * (rows, C), one byte per value, and scales (rows, ceil(C / 32)), one byte e
+ * per block of 32 values along C (the last block of a row may be shorter),
+ * standing for 2^(e - 127).  With a the block's largest magnitude and M = 127
+ * (FMHC_ACT8_INT8: codes are int8) or 448 (FMHC_ACT8_E4M3: codes are e4m3):
+ * e is the smallest byte with a <= M 2^(e - 127), at most 248 (int8) or 246
+ * (e4m3); code = x / 2^(e - 127) rounded to nearest even, kept in [-M, M].
+ * So |restored - x| <= 2^(e - 128) for int8, and <= 2^-4 |x| or 2^(e - 137),
+ * whichever is larger, for e4m3 (below the saturation of the largest f32
+ * values).  A block with an infinity or a NaN gets e = 255 and codes 0 and is
+ * restored as NaN.  Codes and scales need no alignment (8-byte aligned codes
+ * and C % 8 == 0 select the vector path); both formats are exact in bf16.
+ * No counterpart in the reference, whose checkpoints are torch's (recompute).
+ */
+enum fmhc_act8_format { FMHC_ACT8_INT8 = 0, FMHC_ACT8_E4M3 = 1 };
+
+/* x (rows, C) of x_dtype (any of enum fmhc_dtype) -> codes, scales. */
+FMHC_API int fmhc_act_quantize(const void *x, int x_dtype, void *codes, int format,
+                               void *scales, int64_t rows, int64_t C, void *stream);
+/* codes, scales -> x, rounded once to x_dtype (f16: kept within +-65504). */
+FMHC_API int fmhc_act_dequantize(const void *codes, int format, const void *scales, void *x,
+                                 int x_dtype, int64_t rows, int64_t C, void *stream);
+
+/* fmhc_k3_fwd (out bit-identical to it) that also writes x (T, n, C) in 8 bits:
+ * x_codes (T, n, C), x_scales (T, n, ceil(C / 32)). */
+FMHC_API int fmhc_k3_fwd_q8(const void *x, const float *h_pre, void *out, void *x_codes,
+                            void *x_scales, int format, int64_t T, int64_t n, int64_t C,
+                            void *stream);
+/* fmhc_k4_fwd (out bit-identical to it) that also writes lo (T, C) in 8 bits. */
+FMHC_API int fmhc_k4_fwd_q8(const void *x, const void *lo, const float *H,
+                            const float *h_post, void *out, void *lo_codes, void *lo_scales,
+                            int format, int64_t T, int64_t n, int64_t C, void *stream);
+/* fmhc_k3_bwd's grad_h from a checkpoint: grad_h[t,j] = sum_c x8[t,j,c] go[t,c],
+ * x8 the restored x. */
+FMHC_API int fmhc_k3_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scales,
+                            int format, float *grad_h, int64_t T, int64_t n, int64_t C,
+                            void *stream);
+/* fmhc_k4_bwd without grad_x, from checkpoints of x and lo in one format. */
+FMHC_API int fmhc_k4_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scales,
+                            const void *lo_codes, const void *lo_scales, int format,
+                            const float *h_post, void *grad_lo, float *grad_H, float *grad_hp,
+                            int64_t T, int64_t n, int64_t C, void *stream);
+/* fmhc_k1_bwd from a checkpoint of x (T, n, C), D = 32: grad_x (T, n, C) and
+ * grad_W (32, nC).  `workspace` as fmhc_k1_bwd's, of at least
+ * fmhc_k1_bwd_q8_workspace_size(T, C) bytes. */
+FMHC_API int64_t fmhc_k1_bwd_q8_workspace_size(int64_t T, int64_t C);
+FMHC_API int fmhc_k1_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scales,
+                            int format, const void *W, const void *proj,
+                            const float *inv_rms, void *grad_x, void *grad_W, void *workspace,
+                            int64_t workspace_bytes, int64_t T, int64_t n, int64_t C,
+                            void *stream);
+
+/* ------------------------------------------------------------------------
+ * Layer norm over the last dimension of x (rows, C), x_dtype any of enum
+ * fmhc_dtype:
+ *   mean = <x>, rstd = 1 / sqrt(<(x - mean)^2> + eps)            (f32, (rows,))
+ *   y    = (x - mean) rstd weight + bias                         (x_dtype)
+ * weight and bias (C,) of param_dtype; either may be NULL (1 and 0).  With
+ * x_codes and x_scales not NULL, x is also written in 8 bits, so that the
+ * backward needs neither x nor y.
+ * No counterpart in the reference (its users take torch's layer norm).
+ */
+FMHC_API int fmhc_layer_norm_fwd(const void *x, int x_dtype, const void *weight,
+                                 const void *bias, int param_dtype, float eps, void *y,
+                                 float *mean, float *rstd, void *x_codes, int format,
+                                 void *x_scales, int64_t rows, int64_t C, void *stream);
+/* Backward, with xh = (x - mean) rstd and gw = grad_y weight:
+ *   grad_x      = rstd (gw - <gw> - xh <gw xh>)                  (x_dtype)
+ *   grad_weight = sum over rows of grad_y xh, grad_bias = of grad_y  (param_dtype)
+ * from x, or from its checkpoint (x_codes, x_scales; x NULL).  grad_weight and
+ * grad_bias may be NULL; sums are f32 in a fixed order (bitwise reproducible).
+ * rows == 0 writes zero parameter gradients.  `workspace` (256-byte aligned, at
+ * least fmhc_layer_norm_bwd_workspace_size(rows, C) bytes; may be NULL when
+ * both parameter gradients are) holds per-block partial sums. */
+FMHC_API int64_t fmhc_layer_norm_bwd_workspace_size(int64_t rows, int64_t C);
+FMHC_API int fmhc_layer_norm_bwd(const void *grad_y, int x_dtype, const void *x,
+                                 const void *x_codes, int format, const void *x_scales,
+                                 const float *mean, const float *rstd, const void *weight,
+                                 int param_dtype, void *grad_x, void *grad_weight,
+                                 void *grad_bias, void *workspace, int64_t workspace_bytes,
+                                 int64_t rows, int64_t C, void *stream);
 
 #ifdef __cplusplus
 }
