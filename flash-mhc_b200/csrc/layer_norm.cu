@@ -13,17 +13,22 @@
 // mean, never as <x^2> - mean^2: each warp sums the squares about its own mean
 // and warps are joined by  M2 = sum M2_w + n_w (mean_w - mean)^2.
 //
-// One pass over the data: a team of 1..8 warps holds a row in registers (NV
-// chunks of eight values per lane), so x is read once forward, and x and g once
-// backward.  Backward, a lane keeps the same columns for every row its team
-// takes, so its share of grad_w and grad_b stays in registers until the end;
-// blocks write one partial each, and a small kernel adds the partials in block
-// order (no atomics: the same bits every time).
+// One pass over the data: a team of 1..16 warps holds a row, NV chunks of eight
+// values per lane, so x is read once forward, and x and g once backward.
+// Backward, a lane keeps the same columns for every row its team takes, so its
+// share of grad_w and grad_b stays in registers until the end; blocks write one
+// partial each, and a small kernel adds the partials in block order (no
+// atomics: the same bits every time).  Registers for those sums leave at most
+// 16 warps per SM, too few to cover HBM's latency with loads into registers
+// (a first version ran at a third of the copy rate), so the next rows are
+// prefetched into a shared-memory ring (lane_ring.cuh).
 #include "act8.cuh"
 #include "fmhc_launch.h"
 #include "grid.cuh"
+#include "lane_ring.cuh"
 
 #include <algorithm>
+#include <mutex>
 
 namespace fmhc {
 
@@ -31,11 +36,13 @@ using namespace act8;
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kMaxWarps = 16;         // per block, one block per SM
+constexpr int kMaxTeam = kMaxWarps;   // warps per row
+constexpr int kMaxNV = 4;             // chunks of eight values per lane
+constexpr int kThreads = 256;         // of the kernels for any width
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxTeam = kWarps;  // warps per row
-constexpr int kMaxNV = 4;         // chunks of eight values per lane
 constexpr int kMaxParts = 1024;
+constexpr size_t kMaxSmem = 232448 - 1024;  // dynamic, beside the static slots
 
 // w or b at column c, in the parameters' own type (fmhc_dtype); `def` if absent.
 __device__ __forceinline__ float param1(const void *p, int dtype, int64_t c, float def) {
@@ -73,83 +80,131 @@ __device__ __forceinline__ float warp_sum(float v) {
 // different numbers of rows.
 __device__ __forceinline__ float2 team_sum(float2 v, float2 *slot, int team, int warp, int lane) {
   if (team == 1) return v;
-  const int first = warp / team * team;
   if (lane == 0) slot[warp] = v;
   named_bar_sync(1 + warp / team, team * 32);
-  float2 t = slot[first];
-  for (int i = 1; i < team; ++i) {
-    const float2 o = slot[first + i];
-    t.x += o.x;
-    t.y += o.y;
-  }
-  return t;
+  const float2 o = lane < team ? slot[warp / team * team + lane] : make_float2(0.f, 0.f);
+  return make_float2(warp_sum(o.x), warp_sum(o.y));
 }
+
+// Pairs of a chunk's eight values.
+template <class E>
+__device__ __forceinline__ void widen2(const typename Elem<E>::Raw &r, float2 (&f)[4]) {
+  float v[8];
+  Elem<E>::widen(r, v);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) f[k] = make_float2(v[2 * k], v[2 * k + 1]);
+}
+__device__ __forceinline__ void param8x2(const void *p, int dtype, int c, float def, float2 (&f)[4]) {
+  float v[8];
+  param8(p, dtype, c, def, v);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) f[k] = make_float2(v[2 * k], v[2 * k + 1]);
+}
+template <class E>
+__device__ __forceinline__ void copy_raw(typename Elem<E>::Raw *dst, const E *src) {
+  copy_async<16>(dst, src);
+  if constexpr (sizeof(E) == 4) copy_async<16>(reinterpret_cast<char *>(dst) + 16, src + 4);
+}
+
+// Ring depth in rows.  16 warps x NV chunks x 32 lanes x (16 or 32 bytes).
+template <class E> constexpr int kFwdStages = sizeof(E) == 2 ? 4 : 3;
+// Most chunks per lane in the backward: its sums take 16 registers per chunk,
+// and f32 rows twice the ring.
+template <class E> constexpr int kBwdMaxNV = sizeof(E) == 2 ? kMaxNV : 2;
 
 // -------------------------------------------------------------------- forward
 template <class E, int NV, int FMT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(32 * kMaxWarps, 1)
 ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *__restrict__ b,
               int pdt, float eps, E *__restrict__ y, float *__restrict__ mean_out,
               float *__restrict__ rstd_out, uint8_t *__restrict__ codes,
               uint8_t *__restrict__ scales, int64_t rows, int C, int team) {
-  __shared__ float2 slots[2][kWarps];
-  pdl_wait();
+  using Raw = typename Elem<E>::Raw;
+  constexpr int S = kFwdStages<E>;
+  extern __shared__ uint4 dyn[];
+  __shared__ float2 slots[2][kMaxWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int teams = kWarps / team;
-  const int wt = warp % team;
+  const int teams = (blockDim.x >> 5) / team;
+  const int wt = warp % team, first = warp - wt;
   const int nchunk = C / 8, nb = (C + kBlock - 1) / kBlock;
-  // Values of this warp: chunks wt * 32 + lane + i * 32 * team below nchunk.
-  int mine = 0;
+  Raw *ring = reinterpret_cast<Raw *>(dyn) + warp * (S * NV * 32) + lane;
+  // Values of a warp of the team: chunks i * 32 + lane + v * 32 * team below nchunk.
+  const auto count = [&](int i) {
+    int n = 0;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) mine += min(max(nchunk - (wt + i * team) * 32, 0), 32) * 8;
+    for (int v = 0; v < NV; ++v) n += min(max(nchunk - (i + v * team) * 32, 0), 32) * 8;
+    return n;
+  };
+  const int mine = count(wt);
+  // Lane i joins for warp i of the team.
+  const float n_lane = lane < team ? float(count(lane)) : 0.f, inv_n = n_lane > 0.f ? 1.f / n_lane : 0.f;
   const float inv_mine = mine ? 1.f / float(mine) : 0.f, inv_C = 1.f / float(C);
-  int par = 0;
-  for (int64_t r = int64_t(blockIdx.x) * teams + warp / team; r < rows;
-       r += int64_t(gridDim.x) * teams, par ^= 1) {
-    float f[NV][8];
-    float s = 0.f;
+  const int64_t step = int64_t(gridDim.x) * teams;
+  int64_t r = int64_t(blockIdx.x) * teams + warp / team;
+  pdl_wait();
+  const auto fetch = [&](int64_t row, int stage) {
+    if (row < rows) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (wt + i * team) * 32 + lane;
+        if (c < nchunk) copy_raw<E>(ring + (stage * NV + i) * 32, x + row * C + c * 8);
+      }
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch(r + s * step, s);
+  // This lane's columns of the parameters, for every row.
+  float2 fw[NV][4], fb[NV][4];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (wt + i * team) * 32 + lane;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) fw[i][k] = fb[i][k] = both(0.f);
+    if (c < nchunk) {
+      param8x2(w, pdt, c, 1.f, fw[i]);
+      param8x2(b, pdt, c, 0.f, fb[i]);
+    }
+  }
+  int par = 0, stage = 0;
+  for (; r < rows; r += step, par ^= 1) {
+    fetch(r + (S - 1) * step, stage == 0 ? S - 1 : stage - 1);
+    copy_wait<S - 1>();
+    float2 f[NV][4];
+    float2 s2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (wt + i * team) * 32 + lane;
-      typename Elem<E>::Raw raw = {};
-      if (c < nchunk) raw = ld8(x + r * C + c * 8);
-      Elem<E>::widen(raw, f[i]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[i][k] = both(0.f);
+      if ((wt + i * team) * 32 + lane < nchunk) widen2<E>(ring[(stage * NV + i) * 32], f[i]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s2 = add2(s2, f[i][k]);
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) s += f[i][k];
-    s = warp_sum(s);
+    if (++stage == S) stage = 0;
+    const float s = warp_sum(s2.x + s2.y);
     const float m_w = s * inv_mine;
-    float q = 0.f;
+    float2 q2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if ((wt + i * team) * 32 + lane < nchunk) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) q = fmaf(f[i][k] - m_w, f[i][k] - m_w, q);
+        for (int k = 0; k < 4; ++k) {
+          const float2 d = add2(f[i][k], both(-m_w));
+          q2 = fma2(d, d, q2);
+        }
       }
-    q = warp_sum(q);
+    const float q = warp_sum(q2.x + q2.y);
     float mean = m_w, m2 = q;
     if (team > 1) {
       // Join the warps: means first, then the squares about the row's mean.
-      const int first = warp / team * team;
-      float2 *slot = slots[par];
-      if (lane == 0) slot[warp] = make_float2(s, q);
+      // One barrier per row: `slots` alternates (see team_sum).
+      float2 *slot = slots[par] + first;
+      if (lane == 0) slot[wt] = make_float2(s, q);
       named_bar_sync(1 + warp / team, team * 32);
-      float total = 0.f;
-      for (int i = 0; i < team; ++i) total += slot[first + i].x;
-      mean = total * inv_C;
-      m2 = 0.f;
-      for (int i = 0; i < team; ++i) {
-        int n = 0;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) n += min(max(nchunk - (i + v * team) * 32, 0), 32) * 8;
-        if (n) {
-          const float2 o = slot[first + i];
-          const float d = o.x / float(n) - mean;
-          m2 += fmaf(float(n) * d, d, o.y);
-        }
-      }
+      const float2 o = lane < team ? slot[lane] : make_float2(0.f, 0.f);
+      mean = warp_sum(o.x) * inv_C;
+      const float d = n_lane > 0.f ? fmaf(o.x, inv_n, -mean) : 0.f;
+      m2 = warp_sum(fmaf(n_lane * d, d, o.y));
     }
     const float rstd = rsqrtf(fmaf(m2, inv_C, eps));
     if (wt == 0 && lane == 0) {
@@ -159,18 +214,29 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (wt + i * team) * 32 + lane;
-      uint32_t e = 0;
-      if constexpr (FMT != kNone) e = scale_byte<FMT>(amax_block(amax8(f[i])));
-      if (c < nchunk) {
-        if constexpr (FMT != kNone) {
-          __stcs(reinterpret_cast<uint2 *>(codes + r * C + c * 8), encode8<FMT>(f[i], e));
+      const bool in = c < nchunk;
+      if constexpr (FMT != kNone) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[2 * k] = f[i][k].x;
+          v[2 * k + 1] = f[i][k].y;
+        }
+        const uint32_t e = scale_byte<FMT>(amax_block(amax8(v)));
+        if (in) {
+          __stcs(reinterpret_cast<uint2 *>(codes + r * C + c * 8), encode8<FMT>(v, e));
           if ((lane & 3) == 0) __stcs(scales + r * nb + (c >> 2), uint8_t(e));
         }
-        float fw[8], fb[8], o[8];
-        param8(w, pdt, c, 1.f, fw);
-        param8(b, pdt, c, 0.f, fb);
+      }
+      if (in) {
+        float o[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = fmaf((f[i][k] - mean) * rstd, fw[k], fb[k]);
+        for (int k = 0; k < 4; ++k) {
+          const float2 xh = mul2(add2(f[i][k], both(-mean)), both(rstd));
+          const float2 v = fma2(xh, fw[i][k], fb[i][k]);
+          o[2 * k] = v.x;
+          o[2 * k + 1] = v.y;
+        }
         st8(y + r * C + c * 8, o);
       }
     }
@@ -178,74 +244,179 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
 }
 
 // ------------------------------------------------------------------- backward
+// A row's chunk of eight in the backward's ring: g, and x or its codes.
+template <class E, int FMT> struct Input;
+template <class E> struct Input<E, kNone> { using X = typename Elem<E>::Raw; };
+template <class E> struct Input<E, kInt8> { using X = uint2; };
+template <class E> struct Input<E, kE4m3> { using X = uint2; };
+constexpr int kBwdStages = 3;
+
+// xh of a chunk, from x (e unused) or from codes with scale byte e.
+template <class E, int FMT>
+__device__ __forceinline__ void normalised(const typename Input<E, FMT>::X &raw, uint32_t e, float mean,
+                                           float rstd, float2 (&xh)[4]) {
+  if constexpr (FMT == kNone) {
+    widen2<E>(raw, xh);
+  } else {
+    Codes<8> q;
+    q.v = raw;
+    float v[8];
+    restore<FMT, 8>(q, scale_value(e), v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) xh[k] = make_float2(v[2 * k], v[2 * k + 1]);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) xh[k] = mul2(add2(xh[k], both(-mean)), both(rstd));
+}
+
+// The weight's columns of a lane come from shared memory as f32 (or, for rows
+// whose weight does not fit there, from global memory) twice per row; holding
+// them too would pass 128 registers.  For the same reason the second pass reads
+// g and x from the ring again.
 template <class E, int NV, int FMT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(32 * kMaxWarps, 1)
 ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
               const uint8_t *__restrict__ scales, const float *__restrict__ mean,
-              const float *__restrict__ rstd, const void *__restrict__ w, int pdt,
+              const float *__restrict__ rstd, const void *__restrict__ w, int pdt, bool w_shared,
               E *__restrict__ gx, float *__restrict__ part, int64_t rows, int C, int team) {
-  __shared__ float2 slots[2][kWarps];
-  extern __shared__ float joined[];  // [2][C], when a block has several teams
-  pdl_wait();
+  using Raw = typename Elem<E>::Raw;
+  using X = typename Input<E, FMT>::X;
+  constexpr int S = kBwdStages;
+  extern __shared__ uint4 dyn[];
+  __shared__ float2 slots[2][kMaxWarps];
+  const int warps = blockDim.x >> 5;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int teams = kWarps / team;
+  const int teams = warps / team;
   const int wt = warp % team;
   const int nchunk = C / 8, nb = (C + kBlock - 1) / kBlock;
   const float inv_C = 1.f / float(C);
-  float dw[NV][8], db[NV][8];
+  // [warps][S][NV][32] of g, the same of x, then the weight.
+  Raw *ring_g = reinterpret_cast<Raw *>(dyn) + warp * (S * NV * 32) + lane;
+  X *ring_x = reinterpret_cast<X *>(reinterpret_cast<Raw *>(dyn) + warps * (S * NV * 32)) +
+              warp * (S * NV * 32) + lane;
+  float *ws = reinterpret_cast<float *>(
+      reinterpret_cast<X *>(reinterpret_cast<Raw *>(dyn) + warps * (S * NV * 32)) + warps * (S * NV * 32));
+  const int64_t step = int64_t(gridDim.x) * teams;
+  int64_t r = int64_t(blockIdx.x) * teams + warp / team;
+  pdl_wait();
+  const auto fetch = [&](int64_t row, int stage) {
+    if (row < rows) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (wt + i * team) * 32 + lane;
+        if (c < nchunk) {
+          copy_raw<E>(ring_g + (stage * NV + i) * 32, g + row * C + c * 8);
+          if constexpr (FMT == kNone)
+            copy_raw<E>(ring_x + (stage * NV + i) * 32, reinterpret_cast<const E *>(x) + row * C + c * 8);
+          else
+            copy_async<8>(ring_x + (stage * NV + i) * 32, reinterpret_cast<const uint8_t *>(x) + row * C + c * 8);
+        }
+      }
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch(r + s * step, s);
+  if (w_shared) {
+    for (int c = threadIdx.x; c < nchunk; c += blockDim.x) {
+      float f[8];
+      param8(w, pdt, c, 1.f, f);
+      reinterpret_cast<float4 *>(ws)[2 * c] = make_float4(f[0], f[1], f[2], f[3]);
+      reinterpret_cast<float4 *>(ws)[2 * c + 1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+    __syncthreads();
+  }
+  const auto weight = [&](int c, float2 (&f)[4]) {
+    if (w_shared) {
+      const float4 a = reinterpret_cast<const float4 *>(ws)[2 * c];
+      const float4 b = reinterpret_cast<const float4 *>(ws)[2 * c + 1];
+      f[0] = make_float2(a.x, a.y); f[1] = make_float2(a.z, a.w);
+      f[2] = make_float2(b.x, b.y); f[3] = make_float2(b.z, b.w);
+    } else {
+      param8x2(w, pdt, c, 1.f, f);
+    }
+  };
+  float2 dw[NV][4], db[NV][4];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) dw[i][k] = db[i][k] = 0.f;
-  int par = 0;
-  for (int64_t r = int64_t(blockIdx.x) * teams + warp / team; r < rows;
-       r += int64_t(gridDim.x) * teams, par ^= 1) {
-    const float m = __ldg(mean + r), rs = __ldg(rstd + r);
-    float xh[NV][8], gw[NV][8];
-    float2 s = make_float2(0.f, 0.f);
+    for (int k = 0; k < 4; ++k) dw[i][k] = db[i][k] = both(0.f);
+  // mean, rstd and the scale bytes of a row are loaded one row ahead.
+  float next_m = 0.f, next_rs = 0.f;
+  uint32_t next_e[NV], e[NV];
+  const auto ahead = [&](int64_t row) {
+    if (row < rows) {
+      next_m = __ldg(mean + row);
+      next_rs = __ldg(rstd + row);
+      if constexpr (FMT != kNone) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (wt + i * team) * 32 + lane;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) xh[i][k] = gw[i][k] = 0.f;
-      if (c < nchunk) {
-        float fg[8], fw[8];
-        if constexpr (FMT == kNone) {
-          Elem<E>::widen(ld8(reinterpret_cast<const E *>(x) + r * C + c * 8), xh[i]);
-        } else {
-          const Codes<8> q = ld_codes<8>(reinterpret_cast<const uint8_t *>(x) + r * C + c * 8);
-          restore<FMT, 8>(q, scale_value(__ldg(scales + r * nb + (c >> 2))), xh[i]);
-        }
-        Elem<E>::widen(ld8(g + r * C + c * 8), fg);
-        param8(w, pdt, c, 1.f, fw);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          xh[i][k] = (xh[i][k] - m) * rs;
-          gw[i][k] = fg[k] * fw[k];
-          dw[i][k] = fmaf(fg[k], xh[i][k], dw[i][k]);
-          db[i][k] += fg[k];
-          s.x += gw[i][k];
-          s.y = fmaf(gw[i][k], xh[i][k], s.y);
+        for (int i = 0; i < NV; ++i) {
+          const int c = (wt + i * team) * 32 + lane;
+          next_e[i] = c < nchunk ? __ldg(scales + row * nb + (c >> 2)) : 0u;
         }
       }
     }
-    s.x = warp_sum(s.x);
-    s.y = warp_sum(s.y);
-    s = team_sum(s, slots[par], team, warp, lane);
-    const float c1 = s.x * inv_C, c2 = s.y * inv_C;
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) next_e[i] = 0;
+  ahead(r);
+  int par = 0, stage = 0;
+  for (; r < rows; r += step, par ^= 1) {
+    const float m = next_m, rs = next_rs;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) e[i] = next_e[i];
+    fetch(r + (S - 1) * step, stage == 0 ? S - 1 : stage - 1);
+    ahead(r + step);
+    copy_wait<S - 1>();
+    float2 s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (wt + i * team) * 32 + lane;
       if (c < nchunk) {
+        float2 fg[4], xh[4], fw[4];
+        normalised<E, FMT>(ring_x[(stage * NV + i) * 32], e[i], m, rs, xh);
+        widen2<E>(ring_g[(stage * NV + i) * 32], fg);
+        weight(c, fw);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 gw = mul2(fg[k], fw[k]);
+          dw[i][k] = fma2(fg[k], xh[k], dw[i][k]);
+          db[i][k] = add2(db[i][k], fg[k]);
+          s1 = add2(s1, gw);
+          s2 = fma2(gw, xh[k], s2);
+        }
+      }
+    }
+    const float2 sum = team_sum(make_float2(warp_sum(s1.x + s1.y), warp_sum(s2.x + s2.y)), slots[par],
+                                team, warp, lane);
+    const float2 c1 = both(-sum.x * inv_C), c2 = both(-sum.y * inv_C);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (wt + i * team) * 32 + lane;
+      if (c < nchunk) {
+        float2 fg[4], xh[4], fw[4];
+        normalised<E, FMT>(ring_x[(stage * NV + i) * 32], e[i], m, rs, xh);
+        widen2<E>(ring_g[(stage * NV + i) * 32], fg);
+        weight(c, fw);
         float o[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = rs * (gw[i][k] - fmaf(xh[i][k], c2, c1));
+        for (int k = 0; k < 4; ++k) {
+          const float2 v = mul2(both(rs), fma2(fg[k], fw[k], fma2(xh[k], c2, c1)));
+          o[2 * k] = v.x;
+          o[2 * k + 1] = v.y;
+        }
         st8(gx + r * C + c * 8, o);
       }
     }
+    if (++stage == S) stage = 0;
   }
   if (part == nullptr) return;
-  // Join the block's teams in team order, then write the block's partial.
+  // Join the block's teams in team order, then write the block's partial.  The
+  // ring's memory is free: no copy is in flight (a row past the end fetches
+  // nothing) and every warp has passed the barrier below.
+  copy_wait<0>();
+  __syncthreads();
+  float *joined = reinterpret_cast<float *>(dyn);  // [2][C]
   float *dst = part + int64_t(blockIdx.x) * 2 * C;
   for (int t = 0; t < teams; ++t) {
     if (warp / team == t) {
@@ -255,7 +426,7 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
         if (c < nchunk) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            float a = dw[i][k], d = db[i][k];
+            float a = k & 1 ? dw[i][k / 2].y : dw[i][k / 2].x, d = k & 1 ? db[i][k / 2].y : db[i][k / 2].x;
             if (t > 0) {
               a += joined[c * 8 + k];
               d += joined[C + c * 8 + k];
@@ -275,19 +446,21 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
   }
 }
 
-// Adds the partials [n][2][C] in order: grad_w and grad_b in the parameters'
-// type.  Either may be absent.  A block takes 32 columns; each of its 8 warps
-// adds every eighth partial, and the eight sums are added in warp order.
-__global__ void __launch_bounds__(256)
+// Adds the partials [n][2][C] in a fixed order: grad_w and grad_b in the
+// parameters' type.  Either may be absent.  A block takes 32 columns; each of
+// its 32 warps adds every 32nd partial, and the 32 sums are added pairwise.
+constexpr int kSumWarps = 32;
+__global__ void __launch_bounds__(32 * kSumWarps)
 ln_param_grad_kernel(const float *__restrict__ part, void *__restrict__ gw, void *__restrict__ gb,
                      int pdt, int n, int C) {
   pdl_wait();
-  __shared__ float acc[2][8][32];
+  __shared__ float acc[2][kSumWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float a = 0.f, d = 0.f;
   if (c < C) {
-    for (int i = warp; i < n; i += 8) {
+#pragma unroll 8
+    for (int i = warp; i < n; i += kSumWarps) {
       a += part[int64_t(i) * 2 * C + c];
       d += part[int64_t(i) * 2 * C + C + c];
     }
@@ -295,15 +468,16 @@ ln_param_grad_kernel(const float *__restrict__ part, void *__restrict__ gw, void
   acc[0][warp][lane] = a;
   acc[1][warp][lane] = d;
   __syncthreads();
-  if (warp < 2 && c < C) {
-    float s = 0.f;
+  // Warp k adds column k's 32 sums (a butterfly: one order for every lane).
+  const int col = blockIdx.x * 32 + warp;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += acc[warp][i][lane];
-    void *dst = warp == 0 ? gw : gb;
-    if (dst != nullptr) {
-      if (pdt == 0) reinterpret_cast<float *>(dst)[c] = s;
-      else if (pdt == 1) reinterpret_cast<__nv_bfloat16 *>(dst)[c] = __float2bfloat16_rn(s);
-      else reinterpret_cast<__half *>(dst)[c] = __float2half_rn(s);
+  for (int p = 0; p < 2; ++p) {
+    const float s = warp_sum(acc[p][lane][warp]);
+    void *dst = p == 0 ? gw : gb;
+    if (dst != nullptr && lane == 0 && col < C) {
+      if (pdt == 0) reinterpret_cast<float *>(dst)[col] = s;
+      else if (pdt == 1) reinterpret_cast<__nv_bfloat16 *>(dst)[col] = __float2bfloat16_rn(s);
+      else reinterpret_cast<__half *>(dst)[col] = __float2half_rn(s);
     }
   }
 }
@@ -437,26 +611,63 @@ ln_param_part_any_kernel(const E *__restrict__ g, const void *__restrict__ x,
 }
 
 // ------------------------------------------------------------------ launchers
-// Team and chunks per lane for a width the register kernels take.
+// Team and chunks per lane for a width the register kernels take, and the teams
+// per block: as many as keep every SM busy, so that few rows spread over the
+// SMs and many rows fill them.
 struct Shape {
-  int team, nv, teams;
+  int team, nv, teams, threads;
 };
-bool register_shape(int C, Shape *p) {
-  if (C % 8 || C > 256 * kMaxNV * kMaxTeam) return false;
-  const int warps = (C + 255) / 256;  // 256 values per warp and chunk
+int sm_count() {
+  int dev = 0, sms = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms > 0 ? sms : 1;
+}
+bool register_shape(int64_t rows, int C, int max_nv, Shape *p) {
+  if (C % 8 || C > 256 * max_nv * kMaxTeam) return false;
+  const int chunks = (C + 255) / 256;  // 256 values per warp and chunk
   p->team = 1;
-  while (p->team * kMaxNV < warps) p->team *= 2;
-  p->nv = (warps + p->team - 1) / p->team;
+  while (p->team * max_nv < chunks) p->team *= 2;
+  p->nv = (chunks + p->team - 1) / p->team;
   if (p->nv == 3) p->nv = 4;
-  p->teams = kWarps / p->team;
+  const int64_t want = (rows + sm_count() - 1) / sm_count();
+  p->teams = int(std::min<int64_t>(std::max<int64_t>(want, 1), kMaxWarps / p->team));
+  p->threads = p->teams * p->team * 32;
   return true;
 }
+int blocks_for(int64_t rows, const Shape &p) {
+  return int(std::min<int64_t>((rows + p.teams - 1) / p.teams, sm_count()));
+}
 
-#define FMHC_DISPATCH_NV(NV_RT, ...)                        \
-  do {                                                      \
+// Dynamic shared memory beyond the default needs an attribute of the kernel, set
+// once per device to the most it will ask for (and again only where this
+// table's 64 places do not suffice).
+void allow_smem(const void *kernel, size_t bytes) {
+  struct Entry {
+    const void *k;
+    int dev;
+    size_t bytes;
+  };
+  static std::mutex mu;
+  static Entry set[64];
+  static int used = 0;
+  if (bytes <= 48 * 1024) return;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(mu);
+  int at = 0;
+  while (at < used && !(set[at].k == kernel && set[at].dev == dev)) ++at;
+  if (at < used && set[at].bytes >= bytes) return;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) != cudaSuccess) return;
+  if (at == used && used < 64) ++used;
+  if (at < used) set[at] = Entry{kernel, dev, bytes};
+}
+
+#define FMHC_DISPATCH_NV(NV_RT, NV_MAX, ...)                 \
+  do {                                                       \
     if ((NV_RT) == 1) { constexpr int NV = 1; __VA_ARGS__; } \
-    else if ((NV_RT) == 2) { constexpr int NV = 2; __VA_ARGS__; } \
-    else { constexpr int NV = 4; __VA_ARGS__; }             \
+    else if ((NV_RT) == 2 || (NV_MAX) == 2) { constexpr int NV = 2; __VA_ARGS__; } \
+    else { constexpr int NV = (NV_MAX); __VA_ARGS__; }       \
   } while (0)
 #define FMHC_DISPATCH_FMT_OR_NONE(FMT_RT, ...)                                  \
   do {                                                                          \
@@ -464,19 +675,6 @@ bool register_shape(int C, Shape *p) {
     else FMHC_DISPATCH_FMT(FMT_RT, __VA_ARGS__);                                \
   } while (0)
 
-int sm_count() {
-  int dev = 0, sms = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms > 0 ? sms : 1;
-}
-
-// Blocks of the register backward: at most two per SM, no more than the rows.
-int bwd_blocks(int64_t rows, const Shape &p) {
-  const int64_t need = (rows + p.teams - 1) / p.teams;
-  const int64_t cap = std::min<int64_t>(2 * sm_count(), kMaxParts);
-  return int(need < cap ? need : cap);
-}
 int any_slices(int64_t rows, int C) {
   const int64_t cols = (C + 31) / 32;
   int64_t n = (8 * int64_t(sm_count()) + cols - 1) / cols;
@@ -490,28 +688,31 @@ void launch_ln_fwd(const void *x, int dtype, const void *w, const void *b, int p
                    void *y, float *mean, float *rstd, void *codes, int fmt, void *scales,
                    int64_t rows, int C, bool vec, cudaStream_t s) {
   Shape p;
-  if (vec && register_shape(C, &p)) {
-    FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, FMHC_DISPATCH_NV(p.nv, {
+  if (vec && register_shape(rows, C, kMaxNV, &p)) {
+    FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, FMHC_DISPATCH_NV(p.nv, kMaxNV, {
       auto k = ln_fwd_kernel<E, NV, FMT>;
-      launch(k, dim3(grid_for(k, rows * p.team, kThreads)), dim3(kThreads), 0, s, (const E *)x, w,
-             b, pdt, eps, (E *)y, mean, rstd, (uint8_t *)codes, (uint8_t *)scales, rows, C, p.team);
+      const size_t smem = size_t(p.threads) * kFwdStages<E> * NV * sizeof(typename Elem<E>::Raw);
+      allow_smem(reinterpret_cast<const void *>(k), smem);
+      launch(k, dim3(blocks_for(rows, p)), dim3(p.threads), smem, s, (const E *)x, w, b, pdt, eps,
+             (E *)y, mean, rstd, (uint8_t *)codes, (uint8_t *)scales, rows, C, p.team);
     })));
   } else {
     FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, {
       auto k = ln_fwd_any_kernel<E, FMT>;
-      launch(k, dim3(grid_for(k, rows * (kWarps), kThreads)), dim3(kThreads), 0, s,
-             (const E *)x, w, b, pdt, eps, (E *)y, mean, rstd, (uint8_t *)codes, (uint8_t *)scales,
-             rows, C);
+      launch(k, dim3(grid_for(k, rows * kWarps, kThreads)), dim3(kThreads), 0, s, (const E *)x, w, b,
+             pdt, eps, (E *)y, mean, rstd, (uint8_t *)codes, (uint8_t *)scales, rows, C);
     }));
   }
 }
 
 int64_t ln_bwd_workspace_bytes(int64_t rows, int C) {
   if (rows < 1 || C < 1) return 0;
-  // The larger of the two paths, so that the size does not depend on alignment.
+  // The largest of the paths, so that the size depends on neither the type nor
+  // the alignment.
   Shape p;
   int64_t n = any_slices(rows, C);
-  if (register_shape(C, &p)) n = std::max<int64_t>(n, bwd_blocks(rows, p));
+  for (int nv : {kBwdMaxNV<float>, kBwdMaxNV<__half>})
+    if (register_shape(rows, C, nv, &p)) n = std::max<int64_t>(n, blocks_for(rows, p));
   return (n * 2 * C * 4 + 255) & ~int64_t(255);
 }
 
@@ -521,19 +722,27 @@ void launch_ln_bwd(const void *g, int dtype, const void *x, int fmt, const void 
   Shape p;
   float *part = gw != nullptr || gb != nullptr ? ws : nullptr;
   int parts = 0;
-  if (vec && register_shape(C, &p)) {
-    parts = bwd_blocks(rows, p);
-    const size_t smem = part != nullptr && p.teams > 1 ? size_t(2) * C * 4 : 0;
-    FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, FMHC_DISPATCH_NV(p.nv, {
+  if (vec && register_shape(rows, C, dtype == 0 ? kBwdMaxNV<float> : kBwdMaxNV<__half>, &p)) {
+    parts = blocks_for(rows, p);
+    FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, FMHC_DISPATCH_NV(p.nv, kBwdMaxNV<E>, {
       auto k = ln_bwd_kernel<E, NV, FMT>;
-      launch(k, dim3(parts), dim3(kThreads), smem, s, (const E *)g, x, (const uint8_t *)scales,
-             mean, rstd, w, pdt, (E *)gx, part, rows, C, p.team);
+      const size_t ring = size_t(p.threads) * kBwdStages * NV *
+                          (sizeof(typename Elem<E>::Raw) + sizeof(typename Input<E, FMT>::X));
+      // The weight beside the ring where it fits; the ring's memory also holds
+      // the [2][C] sums in which a block's teams are joined.
+      const size_t with_w = ring + size_t(C) * 4;
+      const bool w_shared = w != nullptr && with_w <= kMaxSmem;
+      size_t smem = w_shared ? with_w : ring;
+      if (part != nullptr && p.teams > 1) smem = std::max(smem, size_t(C) * 8);
+      allow_smem(reinterpret_cast<const void *>(k), smem);
+      launch(k, dim3(parts), dim3(p.threads), smem, s, (const E *)g, x, (const uint8_t *)scales, mean,
+             rstd, w, pdt, w_shared, (E *)gx, part, rows, C, p.team);
     })));
   } else {
     FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, {
       auto k = ln_bwd_any_kernel<E, FMT>;
-      launch(k, dim3(grid_for(k, rows * (kWarps), kThreads)), dim3(kThreads), 0, s,
-             (const E *)g, x, (const uint8_t *)scales, mean, rstd, w, pdt, (E *)gx, rows, C);
+      launch(k, dim3(grid_for(k, rows * kWarps, kThreads)), dim3(kThreads), 0, s, (const E *)g, x,
+             (const uint8_t *)scales, mean, rstd, w, pdt, (E *)gx, rows, C);
       if (part != nullptr) {
         parts = any_slices(rows, C);
         launch(ln_param_part_any_kernel<E, FMT>, dim3((C + 31) / 32, parts), dim3(256), 0, s,
@@ -542,8 +751,8 @@ void launch_ln_bwd(const void *g, int dtype, const void *x, int fmt, const void 
     }));
   }
   if (part != nullptr)
-    launch(ln_param_grad_kernel, dim3((C + 31) / 32), dim3(256), 0, s, (const float *)part, gw, gb,
-           pdt, parts, C);
+    launch(ln_param_grad_kernel, dim3((C + 31) / 32), dim3(32 * kSumWarps), 0, s, (const float *)part,
+           gw, gb, pdt, parts, C);
 }
 
 }  // namespace fmhc
