@@ -20,6 +20,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "fmhc_common.cuh"
 
 namespace fmhc {
@@ -225,6 +227,26 @@ __device__ __forceinline__ void st8(E *p, const float (&f)[8]) {
     const typename Elem<E>::Raw r = Elem<E>::narrow(f);
     __stcs(reinterpret_cast<uint4 *>(p), r.a);
     __stcs(reinterpret_cast<uint4 *>(p) + 1, r.b);
+  }
+}
+
+// Largest magnitude among eight raw values, as f32 bits.  Magnitudes of a
+// floating type are ordered like their bits, infinity and NaN above the rest,
+// so 16-bit values are compared two at a time without widening them.
+template <class E>
+__device__ __forceinline__ uint32_t amax8_raw(const typename Elem<E>::Raw &r) {
+  if constexpr (sizeof(E) == 2) {
+    const uint32_t k = 0x7fff7fffu;
+    const uint32_t m = __vmaxu2(__vmaxu2(r.x & k, r.y & k), __vmaxu2(r.z & k, r.w & k));
+    const uint32_t h = max(m & 0xffffu, m >> 16);
+    if constexpr (std::is_same<E, __nv_bfloat16>::value) return h << 16;
+    else return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(h))));
+  } else {
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
+    return m;
   }
 }
 

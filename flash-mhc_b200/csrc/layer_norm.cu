@@ -36,9 +36,13 @@ using namespace act8;
 
 namespace {
 
-constexpr int kMaxWarps = 16;         // per block, one block per SM
-constexpr int kMaxTeam = kMaxWarps;   // warps per row
-constexpr int kMaxNV = 4;             // chunks of eight values per lane
+constexpr int kMaxTeam = 16;          // warps per row
+// Warps per block (one block per SM) and most chunks of eight values per lane.
+#ifndef FMHC_LN_FWD_WARPS
+#define FMHC_LN_FWD_WARPS 24
+#endif
+constexpr int kFwdWarps = FMHC_LN_FWD_WARPS;
+constexpr int kBwdWarps = 16;
 constexpr int kThreads = 256;         // of the kernels for any width
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxParts = 1024;
@@ -106,23 +110,39 @@ __device__ __forceinline__ void copy_raw(typename Elem<E>::Raw *dst, const E *sr
   if constexpr (sizeof(E) == 4) copy_async<16>(reinterpret_cast<char *>(dst) + 16, src + 4);
 }
 
-// Ring depth in rows.  16 warps x NV chunks x 32 lanes x (16 or 32 bytes).
-template <class E> constexpr int kFwdStages = sizeof(E) == 2 ? 4 : 3;
-// Most chunks per lane in the backward: its sums take 16 registers per chunk,
-// and f32 rows twice the ring.
-template <class E> constexpr int kBwdMaxNV = sizeof(E) == 2 ? kMaxNV : 2;
+constexpr int kStages = 3;  // ring depth in rows
+// Most chunks per lane: the backward's sums take 16 registers per chunk, and
+// f32 rows take twice the ring.
+template <class E> constexpr int kMaxNV = sizeof(E) == 2 ? 4 : 2;
+
+// Columns of weight or bias kept in shared memory as f32, the first four values
+// of every chunk and then the last four, so that neighbouring lanes read
+// neighbouring words.
+__device__ __forceinline__ void keep_param(float4 *dst, const void *p, int dtype, float def, int nchunk) {
+  for (int c = threadIdx.x; c < nchunk; c += blockDim.x) {
+    float f[8];
+    param8(p, dtype, c, def, f);
+    dst[c] = make_float4(f[0], f[1], f[2], f[3]);
+    dst[nchunk + c] = make_float4(f[4], f[5], f[6], f[7]);
+  }
+}
+__device__ __forceinline__ void kept_param(const float4 *src, int c, int nchunk, float2 (&f)[4]) {
+  const float4 a = src[c], b = src[nchunk + c];
+  f[0] = make_float2(a.x, a.y); f[1] = make_float2(a.z, a.w);
+  f[2] = make_float2(b.x, b.y); f[3] = make_float2(b.z, b.w);
+}
 
 // -------------------------------------------------------------------- forward
 template <class E, int NV, int FMT>
-__global__ void __launch_bounds__(32 * kMaxWarps, 1)
+__global__ void __launch_bounds__(32 * kFwdWarps, 1)
 ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *__restrict__ b,
               int pdt, float eps, E *__restrict__ y, float *__restrict__ mean_out,
               float *__restrict__ rstd_out, uint8_t *__restrict__ codes,
               uint8_t *__restrict__ scales, int64_t rows, int C, int team) {
   using Raw = typename Elem<E>::Raw;
-  constexpr int S = kFwdStages<E>;
+  constexpr int S = kStages;
   extern __shared__ uint4 dyn[];
-  __shared__ float2 slots[2][kMaxWarps];
+  __shared__ float2 slots[2][kFwdWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int teams = (blockDim.x >> 5) / team;
   const int wt = warp % team, first = warp - wt;
@@ -154,29 +174,28 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
   };
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) fetch(r + s * step, s);
-  // This lane's columns of the parameters, for every row.
-  float2 fw[NV][4], fb[NV][4];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (wt + i * team) * 32 + lane;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) fw[i][k] = fb[i][k] = both(0.f);
-    if (c < nchunk) {
-      param8x2(w, pdt, c, 1.f, fw[i]);
-      param8x2(b, pdt, c, 0.f, fb[i]);
-    }
-  }
+  float4 *ws = reinterpret_cast<float4 *>(reinterpret_cast<Raw *>(dyn) + (blockDim.x >> 5) * (S * NV * 32));
+  float4 *bs = ws + 2 * nchunk;
+  keep_param(ws, w, pdt, 1.f, nchunk);
+  keep_param(bs, b, pdt, 0.f, nchunk);
+  __syncthreads();
   int par = 0, stage = 0;
   for (; r < rows; r += step, par ^= 1) {
     fetch(r + (S - 1) * step, stage == 0 ? S - 1 : stage - 1);
     copy_wait<S - 1>();
     float2 f[NV][4];
+    uint32_t big[NV];  // largest magnitude of the chunk
     float2 s2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) f[i][k] = both(0.f);
-      if ((wt + i * team) * 32 + lane < nchunk) widen2<E>(ring[(stage * NV + i) * 32], f[i]);
+      big[i] = 0;
+      if ((wt + i * team) * 32 + lane < nchunk) {
+        const Raw raw = ring[(stage * NV + i) * 32];
+        widen2<E>(raw, f[i]);
+        if constexpr (FMT != kNone) big[i] = amax8_raw<E>(raw);
+      }
 #pragma unroll
       for (int k = 0; k < 4; ++k) s2 = add2(s2, f[i][k]);
     }
@@ -211,6 +230,7 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
       mean_out[r] = mean;
       rstd_out[r] = rstd;
     }
+    const float2 rs2 = both(rstd), off = both(-mean);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (wt + i * team) * 32 + lane;
@@ -222,18 +242,20 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
           v[2 * k] = f[i][k].x;
           v[2 * k + 1] = f[i][k].y;
         }
-        const uint32_t e = scale_byte<FMT>(amax_block(amax8(v)));
+        const uint32_t e = scale_byte<FMT>(amax_block(big[i]));
         if (in) {
           __stcs(reinterpret_cast<uint2 *>(codes + r * C + c * 8), encode8<FMT>(v, e));
           if ((lane & 3) == 0) __stcs(scales + r * nb + (c >> 2), uint8_t(e));
         }
       }
       if (in) {
+        float2 fw[4], fb[4];
+        kept_param(ws, c, nchunk, fw);
+        kept_param(bs, c, nchunk, fb);
         float o[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float2 xh = mul2(add2(f[i][k], both(-mean)), both(rstd));
-          const float2 v = fma2(xh, fw[i][k], fb[i][k]);
+          const float2 v = fma2(mul2(add2(f[i][k], off), rs2), fw[k], fb[k]);
           o[2 * k] = v.x;
           o[2 * k + 1] = v.y;
         }
@@ -249,24 +271,26 @@ template <class E, int FMT> struct Input;
 template <class E> struct Input<E, kNone> { using X = typename Elem<E>::Raw; };
 template <class E> struct Input<E, kInt8> { using X = uint2; };
 template <class E> struct Input<E, kE4m3> { using X = uint2; };
-constexpr int kBwdStages = 3;
-
-// xh of a chunk, from x (e unused) or from codes with scale byte e.
+// xh of a chunk, from x (e unused) or from codes with scale byte e; off is
+// -mean.  The difference comes first and is rounded once (a code times its
+// scale is exact), so that values near the mean keep their relative precision.
 template <class E, int FMT>
-__device__ __forceinline__ void normalised(const typename Input<E, FMT>::X &raw, uint32_t e, float mean,
-                                           float rstd, float2 (&xh)[4]) {
+__device__ __forceinline__ void normalised(const typename Input<E, FMT>::X &raw, uint32_t e, float rstd,
+                                           float2 off, float2 (&xh)[4]) {
   if constexpr (FMT == kNone) {
     widen2<E>(raw, xh);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xh[i] = mul2(add2(xh[i], off), both(rstd));
   } else {
-    Codes<8> q;
-    q.v = raw;
-    float v[8];
-    restore<FMT, 8>(q, scale_value(e), v);
+    float a[4], b[4];
+    decode4<FMT>(raw.x, a);
+    decode4<FMT>(raw.y, b);
+    xh[0] = make_float2(a[0], a[1]); xh[1] = make_float2(a[2], a[3]);
+    xh[2] = make_float2(b[0], b[1]); xh[3] = make_float2(b[2], b[3]);
+    const float2 s = both(scale_value(e));
 #pragma unroll
-    for (int k = 0; k < 4; ++k) xh[k] = make_float2(v[2 * k], v[2 * k + 1]);
+    for (int i = 0; i < 4; ++i) xh[i] = mul2(fma2(xh[i], s, off), both(rstd));
   }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) xh[k] = mul2(add2(xh[k], both(-mean)), both(rstd));
 }
 
 // The weight's columns of a lane come from shared memory as f32 (or, for rows
@@ -274,16 +298,16 @@ __device__ __forceinline__ void normalised(const typename Input<E, FMT>::X &raw,
 // them too would pass 128 registers.  For the same reason the second pass reads
 // g and x from the ring again.
 template <class E, int NV, int FMT>
-__global__ void __launch_bounds__(32 * kMaxWarps, 1)
+__global__ void __launch_bounds__(32 * kBwdWarps, 1)
 ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
               const uint8_t *__restrict__ scales, const float *__restrict__ mean,
               const float *__restrict__ rstd, const void *__restrict__ w, int pdt, bool w_shared,
               E *__restrict__ gx, float *__restrict__ part, int64_t rows, int C, int team) {
   using Raw = typename Elem<E>::Raw;
   using X = typename Input<E, FMT>::X;
-  constexpr int S = kBwdStages;
+  constexpr int S = kStages;
   extern __shared__ uint4 dyn[];
-  __shared__ float2 slots[2][kMaxWarps];
+  __shared__ float2 slots[2][kBwdWarps];
   const int warps = blockDim.x >> 5;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int teams = warps / team;
@@ -294,7 +318,7 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
   Raw *ring_g = reinterpret_cast<Raw *>(dyn) + warp * (S * NV * 32) + lane;
   X *ring_x = reinterpret_cast<X *>(reinterpret_cast<Raw *>(dyn) + warps * (S * NV * 32)) +
               warp * (S * NV * 32) + lane;
-  float *ws = reinterpret_cast<float *>(
+  float4 *ws = reinterpret_cast<float4 *>(
       reinterpret_cast<X *>(reinterpret_cast<Raw *>(dyn) + warps * (S * NV * 32)) + warps * (S * NV * 32));
   const int64_t step = int64_t(gridDim.x) * teams;
   int64_t r = int64_t(blockIdx.x) * teams + warp / team;
@@ -318,20 +342,12 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) fetch(r + s * step, s);
   if (w_shared) {
-    for (int c = threadIdx.x; c < nchunk; c += blockDim.x) {
-      float f[8];
-      param8(w, pdt, c, 1.f, f);
-      reinterpret_cast<float4 *>(ws)[2 * c] = make_float4(f[0], f[1], f[2], f[3]);
-      reinterpret_cast<float4 *>(ws)[2 * c + 1] = make_float4(f[4], f[5], f[6], f[7]);
-    }
+    keep_param(ws, w, pdt, 1.f, nchunk);
     __syncthreads();
   }
   const auto weight = [&](int c, float2 (&f)[4]) {
     if (w_shared) {
-      const float4 a = reinterpret_cast<const float4 *>(ws)[2 * c];
-      const float4 b = reinterpret_cast<const float4 *>(ws)[2 * c + 1];
-      f[0] = make_float2(a.x, a.y); f[1] = make_float2(a.z, a.w);
-      f[2] = make_float2(b.x, b.y); f[3] = make_float2(b.z, b.w);
+      kept_param(ws, c, nchunk, f);
     } else {
       param8x2(w, pdt, c, 1.f, f);
     }
@@ -362,7 +378,8 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
   ahead(r);
   int par = 0, stage = 0;
   for (; r < rows; r += step, par ^= 1) {
-    const float m = next_m, rs = next_rs;
+    const float rs = next_rs;
+    const float2 off = both(-next_m);
 #pragma unroll
     for (int i = 0; i < NV; ++i) e[i] = next_e[i];
     fetch(r + (S - 1) * step, stage == 0 ? S - 1 : stage - 1);
@@ -374,7 +391,7 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
       const int c = (wt + i * team) * 32 + lane;
       if (c < nchunk) {
         float2 fg[4], xh[4], fw[4];
-        normalised<E, FMT>(ring_x[(stage * NV + i) * 32], e[i], m, rs, xh);
+        normalised<E, FMT>(ring_x[(stage * NV + i) * 32], e[i], rs, off, xh);
         widen2<E>(ring_g[(stage * NV + i) * 32], fg);
         weight(c, fw);
 #pragma unroll
@@ -395,7 +412,7 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
       const int c = (wt + i * team) * 32 + lane;
       if (c < nchunk) {
         float2 fg[4], xh[4], fw[4];
-        normalised<E, FMT>(ring_x[(stage * NV + i) * 32], e[i], m, rs, xh);
+        normalised<E, FMT>(ring_x[(stage * NV + i) * 32], e[i], rs, off, xh);
         widen2<E>(ring_g[(stage * NV + i) * 32], fg);
         weight(c, fw);
         float o[8];
@@ -411,75 +428,72 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
     if (++stage == S) stage = 0;
   }
   if (part == nullptr) return;
-  // Join the block's teams in team order, then write the block's partial.  The
-  // ring's memory is free: no copy is in flight (a row past the end fetches
-  // nothing) and every warp has passed the barrier below.
+  // Join the block's teams: every warp puts its sums into shared memory (the
+  // ring's: no copy is in flight, since a row past the end fetches nothing, and
+  // every warp has passed the barrier), then the block adds them in team order
+  // and writes its partial.  A partial keeps the order of the lanes,
+  // [wt][i * 8 + k, of grad_w then of grad_b][lane], so that all of this is
+  // contiguous; ln_param_grad_kernel puts the columns in their places.
+  constexpr int L = NV * 16 * 32;
   copy_wait<0>();
   __syncthreads();
-  float *joined = reinterpret_cast<float *>(dyn);  // [2][C]
-  float *dst = part + int64_t(blockIdx.x) * 2 * C;
-  for (int t = 0; t < teams; ++t) {
-    if (warp / team == t) {
+  float *sums = reinterpret_cast<float *>(dyn);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = (wt + i * team) * 32 + lane;
-        if (c < nchunk) {
+  for (int i = 0; i < NV; ++i)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            float a = k & 1 ? dw[i][k / 2].y : dw[i][k / 2].x, d = k & 1 ? db[i][k / 2].y : db[i][k / 2].x;
-            if (t > 0) {
-              a += joined[c * 8 + k];
-              d += joined[C + c * 8 + k];
-            }
-            if (t == teams - 1) {
-              dst[c * 8 + k] = a;
-              dst[C + c * 8 + k] = d;
-            } else {
-              joined[c * 8 + k] = a;
-              joined[C + c * 8 + k] = d;
-            }
-          }
-        }
-      }
+    for (int k = 0; k < 8; ++k) {
+      sums[warp * L + (i * 8 + k) * 32 + lane] = k & 1 ? dw[i][k / 2].y : dw[i][k / 2].x;
+      sums[warp * L + ((NV + i) * 8 + k) * 32 + lane] = k & 1 ? db[i][k / 2].y : db[i][k / 2].x;
     }
-    if (t < teams - 1) __syncthreads();
+  __syncthreads();
+  float *dst = part + int64_t(blockIdx.x) * team * L;
+  for (int j = threadIdx.x; j < team * L; j += blockDim.x) {
+    float v = 0.f;
+    for (int t = 0; t < teams; ++t) v += sums[t * team * L + j];
+    dst[j] = v;
   }
 }
 
-// Adds the partials [n][2][C] in a fixed order: grad_w and grad_b in the
-// parameters' type.  Either may be absent.  A block takes 32 columns; each of
-// its 32 warps adds every 32nd partial, and the 32 sums are added pairwise.
+// Adds n partials of `len` sums in a fixed order: grad_w and grad_b in the
+// parameters' type.  Either may be absent.  nv 0: a partial is [2][C]; else it
+// is in the lanes' order (see ln_bwd_kernel).  A block takes 32 sums; each of
+// its 32 warps adds every 32nd partial, and the 32 results are added pairwise.
 constexpr int kSumWarps = 32;
 __global__ void __launch_bounds__(32 * kSumWarps)
 ln_param_grad_kernel(const float *__restrict__ part, void *__restrict__ gw, void *__restrict__ gb,
-                     int pdt, int n, int C) {
+                     int pdt, int n, int64_t len, int C, int nv, int team) {
   pdl_wait();
-  __shared__ float acc[2][kSumWarps][33];
+  __shared__ float acc[kSumWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
-  float a = 0.f, d = 0.f;
-  if (c < C) {
+  const int64_t j0 = int64_t(blockIdx.x) * 32;
+  float a = 0.f;
+  if (j0 + lane < len) {
 #pragma unroll 8
-    for (int i = warp; i < n; i += kSumWarps) {
-      a += part[int64_t(i) * 2 * C + c];
-      d += part[int64_t(i) * 2 * C + C + c];
-    }
+    for (int i = warp; i < n; i += kSumWarps) a += part[i * len + j0 + lane];
   }
-  acc[0][warp][lane] = a;
-  acc[1][warp][lane] = d;
+  acc[warp][lane] = a;
   __syncthreads();
-  // Warp k adds column k's 32 sums (a butterfly: one order for every lane).
-  const int col = blockIdx.x * 32 + warp;
-#pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    const float s = warp_sum(acc[p][lane][warp]);
-    void *dst = p == 0 ? gw : gb;
-    if (dst != nullptr && lane == 0 && col < C) {
-      if (pdt == 0) reinterpret_cast<float *>(dst)[col] = s;
-      else if (pdt == 1) reinterpret_cast<__nv_bfloat16 *>(dst)[col] = __float2bfloat16_rn(s);
-      else reinterpret_cast<__half *>(dst)[col] = __float2half_rn(s);
-    }
+  const float s = warp_sum(acc[lane][warp]);  // sum j0 + warp
+  const int64_t j = j0 + warp;
+  if (lane != 0 || j >= len) return;
+  int c = int(j % C);
+  bool is_b = j >= C;
+  if (nv != 0) {
+    const int l = int(j & 31);
+    int q = int(j >> 5);  // (wt * 2 + which) * nv * 8 + i * 8 + k
+    const int k = q & 7;
+    q >>= 3;
+    const int i = q % nv;
+    q /= nv;
+    is_b = q & 1;
+    c = (((q >> 1) + i * team) * 32 + l) * 8 + k;
+    if (c >= C) return;
   }
+  void *dst = is_b ? gb : gw;
+  if (dst == nullptr) return;
+  if (pdt == 0) reinterpret_cast<float *>(dst)[c] = s;
+  else if (pdt == 1) reinterpret_cast<__nv_bfloat16 *>(dst)[c] = __float2bfloat16_rn(s);
+  else reinterpret_cast<__half *>(dst)[c] = __float2half_rn(s);
 }
 
 // ---------------------------------------------- any width and any alignment
@@ -616,6 +630,7 @@ ln_param_part_any_kernel(const E *__restrict__ g, const void *__restrict__ x,
 // SMs and many rows fill them.
 struct Shape {
   int team, nv, teams, threads;
+  int64_t sums() const { return int64_t(team) * nv * 16 * 32; }  // of a block's partial
 };
 int sm_count() {
   int dev = 0, sms = 0;
@@ -623,7 +638,7 @@ int sm_count() {
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   return sms > 0 ? sms : 1;
 }
-bool register_shape(int64_t rows, int C, int max_nv, Shape *p) {
+bool register_shape(int64_t rows, int C, int max_nv, int max_warps, Shape *p) {
   if (C % 8 || C > 256 * max_nv * kMaxTeam) return false;
   const int chunks = (C + 255) / 256;  // 256 values per warp and chunk
   p->team = 1;
@@ -631,7 +646,7 @@ bool register_shape(int64_t rows, int C, int max_nv, Shape *p) {
   p->nv = (chunks + p->team - 1) / p->team;
   if (p->nv == 3) p->nv = 4;
   const int64_t want = (rows + sm_count() - 1) / sm_count();
-  p->teams = int(std::min<int64_t>(std::max<int64_t>(want, 1), kMaxWarps / p->team));
+  p->teams = int(std::min<int64_t>(std::max<int64_t>(want, 1), max_warps / p->team));
   p->threads = p->teams * p->team * 32;
   return true;
 }
@@ -651,7 +666,7 @@ void allow_smem(const void *kernel, size_t bytes) {
   static std::mutex mu;
   static Entry set[64];
   static int used = 0;
-  if (bytes <= 48 * 1024) return;
+  if (bytes <= 40 * 1024) return;  // beside the static arrays, below the default 48 KiB
   int dev = 0;
   cudaGetDevice(&dev);
   std::lock_guard<std::mutex> lock(mu);
@@ -688,10 +703,10 @@ void launch_ln_fwd(const void *x, int dtype, const void *w, const void *b, int p
                    void *y, float *mean, float *rstd, void *codes, int fmt, void *scales,
                    int64_t rows, int C, bool vec, cudaStream_t s) {
   Shape p;
-  if (vec && register_shape(rows, C, kMaxNV, &p)) {
-    FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, FMHC_DISPATCH_NV(p.nv, kMaxNV, {
+  if (vec && register_shape(rows, C, dtype == 0 ? kMaxNV<float> : kMaxNV<__half>, kFwdWarps, &p)) {
+    FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, FMHC_DISPATCH_NV(p.nv, kMaxNV<E>, {
       auto k = ln_fwd_kernel<E, NV, FMT>;
-      const size_t smem = size_t(p.threads) * kFwdStages<E> * NV * sizeof(typename Elem<E>::Raw);
+      const size_t smem = size_t(p.threads) * kStages * NV * sizeof(typename Elem<E>::Raw) + size_t(C) * 8;
       allow_smem(reinterpret_cast<const void *>(k), smem);
       launch(k, dim3(blocks_for(rows, p)), dim3(p.threads), smem, s, (const E *)x, w, b, pdt, eps,
              (E *)y, mean, rstd, (uint8_t *)codes, (uint8_t *)scales, rows, C, p.team);
@@ -710,30 +725,35 @@ int64_t ln_bwd_workspace_bytes(int64_t rows, int C) {
   // The largest of the paths, so that the size depends on neither the type nor
   // the alignment.
   Shape p;
-  int64_t n = any_slices(rows, C);
-  for (int nv : {kBwdMaxNV<float>, kBwdMaxNV<__half>})
-    if (register_shape(rows, C, nv, &p)) n = std::max<int64_t>(n, blocks_for(rows, p));
-  return (n * 2 * C * 4 + 255) & ~int64_t(255);
+  int64_t n = int64_t(any_slices(rows, C)) * 2 * C;
+  for (int nv : {kMaxNV<float>, kMaxNV<__half>})
+    if (register_shape(rows, C, nv, kBwdWarps, &p)) n = std::max(n, blocks_for(rows, p) * p.sums());
+  return (n * 4 + 255) & ~int64_t(255);
 }
 
 void launch_ln_bwd(const void *g, int dtype, const void *x, int fmt, const void *scales,
                    const float *mean, const float *rstd, const void *w, int pdt, void *gx, void *gw,
                    void *gb, float *ws, int64_t rows, int C, bool vec, cudaStream_t s) {
-  Shape p;
+  Shape p{};
   float *part = gw != nullptr || gb != nullptr ? ws : nullptr;
-  int parts = 0;
-  if (vec && register_shape(rows, C, dtype == 0 ? kBwdMaxNV<float> : kBwdMaxNV<__half>, &p)) {
+  int parts = 0, nv = 0;
+  int64_t len = 2 * int64_t(C);
+  if (vec && register_shape(rows, C, dtype == 0 ? kMaxNV<float> : kMaxNV<__half>,
+                            kBwdWarps, &p)) {
     parts = blocks_for(rows, p);
-    FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, FMHC_DISPATCH_NV(p.nv, kBwdMaxNV<E>, {
+    nv = p.nv;
+    len = p.sums();
+    FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, FMHC_DISPATCH_NV(p.nv, kMaxNV<E>, {
       auto k = ln_bwd_kernel<E, NV, FMT>;
-      const size_t ring = size_t(p.threads) * kBwdStages * NV *
+      const size_t ring = size_t(p.threads) * kStages * NV *
                           (sizeof(typename Elem<E>::Raw) + sizeof(typename Input<E, FMT>::X));
-      // The weight beside the ring where it fits; the ring's memory also holds
-      // the [2][C] sums in which a block's teams are joined.
+      // The ring's memory later holds the 64 NV bytes of sums of every thread.
+      static_assert(kStages * (sizeof(typename Elem<E>::Raw) + sizeof(typename Input<E, FMT>::X)) >= 64,
+                    "sums fit the ring");
+      // The weight goes beside the ring where it fits.
       const size_t with_w = ring + size_t(C) * 4;
       const bool w_shared = w != nullptr && with_w <= kMaxSmem;
-      size_t smem = w_shared ? with_w : ring;
-      if (part != nullptr && p.teams > 1) smem = std::max(smem, size_t(C) * 8);
+      const size_t smem = w_shared ? with_w : ring;
       allow_smem(reinterpret_cast<const void *>(k), smem);
       launch(k, dim3(parts), dim3(p.threads), smem, s, (const E *)g, x, (const uint8_t *)scales, mean,
              rstd, w, pdt, w_shared, (E *)gx, part, rows, C, p.team);
@@ -751,8 +771,8 @@ void launch_ln_bwd(const void *g, int dtype, const void *x, int fmt, const void 
     }));
   }
   if (part != nullptr)
-    launch(ln_param_grad_kernel, dim3((C + 31) / 32), dim3(32 * kSumWarps), 0, s, (const float *)part,
-           gw, gb, pdt, parts, C);
+    launch(ln_param_grad_kernel, dim3(unsigned((len + 31) / 32)), dim3(32 * kSumWarps), 0, s,
+           (const float *)part, gw, gb, pdt, parts, len, C, nv, p.team);
 }
 
 }  // namespace fmhc

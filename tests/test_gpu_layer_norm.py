@@ -133,6 +133,32 @@ def test_missing_parameters(C, which):
     _check_backward(g, _np(x), mean, rstd, w, grads, F32)
 
 
+@pytest.mark.parametrize("C", [64, 256, 512, 1024, 2048])
+def test_every_number_of_rows_per_block(C):
+    """Block and shared-memory sizes follow the rows per SM: one row to two waves of every team count."""
+    w, b = torch.randn(C, device="cuda"), torch.randn(C, device="cuda")
+    for rows in [*range(1, 30, 7), *range(100, 148 * 26, 148 * 2 - 5)]:
+        x, g, _, _ = _inputs(rows, C, BF, BF)
+        for ww, bb in ((w, b), (None, None)):
+            y, mean, rstd = ops.layer_norm(x, ww, bb, EPS)
+            gx, gw, gb = ops.layer_norm_backward(g, x, mean, rstd, ww, bb)
+            xf = x.double()
+            m = xf.mean(-1, keepdim=True)
+            r = 1 / torch.sqrt((xf - m).square().mean(-1, keepdim=True) + EPS)
+            xh = (xf - m) * r
+            want = xh if ww is None else xh * ww.double() + bb.double()
+            # half a bf16 step, and 1e-5 of the terms for the f32 arithmetic
+            assert ((y.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5 * (1 + want.abs() + xh.abs())).all()
+            t = g.double() if ww is None else g.double() * ww.double()
+            want = r * (t - t.mean(-1, keepdim=True) - xh * (t * xh).mean(-1, keepdim=True))
+            lim = 2.0 ** -8 * want.abs() + 1e-5 * r * (1 + t.abs() + xh.abs())
+            assert ((gx.double() - want).abs() <= lim).all()
+            if ww is not None:
+                s = (g.double() * xh).abs().sum(0)
+                assert ((gw.double() - (g.double() * xh).sum(0)).abs() <= 1e-5 * s).all()
+                assert ((gb.double() - g.double().sum(0)).abs() <= 1e-5 * g.double().abs().sum(0)).all()
+
+
 @pytest.mark.parametrize("C", [96, 1023, 2600])
 def test_statistics_of_rows_far_from_zero(C):
     """Mean 1000 times the spread: <x^2> - mean^2 would lose every digit of the variance."""
