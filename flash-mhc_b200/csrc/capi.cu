@@ -624,6 +624,8 @@ int fmhc_k4_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scal
 
 int64_t fmhc_k1_bwd_q8_workspace_size(int64_t T, int64_t C) {
   if (T <= 0 || C <= 0 || C > (int64_t(1) << 26)) return 0;
+  if (fmhc::k1_tc_bwd_q8_shape(T, 4 * C)) return fmhc::k1_tc_bwd_workspace_bytes(T, 4 * C);
+  // Other widths: x restored to bf16, then the workspace of fmhc_k1_bwd.
   return ((T * 4 * C * 2 + 255) & ~int64_t(255)) + fmhc_k1_bwd_workspace_size(T, 4 * C, 32);
 }
 
@@ -633,23 +635,36 @@ int fmhc_k1_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scal
                    int64_t C, void *stream) {
   const char *w = "fmhc_k1_bwd_q8";
   if (int e = check_streams(w, T, n, C)) return e;
-  if (int e = check_k1(w, T, n * C, 32)) return e;
+  const int64_t nC = n * C;
+  if (int e = check_k1(w, T, nC, 32)) return e;
   FMHC_REQUIRE_FMT(w, format);
   FMHC_REQUIRE_PTR(w, grad_W);
   cudaStream_t s = (cudaStream_t)stream;
   if (T == 0) return fmhc_k1_bwd(nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, grad_W, nullptr,
-                                 0, 0, n * C, 32, stream);
-  FMHC_REQUIRE_PTR(w, x_codes); FMHC_REQUIRE_PTR(w, x_scales); FMHC_REQUIRE_PTR(w, workspace);
+                                 0, 0, nC, 32, stream);
+  FMHC_REQUIRE_PTR(w, grad_out); FMHC_REQUIRE_PTR(w, x_codes); FMHC_REQUIRE_PTR(w, x_scales);
+  FMHC_REQUIRE_PTR(w, W); FMHC_REQUIRE_PTR(w, proj); FMHC_REQUIRE_PTR(w, inv_rms);
+  FMHC_REQUIRE_PTR(w, grad_x); FMHC_REQUIRE_PTR(w, workspace);
+  FMHC_REQUIRE_ALIGN2(w, grad_W); FMHC_REQUIRE_ALIGN_TO(w, inv_rms, 4);
   if (!aligned(workspace, 256)) return fail(FMHC_ERR_ALIGNMENT, "%s: workspace must be 256-byte aligned", w);
   const int64_t need = fmhc_k1_bwd_q8_workspace_size(T, C);
   if (workspace_bytes < need)
     return fail(FMHC_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", w,
                 (long long)workspace_bytes, (long long)need);
-  const int64_t x_bytes = (T * 4 * C * 2 + 255) & ~int64_t(255);
+  if (fmhc::k1_tc_bwd_q8_shape(T, nC)) {
+    FMHC_REQUIRE_ALIGN16(w, grad_out); FMHC_REQUIRE_ALIGN16(w, x_codes); FMHC_REQUIRE_ALIGN16(w, W);
+    FMHC_REQUIRE_ALIGN16(w, proj); FMHC_REQUIRE_ALIGN16(w, grad_x);
+    if (!aligned(x_scales, 4)) return fail(FMHC_ERR_ALIGNMENT, "%s: x_scales must be 4-byte aligned", w);
+    if (int e = fmhc::launch_k1_tc_bwd_q8(grad_out, x_codes, x_scales, format, W, proj, inv_rms,
+                                          grad_x, grad_W, workspace, T, int(nC), s))
+      return fail(e, "%s: %s", w, fmhc::k1_tc_error());
+    return check_launch(w);
+  }
+  const int64_t x_bytes = (T * nC * 2 + 255) & ~int64_t(255);
   fmhc::launch_act_dequantize(x_codes, format, x_scales, workspace, FMHC_DTYPE_BF16, 4 * T, int(C),
                               C % 8 == 0 && aligned(x_codes, 8), s);
   return fmhc_k1_bwd(grad_out, workspace, W, proj, inv_rms, grad_x, grad_W,
-                     (char *)workspace + x_bytes, workspace_bytes - x_bytes, T, n * C, 32, stream);
+                     (char *)workspace + x_bytes, workspace_bytes - x_bytes, T, nC, 32, stream);
 }
 
 // ------------------------------------------------------------------ layer norm

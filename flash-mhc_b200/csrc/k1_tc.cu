@@ -745,6 +745,7 @@ k1_fwd_rows_cluster_kernel(const __nv_bfloat16 *__restrict__ x, const __nv_bfloa
 }  // namespace fmhc
 
 #include "k1_tc_bwd.cuh"
+#include "k1_tc_bwd_q8.cuh"
 
 namespace fmhc {
 namespace k1tc {
@@ -798,13 +799,14 @@ int device_sms() {
 // threads, and a first-time attribute call must not land inside a CUDA-graph
 // capture made on another thread).
 int set_smem_attr(const void *kernel, size_t bytes) {
+  constexpr int kKernels = 16;  // more than this file has
   static std::mutex mu;
-  static const void *done_kernel[8][16] = {};
+  static const void *done_kernel[kKernels][16] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 16) dev = 15;
   std::lock_guard<std::mutex> lock(mu);
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < kKernels; ++i) {
     if (done_kernel[i][dev] == kernel) return 0;
     if (done_kernel[i][dev] == nullptr) {
       if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) !=
@@ -834,6 +836,7 @@ bool device_is_sm100() {
 const char *k1_tc_error() { return k1tc::g_msg; }
 
 static_assert(sizeof(k1tc::BwdSmem) + 1024 <= 232448, "K1 backward shared memory");
+static_assert(sizeof(k1tc::BwdQ8Smem) + 1024 <= 232448, "K1 backward shared memory (8-bit x)");
 static_assert((sizeof(k1tc::FwdSmem) + 1024) * FMHC_K1F_CTAS_PER_SM <= 232448,
               "K1 forward shared memory");
 static_assert((sizeof(k1tc::SkSmem<k1tc::kSkStagesShallow>) + 1024) * FMHC_K1F_CTAS_PER_SM <= 232448,
@@ -1073,6 +1076,52 @@ int launch_k1_tc_bwd(const void *go, const void *x, const void *W, const void *p
     launch(k1_bwd_dw_reduce_kernel, dim3(unsigned(p.nkc), kND), dim3(kBwdBK), 0, s, part,
            static_cast<__nv_bfloat16 *>(gW), nC, p.ntt, p.G, p.base, p.rem);
   }
+  return 0;
+}
+
+bool k1_tc_bwd_q8_shape(int64_t T, int64_t nC) {
+  return nC % k1tc::kBwdBK == 0 && T >= 1 && T <= (int64_t(1) << 31) &&
+         nC / k1tc::kBwdBK <= int64_t(k1tc::kBwdMaxG) * k1tc::device_sms() &&
+         k1tc::device_is_sm100() && k1tc::encode_fn() != nullptr;
+}
+
+int launch_k1_tc_bwd_q8(const void *go, const void *codes, const void *scales, int fmt,
+                        const void *W, const void *proj, const float *inv_rms, void *gx, void *gW,
+                        void *ws, int64_t T, int nC, cudaStream_t s) {
+  using namespace k1tc;
+  const BwdPlan p = bwd_plan(T, nC);
+  CUtensorMap mq, mgx, mgo, mproj, mw;
+  // The codes as pairs of bytes: rows of nC / 2, boxes of 64 (128 columns).
+  bool ok = make_map(&mq, codes, uint64_t(nC) / 2, uint64_t(T), uint64_t(nC), 64, kBwdBT,
+                     CU_TENSOR_MAP_SWIZZLE_128B) &&
+            make_map(&mgx, gx, uint64_t(nC), uint64_t(T), uint64_t(nC) * 2, 64, kBwdBT,
+                     CU_TENSOR_MAP_SWIZZLE_128B) &&
+            make_map(&mgo, go, kND, uint64_t(T), kND * 2, kND, kBwdBT, CU_TENSOR_MAP_SWIZZLE_64B) &&
+            make_map(&mproj, proj, kND, uint64_t(T), kND * 2, kND, kBwdBT,
+                     CU_TENSOR_MAP_SWIZZLE_64B) &&
+            make_map(&mw, W, uint64_t(nC), kND, uint64_t(nC) * 2, 64, kND,
+                     CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!ok) {
+    snprintf(g_msg, sizeof(g_msg), "cuTensorMapEncodeTiled failed");
+    return 5;
+  }
+  const size_t smem = sizeof(BwdQ8Smem) + 1024;
+  auto kern = fmt == act8::kInt8 ? k1_bwd_q8_tc_kernel<act8::kInt8> : k1_bwd_q8_tc_kernel<act8::kE4m3>;
+  if (int e = set_smem_attr(reinterpret_cast<const void *>(kern), smem)) return e;
+  BwdArgs args{};
+  args.inv_rms = inv_rms;
+  args.dw_part = static_cast<float *>(ws);
+  args.T = T;
+  args.nC = nC;
+  args.ntt = p.ntt;
+  args.G = p.G;
+  args.base = p.base;
+  args.rem = p.rem;
+  args.with_dw = 1;
+  launch(kern, dim3(unsigned(p.grid)), dim3(kQ8Threads), smem, s, mq, mgx, mgo, mproj, mw,
+         static_cast<const uint8_t *>(scales), args);
+  launch(k1_bwd_dw_reduce_kernel, dim3(unsigned(p.nkc), kND), dim3(kBwdBK), 0, s,
+         (const float *)args.dw_part, static_cast<__nv_bfloat16 *>(gW), nC, p.ntt, p.G, p.base, p.rem);
   return 0;
 }
 

@@ -38,6 +38,14 @@ int launch_k1_tc_bwd(const void *go, const void *x, const void *W, const void *p
                      const float *inv_rms, void *gx, void *gW, void *ws, int64_t ws_bytes,
                      int64_t T, int nC, cudaStream_t s);
 
+// Backward (grad_x and grad_W) from an 8-bit checkpoint of x.  Needs a shape for
+// which k1_tc_bwd_q8_shape holds, go, codes, W, proj and gx 16-byte and scales
+// 4-byte aligned, and a workspace of k1_tc_bwd_workspace_bytes(T, nC).
+bool k1_tc_bwd_q8_shape(int64_t T, int64_t nC);
+int launch_k1_tc_bwd_q8(const void *go, const void *codes, const void *scales, int fmt,
+                        const void *W, const void *proj, const float *inv_rms, void *gx, void *gW,
+                        void *ws, int64_t T, int nC, cudaStream_t s);
+
 // Test hook: the persistent tensor-core forward in which CTA 0 loses its first
 // copy, so its waits on that stage expire (see k1_fwd_tc_kernel's LOSE_COPY).
 // Same preconditions as launch_k1_tc_fwd; the output is not meaningful.

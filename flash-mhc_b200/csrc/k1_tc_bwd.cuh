@@ -151,6 +151,35 @@ __device__ __forceinline__ float go_proj_chunk_dot(const uint4 g, const uint4 p)
   return dot;
 }
 
+// Tile prep of one slot by one warp: gos = bf16(go * inv_rms) and (s, inv_rms)
+// per token, from the slot's go and proj.  Lane l takes the tile rows l, l + 32,
+// l + 64, l + 96, whose inv_rms are invr.
+__device__ __forceinline__ void prep_tile(uint8_t *sb, int lane, const float (&invr)[4], float nC) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = lane + 32 * i;
+    const float rinv = invr[i];
+    float pc[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int off = r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+      const uint4 g = *reinterpret_cast<const uint4 *>(sb + kBwdSlotGo + off);
+      const uint4 pj = *reinterpret_cast<const uint4 *>(sb + kBwdSlotProj + off);
+      pc[c] = go_proj_chunk_dot(g, pj);
+      // gos = bf16(go * inv_rms), as the reference's (grad_out * inv_rms).to(x.dtype)
+      uint4 o;
+      o.x = pack_bf16x2(bf16lo(g.x) * rinv, bf16hi(g.x) * rinv);
+      o.y = pack_bf16x2(bf16lo(g.y) * rinv, bf16hi(g.y) * rinv);
+      o.z = pack_bf16x2(bf16lo(g.z) * rinv, bf16hi(g.z) * rinv);
+      o.w = pack_bf16x2(bf16lo(g.w) * rinv, bf16hi(g.w) * rinv);
+      *reinterpret_cast<uint4 *>(sb + kBwdSlotGos + off) = o;
+    }
+    const float dot = (pc[0] + pc[1]) + (pc[2] + pc[3]);
+    reinterpret_cast<float2 *>(sb + kBwdSlotSinv)[r] =
+        make_float2(dot * (rinv * rinv) / nC, rinv);
+  }
+}
+
 __global__ void __launch_bounds__(kBwdThreads, 1)
 k1_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_x,
                  const __grid_constant__ CUtensorMap tmap_gx,
@@ -423,30 +452,7 @@ k1_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_x,
         invr[i] = t < a.T ? __ldg(a.inv_rms + t) : 0.f;
       }
       if (!mbar_wait(smem_u32(&sm.gfull[slot]), sphase, abort, kSiteBPrepSlot)) break;
-      uint8_t *sb = sm.slot[slot];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = lane + 32 * i;
-        const float rinv = invr[i];
-        float pc[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int off = r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
-          const uint4 g = *reinterpret_cast<const uint4 *>(sb + kBwdSlotGo + off);
-          const uint4 pj = *reinterpret_cast<const uint4 *>(sb + kBwdSlotProj + off);
-          pc[c] = go_proj_chunk_dot(g, pj);
-          // gos = bf16(go * inv_rms), as the reference's (grad_out * inv_rms).to(x.dtype)
-          uint4 o;
-          o.x = pack_bf16x2(bf16lo(g.x) * rinv, bf16hi(g.x) * rinv);
-          o.y = pack_bf16x2(bf16lo(g.y) * rinv, bf16hi(g.y) * rinv);
-          o.z = pack_bf16x2(bf16lo(g.z) * rinv, bf16hi(g.z) * rinv);
-          o.w = pack_bf16x2(bf16lo(g.w) * rinv, bf16hi(g.w) * rinv);
-          *reinterpret_cast<uint4 *>(sb + kBwdSlotGos + off) = o;
-        }
-        const float dot = (pc[0] + pc[1]) + (pc[2] + pc[3]);
-        reinterpret_cast<float2 *>(sb + kBwdSlotSinv)[r] =
-            make_float2(dot * (rinv * rinv) / float(a.nC), rinv);
-      }
+      prep_tile(sm.slot[slot], lane, invr, float(a.nC));
       // gos is read by the MMA (async proxy) and go/proj are refilled by the
       // TMA: order this thread's generic reads and writes before both.
       fence_proxy_async_smem();

@@ -1,0 +1,412 @@
+// K1 backward on the tensor cores from an 8-bit checkpoint of x: grad_x and
+// grad_W in one pass over the codes.  Included by k1_tc.cu after
+// k1_tc_bwd.cuh, whose formulas, work order, token-tile slots and grad_W
+// reduction it shares (x there is the restored x8 here).
+//
+// The tensor cores want x as bf16 in the 128-byte-swizzled layout that the TMA
+// gives the bf16 kernel.  Both code formats are exact in bf16, so here the TMA
+// brings the codes (a quarter of the bytes that the bf16 kernel moves in and
+// out is saved), and four more warps widen them into that layout:
+//
+//   warp 0       TMA producer: go and proj per token tile (slots), and per unit
+//                the codes [128 t x 128 k] and the W chunk into a raw stage.
+//   warps 12-15  converters, thread = token row: codes and scale bytes of the
+//                row -> bf16 x tile in an x stage.  The four scale bytes of a
+//                row's 128 columns are one word, loaded a unit ahead.
+//   warp 1       MMA issuer: as in the bf16 kernel, on the x stage, the raw
+//                stage's W chunk and the slot.
+//   warps 2-9    epilogue, warp 10 store, warp 11 tile prep: as in the bf16
+//                kernel; the epilogue takes its 64 columns in two halves, which
+//                keeps a thread within the 128 registers that 16 warps leave.
+//
+// A raw stage is free again when the converters have read the codes and the
+// MMAs have read W; an x stage when the TMA store has read the grad_x that the
+// epilogue wrote over x.  Every wait is bounded (sm100_ptx.cuh).
+#pragma once
+
+#include "act8.cuh"
+
+namespace fmhc {
+namespace k1tc {
+
+constexpr int kQ8Raw = 3;                             // raw stages: codes and W chunk
+constexpr int kQ8Stages = 3;                          // x stages
+constexpr int kQ8CodeBytes = kBwdBT * kBwdBK;         // 16 KiB
+constexpr int kQ8RawBytes = kQ8CodeBytes + kBwdWBytes;  // 24 KiB
+constexpr int kQ8ConvWarp = kBwdPrepWarp + 1;
+constexpr int kQ8ConvWarps = 4;
+constexpr int kQ8Threads = 32 * (kQ8ConvWarp + kQ8ConvWarps);  // 512
+static_assert(kBwdInflight < kQ8Stages, "stores in flight");
+
+struct alignas(1024) BwdQ8Smem {
+  uint8_t raw[kQ8Raw][kQ8RawBytes];           // codes, then the W chunk
+  uint8_t x[kQ8Stages][kBwdXBytes];           // x tile, later grad_x
+  uint8_t slot[kBwdSlots][kBwdSlotBytes];     // go, proj, gos, (s, inv) of one token tile
+  uint64_t rfull[kQ8Raw];                     // codes and W landed
+  uint64_t rempty[kQ8Raw];                    // converters + MMA commit
+  uint64_t xfull[kQ8Stages];                  // converters wrote x
+  uint64_t xempty[kQ8Stages];                 // the store has read grad_x
+  uint64_t epi[kQ8Stages];                    // the epilogue wrote grad_x
+  uint64_t gfull[kBwdSlots];
+  uint64_t gready[kBwdSlots];
+  uint64_t gempty[kBwdSlots];
+  uint64_t tfull[2];
+  uint64_t tempty[2];
+  uint64_t dwfull;
+  uint64_t mma_done;
+  uint32_t tmem_base;
+  int abort;
+};
+
+enum : unsigned { kSiteQProdRaw = 0x301, kSiteQProdSlot = 0x302, kSiteQMmaRaw = 0x303,
+                  kSiteQMmaX = 0x304, kSiteQMmaTempty = 0x305, kSiteQMmaSlot = 0x306,
+                  kSiteQEpiSlot = 0x307, kSiteQEpiX = 0x308, kSiteQEpiTfull = 0x309,
+                  kSiteQEpiDw = 0x30a, kSiteQStore = 0x30b, kSiteQPrep = 0x30c,
+                  kSiteQConvRaw = 0x30d, kSiteQConvX = 0x30e, kSiteQDrain = 0x30f };
+
+// Eight codes (two words) with scale s -> eight bf16 values (exact).
+template <int FMT>
+__device__ __forceinline__ uint4 codes_to_bf16(uint32_t a, uint32_t b, float s) {
+  float f[4], g[4];
+  act8::decode4<FMT>(a, f);
+  act8::decode4<FMT>(b, g);
+  return make_uint4(pack_bf16x2(f[0] * s, f[1] * s), pack_bf16x2(f[2] * s, f[3] * s),
+                    pack_bf16x2(g[0] * s, g[1] * s), pack_bf16x2(g[2] * s, g[3] * s));
+}
+
+template <int FMT>
+__global__ void __launch_bounds__(kQ8Threads, 1)
+k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
+                    const __grid_constant__ CUtensorMap tmap_gx,
+                    const __grid_constant__ CUtensorMap tmap_go,
+                    const __grid_constant__ CUtensorMap tmap_proj,
+                    const __grid_constant__ CUtensorMap tmap_w,
+                    const uint8_t *__restrict__ scales, const BwdArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  BwdQ8Smem &sm = *reinterpret_cast<BwdQ8Smem *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  volatile int *abort = &sm.abort;
+
+  int grp, gi, ng;
+  bwd_cta_group(int(blockIdx.x), a.base, a.rem, grp, gi, ng);
+  const int G = a.G;
+  const int ntiles = gi < a.ntt ? (a.ntt - gi + ng - 1) / ng : 0;
+  const int nunits = ntiles * G;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kQ8Raw; ++s) {
+      mbar_init(smem_u32(&sm.rfull[s]), 1);
+      mbar_init(smem_u32(&sm.rempty[s]), kQ8ConvWarps + 1);
+    }
+    for (int s = 0; s < kQ8Stages; ++s) {
+      mbar_init(smem_u32(&sm.xfull[s]), kQ8ConvWarps);
+      mbar_init(smem_u32(&sm.xempty[s]), 1);
+      mbar_init(smem_u32(&sm.epi[s]), kBwdEpiWarps);
+    }
+    for (int b = 0; b < kBwdSlots; ++b) {
+      mbar_init(smem_u32(&sm.gfull[b]), 1);
+      mbar_init(smem_u32(&sm.gready[b]), 1);
+      mbar_init(smem_u32(&sm.gempty[b]), 1 + kBwdEpiWarps);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&sm.tfull[b]), 1);
+      mbar_init(smem_u32(&sm.tempty[b]), kBwdEpiWarps);
+    }
+    mbar_init(smem_u32(&sm.dwfull), 1);
+    mbar_init(smem_u32(&sm.mma_done), 1);
+    sm.abort = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tmap_codes);
+    prefetch_tmap(&tmap_gx);
+    prefetch_tmap(&tmap_go);
+    prefetch_tmap(&tmap_proj);
+    prefetch_tmap(&tmap_w);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&sm.tmem_base), kBwdTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  // No global memory is touched before this point (see pdl_wait()).
+  pdl_wait();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      int stage = 0, slot = 0, issued = 0, slots_issued = 0;
+      uint32_t phase = 0, sphase = 0;
+      for (int j = 0; j < nunits && !*abort; ++j) {
+        const int m = j / G, jj = j - m * G;
+        const int32_t row0 = (gi + m * ng) * kBwdBT;
+        const int kc = grp * G + jj;
+        if (jj == 0) {  // new token tile: go and proj into the next slot
+          if (!mbar_wait(smem_u32(&sm.gempty[slot]), sphase ^ 1, abort, kSiteQProdSlot)) break;
+          const uint32_t gf = smem_u32(&sm.gfull[slot]);
+          const uint32_t sb = smem_u32(sm.slot[slot]);
+          mbar_arrive_expect_tx(gf, uint32_t(2 * kBwdGBytes));
+          tma_load_2d(sb + kBwdSlotGo, &tmap_go, gf, 0, row0);
+          tma_load_2d(sb + kBwdSlotProj, &tmap_proj, gf, 0, row0);
+          ++slots_issued;
+          if (++slot == kBwdSlots) { slot = 0; sphase ^= 1; }
+        }
+        if (!mbar_wait(smem_u32(&sm.rempty[stage]), phase ^ 1, abort, kSiteQProdRaw)) break;
+        const uint32_t f = smem_u32(&sm.rfull[stage]);
+        const uint32_t base = smem_u32(sm.raw[stage]);
+        mbar_arrive_expect_tx(f, uint32_t(kQ8RawBytes));
+        // The codes' map counts pairs of bytes: 64 of them are 128 columns.
+        tma_load_2d(base, &tmap_codes, f, kc * (kBwdBK / 2), row0);
+        tma_load_2d(base + kQ8CodeBytes, &tmap_w, f, kc * kBwdBK, 0);
+        tma_load_2d(base + kQ8CodeBytes + kBwdWBytes / 2, &tmap_w, f, kc * kBwdBK + 64, 0);
+        ++issued;
+        if (++stage == kQ8Raw) { stage = 0; phase ^= 1; }
+      }
+      // Drain: every copy issued must have landed before the CTA exits.
+      int n = issued < kQ8Raw ? issued : kQ8Raw;
+      int s = stage;
+      uint32_t ph = phase;
+      for (int i = 0; i < n; ++i) {
+        if (--s < 0) { s = kQ8Raw - 1; ph ^= 1; }
+        mbar_wait(smem_u32(&sm.rfull[s]), ph, abort, kSiteQDrain, true);
+      }
+      n = slots_issued < kBwdSlots ? slots_issued : kBwdSlots;
+      s = slot;
+      ph = sphase;
+      for (int i = 0; i < n; ++i) {
+        if (--s < 0) { s = kBwdSlots - 1; ph ^= 1; }
+        mbar_wait(smem_u32(&sm.gfull[s]), ph, abort, kSiteQDrain, true);
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc_dx = idesc_bf16_f32(kBwdBT, kBwdBK, 0, 1);
+      constexpr uint32_t idesc_dw = idesc_bf16_f32(kBwdBK, kND, 1, 1);
+      int raw = 0, stage = 0, acc = 0, slot = 0;
+      uint32_t rphase = 0, phase = 0, acc_phase = 0, sphase = 0;
+      bool ok = true;
+      for (int j = 0; j < nunits && !*abort; ++j) {
+        const int m = j / G, jj = j - m * G;
+        if (jj == 0 &&
+            !mbar_wait(smem_u32(&sm.gready[slot]), sphase, abort, kSiteQMmaSlot)) { ok = false; break; }
+        if (!mbar_wait(smem_u32(&sm.tempty[acc]), acc_phase ^ 1, abort, kSiteQMmaTempty)) { ok = false; break; }
+        if (!mbar_wait(smem_u32(&sm.rfull[raw]), rphase, abort, kSiteQMmaRaw)) { ok = false; break; }
+        if (!mbar_wait(smem_u32(&sm.xfull[stage]), phase, abort, kSiteQMmaX)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t base = smem_u32(sm.x[stage]);
+        const uint32_t wb = smem_u32(sm.raw[raw]) + kQ8CodeBytes;
+        const uint32_t gs = smem_u32(sm.slot[slot]);
+        // grad_W: M = k (two 64-wide MN blocks 16 KiB apart), N = d, K = tokens.
+#pragma unroll
+        for (int k = 0; k < kBwdBT / 16; ++k) {
+          const uint64_t ad = smem_desc(base + k * 2048, kBwdXBox, 1024, 2);
+          const uint64_t bd = smem_desc(gs + kBwdSlotGos + k * 1024, 512, 512, 4);
+          mma_bf16_ss(tmem + kBwdDwCol + uint32_t(jj * kND), ad, bd, idesc_dw,
+                      (m > 0 || k > 0) ? 1u : 0u);
+        }
+        // grad_x: M = tokens, N = 128 k (two 64-wide MN blocks 4 KiB apart), K = d.
+#pragma unroll
+        for (int k = 0; k < kND / 16; ++k) {
+          const uint64_t ad = smem_desc(gs + kBwdSlotGo + k * 32, 16, 512, 4);
+          const uint64_t bd = smem_desc(wb + k * 2048, kBwdWBytes / 2, 1024, 2);
+          mma_bf16_ss(tmem + uint32_t(acc * kBwdBK), ad, bd, idesc_dx, k != 0);
+        }
+        mma_commit(smem_u32(&sm.tfull[acc]));
+        mma_commit(smem_u32(&sm.rempty[raw]));
+        if (jj == G - 1) {
+          mma_commit(smem_u32(&sm.gempty[slot]));
+          if (++slot == kBwdSlots) { slot = 0; sphase ^= 1; }
+        }
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+        if (++raw == kQ8Raw) { raw = 0; rphase ^= 1; }
+        if (++stage == kQ8Stages) { stage = 0; phase ^= 1; }
+      }
+      if (ok && !*abort && nunits > 0) mma_commit(smem_u32(&sm.dwfull));
+      mma_commit(smem_u32(&sm.mma_done));
+      mbar_wait(smem_u32(&sm.mma_done), 0, abort, kSiteQDrain, true);
+    }
+  } else if (warp < kBwdStoreWarp) {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;           // TMEM lane quarter
+    const int h = (warp - 2) >> 2;    // column half of the unit (0: 0-63, 1: 64-127)
+    const int r = q * 32 + lane;      // token row of the unit / k row of the grad_W partial
+    int stage = 0, acc = 0, slot = 0;
+    uint32_t phase = 0, acc_phase = 0, sphase = 0;
+    float s = 0.f, inv = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nunits && !*abort; ++j) {
+      const int m = j / G, jj = j - m * G;
+      if (jj == 0) {
+        // (s, inv_rms) of this thread's token, kept in registers for the tile.
+        if (!mbar_wait(smem_u32(&sm.gready[slot]), sphase, abort, kSiteQEpiSlot)) { ok = false; break; }
+        const float2 si = reinterpret_cast<const float2 *>(sm.slot[slot] + kBwdSlotSinv)[r];
+        s = si.x;
+        inv = si.y;
+        // The slot's refill is a TMA (async-proxy) write: order this thread's
+        // generic-proxy read before it, then release (one arrive per warp).
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.gempty[slot]));
+        if (++slot == kBwdSlots) { slot = 0; sphase ^= 1; }
+      }
+      if (!mbar_wait(smem_u32(&sm.xfull[stage]), phase, abort, kSiteQEpiX)) { ok = false; break; }
+      if (!mbar_wait(smem_u32(&sm.tfull[acc]), acc_phase, abort, kSiteQEpiTfull)) { ok = false; break; }
+      tc_fence_after();
+      // Columns 64h .. 64h+63 of row r are one 128-byte row of x box h.
+      uint8_t *rowp = sm.x[stage] + h * kBwdXBox + r * 128;
+      const uint32_t tl = tmem + (uint32_t(q * 32) << 16) + uint32_t(acc * kBwdBK + 64 * h);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tl + 32 * p, v);
+        uint4 xv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          xv[i] = *reinterpret_cast<const uint4 *>(rowp + (((4 * p + i) ^ (r & 7)) << 4));
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float *dv = reinterpret_cast<const float *>(v + 8 * i);
+          uint4 o;
+          o.x = pack_bf16x2(fmaf(-s, bf16lo(xv[i].x), inv * dv[0]), fmaf(-s, bf16hi(xv[i].x), inv * dv[1]));
+          o.y = pack_bf16x2(fmaf(-s, bf16lo(xv[i].y), inv * dv[2]), fmaf(-s, bf16hi(xv[i].y), inv * dv[3]));
+          o.z = pack_bf16x2(fmaf(-s, bf16lo(xv[i].z), inv * dv[4]), fmaf(-s, bf16hi(xv[i].z), inv * dv[5]));
+          o.w = pack_bf16x2(fmaf(-s, bf16lo(xv[i].w), inv * dv[6]), fmaf(-s, bf16hi(xv[i].w), inv * dv[7]));
+          *reinterpret_cast<uint4 *>(rowp + (((4 * p + i) ^ (r & 7)) << 4)) = o;
+        }
+      }
+      // Every writer makes its grad_x visible to the TMA (async proxy), then
+      // one arrive per warp on epi[stage] for the store warp and on tempty.
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(smem_u32(&sm.epi[stage]));
+        mbar_arrive(smem_u32(&sm.tempty[acc]));
+      }
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      if (++stage == kQ8Stages) { stage = 0; phase ^= 1; }
+    }
+    if (ok && nunits > 0 && mbar_wait(smem_u32(&sm.dwfull), 0, abort, kSiteQEpiDw)) {
+      // grad_W partials of the group's G k-chunks: thread r owns k row r of
+      // each, 32 d columns; warps 2-5 take the even chunks, warps 6-9 the odd.
+      tc_fence_after();
+      float *dst0 = a.dw_part + int64_t(blockIdx.x) * G * (kND * kBwdBK) + r;
+      for (int jj = h; jj < G; jj += 2) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tmem + (uint32_t(q * 32) << 16) + kBwdDwCol + uint32_t(jj * kND), v);
+        tmem_wait_ld();
+        float *dst = dst0 + int64_t(jj) * (kND * kBwdBK);
+#pragma unroll
+        for (int d = 0; d < kND; ++d) __stcg(dst + d * kBwdBK, __uint_as_float(v[d]));
+      }
+    }
+  } else if (warp == kBwdStoreWarp) {
+    // --------------------------------------------------------------- store
+    if (lane == 0) {
+      int stage = 0, npend = 0;
+      int pend[kBwdInflight];
+      uint32_t phase = 0;
+      for (int j = 0; j < nunits && !*abort; ++j) {
+        const int m = j / G, jj = j - m * G;
+        const int32_t row0 = (gi + m * ng) * kBwdBT;
+        const int kc = grp * G + jj;
+        if (!mbar_wait(smem_u32(&sm.epi[stage]), phase, abort, kSiteQStore)) break;
+        const uint32_t base = smem_u32(sm.x[stage]);
+        tma_store_2d(&tmap_gx, base, kc * kBwdBK, row0);
+        tma_store_2d(&tmap_gx, base + kBwdXBox, kc * kBwdBK + 64, row0);
+        tma_store_commit();
+        pend[npend++] = stage;
+        tma_store_wait_read<kBwdInflight - 1>();
+        while (npend > kBwdInflight - 1) {
+          mbar_arrive(smem_u32(&sm.xempty[pend[0]]));
+          for (int i = 1; i < npend; ++i) pend[i - 1] = pend[i];
+          --npend;
+        }
+        if (++stage == kQ8Stages) { stage = 0; phase ^= 1; }
+      }
+      tma_store_wait_all<0>();
+      for (int i = 0; i < npend; ++i) mbar_arrive(smem_u32(&sm.xempty[pend[i]]));
+    }
+  } else if (warp == kBwdPrepWarp) {
+    // ----------------------------------------------------------- tile prep
+    // As in the bf16 kernel: lane l takes the tile rows l, l + 32, l + 64, l + 96.
+    int slot = 0;
+    uint32_t sphase = 0;
+    for (int m = 0; m < ntiles && !*abort; ++m) {
+      const int64_t t0 = int64_t(gi + m * ng) * kBwdBT;
+      float invr[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t t = t0 + lane + 32 * i;
+        invr[i] = t < a.T ? __ldg(a.inv_rms + t) : 0.f;
+      }
+      if (!mbar_wait(smem_u32(&sm.gfull[slot]), sphase, abort, kSiteQPrep)) break;
+      prep_tile(sm.slot[slot], lane, invr, float(a.nC));
+      // gos is read by the MMA (async proxy) and go/proj are refilled by the
+      // TMA: order this thread's generic reads and writes before both.
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sm.gready[slot]));
+      if (++slot == kBwdSlots) { slot = 0; sphase ^= 1; }
+    }
+  } else {
+    // ----------------------------------------------------------- converters
+    const int r = (warp - kQ8ConvWarp) * 32 + lane;  // token row of the unit
+    const int64_t words = a.nC / 128;                // scale words per token (4 bytes: 128 columns)
+    const auto scale_word = [&](int j) {
+      const int m = j / G, jj = j - m * G;
+      const int64_t t = int64_t(gi + m * ng) * kBwdBT + r;
+      return j < nunits && t < a.T
+                 ? __ldg(reinterpret_cast<const uint32_t *>(scales) + t * words + grp * G + jj)
+                 : 0u;
+    };
+    int raw = 0, stage = 0;
+    uint32_t rphase = 0, phase = 0;
+    uint32_t next = scale_word(0);
+    for (int j = 0; j < nunits && !*abort; ++j) {
+      const uint32_t sw = next;
+      next = scale_word(j + 1);
+      if (!mbar_wait(smem_u32(&sm.rfull[raw]), rphase, abort, kSiteQConvRaw)) break;
+      if (!mbar_wait(smem_u32(&sm.xempty[stage]), phase ^ 1, abort, kSiteQConvX)) break;
+      // Row r of the codes: 128 bytes, 16-byte chunk c at position c ^ (r & 7).
+      // Columns 16c .. 16c+15 go to chunks 2(c & 3) and 2(c & 3) + 1 of the
+      // 128-byte row r of x box c / 4, swizzled the same way.
+      const uint8_t *src = sm.raw[raw] + r * 128;
+      uint8_t *dst = sm.x[stage] + r * 128;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(src + ((c ^ (r & 7)) << 4));
+        const float s = act8::scale_value((sw >> (8 * (c >> 1))) & 0xffu);
+        uint8_t *row = dst + (c >> 2) * kBwdXBox;
+        const int i = 2 * (c & 3);
+        *reinterpret_cast<uint4 *>(row + ((i ^ (r & 7)) << 4)) = codes_to_bf16<FMT>(v.x, v.y, s);
+        *reinterpret_cast<uint4 *>(row + (((i + 1) ^ (r & 7)) << 4)) = codes_to_bf16<FMT>(v.z, v.w, s);
+      }
+      // x is read by the MMA (async proxy) and the raw stage is refilled by the
+      // TMA: order this thread's writes and reads before both.
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(smem_u32(&sm.xfull[stage]));
+        mbar_arrive(smem_u32(&sm.rempty[raw]));
+      }
+      if (++raw == kQ8Raw) { raw = 0; rphase ^= 1; }
+      if (++stage == kQ8Stages) { stage = 0; phase ^= 1; }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kBwdTmemCols);
+  }
+}
+
+}  // namespace k1tc
+}  // namespace fmhc

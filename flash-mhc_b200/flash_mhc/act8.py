@@ -110,6 +110,11 @@ def _new_checkpoint(x: torch.Tensor, code_dtype: torch.dtype):
             torch.empty(_scales_shape(x.shape), device=x.device, dtype=torch.uint8))
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` at an address that is a multiple of 16 (a copy if it is a view at another one)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _streams(op: str, name: str, x: torch.Tensor):
     if x.dim() != 3:
         raise ValueError(f"flash_mhc::{op}: {name} must be (T, n, C) (got {tuple(x.shape)})")
@@ -317,6 +322,7 @@ def _fused_rmsnorm_project_backward_q8_cuda(grad_out, x_codes, x_scales, W, proj
                  inv_rms=inv_rms)
     x_codes, x_scales, fmt = _checkpoint(op, "x", x_codes, x_scales)
     grad_out, W, proj_out = _bf16("grad_out", grad_out), _bf16("W", W), _bf16("proj_out", proj_out)
+    grad_out, W, proj_out, x_codes, x_scales = (_aligned(t) for t in (grad_out, W, proj_out, x_codes, x_scales))
     inv_rms = inv_rms.to(torch.float32).contiguous()
     dev, dt = grad_out.device, grad_out.dtype
     grad_x = torch.empty((T, n, C), device=dev, dtype=dt)

@@ -232,6 +232,30 @@ def test_projection_backward_from_a_checkpoint(T, C, fmt):
     _within("grad_W", gW, want, BF16_HALF * np.abs(want) + (T + 8) * U23 * (np.abs(gos).T @ np.abs(x8)) + 1e-30)
 
 
+def test_projection_backward_of_views_at_odd_addresses_and_of_non_finite_streams():
+    T, C = 200, 64
+    x, W, go, proj, inv = _projection(T, C)
+    xc, xs = act8.quantize(x)
+    want = ops.fused_rmsnorm_project_backward_q8(go, xc, xs, W, proj, inv)
+
+    def moved(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        v = flat[1:].view(t.shape)
+        v.copy_(t)
+        return v
+
+    got = ops.fused_rmsnorm_project_backward_q8(*(moved(t) for t in (go, xc, xs, W, proj, inv)))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # a block of a checkpoint that stands for NaN reaches exactly its columns
+    bad = xs.clone()
+    bad[17, 2, 1] = 255
+    gx, gW = ops.fused_rmsnorm_project_backward_q8(go, xc, bad, W, proj, inv)
+    nan = torch.zeros(T, 4, C, dtype=torch.bool, device="cuda")
+    nan[17, 2, 32:] = True
+    assert torch.equal(torch.isnan(gx), nan) and torch.equal(gx[~nan], want[0][~nan])
+    assert torch.equal(torch.isnan(gW).all(0), nan[17].reshape(-1)) and not torch.isnan(gW[:, ~nan[17].reshape(-1)]).any()
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_projection_backward_against_differences(fmt):
     """d/dt <g, project(x + t dx, W + t dW)> at t = 0, for x that a checkpoint holds exactly."""
