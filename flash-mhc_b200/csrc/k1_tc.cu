@@ -836,7 +836,7 @@ bool device_is_sm100() {
 const char *k1_tc_error() { return k1tc::g_msg; }
 
 static_assert(sizeof(k1tc::BwdSmem) + 1024 <= 232448, "K1 backward shared memory");
-static_assert(sizeof(k1tc::BwdQ8Smem) + 1024 <= 232448, "K1 backward shared memory (8-bit x)");
+static_assert(sizeof(k1tc::BwdQ8Smem) <= 232448, "K1 backward shared memory (8-bit x)");
 static_assert((sizeof(k1tc::FwdSmem) + 1024) * FMHC_K1F_CTAS_PER_SM <= 232448,
               "K1 forward shared memory");
 static_assert((sizeof(k1tc::SkSmem<k1tc::kSkStagesShallow>) + 1024) * FMHC_K1F_CTAS_PER_SM <= 232448,
@@ -1105,7 +1105,7 @@ int launch_k1_tc_bwd_q8(const void *go, const void *codes, const void *scales, i
     snprintf(g_msg, sizeof(g_msg), "cuTensorMapEncodeTiled failed");
     return 5;
   }
-  const size_t smem = sizeof(BwdQ8Smem) + 1024;
+  const size_t smem = sizeof(BwdQ8Smem);
   auto kern = fmt == act8::kInt8 ? k1_bwd_q8_tc_kernel<act8::kInt8> : k1_bwd_q8_tc_kernel<act8::kE4m3>;
   if (int e = set_smem_attr(reinterpret_cast<const void *>(kern), smem)) return e;
   BwdArgs args{};

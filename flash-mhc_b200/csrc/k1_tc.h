@@ -40,7 +40,7 @@ int launch_k1_tc_bwd(const void *go, const void *x, const void *W, const void *p
 
 // Backward (grad_x and grad_W) from an 8-bit checkpoint of x.  Needs a shape for
 // which k1_tc_bwd_q8_shape holds, go, codes, W, proj and gx 16-byte and scales
-// 4-byte aligned, and a workspace of k1_tc_bwd_workspace_bytes(T, nC).
+// 2-byte aligned, and a workspace of k1_tc_bwd_workspace_bytes(T, nC).
 bool k1_tc_bwd_q8_shape(int64_t T, int64_t nC);
 int launch_k1_tc_bwd_q8(const void *go, const void *codes, const void *scales, int fmt,
                         const void *W, const void *proj, const float *inv_rms, void *gx, void *gW,

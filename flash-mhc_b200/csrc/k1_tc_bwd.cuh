@@ -153,7 +153,9 @@ __device__ __forceinline__ float go_proj_chunk_dot(const uint4 g, const uint4 p)
 
 // Tile prep of one slot by one warp: gos = bf16(go * inv_rms) and (s, inv_rms)
 // per token, from the slot's go and proj.  Lane l takes the tile rows l, l + 32,
-// l + 64, l + 96, whose inv_rms are invr.
+// l + 64, l + 96, whose inv_rms are invr.  GOS may be proj's own place: a chunk
+// of gos is written after the chunk of proj there has been read.
+template <int GOS, int SINV>
 __device__ __forceinline__ void prep_tile(uint8_t *sb, int lane, const float (&invr)[4], float nC) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -172,10 +174,10 @@ __device__ __forceinline__ void prep_tile(uint8_t *sb, int lane, const float (&i
       o.y = pack_bf16x2(bf16lo(g.y) * rinv, bf16hi(g.y) * rinv);
       o.z = pack_bf16x2(bf16lo(g.z) * rinv, bf16hi(g.z) * rinv);
       o.w = pack_bf16x2(bf16lo(g.w) * rinv, bf16hi(g.w) * rinv);
-      *reinterpret_cast<uint4 *>(sb + kBwdSlotGos + off) = o;
+      *reinterpret_cast<uint4 *>(sb + GOS + off) = o;
     }
     const float dot = (pc[0] + pc[1]) + (pc[2] + pc[3]);
-    reinterpret_cast<float2 *>(sb + kBwdSlotSinv)[r] =
+    reinterpret_cast<float2 *>(sb + SINV)[r] =
         make_float2(dot * (rinv * rinv) / nC, rinv);
   }
 }
@@ -452,7 +454,7 @@ k1_bwd_tc_kernel(const __grid_constant__ CUtensorMap tmap_x,
         invr[i] = t < a.T ? __ldg(a.inv_rms + t) : 0.f;
       }
       if (!mbar_wait(smem_u32(&sm.gfull[slot]), sphase, abort, kSiteBPrepSlot)) break;
-      prep_tile(sm.slot[slot], lane, invr, float(a.nC));
+      prep_tile<kBwdSlotGos, kBwdSlotSinv>(sm.slot[slot], lane, invr, float(a.nC));
       // gos is read by the MMA (async proxy) and go/proj are refilled by the
       // TMA: order this thread's generic reads and writes before both.
       fence_proxy_async_smem();

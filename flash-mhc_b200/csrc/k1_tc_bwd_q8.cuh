@@ -4,48 +4,57 @@
 // reduction it shares (x there is the restored x8 here).
 //
 // The tensor cores want x as bf16 in the 128-byte-swizzled layout that the TMA
-// gives the bf16 kernel.  Both code formats are exact in bf16, so here the TMA
-// brings the codes (a quarter of the bytes that the bf16 kernel moves in and
-// out is saved), and four more warps widen them into that layout:
+// gives the bf16 kernel.  Both code formats are exact in bf16, so eight more
+// warps widen the codes into that layout:
 //
 //   warp 0       TMA producer: go and proj per token tile (slots), and per unit
-//                the codes [128 t x 128 k] and the W chunk into a raw stage.
-//   warps 12-15  converters, thread = token row: codes and scale bytes of the
-//                row -> bf16 x tile in an x stage.  The four scale bytes of a
-//                row's 128 columns are one word, loaded a unit ahead.
-//   warp 1       MMA issuer: as in the bf16 kernel, on the x stage, the raw
-//                stage's W chunk and the slot.
-//   warps 2-9    epilogue, warp 10 store, warp 11 tile prep: as in the bf16
-//                kernel; the epilogue takes its 64 columns in two halves, which
-//                keeps a thread within the 128 registers that 16 warps leave.
+//                the codes [128 t x 128 k] and the W chunk, each into a ring of
+//                its own.
+//   warps 12-19  converters, two warps per 32 token rows, thread = token row and
+//                64 columns: codes and scale bytes -> bf16 x tile in a stage.
+//                The four scale bytes of a row's 128 columns are one word,
+//                loaded a unit ahead.
+//   warp 1       MMA issuer, warps 2-9 epilogue, warp 10 store, warp 11 tile
+//                prep: as in the bf16 kernel; the epilogue takes its 64 columns
+//                in two halves, which keeps a thread within the 96 registers
+//                that 20 warps leave, and the prep writes gos over proj.
 //
-// A raw stage is free again when the converters have read the codes and the
-// MMAs have read W; an x stage when the TMA store has read the grad_x that the
-// epilogue wrote over x.  Every wait is bounded (sm100_ptx.cuh).
+// Codes are free again once converted, W once the MMAs of its unit are done, a
+// stage once the store has read the grad_x that the epilogue wrote over x.
+// Shared memory is filled to the last KiB: the stages in flight hide the latency
+// of a unit's chain (load, convert, MMA, epilogue, store).
+// Every wait is bounded (sm100_ptx.cuh).
 #pragma once
 
 #include "act8.cuh"
+#include "lane_ring.cuh"
 
 namespace fmhc {
 namespace k1tc {
 
-constexpr int kQ8Raw = 3;                             // raw stages: codes and W chunk
-constexpr int kQ8Stages = 3;                          // x stages
-constexpr int kQ8CodeBytes = kBwdBT * kBwdBK;         // 16 KiB
-constexpr int kQ8RawBytes = kQ8CodeBytes + kBwdWBytes;  // 24 KiB
+constexpr int kQ8Codes = 3;                   // code tiles in flight
+constexpr int kQ8W = 2;                       // W chunks in flight
+constexpr int kQ8Stages = 4;                  // x tiles
+constexpr int kQ8CodeBytes = kBwdBT * kBwdBK;  // 16 KiB
 constexpr int kQ8ConvWarp = kBwdPrepWarp + 1;
-constexpr int kQ8ConvWarps = 4;
-constexpr int kQ8Threads = 32 * (kQ8ConvWarp + kQ8ConvWarps);  // 512
+constexpr int kQ8ConvWarps = 8;
+constexpr int kQ8Threads = 32 * (kQ8ConvWarp + kQ8ConvWarps);  // 640
 static_assert(kBwdInflight < kQ8Stages, "stores in flight");
+// Slot layout: go at 0, proj and later gos at 8 KiB, (s, inv) at 16 KiB.
+constexpr int kQ8SlotGos = kBwdSlotProj, kQ8SlotSinv = 2 * kBwdGBytes;
+constexpr int kQ8SlotBytes = 2 * kBwdGBytes + kBwdSBytes;
 
 struct alignas(1024) BwdQ8Smem {
-  uint8_t raw[kQ8Raw][kQ8RawBytes];           // codes, then the W chunk
   uint8_t x[kQ8Stages][kBwdXBytes];           // x tile, later grad_x
-  uint8_t slot[kBwdSlots][kBwdSlotBytes];     // go, proj, gos, (s, inv) of one token tile
-  uint64_t rfull[kQ8Raw];                     // codes and W landed
-  uint64_t rempty[kQ8Raw];                    // converters + MMA commit
+  uint8_t codes[kQ8Codes][kQ8CodeBytes];
+  uint8_t w[kQ8W][kBwdWBytes];
+  uint8_t slot[kBwdSlots][kQ8SlotBytes];      // go, proj or gos, (s, inv) of one token tile
+  uint64_t cfull[kQ8Codes];                   // codes landed
+  uint64_t cempty[kQ8Codes];                  // converters have read them
+  uint64_t wfull[kQ8W];                       // W landed
+  uint64_t wempty[kQ8W];                      // the MMAs have read it
   uint64_t xfull[kQ8Stages];                  // converters wrote x
-  uint64_t xempty[kQ8Stages];                 // the store has read grad_x
+  uint64_t empty[kQ8Stages];                  // the store has read grad_x
   uint64_t epi[kQ8Stages];                    // the epilogue wrote grad_x
   uint64_t gfull[kBwdSlots];
   uint64_t gready[kBwdSlots];
@@ -58,20 +67,52 @@ struct alignas(1024) BwdQ8Smem {
   int abort;
 };
 
-enum : unsigned { kSiteQProdRaw = 0x301, kSiteQProdSlot = 0x302, kSiteQMmaRaw = 0x303,
+enum : unsigned { kSiteQProdCodes = 0x301, kSiteQProdSlot = 0x302, kSiteQMmaW = 0x303,
                   kSiteQMmaX = 0x304, kSiteQMmaTempty = 0x305, kSiteQMmaSlot = 0x306,
                   kSiteQEpiSlot = 0x307, kSiteQEpiX = 0x308, kSiteQEpiTfull = 0x309,
                   kSiteQEpiDw = 0x30a, kSiteQStore = 0x30b, kSiteQPrep = 0x30c,
-                  kSiteQConvRaw = 0x30d, kSiteQConvX = 0x30e, kSiteQDrain = 0x30f };
+                  kSiteQConvX = 0x30d, kSiteQConvCodes = 0x30e, kSiteQProdW = 0x30f,
+                  kSiteQDrain = 0x310 };
 
-// Eight codes (two words) with scale s -> eight bf16 values (exact).
+// mbar_wait by a whole warp with one outcome: a lane whose wait expires takes the
+// others with it, so that no lane is left at a warp barrier.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int *abort,
+                                               unsigned site) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, site));
+}
+
+// Scale byte -> the factor that widen4 takes: 2^(e - 127) as two bf16 or as f32.
 template <int FMT>
-__device__ __forceinline__ uint4 codes_to_bf16(uint32_t a, uint32_t b, float s) {
-  float f[4], g[4];
-  act8::decode4<FMT>(a, f);
-  act8::decode4<FMT>(b, g);
-  return make_uint4(pack_bf16x2(f[0] * s, f[1] * s), pack_bf16x2(f[2] * s, f[3] * s),
-                    pack_bf16x2(g[0] * s, g[1] * s), pack_bf16x2(g[2] * s, g[3] * s));
+__device__ __forceinline__ uint32_t widen_factor(uint32_t e) {
+  const uint32_t f = __float_as_uint(act8::scale_value(e));
+  return FMT == act8::kInt8 ? __byte_perm(f, 0, 0x3232) : f;
+}
+
+// Four codes -> four bf16 values (exact: at most 7 significant bits).
+template <int FMT>
+__device__ __forceinline__ uint2 widen4(uint32_t w, uint32_t factor) {
+  if constexpr (FMT == act8::kInt8) {
+    // 0x4300 | code is, as bf16, 128 + (code & 127) once bit 7 is cleared, and
+    // 128 or 256 (for a negative code) once bits 0-6 are: the difference is the
+    // code.  Two codes per instruction, exact in bf16.
+    uint32_t o[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t p = __byte_perm(w, 0x43434343u, i ? 0x7372 : 0x7170);
+      const uint32_t hi = p & 0xff7fff7fu, lo = p & 0xff80ff80u;
+      const __nv_bfloat162 v = __hmul2(__hsub2(reinterpret_cast<const __nv_bfloat162 &>(hi),
+                                               reinterpret_cast<const __nv_bfloat162 &>(lo)),
+                                       reinterpret_cast<const __nv_bfloat162 &>(factor));
+      o[i] = reinterpret_cast<const uint32_t &>(v);
+    }
+    return make_uint2(o[0], o[1]);
+  } else {
+    float f[4];
+    act8::decode4<FMT>(w, f);
+    const float2 s = both(__uint_as_float(factor));
+    const float2 a = mul2(make_float2(f[0], f[1]), s), b = mul2(make_float2(f[2], f[3]), s);
+    return make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(b.x, b.y));
+  }
 }
 
 template <int FMT>
@@ -82,9 +123,9 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
                     const __grid_constant__ CUtensorMap tmap_proj,
                     const __grid_constant__ CUtensorMap tmap_w,
                     const uint8_t *__restrict__ scales, const BwdArgs a) {
-  extern __shared__ uint8_t smem_raw[];
-  BwdQ8Smem &sm = *reinterpret_cast<BwdQ8Smem *>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // No static shared memory beside it, so it starts on a 1 KiB boundary.
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  BwdQ8Smem &sm = *reinterpret_cast<BwdQ8Smem *>(smem_raw);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   volatile int *abort = &sm.abort;
@@ -96,13 +137,17 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
   const int nunits = ntiles * G;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kQ8Raw; ++s) {
-      mbar_init(smem_u32(&sm.rfull[s]), 1);
-      mbar_init(smem_u32(&sm.rempty[s]), kQ8ConvWarps + 1);
+    for (int s = 0; s < kQ8Codes; ++s) {
+      mbar_init(smem_u32(&sm.cfull[s]), 1);
+      mbar_init(smem_u32(&sm.cempty[s]), kQ8ConvWarps);
+    }
+    for (int s = 0; s < kQ8W; ++s) {
+      mbar_init(smem_u32(&sm.wfull[s]), 1);
+      mbar_init(smem_u32(&sm.wempty[s]), 1);
     }
     for (int s = 0; s < kQ8Stages; ++s) {
       mbar_init(smem_u32(&sm.xfull[s]), kQ8ConvWarps);
-      mbar_init(smem_u32(&sm.xempty[s]), 1);
+      mbar_init(smem_u32(&sm.empty[s]), 1);
       mbar_init(smem_u32(&sm.epi[s]), kBwdEpiWarps);
     }
     for (int b = 0; b < kBwdSlots; ++b) {
@@ -138,8 +183,8 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
-      int stage = 0, slot = 0, issued = 0, slots_issued = 0;
-      uint32_t phase = 0, sphase = 0;
+      int cs = 0, ws = 0, slot = 0, issued = 0, w_issued = 0, slots_issued = 0;
+      uint32_t cphase = 0, wphase = 0, sphase = 0;
       for (int j = 0; j < nunits && !*abort; ++j) {
         const int m = j / G, jj = j - m * G;
         const int32_t row0 = (gi + m * ng) * kBwdBT;
@@ -154,24 +199,35 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
           ++slots_issued;
           if (++slot == kBwdSlots) { slot = 0; sphase ^= 1; }
         }
-        if (!mbar_wait(smem_u32(&sm.rempty[stage]), phase ^ 1, abort, kSiteQProdRaw)) break;
-        const uint32_t f = smem_u32(&sm.rfull[stage]);
-        const uint32_t base = smem_u32(sm.raw[stage]);
-        mbar_arrive_expect_tx(f, uint32_t(kQ8RawBytes));
+        if (!mbar_wait(smem_u32(&sm.cempty[cs]), cphase ^ 1, abort, kSiteQProdCodes)) break;
+        const uint32_t cf = smem_u32(&sm.cfull[cs]);
+        mbar_arrive_expect_tx(cf, uint32_t(kQ8CodeBytes));
         // The codes' map counts pairs of bytes: 64 of them are 128 columns.
-        tma_load_2d(base, &tmap_codes, f, kc * (kBwdBK / 2), row0);
-        tma_load_2d(base + kQ8CodeBytes, &tmap_w, f, kc * kBwdBK, 0);
-        tma_load_2d(base + kQ8CodeBytes + kBwdWBytes / 2, &tmap_w, f, kc * kBwdBK + 64, 0);
+        tma_load_2d(smem_u32(sm.codes[cs]), &tmap_codes, cf, kc * (kBwdBK / 2), row0);
         ++issued;
-        if (++stage == kQ8Raw) { stage = 0; phase ^= 1; }
+        if (++cs == kQ8Codes) { cs = 0; cphase ^= 1; }
+        if (!mbar_wait(smem_u32(&sm.wempty[ws]), wphase ^ 1, abort, kSiteQProdW)) break;
+        const uint32_t wf = smem_u32(&sm.wfull[ws]);
+        mbar_arrive_expect_tx(wf, uint32_t(kBwdWBytes));
+        tma_load_2d(smem_u32(sm.w[ws]), &tmap_w, wf, kc * kBwdBK, 0);
+        tma_load_2d(smem_u32(sm.w[ws]) + kBwdWBytes / 2, &tmap_w, wf, kc * kBwdBK + 64, 0);
+        ++w_issued;
+        if (++ws == kQ8W) { ws = 0; wphase ^= 1; }
       }
       // Drain: every copy issued must have landed before the CTA exits.
-      int n = issued < kQ8Raw ? issued : kQ8Raw;
-      int s = stage;
-      uint32_t ph = phase;
+      int n = issued < kQ8Codes ? issued : kQ8Codes;
+      int s = cs;
+      uint32_t ph = cphase;
       for (int i = 0; i < n; ++i) {
-        if (--s < 0) { s = kQ8Raw - 1; ph ^= 1; }
-        mbar_wait(smem_u32(&sm.rfull[s]), ph, abort, kSiteQDrain, true);
+        if (--s < 0) { s = kQ8Codes - 1; ph ^= 1; }
+        mbar_wait(smem_u32(&sm.cfull[s]), ph, abort, kSiteQDrain, true);
+      }
+      n = w_issued < kQ8W ? w_issued : kQ8W;
+      s = ws;
+      ph = wphase;
+      for (int i = 0; i < n; ++i) {
+        if (--s < 0) { s = kQ8W - 1; ph ^= 1; }
+        mbar_wait(smem_u32(&sm.wfull[s]), ph, abort, kSiteQDrain, true);
       }
       n = slots_issued < kBwdSlots ? slots_issued : kBwdSlots;
       s = slot;
@@ -186,25 +242,25 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
     if (lane == 0) {
       constexpr uint32_t idesc_dx = idesc_bf16_f32(kBwdBT, kBwdBK, 0, 1);
       constexpr uint32_t idesc_dw = idesc_bf16_f32(kBwdBK, kND, 1, 1);
-      int raw = 0, stage = 0, acc = 0, slot = 0;
-      uint32_t rphase = 0, phase = 0, acc_phase = 0, sphase = 0;
+      int stage = 0, ws = 0, acc = 0, slot = 0;
+      uint32_t phase = 0, wphase = 0, acc_phase = 0, sphase = 0;
       bool ok = true;
       for (int j = 0; j < nunits && !*abort; ++j) {
         const int m = j / G, jj = j - m * G;
         if (jj == 0 &&
             !mbar_wait(smem_u32(&sm.gready[slot]), sphase, abort, kSiteQMmaSlot)) { ok = false; break; }
         if (!mbar_wait(smem_u32(&sm.tempty[acc]), acc_phase ^ 1, abort, kSiteQMmaTempty)) { ok = false; break; }
-        if (!mbar_wait(smem_u32(&sm.rfull[raw]), rphase, abort, kSiteQMmaRaw)) { ok = false; break; }
+        if (!mbar_wait(smem_u32(&sm.wfull[ws]), wphase, abort, kSiteQMmaW)) { ok = false; break; }
         if (!mbar_wait(smem_u32(&sm.xfull[stage]), phase, abort, kSiteQMmaX)) { ok = false; break; }
         tc_fence_after();
         const uint32_t base = smem_u32(sm.x[stage]);
-        const uint32_t wb = smem_u32(sm.raw[raw]) + kQ8CodeBytes;
+        const uint32_t wb = smem_u32(sm.w[ws]);
         const uint32_t gs = smem_u32(sm.slot[slot]);
         // grad_W: M = k (two 64-wide MN blocks 16 KiB apart), N = d, K = tokens.
 #pragma unroll
         for (int k = 0; k < kBwdBT / 16; ++k) {
           const uint64_t ad = smem_desc(base + k * 2048, kBwdXBox, 1024, 2);
-          const uint64_t bd = smem_desc(gs + kBwdSlotGos + k * 1024, 512, 512, 4);
+          const uint64_t bd = smem_desc(gs + kQ8SlotGos + k * 1024, 512, 512, 4);
           mma_bf16_ss(tmem + kBwdDwCol + uint32_t(jj * kND), ad, bd, idesc_dw,
                       (m > 0 || k > 0) ? 1u : 0u);
         }
@@ -216,13 +272,13 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
           mma_bf16_ss(tmem + uint32_t(acc * kBwdBK), ad, bd, idesc_dx, k != 0);
         }
         mma_commit(smem_u32(&sm.tfull[acc]));
-        mma_commit(smem_u32(&sm.rempty[raw]));
+        mma_commit(smem_u32(&sm.wempty[ws]));
+        if (++ws == kQ8W) { ws = 0; wphase ^= 1; }
         if (jj == G - 1) {
           mma_commit(smem_u32(&sm.gempty[slot]));
           if (++slot == kBwdSlots) { slot = 0; sphase ^= 1; }
         }
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
-        if (++raw == kQ8Raw) { raw = 0; rphase ^= 1; }
         if (++stage == kQ8Stages) { stage = 0; phase ^= 1; }
       }
       if (ok && !*abort && nunits > 0) mma_commit(smem_u32(&sm.dwfull));
@@ -242,8 +298,8 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
       const int m = j / G, jj = j - m * G;
       if (jj == 0) {
         // (s, inv_rms) of this thread's token, kept in registers for the tile.
-        if (!mbar_wait(smem_u32(&sm.gready[slot]), sphase, abort, kSiteQEpiSlot)) { ok = false; break; }
-        const float2 si = reinterpret_cast<const float2 *>(sm.slot[slot] + kBwdSlotSinv)[r];
+        if (!mbar_wait_warp(smem_u32(&sm.gready[slot]), sphase, abort, kSiteQEpiSlot)) { ok = false; break; }
+        const float2 si = reinterpret_cast<const float2 *>(sm.slot[slot] + kQ8SlotSinv)[r];
         s = si.x;
         inv = si.y;
         // The slot's refill is a TMA (async-proxy) write: order this thread's
@@ -253,8 +309,8 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
         if (lane == 0) mbar_arrive(smem_u32(&sm.gempty[slot]));
         if (++slot == kBwdSlots) { slot = 0; sphase ^= 1; }
       }
-      if (!mbar_wait(smem_u32(&sm.xfull[stage]), phase, abort, kSiteQEpiX)) { ok = false; break; }
-      if (!mbar_wait(smem_u32(&sm.tfull[acc]), acc_phase, abort, kSiteQEpiTfull)) { ok = false; break; }
+      if (!mbar_wait_warp(smem_u32(&sm.xfull[stage]), phase, abort, kSiteQEpiX)) { ok = false; break; }
+      if (!mbar_wait_warp(smem_u32(&sm.tfull[acc]), acc_phase, abort, kSiteQEpiTfull)) { ok = false; break; }
       tc_fence_after();
       // Columns 64h .. 64h+63 of row r are one 128-byte row of x box h.
       uint8_t *rowp = sm.x[stage] + h * kBwdXBox + r * 128;
@@ -291,7 +347,7 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       if (++stage == kQ8Stages) { stage = 0; phase ^= 1; }
     }
-    if (ok && nunits > 0 && mbar_wait(smem_u32(&sm.dwfull), 0, abort, kSiteQEpiDw)) {
+    if (ok && nunits > 0 && mbar_wait_warp(smem_u32(&sm.dwfull), 0, abort, kSiteQEpiDw)) {
       // grad_W partials of the group's G k-chunks: thread r owns k row r of
       // each, 32 d columns; warps 2-5 take the even chunks, warps 6-9 the odd.
       tc_fence_after();
@@ -323,14 +379,14 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
         pend[npend++] = stage;
         tma_store_wait_read<kBwdInflight - 1>();
         while (npend > kBwdInflight - 1) {
-          mbar_arrive(smem_u32(&sm.xempty[pend[0]]));
+          mbar_arrive(smem_u32(&sm.empty[pend[0]]));
           for (int i = 1; i < npend; ++i) pend[i - 1] = pend[i];
           --npend;
         }
         if (++stage == kQ8Stages) { stage = 0; phase ^= 1; }
       }
       tma_store_wait_all<0>();
-      for (int i = 0; i < npend; ++i) mbar_arrive(smem_u32(&sm.xempty[pend[i]]));
+      for (int i = 0; i < npend; ++i) mbar_arrive(smem_u32(&sm.empty[pend[i]]));
     }
   } else if (warp == kBwdPrepWarp) {
     // ----------------------------------------------------------- tile prep
@@ -345,8 +401,8 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
         const int64_t t = t0 + lane + 32 * i;
         invr[i] = t < a.T ? __ldg(a.inv_rms + t) : 0.f;
       }
-      if (!mbar_wait(smem_u32(&sm.gfull[slot]), sphase, abort, kSiteQPrep)) break;
-      prep_tile(sm.slot[slot], lane, invr, float(a.nC));
+      if (!mbar_wait_warp(smem_u32(&sm.gfull[slot]), sphase, abort, kSiteQPrep)) break;
+      prep_tile<kQ8SlotGos, kQ8SlotSinv>(sm.slot[slot], lane, invr, float(a.nC));
       // gos is read by the MMA (async proxy) and go/proj are refilled by the
       // TMA: order this thread's generic reads and writes before both.
       fence_proxy_async_smem();
@@ -356,46 +412,52 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
     }
   } else {
     // ----------------------------------------------------------- converters
-    const int r = (warp - kQ8ConvWarp) * 32 + lane;  // token row of the unit
-    const int64_t words = a.nC / 128;                // scale words per token (4 bytes: 128 columns)
-    const auto scale_word = [&](int j) {
-      const int m = j / G, jj = j - m * G;
+    const int r = ((warp - kQ8ConvWarp) & 3) * 32 + lane;  // token row of the unit
+    const int h = (warp - kQ8ConvWarp) >> 2;               // x box: columns 64h .. 64h+63
+    // Scale bytes 2h and 2h + 1 of the row's 128 columns (even addresses: nC / 32
+    // is a multiple of 4, and the base is checked).
+    const auto scale_pair = [&](int j) {
+      const int m = j / G, kc = grp * G + (j - m * G);
       const int64_t t = int64_t(gi + m * ng) * kBwdBT + r;
       return j < nunits && t < a.T
-                 ? __ldg(reinterpret_cast<const uint32_t *>(scales) + t * words + grp * G + jj)
+                 ? uint32_t(__ldg(reinterpret_cast<const uint16_t *>(
+                       scales + t * (a.nC / act8::kBlock) + kc * (kBwdBK / act8::kBlock) + 2 * h)))
                  : 0u;
     };
-    int raw = 0, stage = 0;
-    uint32_t rphase = 0, phase = 0;
-    uint32_t next = scale_word(0);
+    int cs = 0, stage = 0;
+    uint32_t cphase = 0, phase = 0;
+    uint32_t next = scale_pair(0);
     for (int j = 0; j < nunits && !*abort; ++j) {
       const uint32_t sw = next;
-      next = scale_word(j + 1);
-      if (!mbar_wait(smem_u32(&sm.rfull[raw]), rphase, abort, kSiteQConvRaw)) break;
-      if (!mbar_wait(smem_u32(&sm.xempty[stage]), phase ^ 1, abort, kSiteQConvX)) break;
-      // Row r of the codes: 128 bytes, 16-byte chunk c at position c ^ (r & 7).
-      // Columns 16c .. 16c+15 go to chunks 2(c & 3) and 2(c & 3) + 1 of the
-      // 128-byte row r of x box c / 4, swizzled the same way.
-      const uint8_t *src = sm.raw[raw] + r * 128;
-      uint8_t *dst = sm.x[stage] + r * 128;
+      next = scale_pair(j + 1);
+      if (!mbar_wait_warp(smem_u32(&sm.cfull[cs]), cphase, abort, kSiteQConvCodes)) break;
+      // Row r of the codes: 128 bytes, 16-byte chunk c at position c ^ (r & 7);
+      // chunks 4h .. 4h+3 are this thread's.  Chunk 4h + i goes to chunks 2i and
+      // 2i + 1 of the 128-byte row r of x box h, swizzled the same way.
+      const uint8_t *src = sm.codes[cs] + r * 128;
+      uint4 v[4];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(src + ((c ^ (r & 7)) << 4));
-        const float s = act8::scale_value((sw >> (8 * (c >> 1))) & 0xffu);
-        uint8_t *row = dst + (c >> 2) * kBwdXBox;
-        const int i = 2 * (c & 3);
-        *reinterpret_cast<uint4 *>(row + ((i ^ (r & 7)) << 4)) = codes_to_bf16<FMT>(v.x, v.y, s);
-        *reinterpret_cast<uint4 *>(row + (((i + 1) ^ (r & 7)) << 4)) = codes_to_bf16<FMT>(v.z, v.w, s);
+      for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4 *>(src + (((4 * h + i) ^ (r & 7)) << 4));
+      const uint32_t f0 = widen_factor<FMT>(sw & 0xffu), f1 = widen_factor<FMT>(sw >> 8);
+      if (!mbar_wait_warp(smem_u32(&sm.empty[stage]), phase ^ 1, abort, kSiteQConvX)) break;
+      uint8_t *row = sm.x[stage] + h * kBwdXBox + r * 128;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t f = i < 2 ? f0 : f1;
+        const uint2 a0 = widen4<FMT>(v[i].x, f), a1 = widen4<FMT>(v[i].y, f);
+        const uint2 b0 = widen4<FMT>(v[i].z, f), b1 = widen4<FMT>(v[i].w, f);
+        *reinterpret_cast<uint4 *>(row + (((2 * i) ^ (r & 7)) << 4)) = make_uint4(a0.x, a0.y, a1.x, a1.y);
+        *reinterpret_cast<uint4 *>(row + (((2 * i + 1) ^ (r & 7)) << 4)) = make_uint4(b0.x, b0.y, b1.x, b1.y);
       }
-      // x is read by the MMA (async proxy) and the raw stage is refilled by the
-      // TMA: order this thread's writes and reads before both.
+      // x is read by the MMA (async proxy) and the codes' place is refilled by
+      // the TMA: order this thread's writes and reads before both.
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(smem_u32(&sm.xfull[stage]));
-        mbar_arrive(smem_u32(&sm.rempty[raw]));
+        mbar_arrive(smem_u32(&sm.cempty[cs]));
       }
-      if (++raw == kQ8Raw) { raw = 0; rphase ^= 1; }
+      if (++cs == kQ8Codes) { cs = 0; cphase ^= 1; }
       if (++stage == kQ8Stages) { stage = 0; phase ^= 1; }
     }
   }
