@@ -39,7 +39,10 @@ constexpr int kQ8CodeBytes = kBwdBT * kBwdBK;  // 16 KiB
 constexpr int kQ8ConvWarp = kBwdPrepWarp + 1;
 constexpr int kQ8ConvWarps = 8;
 constexpr int kQ8Threads = 32 * (kQ8ConvWarp + kQ8ConvWarps);  // 640
-static_assert(kBwdInflight < kQ8Stages, "stores in flight");
+#ifndef FMHC_K1Q_STORES_IN_FLIGHT
+#define FMHC_K1Q_STORES_IN_FLIGHT 1
+#endif
+constexpr int kQ8Inflight = FMHC_K1Q_STORES_IN_FLIGHT;  // grad_x stores whose stages are held
 // Slot layout: go at 0, proj and later gos at 8 KiB, (s, inv) at 16 KiB.
 constexpr int kQ8SlotGos = kBwdSlotProj, kQ8SlotSinv = 2 * kBwdGBytes;
 constexpr int kQ8SlotBytes = 2 * kBwdGBytes + kBwdSBytes;
@@ -185,34 +188,41 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
     if (lane == 0) {
       int cs = 0, ws = 0, slot = 0, issued = 0, w_issued = 0, slots_issued = 0;
       uint32_t cphase = 0, wphase = 0, sphase = 0;
-      for (int j = 0; j < nunits && !*abort; ++j) {
+      // Unit j's codes go out before unit j - 1's W chunk: waiting for the MMAs
+      // to release a W chunk must not hold back the codes.
+      for (int j = 0; j <= nunits && !*abort; ++j) {
         const int m = j / G, jj = j - m * G;
         const int32_t row0 = (gi + m * ng) * kBwdBT;
         const int kc = grp * G + jj;
-        if (jj == 0) {  // new token tile: go and proj into the next slot
-          if (!mbar_wait(smem_u32(&sm.gempty[slot]), sphase ^ 1, abort, kSiteQProdSlot)) break;
-          const uint32_t gf = smem_u32(&sm.gfull[slot]);
-          const uint32_t sb = smem_u32(sm.slot[slot]);
-          mbar_arrive_expect_tx(gf, uint32_t(2 * kBwdGBytes));
-          tma_load_2d(sb + kBwdSlotGo, &tmap_go, gf, 0, row0);
-          tma_load_2d(sb + kBwdSlotProj, &tmap_proj, gf, 0, row0);
-          ++slots_issued;
-          if (++slot == kBwdSlots) { slot = 0; sphase ^= 1; }
+        if (j < nunits) {
+          if (jj == 0) {  // new token tile: go and proj into the next slot
+            if (!mbar_wait(smem_u32(&sm.gempty[slot]), sphase ^ 1, abort, kSiteQProdSlot)) break;
+            const uint32_t gf = smem_u32(&sm.gfull[slot]);
+            const uint32_t sb = smem_u32(sm.slot[slot]);
+            mbar_arrive_expect_tx(gf, uint32_t(2 * kBwdGBytes));
+            tma_load_2d(sb + kBwdSlotGo, &tmap_go, gf, 0, row0);
+            tma_load_2d(sb + kBwdSlotProj, &tmap_proj, gf, 0, row0);
+            ++slots_issued;
+            if (++slot == kBwdSlots) { slot = 0; sphase ^= 1; }
+          }
+          if (!mbar_wait(smem_u32(&sm.cempty[cs]), cphase ^ 1, abort, kSiteQProdCodes)) break;
+          const uint32_t cf = smem_u32(&sm.cfull[cs]);
+          mbar_arrive_expect_tx(cf, uint32_t(kQ8CodeBytes));
+          // The codes' map counts pairs of bytes: 64 of them are 128 columns.
+          tma_load_2d(smem_u32(sm.codes[cs]), &tmap_codes, cf, kc * (kBwdBK / 2), row0);
+          ++issued;
+          if (++cs == kQ8Codes) { cs = 0; cphase ^= 1; }
         }
-        if (!mbar_wait(smem_u32(&sm.cempty[cs]), cphase ^ 1, abort, kSiteQProdCodes)) break;
-        const uint32_t cf = smem_u32(&sm.cfull[cs]);
-        mbar_arrive_expect_tx(cf, uint32_t(kQ8CodeBytes));
-        // The codes' map counts pairs of bytes: 64 of them are 128 columns.
-        tma_load_2d(smem_u32(sm.codes[cs]), &tmap_codes, cf, kc * (kBwdBK / 2), row0);
-        ++issued;
-        if (++cs == kQ8Codes) { cs = 0; cphase ^= 1; }
-        if (!mbar_wait(smem_u32(&sm.wempty[ws]), wphase ^ 1, abort, kSiteQProdW)) break;
-        const uint32_t wf = smem_u32(&sm.wfull[ws]);
-        mbar_arrive_expect_tx(wf, uint32_t(kBwdWBytes));
-        tma_load_2d(smem_u32(sm.w[ws]), &tmap_w, wf, kc * kBwdBK, 0);
-        tma_load_2d(smem_u32(sm.w[ws]) + kBwdWBytes / 2, &tmap_w, wf, kc * kBwdBK + 64, 0);
-        ++w_issued;
-        if (++ws == kQ8W) { ws = 0; wphase ^= 1; }
+        if (j > 0) {
+          const int kw = grp * G + (j - 1) % G;
+          if (!mbar_wait(smem_u32(&sm.wempty[ws]), wphase ^ 1, abort, kSiteQProdW)) break;
+          const uint32_t wf = smem_u32(&sm.wfull[ws]);
+          mbar_arrive_expect_tx(wf, uint32_t(kBwdWBytes));
+          tma_load_2d(smem_u32(sm.w[ws]), &tmap_w, wf, kw * kBwdBK, 0);
+          tma_load_2d(smem_u32(sm.w[ws]) + kBwdWBytes / 2, &tmap_w, wf, kw * kBwdBK + 64, 0);
+          ++w_issued;
+          if (++ws == kQ8W) { ws = 0; wphase ^= 1; }
+        }
       }
       // Drain: every copy issued must have landed before the CTA exits.
       int n = issued < kQ8Codes ? issued : kQ8Codes;
@@ -365,7 +375,7 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
     // --------------------------------------------------------------- store
     if (lane == 0) {
       int stage = 0, npend = 0;
-      int pend[kBwdInflight];
+      int pend[kQ8Inflight];
       uint32_t phase = 0;
       for (int j = 0; j < nunits && !*abort; ++j) {
         const int m = j / G, jj = j - m * G;
@@ -377,8 +387,8 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
         tma_store_2d(&tmap_gx, base + kBwdXBox, kc * kBwdBK + 64, row0);
         tma_store_commit();
         pend[npend++] = stage;
-        tma_store_wait_read<kBwdInflight - 1>();
-        while (npend > kBwdInflight - 1) {
+        tma_store_wait_read<kQ8Inflight - 1>();
+        while (npend > kQ8Inflight - 1) {
           mbar_arrive(smem_u32(&sm.empty[pend[0]]));
           for (int i = 1; i < npend; ++i) pend[i - 1] = pend[i];
           --npend;
