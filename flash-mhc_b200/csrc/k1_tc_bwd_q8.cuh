@@ -21,8 +21,17 @@
 //
 // Codes are free again once converted, W once the MMAs of its unit are done, a
 // stage once the store has read the grad_x that the epilogue wrote over x.
-// Shared memory is filled to the last KiB: the stages in flight hide the latency
-// of a unit's chain (load, convert, MMA, epilogue, store).
+//
+// What bounds it: shared memory.  A unit moves 48 KiB of HBM traffic but about
+// 220 KiB through shared memory (codes in and out, x in, to the MMAs and to the
+// epilogue, grad_x in and out), on top of the 64 KiB of HBM and 180 KiB of the
+// bf16 kernel.  T = 65536, C = 1024, int8, us (bf16 kernel: 181; floor of the
+// bytes: 126): four converter warps 216; eight 189; codes and W in rings of
+// their own 182; codes ahead of W and one store held 174; rings of 4 codes, 4 W,
+// 3 stages instead of 3, 2, 4: 166.  Not faster: codes loaded into registers
+// (241), converter and epilogue in one warp with x kept in registers (171), the
+// same with D1 a unit ahead and grad_x in tiles of its own (193), codes of two
+// chunks at a time (175), a slot loaded half a tile ahead (172).
 // Every wait is bounded (sm100_ptx.cuh).
 #pragma once
 
@@ -32,17 +41,13 @@
 namespace fmhc {
 namespace k1tc {
 
-constexpr int kQ8Codes = 3;                   // code tiles in flight
-constexpr int kQ8W = 2;                       // W chunks in flight
-constexpr int kQ8Stages = 4;                  // x tiles
+constexpr int kQ8Codes = 4;                   // code tiles in flight
+constexpr int kQ8W = 4;                       // W chunks in flight
+constexpr int kQ8Stages = 3;                  // x tiles
 constexpr int kQ8CodeBytes = kBwdBT * kBwdBK;  // 16 KiB
 constexpr int kQ8ConvWarp = kBwdPrepWarp + 1;
 constexpr int kQ8ConvWarps = 8;
 constexpr int kQ8Threads = 32 * (kQ8ConvWarp + kQ8ConvWarps);  // 640
-#ifndef FMHC_K1Q_STORES_IN_FLIGHT
-#define FMHC_K1Q_STORES_IN_FLIGHT 1
-#endif
-constexpr int kQ8Inflight = FMHC_K1Q_STORES_IN_FLIGHT;  // grad_x stores whose stages are held
 // Slot layout: go at 0, proj and later gos at 8 KiB, (s, inv) at 16 KiB.
 constexpr int kQ8SlotGos = kBwdSlotProj, kQ8SlotSinv = 2 * kBwdGBytes;
 constexpr int kQ8SlotBytes = 2 * kBwdGBytes + kBwdSBytes;
@@ -374,8 +379,7 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
   } else if (warp == kBwdStoreWarp) {
     // --------------------------------------------------------------- store
     if (lane == 0) {
-      int stage = 0, npend = 0;
-      int pend[kQ8Inflight];
+      int stage = 0;
       uint32_t phase = 0;
       for (int j = 0; j < nunits && !*abort; ++j) {
         const int m = j / G, jj = j - m * G;
@@ -386,17 +390,13 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
         tma_store_2d(&tmap_gx, base, kc * kBwdBK, row0);
         tma_store_2d(&tmap_gx, base + kBwdXBox, kc * kBwdBK + 64, row0);
         tma_store_commit();
-        pend[npend++] = stage;
-        tma_store_wait_read<kQ8Inflight - 1>();
-        while (npend > kQ8Inflight - 1) {
-          mbar_arrive(smem_u32(&sm.empty[pend[0]]));
-          for (int i = 1; i < npend; ++i) pend[i - 1] = pend[i];
-          --npend;
-        }
+        // Free the stage as soon as this store has read it (holding it until
+        // the next store is issued, as the bf16 kernel does: 176 against 174 us).
+        tma_store_wait_read<0>();
+        mbar_arrive(smem_u32(&sm.empty[stage]));
         if (++stage == kQ8Stages) { stage = 0; phase ^= 1; }
       }
       tma_store_wait_all<0>();
-      for (int i = 0; i < npend; ++i) mbar_arrive(smem_u32(&sm.empty[pend[i]]));
     }
   } else if (warp == kBwdPrepWarp) {
     // ----------------------------------------------------------- tile prep
