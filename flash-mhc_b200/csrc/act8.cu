@@ -61,7 +61,7 @@ dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__
   pdl_wait();
   const int64_t step = int64_t(gridDim.x) * kThreads * kUnroll;
   for (int64_t i0 = int64_t(blockIdx.x) * kThreads * kUnroll; i0 < chunks; i0 += step) {
-    Codes<8> raw[kUnroll];
+    uint2 raw[kUnroll];
     uint32_t e[kUnroll];
     int64_t at[kUnroll];
     bool in[kUnroll];
@@ -77,7 +77,7 @@ dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__
         at[u] = row * C + c;
       }
       if (in[u]) {
-        raw[u] = ld_codes<8>(codes + at[u]);
+        raw[u] = ld_codes8(codes + at[u]);
         e[u] = __ldg(scales + (i >> 2));
       }
     }
@@ -85,7 +85,7 @@ dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__
     for (int u = 0; u < kUnroll; ++u) {
       if (in[u]) {
         float f[8];
-        restore<FMT, 8>(raw[u], scale_value(e[u]), f);
+        restore<FMT>(raw[u], scale_value(e[u]), f);
 #pragma unroll
         for (int k = 0; k < 8; ++k) f[k] = Elem<E>::fit(f[k]);
         st8(x + at[u], f);

@@ -111,32 +111,19 @@ __device__ __forceinline__ float decode1(uint8_t c) {
   return f[0];
 }
 
-// VEC codes (8 or 1) loaded as one access and widened to scaled f32 values.
-template <int VEC> struct Codes;
-template <> struct Codes<8> { uint2 v; };
-template <> struct Codes<1> { uint8_t v; };
-
-template <int VEC>
-__device__ __forceinline__ Codes<VEC> ld_codes(const uint8_t *p) {
-  Codes<VEC> c;
-  if constexpr (VEC == 8) c.v = __ldcs(reinterpret_cast<const uint2 *>(p));
-  else c.v = __ldcs(p);
-  return c;
+// Eight codes loaded as one access, and widened to scaled f32 values.
+__device__ __forceinline__ uint2 ld_codes8(const uint8_t *p) {
+  return __ldcs(reinterpret_cast<const uint2 *>(p));
 }
-
-template <int FMT, int VEC>
-__device__ __forceinline__ void restore(const Codes<VEC> &c, float s, float (&f)[VEC]) {
-  if constexpr (VEC == 8) {
-    float a[4], b[4];
-    decode4<FMT>(c.v.x, a);
-    decode4<FMT>(c.v.y, b);
+template <int FMT>
+__device__ __forceinline__ void restore(uint2 c, float s, float (&f)[8]) {
+  float a[4], b[4];
+  decode4<FMT>(c.x, a);
+  decode4<FMT>(c.y, b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[i] = a[i] * s;
-      f[i + 4] = b[i] * s;
-    }
-  } else {
-    f[0] = decode1<FMT>(c.v) * s;
+  for (int i = 0; i < 4; ++i) {
+    f[i] = a[i] * s;
+    f[i + 4] = b[i] * s;
   }
 }
 

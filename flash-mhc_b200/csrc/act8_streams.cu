@@ -5,9 +5,16 @@
 // Work mapping as in k3k4_stream.cu: one warp per token, lanes walk C in chunks
 // of eight values.  Four neighbouring lanes hold one block of 32 values, so a
 // block's maximum takes two shuffles, and lane 4k writes or reads its scale.
+//
+// The backwards read less per lane and iteration than the bf16 kernels (codes
+// are half as wide) and need the registers for their sums, so loads into
+// registers leave too few bytes in flight: a first version, shaped like the bf16
+// kernels, reached 0.56-0.66 of the copy rate.  They prefetch through a
+// shared-memory ring instead (lane_ring.cuh), one block per SM.
 #include "act8.cuh"
 #include "fmhc_launch.h"
 #include "grid.cuh"
+#include "lane_ring.cuh"
 
 namespace fmhc {
 
@@ -119,46 +126,115 @@ k4_fwd_q8_kernel(const bf16 *__restrict__ x, const bf16 *__restrict__ lo,
   }
 }
 
-// VEC bf16 values -> f32 (VEC 8 or 1).
-template <int VEC>
-__device__ __forceinline__ void load_f32(const bf16 *p, float (&f)[VEC]) {
-  if constexpr (VEC == 8) Elem<bf16>::widen(ld8(p), f);
-  else f[0] = Elem<bf16>::widen1(*p);
+// --------------------------------------------------------- backward rings
+// Position of a warp's pipeline: token t, and this lane's chunk of eight values.
+struct Cursor {
+  int64_t t;
+  int c;
+};
+__device__ __forceinline__ void advance(Cursor &p, int lane, int nchunk, int64_t nwarps) {
+  p.c += 32;
+  if (p.c - lane >= nchunk) {
+    p.c = lane;
+    p.t += nwarps;
+  }
+}
+
+// Four codes in a word -> two pairs of unscaled values.
+template <int FMT>
+__device__ __forceinline__ void decode4x2(uint32_t w, float2 &a, float2 &b) {
+  float f[4];
+  decode4<FMT>(w, f);
+  a = make_float2(f[0], f[1]);
+  b = make_float2(f[2], f[3]);
+}
+// Eight codes, scaled.
+template <int FMT>
+__device__ __forceinline__ void restore8(uint2 q, uint32_t e, float2 (&f)[4]) {
+  decode4x2<FMT>(q.x, f[0], f[1]);
+  decode4x2<FMT>(q.y, f[2], f[3]);
+  const float2 s = both(scale_value(e));
+#pragma unroll
+  for (int k = 0; k < 4; ++k) f[k] = mul2(f[k], s);
+}
+__device__ __forceinline__ void widen8(uint4 r, float2 (&f)[4]) {
+  f[0] = make_float2(bf16lo(r.x), bf16hi(r.x));
+  f[1] = make_float2(bf16lo(r.y), bf16hi(r.y));
+  f[2] = make_float2(bf16lo(r.z), bf16hi(r.z));
+  f[3] = make_float2(bf16lo(r.w), bf16hi(r.w));
 }
 
 // --------------------------------------------------------------- K3 backward
 //   grad_h[t,j] = sum_c x8[t,j,c] go[t,c]
-template <int FMT, int VEC>
-__global__ void __launch_bounds__(kThreads)
+constexpr int kK3Warps = 32, kK3Stages = 4;
+struct K3Stage {  // of one warp
+  uint4 go[32];
+  uint2 x[4][32];
+};
+template <int FMT>
+__global__ void __launch_bounds__(32 * kK3Warps, 1)
 k3_bwd_q8_kernel(const bf16 *__restrict__ go, const uint8_t *__restrict__ codes,
                  const uint8_t *__restrict__ scales, float *__restrict__ gh, int64_t T, int C) {
+  extern __shared__ uint4 dyn[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t nwarps = int64_t(gridDim.x) * (blockDim.x >> 5);
+  const int nchunk = C / 8, nb = (C + kBlock - 1) / kBlock;
+  K3Stage *ring = reinterpret_cast<K3Stage *>(dyn) + warp * kK3Stages;
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
-  const int64_t nwarps = (int64_t(gridDim.x) * kThreads) >> 5;
-  const int nchunk = C / VEC, nb = (C + kBlock - 1) / kBlock;
-  for (int64_t t = warp; t < T; t += nwarps) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c = lane; c < nchunk; c += 32) {
-      Codes<VEC> q[4];
-      uint32_t e[4];
-      float g[VEC];
+  const auto fetch = [&](const Cursor &p, int stage) {
+    if (p.t < T && p.c < nchunk) {
+      copy_async<16>(&ring[stage].go[lane], go + p.t * C + p.c * 8);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) copy_async<8>(&ring[stage].x[j][lane], codes + (p.t * 4 + j) * C + p.c * 8);
+    }
+    copy_commit();
+  };
+  uint32_t e[4] = {0, 0, 0, 0};
+  const auto fetch_scales = [&](const Cursor &p) {
+    if (p.t < T && p.c < nchunk) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) e[j] = __ldg(scales + (p.t * 4 + j) * nb + (p.c >> 2));
+    }
+  };
+  Cursor now{int64_t(warp) * gridDim.x + blockIdx.x, lane}, ahead = now;
+#pragma unroll
+  for (int s = 0; s < kK3Stages - 1; ++s) {
+    fetch(ahead, s);
+    advance(ahead, lane, nchunk, nwarps);
+  }
+  fetch_scales(now);
+  int stage = 0;
+  float2 acc[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
+  while (now.t < T) {
+    fetch(ahead, stage == 0 ? kK3Stages - 1 : stage - 1);
+    advance(ahead, lane, nchunk, nwarps);
+    const uint32_t e0[4] = {e[0], e[1], e[2], e[3]};
+    Cursor next = now;
+    advance(next, lane, nchunk, nwarps);
+    fetch_scales(next);
+    copy_wait<kK3Stages - 1>();
+    if (now.c < nchunk) {
+      float2 g[4], f[4];
+      widen8(ring[stage].go[lane], g);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        q[j] = ld_codes<VEC>(codes + (t * 4 + j) * C + c * VEC);
-        e[j] = __ldg(scales + (t * 4 + j) * nb + c * VEC / kBlock);
-      }
-      load_f32<VEC>(go + t * C + c * VEC, g);
+        restore8<FMT>(ring[stage].x[j][lane], e0[j], f);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float f[VEC];
-        restore<FMT, VEC>(q[j], scale_value(e[j]), f);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[j] = fmaf(f[k], g[k], acc[j]);
+        for (int k = 0; k < 4; ++k) acc[j] = fma2(f[k], g[k], acc[j]);
       }
     }
-    warp_reduce_scatter<4>(acc, lane);
-    if ((lane & 7) == 0) __stcs(gh + t * 4 + scatter_index<4>(lane), acc[0]);
+    if (next.t != now.t) {  // the token's last chunks
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] = acc[j].x + acc[j].y;
+        acc[j] = both(0.f);
+      }
+      warp_reduce_scatter<4>(v, lane);
+      if ((lane & 7) == 0) __stcs(gh + now.t * 4 + scatter_index<4>(lane), v[0]);
+    }
+    now = next;
+    if (++stage == kK3Stages) stage = 0;
   }
 }
 
@@ -166,67 +242,194 @@ k3_bwd_q8_kernel(const bf16 *__restrict__ go, const uint8_t *__restrict__ codes,
 //   grad_lo[t,c]  = bf16( sum_i h_post[t,i] go[t,i,c] )
 //   grad_hp[t,i]  = sum_c go[t,i,c] lo8[t,c]
 //   grad_H[t,i,j] = sum_c go[t,i,c] x8[t,j,c]
-template <int FMT, int VEC>
-__global__ void __launch_bounds__(kThreads)
+constexpr int kK4Warps = 16, kK4Stages = 4;
+struct K4Stage {  // of one warp
+  uint4 go[4][32];
+  uint2 x[5][32];  // the four streams and lo
+};
+template <int FMT>
+__global__ void __launch_bounds__(32 * kK4Warps, 1)
 k4_bwd_q8_kernel(const bf16 *__restrict__ go, const uint8_t *__restrict__ xc,
                  const uint8_t *__restrict__ xs, const uint8_t *__restrict__ lc,
                  const uint8_t *__restrict__ ls, const float4 *__restrict__ hpost,
                  bf16 *__restrict__ glo, float *__restrict__ gH, float *__restrict__ ghp,
                  int64_t T, int C) {
+  extern __shared__ uint4 dyn[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t nwarps = int64_t(gridDim.x) * (blockDim.x >> 5);
+  const int nchunk = C / 8, nb = (C + kBlock - 1) / kBlock;
+  K4Stage *ring = reinterpret_cast<K4Stage *>(dyn) + warp * kK4Stages;
+  pdl_wait();
+  const auto fetch = [&](const Cursor &p, int stage) {
+    if (p.t < T && p.c < nchunk) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) copy_async<16>(&ring[stage].go[i][lane], go + (p.t * 4 + i) * C + p.c * 8);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) copy_async<8>(&ring[stage].x[j][lane], xc + (p.t * 4 + j) * C + p.c * 8);
+      copy_async<8>(&ring[stage].x[4][lane], lc + p.t * C + p.c * 8);
+    }
+    copy_commit();
+  };
+  uint32_t e[5] = {0, 0, 0, 0, 0};
+  float4 hp = make_float4(0.f, 0.f, 0.f, 0.f);
+  const auto fetch_scales = [&](const Cursor &p) {
+    if (p.t < T) {
+      hp = __ldg(hpost + p.t);
+      if (p.c < nchunk) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = __ldg(xs + (p.t * 4 + j) * nb + (p.c >> 2));
+        e[4] = __ldg(ls + p.t * nb + (p.c >> 2));
+      }
+    }
+  };
+  Cursor now{int64_t(warp) * gridDim.x + blockIdx.x, lane}, ahead = now;
+#pragma unroll
+  for (int s = 0; s < kK4Stages - 1; ++s) {
+    fetch(ahead, s);
+    advance(ahead, lane, nchunk, nwarps);
+  }
+  fetch_scales(now);
+  int stage = 0;
+  float2 accH[4][4], accP[4];  // of even and odd columns
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    accP[i] = both(0.f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) accH[i][j] = both(0.f);
+  }
+  while (now.t < T) {
+    fetch(ahead, stage == 0 ? kK4Stages - 1 : stage - 1);
+    advance(ahead, lane, nchunk, nwarps);
+    const uint32_t e0[5] = {e[0], e[1], e[2], e[3], e[4]};
+    const float4 h = hp;
+    Cursor next = now;
+    advance(next, lane, nchunk, nwarps);
+    fetch_scales(next);
+    copy_wait<kK4Stages - 1>();
+    if (now.c < nchunk) {
+      float2 g[4][4], f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) widen8(ring[stage].go[i][lane], g[i]);
+      restore8<FMT>(ring[stage].x[4][lane], e0[4], f);
+      float o[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float2 s = mul2(both(h.x), g[0][k]);  // in the order of fmhc_k4_bwd
+        s = fma2(both(h.y), g[1][k], s);
+        s = fma2(both(h.z), g[2][k], s);
+        s = fma2(both(h.w), g[3][k], s);
+        o[2 * k] = s.x;
+        o[2 * k + 1] = s.y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) accP[i] = fma2(g[i][k], f[k], accP[i]);
+      }
+      st8(glo + now.t * C + now.c * 8, o);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        restore8<FMT>(ring[stage].x[j][lane], e0[j], f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) accH[i][j] = fma2(g[i][k], f[k], accH[i][j]);
+      }
+    }
+    if (next.t != now.t) {  // the token's last chunks
+      float v[16], w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = accP[i].x + accP[i].y;
+        accP[i] = both(0.f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[i * 4 + j] = accH[i][j].x + accH[i][j].y;
+          accH[i][j] = both(0.f);
+        }
+      }
+      warp_reduce_scatter<16>(v, lane);
+      warp_reduce_scatter<4>(w, lane);
+      if ((lane & 1) == 0) __stcs(gH + now.t * 16 + scatter_index<16>(lane), v[0]);
+      if ((lane & 7) == 0) __stcs(ghp + now.t * 4 + scatter_index<4>(lane), w[0]);
+    }
+    now = next;
+    if (++stage == kK4Stages) stage = 0;
+  }
+}
+
+// ---------------------------------------------- any width and any alignment
+// One warp per token, one value per lane at a time.
+template <int FMT>
+__global__ void __launch_bounds__(kThreads)
+k3_bwd_q8_any_kernel(const bf16 *__restrict__ go, const uint8_t *__restrict__ codes,
+                     const uint8_t *__restrict__ scales, float *__restrict__ gh, int64_t T, int C) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
   const int64_t nwarps = (int64_t(gridDim.x) * kThreads) >> 5;
-  const int nchunk = C / VEC, nb = (C + kBlock - 1) / kBlock;
+  const int nb = (C + kBlock - 1) / kBlock;
   for (int64_t t = warp; t < T; t += nwarps) {
-    const float4 hp4 = __ldg(hpost + t);
-    const float hp[4] = {hp4.x, hp4.y, hp4.z, hp4.w};
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = lane; c < C; c += 32) {
+      const float g = Elem<bf16>::widen1(go[t * C + c]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        acc[j] = fmaf(decode1<FMT>(codes[(t * 4 + j) * C + c]) * scale_value(scales[(t * 4 + j) * nb + c / kBlock]),
+                      g, acc[j]);
+    }
+    warp_reduce_scatter<4>(acc, lane);
+    if ((lane & 7) == 0) gh[t * 4 + scatter_index<4>(lane)] = acc[0];
+  }
+}
+
+template <int FMT>
+__global__ void __launch_bounds__(kThreads)
+k4_bwd_q8_any_kernel(const bf16 *__restrict__ go, const uint8_t *__restrict__ xc,
+                     const uint8_t *__restrict__ xs, const uint8_t *__restrict__ lc,
+                     const uint8_t *__restrict__ ls, const float4 *__restrict__ hpost,
+                     bf16 *__restrict__ glo, float *__restrict__ gH, float *__restrict__ ghp,
+                     int64_t T, int C) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
+  const int64_t nwarps = (int64_t(gridDim.x) * kThreads) >> 5;
+  const int nb = (C + kBlock - 1) / kBlock;
+  for (int64_t t = warp; t < T; t += nwarps) {
+    const float4 h = __ldg(hpost + t);
     float accH[16], accP[4];
 #pragma unroll
     for (int k = 0; k < 16; ++k) accH[k] = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) accP[k] = 0.f;
-    for (int c = lane; c < nchunk; c += 32) {
-      Codes<VEC> q[5];
-      uint32_t e[5];
-      float g[4][VEC];
+    for (int c = lane; c < C; c += 32) {
+      float g[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) g[i] = Elem<bf16>::widen1(go[(t * 4 + i) * C + c]);
+      const float l = decode1<FMT>(lc[t * C + c]) * scale_value(ls[t * nb + c / kBlock]);
+      glo[t * C + c] = __float2bfloat16_rn(fmaf(h.w, g[3], fmaf(h.z, g[2], fmaf(h.y, g[1], h.x * g[0]))));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) accP[i] = fmaf(g[i], l, accP[i]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        q[j] = ld_codes<VEC>(xc + (t * 4 + j) * C + c * VEC);
-        e[j] = __ldg(xs + (t * 4 + j) * nb + c * VEC / kBlock);
-      }
-      q[4] = ld_codes<VEC>(lc + t * C + c * VEC);
-      e[4] = __ldg(ls + t * nb + c * VEC / kBlock);
+        const float x = decode1<FMT>(xc[(t * 4 + j) * C + c]) * scale_value(xs[(t * 4 + j) * nb + c / kBlock]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) load_f32<VEC>(go + (t * 4 + i) * C + c * VEC, g[i]);
-      float f[VEC], o[VEC];
-      restore<FMT, VEC>(q[4], scale_value(e[4]), f);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        float s = hp[0] * g[0][k];
-        s = fmaf(hp[1], g[1][k], s);
-        s = fmaf(hp[2], g[2][k], s);
-        o[k] = fmaf(hp[3], g[3][k], s);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) accP[i] = fmaf(g[i][k], f[k], accP[i]);
-      }
-      if constexpr (VEC == 8) st8(glo + t * C + c * 8, o);
-      else glo[t * C + c] = __float2bfloat16_rn(o[0]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        restore<FMT, VEC>(q[j], scale_value(e[j]), f);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) accH[i * 4 + j] = fmaf(g[i][k], f[k], accH[i * 4 + j]);
-        }
+        for (int i = 0; i < 4; ++i) accH[i * 4 + j] = fmaf(g[i], x, accH[i * 4 + j]);
       }
     }
     warp_reduce_scatter<16>(accH, lane);
     warp_reduce_scatter<4>(accP, lane);
-    if ((lane & 1) == 0) __stcs(gH + t * 16 + scatter_index<16>(lane), accH[0]);
-    if ((lane & 7) == 0) __stcs(ghp + t * 4 + scatter_index<4>(lane), accP[0]);
+    if ((lane & 1) == 0) gH[t * 16 + scatter_index<16>(lane)] = accH[0];
+    if ((lane & 7) == 0) ghp[t * 4 + scatter_index<4>(lane)] = accP[0];
   }
+}
+
+// Warps per block of the ring kernels: few tokens spread over the SMs, many
+// fill them.
+int ring_warps(int64_t T, int most) {
+  const int64_t per_sm = (T + sm_count() - 1) / sm_count();
+  return int(per_sm < most ? (per_sm < 1 ? 1 : per_sm) : most);
+}
+int ring_blocks(int64_t T, int warps) {
+  const int64_t need = (T + warps - 1) / warps;
+  return int(need < sm_count() ? need : sm_count());
 }
 
 }  // namespace
@@ -256,9 +459,18 @@ void launch_k4_fwd_q8(const void *x, const void *lo, const float *H, const float
 void launch_k3_bwd_q8(const void *go, const void *codes, const void *scales, int fmt, float *gh,
                       int64_t T, int C, int vec, cudaStream_t s) {
   FMHC_DISPATCH_FMT(fmt, {
-    auto k = vec == 8 ? k3_bwd_q8_kernel<FMT, 8> : k3_bwd_q8_kernel<FMT, 1>;
-    launch(k, dim3(grid_for(k, T, kThreads)), dim3(kThreads), 0, s, (const bf16 *)go,
-           (const uint8_t *)codes, (const uint8_t *)scales, gh, T, C);
+    if (vec == 8) {
+      const int warps = ring_warps(T, kK3Warps);
+      const size_t smem = sizeof(K3Stage) * kK3Stages * warps;
+      auto k = k3_bwd_q8_kernel<FMT>;
+      allow_smem(reinterpret_cast<const void *>(k), smem);
+      launch(k, dim3(ring_blocks(T, warps)), dim3(32 * warps), smem, s, (const bf16 *)go,
+             (const uint8_t *)codes, (const uint8_t *)scales, gh, T, C);
+    } else {
+      auto k = k3_bwd_q8_any_kernel<FMT>;
+      launch(k, dim3(grid_for(k, T, kThreads)), dim3(kThreads), 0, s, (const bf16 *)go,
+             (const uint8_t *)codes, (const uint8_t *)scales, gh, T, C);
+    }
   });
 }
 
@@ -266,10 +478,20 @@ void launch_k4_bwd_q8(const void *go, const void *xc, const void *xs, const void
                       const void *ls, int fmt, const float *hp, void *glo, float *gH, float *ghp,
                       int64_t T, int C, int vec, cudaStream_t s) {
   FMHC_DISPATCH_FMT(fmt, {
-    auto k = vec == 8 ? k4_bwd_q8_kernel<FMT, 8> : k4_bwd_q8_kernel<FMT, 1>;
-    launch(k, dim3(grid_for(k, T, kThreads)), dim3(kThreads), 0, s, (const bf16 *)go,
-           (const uint8_t *)xc, (const uint8_t *)xs, (const uint8_t *)lc, (const uint8_t *)ls,
-           (const float4 *)hp, (bf16 *)glo, gH, ghp, T, C);
+    if (vec == 8) {
+      const int warps = ring_warps(T, kK4Warps);
+      const size_t smem = sizeof(K4Stage) * kK4Stages * warps;
+      auto k = k4_bwd_q8_kernel<FMT>;
+      allow_smem(reinterpret_cast<const void *>(k), smem);
+      launch(k, dim3(ring_blocks(T, warps)), dim3(32 * warps), smem, s, (const bf16 *)go,
+             (const uint8_t *)xc, (const uint8_t *)xs, (const uint8_t *)lc, (const uint8_t *)ls,
+             (const float4 *)hp, (bf16 *)glo, gH, ghp, T, C);
+    } else {
+      auto k = k4_bwd_q8_any_kernel<FMT>;
+      launch(k, dim3(grid_for(k, T, kThreads)), dim3(kThreads), 0, s, (const bf16 *)go,
+             (const uint8_t *)xc, (const uint8_t *)xs, (const uint8_t *)lc, (const uint8_t *)ls,
+             (const float4 *)hp, (bf16 *)glo, gH, ghp, T, C);
+    }
   });
 }
 

@@ -1,4 +1,4 @@
-// Grid size of the persistent streaming kernels.
+// Grid and shared-memory set-up of the persistent streaming kernels.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -41,6 +41,39 @@ int grid_for(K kernel, int64_t T, int threads) {
   const int64_t need = (T + warps_per_block - 1) / warps_per_block;
   const int64_t cap = int64_t(sms) * per_sm;
   return int(need < cap ? need : cap);
+}
+
+inline int sm_count() {
+  int dev = 0, sms = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms > 0 ? sms : 1;
+}
+
+constexpr size_t kMaxSmem = 232448 - 1024;  // dynamic shared memory beside a little static
+
+// Dynamic shared memory beyond the default needs an attribute of the kernel, set
+// once per device to the most it will ask for (and again only where this
+// table's 128 places do not suffice).
+inline void allow_smem(const void *kernel, size_t bytes) {
+  struct Entry {
+    const void *k;
+    int dev;
+    size_t bytes;
+  };
+  static std::mutex mu;
+  static Entry set[128];
+  static int used = 0;
+  if (bytes <= 40 * 1024) return;  // beside the static arrays, below the default 48 KiB
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(mu);
+  int at = 0;
+  while (at < used && !(set[at].k == kernel && set[at].dev == dev)) ++at;
+  if (at < used && set[at].bytes >= bytes) return;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) != cudaSuccess) return;
+  if (at == used && used < 128) ++used;
+  if (at < used) set[at] = Entry{kernel, dev, bytes};
 }
 
 }  // namespace fmhc

@@ -28,7 +28,6 @@
 #include "lane_ring.cuh"
 
 #include <algorithm>
-#include <mutex>
 
 namespace fmhc {
 
@@ -46,7 +45,6 @@ constexpr int kBwdWarps = 16;
 constexpr int kThreads = 256;         // of the kernels for any width
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxParts = 1024;
-constexpr size_t kMaxSmem = 232448 - 1024;  // dynamic, beside the static slots
 
 // w or b at column c, in the parameters' own type (fmhc_dtype); `def` if absent.
 __device__ __forceinline__ float param1(const void *p, int dtype, int64_t c, float def) {
@@ -632,12 +630,6 @@ struct Shape {
   int team, nv, teams, threads;
   int64_t sums() const { return int64_t(team) * nv * 16 * 32; }  // of a block's partial
 };
-int sm_count() {
-  int dev = 0, sms = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms > 0 ? sms : 1;
-}
 bool register_shape(int64_t rows, int C, int max_nv, int max_warps, Shape *p) {
   if (C % 8 || C > 256 * max_nv * kMaxTeam) return false;
   const int chunks = (C + 255) / 256;  // 256 values per warp and chunk
@@ -652,30 +644,6 @@ bool register_shape(int64_t rows, int C, int max_nv, int max_warps, Shape *p) {
 }
 int blocks_for(int64_t rows, const Shape &p) {
   return int(std::min<int64_t>((rows + p.teams - 1) / p.teams, sm_count()));
-}
-
-// Dynamic shared memory beyond the default needs an attribute of the kernel, set
-// once per device to the most it will ask for (and again only where this
-// table's 64 places do not suffice).
-void allow_smem(const void *kernel, size_t bytes) {
-  struct Entry {
-    const void *k;
-    int dev;
-    size_t bytes;
-  };
-  static std::mutex mu;
-  static Entry set[64];
-  static int used = 0;
-  if (bytes <= 40 * 1024) return;  // beside the static arrays, below the default 48 KiB
-  int dev = 0;
-  cudaGetDevice(&dev);
-  std::lock_guard<std::mutex> lock(mu);
-  int at = 0;
-  while (at < used && !(set[at].k == kernel && set[at].dev == dev)) ++at;
-  if (at < used && set[at].bytes >= bytes) return;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) != cudaSuccess) return;
-  if (at == used && used < 64) ++used;
-  if (at < used) set[at] = Entry{kernel, dev, bytes};
 }
 
 #define FMHC_DISPATCH_NV(NV_RT, NV_MAX, ...)                 \
