@@ -146,13 +146,10 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
   const int wt = warp % team, first = warp - wt;
   const int nchunk = C / 8, nb = (C + kBlock - 1) / kBlock;
   Raw *ring = reinterpret_cast<Raw *>(dyn) + warp * (S * NV * 32) + lane;
-  // Values of a warp of the team: chunks i * 32 + lane + v * 32 * team below nchunk.
-  const auto count = [&](int i) {
-    int n = 0;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) n += min(max(nchunk - (i + v * team) * 32, 0), 32) * 8;
-    return n;
-  };
+  // Warp i of the team holds the NV * 32 chunks from i * NV * 32, those below
+  // nchunk; this lane every 32nd, from c0: its chunk i exists if i * 32 < left.
+  const auto count = [&](int i) { return min(max(nchunk - i * NV * 32, 0), NV * 32) * 8; };
+  const int c0 = wt * NV * 32 + lane, left = nchunk - c0;
   const int mine = count(wt);
   // Lane i joins for warp i of the team.
   const float n_lane = lane < team ? float(count(lane)) : 0.f, inv_n = n_lane > 0.f ? 1.f / n_lane : 0.f;
@@ -160,18 +157,25 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
   const int64_t step = int64_t(gridDim.x) * teams;
   int64_t r = int64_t(blockIdx.x) * teams + warp / team;
   pdl_wait();
-  const auto fetch = [&](int64_t row, int stage) {
-    if (row < rows) {
+  // Pointers that move on by one step of rows.
+  const int64_t hop = step * C;
+  const E *src = x + r * C + c0 * 8;
+  E *dst = y + r * C + c0 * 8;
+  uint8_t *code_dst = FMT == kNone ? nullptr : codes + r * C + c0 * 8;
+  uint8_t *scale_dst = FMT == kNone ? nullptr : scales + r * nb + (c0 >> 2);
+  int64_t fetched = r;
+  const auto fetch = [&](int stage) {
+    if (fetched < rows) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = (wt + i * team) * 32 + lane;
-        if (c < nchunk) copy_raw<E>(ring + (stage * NV + i) * 32, x + row * C + c * 8);
-      }
+      for (int i = 0; i < NV; ++i)
+        if (i * 32 < left) copy_raw<E>(ring + (stage * NV + i) * 32, src + i * 256);
     }
+    fetched += step;
+    src += hop;
     copy_commit();
   };
 #pragma unroll
-  for (int s = 0; s < S - 1; ++s) fetch(r + s * step, s);
+  for (int s = 0; s < S - 1; ++s) fetch(s);
   float4 *ws = reinterpret_cast<float4 *>(reinterpret_cast<Raw *>(dyn) + (blockDim.x >> 5) * (S * NV * 32));
   float4 *bs = ws + 2 * nchunk;
   keep_param(ws, w, pdt, 1.f, nchunk);
@@ -179,7 +183,7 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
   __syncthreads();
   int par = 0, stage = 0;
   for (; r < rows; r += step, par ^= 1) {
-    fetch(r + (S - 1) * step, stage == 0 ? S - 1 : stage - 1);
+    fetch(stage == 0 ? S - 1 : stage - 1);
     copy_wait<S - 1>();
     float2 f[NV][4];
     uint32_t big[NV];  // largest magnitude of the chunk
@@ -189,7 +193,7 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
 #pragma unroll
       for (int k = 0; k < 4; ++k) f[i][k] = both(0.f);
       big[i] = 0;
-      if ((wt + i * team) * 32 + lane < nchunk) {
+      if (i * 32 < left) {
         const Raw raw = ring[(stage * NV + i) * 32];
         widen2<E>(raw, f[i]);
         if constexpr (FMT != kNone) big[i] = amax8_raw<E>(raw);
@@ -203,7 +207,7 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
     float2 q2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if ((wt + i * team) * 32 + lane < nchunk) {
+      if (i * 32 < left) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float2 d = add2(f[i][k], both(-m_w));
@@ -231,8 +235,7 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
     const float2 rs2 = both(rstd), off = both(-mean);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (wt + i * team) * 32 + lane;
-      const bool in = c < nchunk;
+      const bool in = i * 32 < left;
       if constexpr (FMT != kNone) {
         float v[8];
 #pragma unroll
@@ -242,14 +245,14 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
         }
         const uint32_t e = scale_byte<FMT>(amax_block(big[i]));
         if (in) {
-          __stcs(reinterpret_cast<uint2 *>(codes + r * C + c * 8), encode8<FMT>(v, e));
-          if ((lane & 3) == 0) __stcs(scales + r * nb + (c >> 2), uint8_t(e));
+          __stcs(reinterpret_cast<uint2 *>(code_dst + i * 256), encode8<FMT>(v, e));
+          if ((lane & 3) == 0) __stcs(scale_dst + i * 8, uint8_t(e));
         }
       }
       if (in) {
         float2 fw[4], fb[4];
-        kept_param(ws, c, nchunk, fw);
-        kept_param(bs, c, nchunk, fb);
+        kept_param(ws, c0 + i * 32, nchunk, fw);
+        kept_param(bs, c0 + i * 32, nchunk, fb);
         float o[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -257,8 +260,13 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
           o[2 * k] = v.x;
           o[2 * k + 1] = v.y;
         }
-        st8(y + r * C + c * 8, o);
+        st8(dst + i * 256, o);
       }
+    }
+    dst += hop;
+    if constexpr (FMT != kNone) {
+      code_dst += hop;
+      scale_dst += step * nb;
     }
   }
 }
@@ -321,24 +329,34 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
   const int64_t step = int64_t(gridDim.x) * teams;
   int64_t r = int64_t(blockIdx.x) * teams + warp / team;
   pdl_wait();
-  const auto fetch = [&](int64_t row, int stage) {
-    if (row < rows) {
+  // This lane's chunks: every 32nd of its warp's NV * 32, from c0 (as in the
+  // forward); pointers that move on by one step of rows.
+  const int c0 = wt * NV * 32 + lane, left = nchunk - c0;
+  const int64_t hop = step * C;
+  const E *g_src = g + r * C + c0 * 8;
+  const E *x_src = FMT == kNone ? reinterpret_cast<const E *>(x) + r * C + c0 * 8 : nullptr;
+  const uint8_t *q_src = FMT == kNone ? nullptr : reinterpret_cast<const uint8_t *>(x) + r * C + c0 * 8;
+  E *dst = gx + r * C + c0 * 8;
+  int64_t fetched = r;
+  const auto fetch = [&](int stage) {
+    if (fetched < rows) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (wt + i * team) * 32 + lane;
-        if (c < nchunk) {
-          copy_raw<E>(ring_g + (stage * NV + i) * 32, g + row * C + c * 8);
-          if constexpr (FMT == kNone)
-            copy_raw<E>(ring_x + (stage * NV + i) * 32, reinterpret_cast<const E *>(x) + row * C + c * 8);
-          else
-            copy_async<8>(ring_x + (stage * NV + i) * 32, reinterpret_cast<const uint8_t *>(x) + row * C + c * 8);
+        if (i * 32 < left) {
+          copy_raw<E>(ring_g + (stage * NV + i) * 32, g_src + i * 256);
+          if constexpr (FMT == kNone) copy_raw<E>(ring_x + (stage * NV + i) * 32, x_src + i * 256);
+          else copy_async<8>(ring_x + (stage * NV + i) * 32, q_src + i * 256);
         }
       }
     }
+    fetched += step;
+    g_src += hop;
+    if constexpr (FMT == kNone) x_src += hop;
+    else q_src += hop;
     copy_commit();
   };
 #pragma unroll
-  for (int s = 0; s < S - 1; ++s) fetch(r + s * step, s);
+  for (int s = 0; s < S - 1; ++s) fetch(s);
   if (w_shared) {
     keep_param(ws, w, pdt, 1.f, nchunk);
     __syncthreads();
@@ -358,16 +376,16 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
   // mean, rstd and the scale bytes of a row are loaded one row ahead.
   float next_m = 0.f, next_rs = 0.f;
   uint32_t next_e[NV], e[NV];
+  const uint8_t *s_src = FMT == kNone ? nullptr : scales + r * nb + (c0 >> 2);
   const auto ahead = [&](int64_t row) {
     if (row < rows) {
       next_m = __ldg(mean + row);
       next_rs = __ldg(rstd + row);
       if constexpr (FMT != kNone) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int c = (wt + i * team) * 32 + lane;
-          next_e[i] = c < nchunk ? __ldg(scales + row * nb + (c >> 2)) : 0u;
-        }
+        for (int i = 0; i < NV; ++i)
+          if (i * 32 < left) next_e[i] = __ldg(s_src + i * 8);
+        s_src += step * nb;
       }
     }
   };
@@ -380,18 +398,17 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
     const float2 off = both(-next_m);
 #pragma unroll
     for (int i = 0; i < NV; ++i) e[i] = next_e[i];
-    fetch(r + (S - 1) * step, stage == 0 ? S - 1 : stage - 1);
+    fetch(stage == 0 ? S - 1 : stage - 1);
     ahead(r + step);
     copy_wait<S - 1>();
     float2 s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (wt + i * team) * 32 + lane;
-      if (c < nchunk) {
+      if (i * 32 < left) {
         float2 fg[4], xh[4], fw[4];
         normalised<E, FMT>(ring_x[(stage * NV + i) * 32], e[i], rs, off, xh);
         widen2<E>(ring_g[(stage * NV + i) * 32], fg);
-        weight(c, fw);
+        weight(c0 + i * 32, fw);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float2 gw = mul2(fg[k], fw[k]);
@@ -407,12 +424,11 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
     const float2 c1 = both(-sum.x * inv_C), c2 = both(-sum.y * inv_C);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (wt + i * team) * 32 + lane;
-      if (c < nchunk) {
+      if (i * 32 < left) {
         float2 fg[4], xh[4], fw[4];
         normalised<E, FMT>(ring_x[(stage * NV + i) * 32], e[i], rs, off, xh);
         widen2<E>(ring_g[(stage * NV + i) * 32], fg);
-        weight(c, fw);
+        weight(c0 + i * 32, fw);
         float o[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -420,9 +436,10 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
           o[2 * k] = v.x;
           o[2 * k + 1] = v.y;
         }
-        st8(gx + r * C + c * 8, o);
+        st8(dst + i * 256, o);
       }
     }
+    dst += hop;
     if (++stage == S) stage = 0;
   }
   if (part == nullptr) return;
@@ -444,11 +461,11 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
       sums[warp * L + ((NV + i) * 8 + k) * 32 + lane] = k & 1 ? db[i][k / 2].y : db[i][k / 2].x;
     }
   __syncthreads();
-  float *dst = part + int64_t(blockIdx.x) * team * L;
+  float *out = part + int64_t(blockIdx.x) * team * L;
   for (int j = threadIdx.x; j < team * L; j += blockDim.x) {
     float v = 0.f;
     for (int t = 0; t < teams; ++t) v += sums[t * team * L + j];
-    dst[j] = v;
+    out[j] = v;
   }
 }
 
@@ -459,7 +476,7 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
 constexpr int kSumWarps = 32;
 __global__ void __launch_bounds__(32 * kSumWarps)
 ln_param_grad_kernel(const float *__restrict__ part, void *__restrict__ gw, void *__restrict__ gb,
-                     int pdt, int n, int64_t len, int C, int nv, int team) {
+                     int pdt, int n, int64_t len, int C, int nv) {
   pdl_wait();
   __shared__ float acc[kSumWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -484,7 +501,7 @@ ln_param_grad_kernel(const float *__restrict__ part, void *__restrict__ gw, void
     const int i = q % nv;
     q /= nv;
     is_b = q & 1;
-    c = (((q >> 1) + i * team) * 32 + l) * 8 + k;
+    c = (((q >> 1) * nv + i) * 32 + l) * 8 + k;
     if (c >= C) return;
   }
   void *dst = is_b ? gb : gw;
@@ -740,7 +757,7 @@ void launch_ln_bwd(const void *g, int dtype, const void *x, int fmt, const void 
   }
   if (part != nullptr)
     launch(ln_param_grad_kernel, dim3(unsigned((len + 31) / 32)), dim3(32 * kSumWarps), 0, s,
-           (const float *)part, gw, gb, pdt, parts, len, C, nv, p.team);
+           (const float *)part, gw, gb, pdt, parts, len, C, nv);
 }
 
 }  // namespace fmhc
