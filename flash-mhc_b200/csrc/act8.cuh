@@ -23,6 +23,7 @@
 #include <type_traits>
 
 #include "fmhc_common.cuh"
+#include "lane_ring.cuh"
 
 namespace fmhc {
 namespace act8 {
@@ -102,6 +103,21 @@ __device__ __forceinline__ void decode4(uint32_t w, float (&f)[4]) {
     const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&a));
     const float2 q = __half22float2(*reinterpret_cast<const __half2 *>(&b));
     f[0] = p.x; f[1] = p.y; f[2] = q.x; f[3] = q.y;
+  }
+}
+// The same as two pairs.
+template <int FMT>
+__device__ __forceinline__ void decode4x2(uint32_t w, float2 &a, float2 &b) {
+  if constexpr (FMT == kInt8) {
+    const uint32_t u = w ^ 0x80808080u, m = 0x4b000000u;
+    const float2 o = both(-8388736.f);
+    a = add2(make_float2(__uint_as_float(__byte_perm(u, m, 0x7650)), __uint_as_float(__byte_perm(u, m, 0x7651))), o);
+    b = add2(make_float2(__uint_as_float(__byte_perm(u, m, 0x7652)), __uint_as_float(__byte_perm(u, m, 0x7653))), o);
+  } else {
+    float f[4];
+    decode4<FMT>(w, f);
+    a = make_float2(f[0], f[1]);
+    b = make_float2(f[2], f[3]);
   }
 }
 template <int FMT>

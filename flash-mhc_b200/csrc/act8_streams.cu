@@ -140,14 +140,6 @@ __device__ __forceinline__ void advance(Cursor &p, int lane, int nchunk, int64_t
   }
 }
 
-// Four codes in a word -> two pairs of unscaled values.
-template <int FMT>
-__device__ __forceinline__ void decode4x2(uint32_t w, float2 &a, float2 &b) {
-  float f[4];
-  decode4<FMT>(w, f);
-  a = make_float2(f[0], f[1]);
-  b = make_float2(f[2], f[3]);
-}
 // Eight codes, scaled.
 template <int FMT>
 __device__ __forceinline__ void restore8(uint2 q, uint32_t e, float2 (&f)[4]) {

@@ -11,7 +11,20 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <utility>
+
 namespace fmhc {
+
+// f(std::integral_constant<int, i>) for i = 0 .. N - 1: unrolled, with the index
+// a constant (offsets of the asm below).
+template <class F, int... I>
+__device__ __forceinline__ void unrolled_(F &&f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void unrolled(F &&f) {
+  unrolled_(f, std::make_integer_sequence<int, N>{});
+}
 
 // ------------------------------------------------- two f32 in one instruction
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -50,6 +63,31 @@ __device__ __forceinline__ void copy_async(void *dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_addr(dst)), "l"(src) : "memory");
   else
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(shared_addr(dst)), "l"(src) : "memory");
+}
+// The same with a shared-memory address plus a constant.
+template <int BYTES, int OFF>
+__device__ __forceinline__ void copy_async_at(uint32_t dst, const void *src) {
+  static_assert(BYTES == 16 || BYTES == 8, "copy size");
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0 + %2], [%1], 16;" ::"r"(dst), "l"(src), "n"(OFF) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0 + %2], [%1], 8;" ::"r"(dst), "l"(src), "n"(OFF) : "memory");
+}
+// Shared-memory loads at an address plus a constant.
+template <int OFF>
+__device__ __forceinline__ uint4 load_shared16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a), "n"(OFF)
+               : "memory");
+  return v;
+}
+template <int OFF>
+__device__ __forceinline__ uint2 load_shared8(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2 + %3];" : "=r"(v.x), "=r"(v.y) : "r"(a), "n"(OFF) : "memory");
+  return v;
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Wait until at most N of this thread's latest groups are still in flight.

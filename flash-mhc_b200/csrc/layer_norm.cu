@@ -102,10 +102,16 @@ __device__ __forceinline__ void param8x2(const void *p, int dtype, int c, float 
 #pragma unroll
   for (int k = 0; k < 4; ++k) f[k] = make_float2(v[2 * k], v[2 * k + 1]);
 }
-template <class E>
-__device__ __forceinline__ void copy_raw(typename Elem<E>::Raw *dst, const E *src) {
-  copy_async<16>(dst, src);
-  if constexpr (sizeof(E) == 4) copy_async<16>(reinterpret_cast<char *>(dst) + 16, src + 4);
+// One raw chunk of eight values to and from shared memory.
+template <class E, int OFF>
+__device__ __forceinline__ void copy_raw(uint32_t dst, const E *src) {
+  copy_async_at<16, OFF>(dst, src);
+  if constexpr (sizeof(E) == 4) copy_async_at<16, OFF + 16>(dst, src + 4);
+}
+template <class E, int OFF>
+__device__ __forceinline__ typename Elem<E>::Raw load_raw(uint32_t a) {
+  if constexpr (sizeof(E) == 4) return {load_shared16<OFF>(a), load_shared16<OFF + 16>(a)};
+  else return load_shared16<OFF>(a);
 }
 
 constexpr int kStages = 3;  // ring depth in rows
@@ -124,10 +130,15 @@ __device__ __forceinline__ void keep_param(float4 *dst, const void *p, int dtype
     dst[nchunk + c] = make_float4(f[4], f[5], f[6], f[7]);
   }
 }
-__device__ __forceinline__ void kept_param(const float4 *src, int c, int nchunk, float2 (&f)[4]) {
-  const float4 a = src[c], b = src[nchunk + c];
-  f[0] = make_float2(a.x, a.y); f[1] = make_float2(a.z, a.w);
-  f[2] = make_float2(b.x, b.y); f[3] = make_float2(b.z, b.w);
+// Chunk of a lane whose first chunk is at `lo` (first halves) and `hi`, I * 32
+// chunks on.
+template <int I>
+__device__ __forceinline__ void kept_param(uint32_t lo, uint32_t hi, float2 (&f)[4]) {
+  const uint4 a = load_shared16<I * 512>(lo), b = load_shared16<I * 512>(hi);
+  f[0] = make_float2(__uint_as_float(a.x), __uint_as_float(a.y));
+  f[1] = make_float2(__uint_as_float(a.z), __uint_as_float(a.w));
+  f[2] = make_float2(__uint_as_float(b.x), __uint_as_float(b.y));
+  f[3] = make_float2(__uint_as_float(b.z), __uint_as_float(b.w));
 }
 
 // -------------------------------------------------------------------- forward
@@ -145,7 +156,8 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
   const int teams = (blockDim.x >> 5) / team;
   const int wt = warp % team, first = warp - wt;
   const int nchunk = C / 8, nb = (C + kBlock - 1) / kBlock;
-  Raw *ring = reinterpret_cast<Raw *>(dyn) + warp * (S * NV * 32) + lane;
+  constexpr int kChunk = 32 * int(sizeof(Raw));  // a warp's chunk in the ring
+  const uint32_t ring = shared_addr(dyn) + warp * (S * NV * kChunk) + lane * int(sizeof(Raw));
   // Warp i of the team holds the NV * 32 chunks from i * NV * 32, those below
   // nchunk; this lane every 32nd, from c0: its chunk i exists if i * 32 < left.
   const auto count = [&](int i) { return min(max(nchunk - i * NV * 32, 0), NV * 32) * 8; };
@@ -166,9 +178,10 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
   int64_t fetched = r;
   const auto fetch = [&](int stage) {
     if (fetched < rows) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (i * 32 < left) copy_raw<E>(ring + (stage * NV + i) * 32, src + i * 256);
+      const uint32_t to = ring + stage * (NV * kChunk);
+      unrolled<NV>([&](auto i) {
+        if (i * 32 < left) copy_raw<E, i * kChunk>(to, src + i * 256);
+      });
     }
     fetched += step;
     src += hop;
@@ -181,6 +194,8 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
   keep_param(ws, w, pdt, 1.f, nchunk);
   keep_param(bs, b, pdt, 0.f, nchunk);
   __syncthreads();
+  const uint32_t w_lo = shared_addr(ws + c0), w_hi = shared_addr(ws + nchunk + c0);
+  const uint32_t b_lo = shared_addr(bs + c0), b_hi = shared_addr(bs + nchunk + c0);
   int par = 0, stage = 0;
   for (; r < rows; r += step, par ^= 1) {
     fetch(stage == 0 ? S - 1 : stage - 1);
@@ -188,19 +203,19 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
     float2 f[NV][4];
     uint32_t big[NV];  // largest magnitude of the chunk
     float2 s2 = both(0.f);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
+    const uint32_t from = ring + stage * (NV * kChunk);
+    unrolled<NV>([&](auto i) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) f[i][k] = both(0.f);
       big[i] = 0;
       if (i * 32 < left) {
-        const Raw raw = ring[(stage * NV + i) * 32];
+        const Raw raw = load_raw<E, i * kChunk>(from);
         widen2<E>(raw, f[i]);
         if constexpr (FMT != kNone) big[i] = amax8_raw<E>(raw);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) s2 = add2(s2, f[i][k]);
-    }
+    });
     if (++stage == S) stage = 0;
     const float s = warp_sum(s2.x + s2.y);
     const float m_w = s * inv_mine;
@@ -233,8 +248,7 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
       rstd_out[r] = rstd;
     }
     const float2 rs2 = both(rstd), off = both(-mean);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
+    unrolled<NV>([&](auto i) {
       const bool in = i * 32 < left;
       if constexpr (FMT != kNone) {
         float v[8];
@@ -251,8 +265,8 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
       }
       if (in) {
         float2 fw[4], fb[4];
-        kept_param(ws, c0 + i * 32, nchunk, fw);
-        kept_param(bs, c0 + i * 32, nchunk, fb);
+        kept_param<i>(w_lo, w_hi, fw);
+        kept_param<i>(b_lo, b_hi, fb);
         float o[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -262,7 +276,7 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
         }
         st8(dst + i * 256, o);
       }
-    }
+    });
     dst += hop;
     if constexpr (FMT != kNone) {
       code_dst += hop;
@@ -288,11 +302,8 @@ __device__ __forceinline__ void normalised(const typename Input<E, FMT>::X &raw,
 #pragma unroll
     for (int i = 0; i < 4; ++i) xh[i] = mul2(add2(xh[i], off), both(rstd));
   } else {
-    float a[4], b[4];
-    decode4<FMT>(raw.x, a);
-    decode4<FMT>(raw.y, b);
-    xh[0] = make_float2(a[0], a[1]); xh[1] = make_float2(a[2], a[3]);
-    xh[2] = make_float2(b[0], b[1]); xh[3] = make_float2(b[2], b[3]);
+    decode4x2<FMT>(raw.x, xh[0], xh[1]);
+    decode4x2<FMT>(raw.y, xh[2], xh[3]);
     const float2 s = both(scale_value(e));
 #pragma unroll
     for (int i = 0; i < 4; ++i) xh[i] = mul2(fma2(xh[i], s, off), both(rstd));
@@ -321,9 +332,10 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
   const int nchunk = C / 8, nb = (C + kBlock - 1) / kBlock;
   const float inv_C = 1.f / float(C);
   // [warps][S][NV][32] of g, the same of x, then the weight.
-  Raw *ring_g = reinterpret_cast<Raw *>(dyn) + warp * (S * NV * 32) + lane;
-  X *ring_x = reinterpret_cast<X *>(reinterpret_cast<Raw *>(dyn) + warps * (S * NV * 32)) +
-              warp * (S * NV * 32) + lane;
+  constexpr int kChunkG = 32 * int(sizeof(Raw)), kChunkX = 32 * int(sizeof(X));
+  const uint32_t ring_g = shared_addr(dyn) + warp * (S * NV * kChunkG) + lane * int(sizeof(Raw));
+  const uint32_t ring_x = shared_addr(dyn) + warps * (S * NV * kChunkG) + warp * (S * NV * kChunkX) +
+                          lane * int(sizeof(X));
   float4 *ws = reinterpret_cast<float4 *>(
       reinterpret_cast<X *>(reinterpret_cast<Raw *>(dyn) + warps * (S * NV * 32)) + warps * (S * NV * 32));
   const int64_t step = int64_t(gridDim.x) * teams;
@@ -340,14 +352,14 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
   int64_t fetched = r;
   const auto fetch = [&](int stage) {
     if (fetched < rows) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
+      const uint32_t to_g = ring_g + stage * (NV * kChunkG), to_x = ring_x + stage * (NV * kChunkX);
+      unrolled<NV>([&](auto i) {
         if (i * 32 < left) {
-          copy_raw<E>(ring_g + (stage * NV + i) * 32, g_src + i * 256);
-          if constexpr (FMT == kNone) copy_raw<E>(ring_x + (stage * NV + i) * 32, x_src + i * 256);
-          else copy_async<8>(ring_x + (stage * NV + i) * 32, q_src + i * 256);
+          copy_raw<E, i * kChunkG>(to_g, g_src + i * 256);
+          if constexpr (FMT == kNone) copy_raw<E, i * kChunkX>(to_x, x_src + i * 256);
+          else copy_async_at<8, i * kChunkX>(to_x, q_src + i * 256);
         }
-      }
+      });
     }
     fetched += step;
     g_src += hop;
@@ -361,12 +373,14 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
     keep_param(ws, w, pdt, 1.f, nchunk);
     __syncthreads();
   }
-  const auto weight = [&](int c, float2 (&f)[4]) {
-    if (w_shared) {
-      kept_param(ws, c, nchunk, f);
-    } else {
-      param8x2(w, pdt, c, 1.f, f);
-    }
+  const uint32_t w_lo = shared_addr(ws + c0), w_hi = shared_addr(ws + nchunk + c0);
+  const auto weight = [&](auto i, float2 (&f)[4]) {
+    if (w_shared) kept_param<i>(w_lo, w_hi, f);
+    else param8x2(w, pdt, c0 + i * 32, 1.f, f);
+  };
+  const auto load_x = [&](auto i, uint32_t from) -> X {
+    if constexpr (FMT == kNone) return load_raw<E, i * kChunkX>(from);
+    else return load_shared8<i * kChunkX>(from);
   };
   float2 dw[NV][4], db[NV][4];
 #pragma unroll
@@ -402,13 +416,13 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
     ahead(r + step);
     copy_wait<S - 1>();
     float2 s1 = both(0.f), s2 = both(0.f);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
+    const uint32_t from_g = ring_g + stage * (NV * kChunkG), from_x = ring_x + stage * (NV * kChunkX);
+    unrolled<NV>([&](auto i) {
       if (i * 32 < left) {
         float2 fg[4], xh[4], fw[4];
-        normalised<E, FMT>(ring_x[(stage * NV + i) * 32], e[i], rs, off, xh);
-        widen2<E>(ring_g[(stage * NV + i) * 32], fg);
-        weight(c0 + i * 32, fw);
+        normalised<E, FMT>(load_x(i, from_x), e[i], rs, off, xh);
+        widen2<E>(load_raw<E, i * kChunkG>(from_g), fg);
+        weight(i, fw);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float2 gw = mul2(fg[k], fw[k]);
@@ -418,17 +432,16 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
           s2 = fma2(gw, xh[k], s2);
         }
       }
-    }
+    });
     const float2 sum = team_sum(make_float2(warp_sum(s1.x + s1.y), warp_sum(s2.x + s2.y)), slots[par],
                                 team, warp, lane);
     const float2 c1 = both(-sum.x * inv_C), c2 = both(-sum.y * inv_C);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
+    unrolled<NV>([&](auto i) {
       if (i * 32 < left) {
         float2 fg[4], xh[4], fw[4];
-        normalised<E, FMT>(ring_x[(stage * NV + i) * 32], e[i], rs, off, xh);
-        widen2<E>(ring_g[(stage * NV + i) * 32], fg);
-        weight(c0 + i * 32, fw);
+        normalised<E, FMT>(load_x(i, from_x), e[i], rs, off, xh);
+        widen2<E>(load_raw<E, i * kChunkG>(from_g), fg);
+        weight(i, fw);
         float o[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -438,7 +451,7 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
         }
         st8(dst + i * 256, o);
       }
-    }
+    });
     dst += hop;
     if (++stage == S) stage = 0;
   }
