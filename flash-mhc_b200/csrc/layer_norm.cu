@@ -133,15 +133,24 @@ __device__ __forceinline__ void keep_param(float4 *dst, const void *p, int dtype
 // Chunk of a lane whose first chunk is at `lo` (first halves) and `hi`, I * 32
 // chunks on.
 template <int I>
-__device__ __forceinline__ void kept_param(uint32_t lo, uint32_t hi, float2 (&f)[4]) {
+__device__ __forceinline__ void kept_param(uint32_t lo, uint32_t hi, float (&f)[8]) {
   const uint4 a = load_shared16<I * 512>(lo), b = load_shared16<I * 512>(hi);
-  f[0] = make_float2(__uint_as_float(a.x), __uint_as_float(a.y));
-  f[1] = make_float2(__uint_as_float(a.z), __uint_as_float(a.w));
-  f[2] = make_float2(__uint_as_float(b.x), __uint_as_float(b.y));
-  f[3] = make_float2(__uint_as_float(b.z), __uint_as_float(b.w));
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(w[k]);
+}
+template <int I>
+__device__ __forceinline__ void kept_param(uint32_t lo, uint32_t hi, float2 (&f)[4]) {
+  float v[8];
+  kept_param<I>(lo, hi, v);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) f[k] = make_float2(v[2 * k], v[2 * k + 1]);
 }
 
 // -------------------------------------------------------------------- forward
+// Scalar arithmetic: packed pairs, as in the backward, were no faster without
+// and slower with the 8-bit copy (131072 x 1024: 98.5 against 100.2 us, with
+// int8 113 against 125).
 template <class E, int NV, int FMT>
 __global__ void __launch_bounds__(32 * kFwdWarps, 1)
 ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *__restrict__ b,
@@ -200,36 +209,39 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
   for (; r < rows; r += step, par ^= 1) {
     fetch(stage == 0 ? S - 1 : stage - 1);
     copy_wait<S - 1>();
-    float2 f[NV][4];
+    float f[NV][8];
     uint32_t big[NV];  // largest magnitude of the chunk
-    float2 s2 = both(0.f);
+    float s = 0.f;
     const uint32_t from = ring + stage * (NV * kChunk);
     unrolled<NV>([&](auto i) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) f[i][k] = both(0.f);
+      for (int k = 0; k < 8; ++k) f[i][k] = 0.f;
       big[i] = 0;
       if (i * 32 < left) {
         const Raw raw = load_raw<E, i * kChunk>(from);
-        widen2<E>(raw, f[i]);
+        Elem<E>::widen(raw, f[i]);
         if constexpr (FMT != kNone) big[i] = amax8_raw<E>(raw);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s2 = add2(s2, f[i][k]);
+      for (int k = 0; k < 8; k += 2) s += f[i][k] + f[i][k + 1];
     });
     if (++stage == S) stage = 0;
-    const float s = warp_sum(s2.x + s2.y);
-    const float m_w = s * inv_mine;
-    float2 q2 = both(0.f);
+    s = warp_sum(s);
+    // (__fmul_rn: not to be contracted with the differences below, so that every
+    // instantiation gives the same bits.)
+    const float m_w = __fmul_rn(s, inv_mine);
+    float q = 0.f, q1 = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (i * 32 < left) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 d = add2(f[i][k], both(-m_w));
-          q2 = fma2(d, d, q2);
+        for (int k = 0; k < 8; k += 2) {
+          const float d = f[i][k] - m_w, d1 = f[i][k + 1] - m_w;
+          q = fmaf(d, d, q);
+          q1 = fmaf(d1, d1, q1);
         }
       }
-    const float q = warp_sum(q2.x + q2.y);
+    q = warp_sum(q + q1);
     float mean = m_w, m2 = q;
     if (team > 1) {
       // Join the warps: means first, then the squares about the row's mean.
@@ -238,7 +250,7 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
       if (lane == 0) slot[wt] = make_float2(s, q);
       named_bar_sync(1 + warp / team, team * 32);
       const float2 o = lane < team ? slot[lane] : make_float2(0.f, 0.f);
-      mean = warp_sum(o.x) * inv_C;
+      mean = __fmul_rn(warp_sum(o.x), inv_C);
       const float d = n_lane > 0.f ? fmaf(o.x, inv_n, -mean) : 0.f;
       m2 = warp_sum(fmaf(n_lane * d, d, o.y));
     }
@@ -247,33 +259,21 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
       mean_out[r] = mean;
       rstd_out[r] = rstd;
     }
-    const float2 rs2 = both(rstd), off = both(-mean);
     unrolled<NV>([&](auto i) {
       const bool in = i * 32 < left;
       if constexpr (FMT != kNone) {
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          v[2 * k] = f[i][k].x;
-          v[2 * k + 1] = f[i][k].y;
-        }
         const uint32_t e = scale_byte<FMT>(amax_block(big[i]));
         if (in) {
-          __stcs(reinterpret_cast<uint2 *>(code_dst + i * 256), encode8<FMT>(v, e));
+          __stcs(reinterpret_cast<uint2 *>(code_dst + i * 256), encode8<FMT>(f[i], e));
           if ((lane & 3) == 0) __stcs(scale_dst + i * 8, uint8_t(e));
         }
       }
       if (in) {
-        float2 fw[4], fb[4];
+        float fw[8], fb[8], o[8];
         kept_param<i>(w_lo, w_hi, fw);
         kept_param<i>(b_lo, b_hi, fb);
-        float o[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 v = fma2(mul2(add2(f[i][k], off), rs2), fw[k], fb[k]);
-          o[2 * k] = v.x;
-          o[2 * k + 1] = v.y;
-        }
+        for (int k = 0; k < 8; ++k) o[k] = fmaf((f[i][k] - mean) * rstd, fw[k], fb[k]);
         st8(dst + i * 256, o);
       }
     });
