@@ -62,14 +62,19 @@ __device__ __forceinline__ float scale_value(uint32_t e) {
   return __uint_as_float(b);
 }
 
-// Four values -> four codes in one word (value 0 in the lowest byte).
-template <int FMT>
+// The scale bytes below this one need no care in encode4: no value of their
+// block is above M times the scale, and none is infinite or NaN.
+template <int FMT> constexpr uint32_t kTopScale = 254u - Format<FMT>::kTop;
+
+// Four values -> four codes in one word (value 0 in the lowest byte).  CARE: the
+// scale byte may be kTopScale (saturate) or 255 (codes 0).
+template <int FMT, bool CARE>
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, uint32_t e) {
-  const float inv = __uint_as_float((254u - min(e, 254u - Format<FMT>::kTop)) << 23);
+  const float inv = __uint_as_float((254u - (CARE ? min(e, kTopScale<FMT>) : e)) << 23);
   float v[4] = {a * inv, b * inv, c * inv, d * inv};
   uint32_t w;
   if constexpr (FMT == kInt8) {
-    if (e == 254u - Format<FMT>::kTop) {  // only here can a value exceed M
+    if constexpr (CARE) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = fminf(fmaxf(v[i], -Format<FMT>::kMax), Format<FMT>::kMax);
     }
@@ -85,7 +90,7 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, 
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(v[3]), "f"(v[2]));
     w = uint32_t(lo) | (uint32_t(hi) << 16);
   }
-  return e == 255u ? 0u : w;
+  return CARE && e == 255u ? 0u : w;
 }
 
 // One word of codes -> four unscaled f32 values (exact).
@@ -253,14 +258,6 @@ __device__ __forceinline__ uint32_t amax8_raw(const typename Elem<E>::Raw &r) {
   }
 }
 
-// f32 bits of the largest magnitude of eight values (NaN above infinity above
-// everything finite, as unsigned integers order them).
-__device__ __forceinline__ uint32_t amax8(const float (&f)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
-  return m;
-}
 // The same over the four lanes that share a block (lanes 4k .. 4k+3, eight
 // values each); every lane of the warp takes part.
 __device__ __forceinline__ uint32_t amax_block(uint32_t m) {
@@ -268,10 +265,16 @@ __device__ __forceinline__ uint32_t amax_block(uint32_t m) {
   return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
 }
 
-// Encodes eight values of a block with scale byte e.
+// Encodes eight values of a block with scale byte e, or one.
 template <int FMT>
 __device__ __forceinline__ uint2 encode8(const float (&f)[8], uint32_t e) {
-  return make_uint2(encode4<FMT>(f[0], f[1], f[2], f[3], e), encode4<FMT>(f[4], f[5], f[6], f[7], e));
+  if (e < kTopScale<FMT>)
+    return make_uint2(encode4<FMT, false>(f[0], f[1], f[2], f[3], e), encode4<FMT, false>(f[4], f[5], f[6], f[7], e));
+  return make_uint2(encode4<FMT, true>(f[0], f[1], f[2], f[3], e), encode4<FMT, true>(f[4], f[5], f[6], f[7], e));
+}
+template <int FMT>
+__device__ __forceinline__ uint8_t encode1(float f, uint32_t e) {
+  return uint8_t(encode4<FMT, true>(f, 0.f, 0.f, 0.f, e));
 }
 
 }  // namespace act8

@@ -25,12 +25,31 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Position of a warp's pipeline: token t, and this lane's chunk of eight values.
+struct Cursor {
+  int64_t t;
+  int c;
+};
+__device__ __forceinline__ void advance(Cursor &p, int lane, int nchunk, int64_t nwarps) {
+  p.c += 32;
+  if (p.c - lane >= nchunk) {
+    p.c = lane;
+    p.t += nwarps;
+  }
+}
+
 // ---------------------------------------------------------------- K3 forward
 //   out[t,c] = bf16( sum_j h_pre[t,j] x[t,j,c] ), and x in 8 bits.
+// Chunks per lane in flight and resident blocks per SM, measured at T = 65536
+// (C = 1024 int8 / C = 2048 e4m3, us): 2 and 3 158 / 318; 1: 200 / 387; 2 and 4:
+// 173 / 343; 4: 225 / 437; 2 with 2 blocks: 172 / 334; a shared-memory ring as
+// in the backwards 158 / 350.
+constexpr int kF3U = 2, kF3Blocks = 3;
 template <int FMT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kF3Blocks)
 k3_fwd_q8_kernel(const bf16 *__restrict__ x, const float4 *__restrict__ hp, bf16 *__restrict__ out,
                  uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, int64_t T, int C) {
+  constexpr int U = kF3U;
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
@@ -40,29 +59,38 @@ k3_fwd_q8_kernel(const bf16 *__restrict__ x, const float4 *__restrict__ hp, bf16
     const float4 h = __ldg(hp + t);
     const float hj[4] = {h.x, h.y, h.z, h.w};
     const bf16 *xr = x + t * 4 * C;
-    for (int c0 = 0; c0 < nchunk; c0 += 32) {
-      const int c = c0 + lane;
-      const bool in = c < nchunk;
-      uint4 a[4] = {};
-      if (in) {
+    for (int c0 = 0; c0 < nchunk; c0 += 32 * U) {
+      uint4 a[U][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) a[j] = ld8(xr + j * C + c * 8);
-      }
-      float o[8];
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + 32 * u + lane;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float f[8];
-        Elem<bf16>::widen(a[j], f);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = j ? fmaf(hj[j], f[k], o[k]) : hj[0] * f[k];
-        const uint32_t e = scale_byte<FMT>(amax_block(amax8(f)));
-        const int64_t row = t * 4 + j;
-        if (in) {
-          __stcs(reinterpret_cast<uint2 *>(codes + row * C + c * 8), encode8<FMT>(f, e));
-          if ((lane & 3) == 0) __stcs(scales + row * nb + (c >> 2), uint8_t(e));
+        for (int j = 0; j < 4; ++j) {
+          a[u][j] = make_uint4(0, 0, 0, 0);
+          if (c < nchunk) a[u][j] = ld8(xr + j * C + c * 8);
         }
       }
-      if (in) st8(out + t * C + c * 8, o);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + 32 * u + lane;
+        if (c - lane >= nchunk) break;  // the whole warp is past the row
+        const bool in = c < nchunk;
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float f[8];
+          Elem<bf16>::widen(a[u][j], f);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o[k] = j ? fmaf(hj[j], f[k], o[k]) : hj[0] * f[k];
+          const uint32_t e = scale_byte<FMT>(amax_block(amax8_raw<bf16>(a[u][j])));
+          const int64_t row = t * 4 + j;
+          if (in) {
+            __stcs(reinterpret_cast<uint2 *>(codes + row * C + c * 8), encode8<FMT>(f, e));
+            if ((lane & 3) == 0) __stcs(scales + row * nb + (c >> 2), uint8_t(e));
+          }
+        }
+        if (in) st8(out + t * C + c * 8, o);
+      }
     }
   }
 }
@@ -70,12 +98,17 @@ k3_fwd_q8_kernel(const bf16 *__restrict__ x, const float4 *__restrict__ hp, bf16
 // ---------------------------------------------------------------- K4 forward
 //   out[t,i,c] = bf16( sum_j H[t,i,j] x[t,j,c] + h_post[t,i] lo[t,c] ), and lo
 //   in 8 bits.
+// Chunks per lane in flight and resident blocks per SM, as above: 2 and 2 208 /
+// 408 us; 4 and 1: 211 / 403; 1 and 2: 224 / 438; 2 and 1: 245 / 474; a ring:
+// 224 / 434.
+constexpr int kF4U = 2, kF4Blocks = 2;
 template <int FMT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kF4Blocks)
 k4_fwd_q8_kernel(const bf16 *__restrict__ x, const bf16 *__restrict__ lo,
                  const float4 *__restrict__ H, const float4 *__restrict__ hpost,
                  bf16 *__restrict__ out, uint8_t *__restrict__ codes,
                  uint8_t *__restrict__ scales, int64_t T, int C) {
+  constexpr int U = kF4U;
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
@@ -91,35 +124,44 @@ k4_fwd_q8_kernel(const bf16 *__restrict__ x, const bf16 *__restrict__ lo,
     const float4 hp4 = __ldg(hpost + t);
     const float hp[4] = {hp4.x, hp4.y, hp4.z, hp4.w};
     const bf16 *xr = x + t * 4 * C;
-    for (int c0 = 0; c0 < nchunk; c0 += 32) {
-      const int c = c0 + lane;
-      const bool in = c < nchunk;
-      uint4 a[4] = {}, l = {};
-      if (in) {
-        l = ld8(lo + t * C + c * 8);
+    for (int c0 = 0; c0 < nchunk; c0 += 32 * U) {
+      uint4 a[U][4], l[U];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) a[j] = ld8(xr + j * C + c * 8);
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + 32 * u + lane;
+        l[u] = make_uint4(0, 0, 0, 0);
+        if (c < nchunk) {
+          l[u] = ld8(lo + t * C + c * 8);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) a[u][j] = ld8(xr + j * C + c * 8);
+        }
       }
-      float fl[8], fx[4][8];
-      Elem<bf16>::widen(l, fl);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) Elem<bf16>::widen(a[j], fx[j]);
-      const uint32_t e = scale_byte<FMT>(amax_block(amax8(fl)));
-      if (in) {
-        __stcs(reinterpret_cast<uint2 *>(codes + t * C + c * 8), encode8<FMT>(fl, e));
-        if ((lane & 3) == 0) __stcs(scales + t * nb + (c >> 2), uint8_t(e));
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + 32 * u + lane;
+        if (c - lane >= nchunk) break;  // the whole warp is past the row
+        float fl[8];
+        Elem<bf16>::widen(l[u], fl);
+        const uint32_t e = scale_byte<FMT>(amax_block(amax8_raw<bf16>(l[u])));
+        if (c < nchunk) {
+          float fx[4][8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float o[8];
+          for (int j = 0; j < 4; ++j) Elem<bf16>::widen(a[u][j], fx[j]);
+          __stcs(reinterpret_cast<uint2 *>(codes + t * C + c * 8), encode8<FMT>(fl, e));
+          if ((lane & 3) == 0) __stcs(scales + t * nb + (c >> 2), uint8_t(e));
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {  // in the order of fmhc_k4_fwd
-            float acc = hp[i] * fl[k];
-            acc = fmaf(Hm[i][0], fx[0][k], acc);
-            acc = fmaf(Hm[i][1], fx[1][k], acc);
-            acc = fmaf(Hm[i][2], fx[2][k], acc);
-            o[k] = fmaf(Hm[i][3], fx[3][k], acc);
+          for (int i = 0; i < 4; ++i) {
+            float o[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {  // in the order of fmhc_k4_fwd
+              float acc = hp[i] * fl[k];
+              acc = fmaf(Hm[i][0], fx[0][k], acc);
+              acc = fmaf(Hm[i][1], fx[1][k], acc);
+              acc = fmaf(Hm[i][2], fx[2][k], acc);
+              o[k] = fmaf(Hm[i][3], fx[3][k], acc);
+            }
+            st8(out + (t * 4 + i) * C + c * 8, o);
           }
-          st8(out + (t * 4 + i) * C + c * 8, o);
         }
       }
     }
@@ -127,19 +169,6 @@ k4_fwd_q8_kernel(const bf16 *__restrict__ x, const bf16 *__restrict__ lo,
 }
 
 // --------------------------------------------------------- backward rings
-// Position of a warp's pipeline: token t, and this lane's chunk of eight values.
-struct Cursor {
-  int64_t t;
-  int c;
-};
-__device__ __forceinline__ void advance(Cursor &p, int lane, int nchunk, int64_t nwarps) {
-  p.c += 32;
-  if (p.c - lane >= nchunk) {
-    p.c = lane;
-    p.t += nwarps;
-  }
-}
-
 // Eight codes, scaled.
 template <int FMT>
 __device__ __forceinline__ void restore8(uint2 q, uint32_t e, float2 (&f)[4]) {

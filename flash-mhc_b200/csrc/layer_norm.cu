@@ -574,7 +574,7 @@ ln_fwd_any_kernel(const E *__restrict__ x, const void *__restrict__ w, const voi
         const float f = c < C ? Elem<E>::widen1(xr[c]) : 0.f;
         const uint32_t e = scale_byte<FMT>(
             __reduce_max_sync(0xffffffffu, __float_as_uint(f) & 0x7fffffffu));
-        if (c < C) codes[r * C + c] = uint8_t(encode4<FMT>(f, 0.f, 0.f, 0.f, e));
+        if (c < C) codes[r * C + c] = encode1<FMT>(f, e);
         if (lane == 0) scales[r * nb + k] = uint8_t(e);
       }
     }
