@@ -26,7 +26,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .ops import _bf16, _coef, _k2_typed_args, _lib, _n4, _on_device, _stream
+from .ops import _bf16, _coef, _k2_typed_args, _lib, _n4, _on_device
 
 BLOCK = 32  # values per scale
 # format name -> (FMHC_ACT8_*, dtype of the codes)
@@ -106,8 +106,29 @@ def _checkpoint(op: str, name: str, codes: torch.Tensor, scales: torch.Tensor):
 
 
 def _new_checkpoint(x: torch.Tensor, code_dtype: torch.dtype):
-    return (torch.empty(x.shape, device=x.device, dtype=code_dtype),
-            torch.empty(_scales_shape(x.shape), device=x.device, dtype=torch.uint8))
+    return (torch.empty_like(x, dtype=code_dtype, memory_format=torch.contiguous_format),
+            x.new_empty(_scales_shape(x.shape), dtype=torch.uint8))
+
+
+def _launch(t: torch.Tensor, name: str, *args) -> None:
+    """C-ABI call ``name`` on ``t``'s device and current stream (the last argument).
+
+    At few tokens a call costs what Python spends on it, so the device is
+    switched only if it has to be and the stream is taken as its raw handle."""
+    index = t.device.index
+    if index == torch._C._cuda_getDevice():
+        _native.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with _on_device(t):
+            _native.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _workspace(t: torch.Tensor, size_fn: str, *args):
+    """(pointer, bytes, tensor) of the scratch that ``size_fn`` asks for on ``t``'s device."""
+    with _on_device(t):
+        n = int(getattr(_native.lib(), size_fn)(*args))
+    ws = t.new_empty((max(n, 1),), dtype=torch.uint8)
+    return ws.data_ptr(), n, ws
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -184,9 +205,8 @@ def _act_quantize_cuda(x, format):
     fmt, code_dtype = _format("act_quantize", format)
     x = _act("act_quantize", "x", x)
     codes, scales = _new_checkpoint(x, code_dtype)
-    with _on_device(x):
-        _native.call("fmhc_act_quantize", x.data_ptr(), _DTYPES[x.dtype], codes.data_ptr(), fmt,
-                     scales.data_ptr(), _rows(x), x.shape[-1], _stream(x))
+    _launch(x, "fmhc_act_quantize", x.data_ptr(), _DTYPES[x.dtype], codes.data_ptr(), fmt,
+            scales.data_ptr(), _rows(x), x.shape[-1])
     return codes, scales
 
 
@@ -197,10 +217,9 @@ def _act_dequantize_cuda(codes, scales, dtype):
     codes, scales, fmt = _checkpoint(op, "the", codes, scales)
     if dtype not in _DTYPES:
         raise ValueError(f"flash_mhc::{op}: dtype must be float32, bfloat16 or float16 (got {dtype})")
-    x = torch.empty(codes.shape, device=codes.device, dtype=dtype)
-    with _on_device(codes):
-        _native.call("fmhc_act_dequantize", codes.data_ptr(), fmt, scales.data_ptr(), x.data_ptr(),
-                     _DTYPES[dtype], _rows(codes), codes.shape[-1], _stream(codes))
+    x = torch.empty_like(codes, dtype=dtype)
+    _launch(codes, "fmhc_act_dequantize", codes.data_ptr(), fmt, scales.data_ptr(), x.data_ptr(),
+            _DTYPES[dtype], _rows(codes), codes.shape[-1])
     return x
 
 
@@ -212,11 +231,10 @@ def _fused_pre_map_q8_cuda(x_streams, h_pre, format):
     _shape(op, "h_pre", h_pre, (T, n))
     _same_device(op, x_streams, h_pre=h_pre)
     x_streams, h_pre = _bf16("x_streams", x_streams), _coef(h_pre)
-    out = torch.empty((T, C), device=x_streams.device, dtype=x_streams.dtype)
+    out = x_streams.new_empty((T, C))
     codes, scales = _new_checkpoint(x_streams, code_dtype)
-    with _on_device(x_streams):
-        _native.call("fmhc_k3_fwd_q8", x_streams.data_ptr(), h_pre.data_ptr(), out.data_ptr(),
-                     codes.data_ptr(), scales.data_ptr(), fmt, T, n, C, _stream(x_streams))
+    _launch(x_streams, "fmhc_k3_fwd_q8", x_streams.data_ptr(), h_pre.data_ptr(), out.data_ptr(),
+            codes.data_ptr(), scales.data_ptr(), fmt, T, n, C)
     return out, codes, scales
 
 
@@ -234,10 +252,9 @@ def _fused_post_res_q8_cuda(x_streams, layer_output, H_merged, h_post, format):
     H_merged, h_post = _coef(H_merged), _coef(h_post)
     out = torch.empty_like(x_streams)
     codes, scales = _new_checkpoint(layer_output, code_dtype)
-    with _on_device(x_streams):
-        _native.call("fmhc_k4_fwd_q8", x_streams.data_ptr(), layer_output.data_ptr(),
-                     H_merged.data_ptr(), h_post.data_ptr(), out.data_ptr(), codes.data_ptr(),
-                     scales.data_ptr(), fmt, T, n, C, _stream(x_streams))
+    _launch(x_streams, "fmhc_k4_fwd_q8", x_streams.data_ptr(), layer_output.data_ptr(),
+            H_merged.data_ptr(), h_post.data_ptr(), out.data_ptr(), codes.data_ptr(),
+            scales.data_ptr(), fmt, T, n, C)
     return out, codes, scales
 
 
@@ -251,21 +268,16 @@ def _mhc_pre_forward_q8_cuda(x_streams, W, alpha_pre, alpha_post, alpha_res, bia
                  alpha_res=alpha_res, bias=bias, perm=perm)
     x_streams, W = _bf16("x_streams", x_streams), _bf16("W", W)
     args, _keep = _k2_typed_args(alpha_pre, alpha_post, alpha_res, bias, perm)
-    dev, dt = x_streams.device, x_streams.dtype
-    f = dict(device=dev, dtype=torch.float32)
-    layer_input = torch.empty((T, C), device=dev, dtype=dt)
-    proj = torch.empty((T, 32), device=dev, dtype=dt)
-    inv_rms = torch.empty((T,), **f)
-    h_pre, h_post, H = torch.empty((T, 4), **f), torch.empty((T, 4), **f), torch.empty((T, 4, 4), **f)
+    new = lambda *shape, dtype=torch.float32: x_streams.new_empty(shape, dtype=dtype)  # noqa: E731
+    layer_input, proj = new(T, C, dtype=x_streams.dtype), new(T, 32, dtype=x_streams.dtype)
+    inv_rms, h_pre, h_post, H = new(T), new(T, 4), new(T, 4), new(T, 4, 4)
     codes, scales = _new_checkpoint(x_streams, code_dtype)
-    with _on_device(x_streams):
-        s = _stream(x_streams)
-        # K1 and K2 in one kernel, then K3 with the checkpoint of x.
-        _native.call("fmhc_mhc_pre_fwd", x_streams.data_ptr(), W.data_ptr(), *args,
-                     proj.data_ptr(), inv_rms.data_ptr(), h_pre.data_ptr(), h_post.data_ptr(),
-                     H.data_ptr(), None, T, n, C, s)
-        _native.call("fmhc_k3_fwd_q8", x_streams.data_ptr(), h_pre.data_ptr(),
-                     layer_input.data_ptr(), codes.data_ptr(), scales.data_ptr(), fmt, T, n, C, s)
+    # K1 and K2 in one kernel, then K3 with the checkpoint of x.
+    _launch(x_streams, "fmhc_mhc_pre_fwd", x_streams.data_ptr(), W.data_ptr(), *args,
+            proj.data_ptr(), inv_rms.data_ptr(), h_pre.data_ptr(), h_post.data_ptr(),
+            H.data_ptr(), None, T, n, C)
+    _launch(x_streams, "fmhc_k3_fwd_q8", x_streams.data_ptr(), h_pre.data_ptr(),
+            layer_input.data_ptr(), codes.data_ptr(), scales.data_ptr(), fmt, T, n, C)
     return layer_input, proj, inv_rms, h_pre, h_post, H, codes, scales
 
 
@@ -277,10 +289,9 @@ def _pre_map_grad_h_q8_cuda(grad_out, x_codes, x_scales):
     _same_device(op, grad_out, x_codes=x_codes, x_scales=x_scales)
     x_codes, x_scales, fmt = _checkpoint(op, "x", x_codes, x_scales)
     grad_out = _bf16("grad_out", grad_out)
-    grad_h_pre = torch.empty((T, n), device=grad_out.device, dtype=torch.float32)
-    with _on_device(grad_out):
-        _native.call("fmhc_k3_bwd_q8", grad_out.data_ptr(), x_codes.data_ptr(), x_scales.data_ptr(),
-                     fmt, grad_h_pre.data_ptr(), T, n, C, _stream(grad_out))
+    grad_h_pre = grad_out.new_empty((T, n), dtype=torch.float32)
+    _launch(grad_out, "fmhc_k3_bwd_q8", grad_out.data_ptr(), x_codes.data_ptr(),
+            x_scales.data_ptr(), fmt, grad_h_pre.data_ptr(), T, n, C)
     return grad_h_pre
 
 
@@ -299,14 +310,12 @@ def _post_res_grad_params_q8_cuda(grad_out, x_codes, x_scales, lo_codes, lo_scal
         raise ValueError(f"flash_mhc::{op}: x_codes and lo_codes must have one format "
                          f"(got {x_codes.dtype} and {lo_codes.dtype})")
     grad_out, h_post = _bf16("grad_out", grad_out), _coef(h_post)
-    f = dict(device=grad_out.device, dtype=torch.float32)
-    grad_lo = torch.empty((T, C), device=grad_out.device, dtype=grad_out.dtype)
-    grad_H, grad_hp = torch.empty((T, n, n), **f), torch.empty((T, n), **f)
-    with _on_device(grad_out):
-        _native.call("fmhc_k4_bwd_q8", grad_out.data_ptr(), x_codes.data_ptr(), x_scales.data_ptr(),
-                     lo_codes.data_ptr(), lo_scales.data_ptr(), fmt, h_post.data_ptr(),
-                     grad_lo.data_ptr(), grad_H.data_ptr(), grad_hp.data_ptr(), T, n, C,
-                     _stream(grad_out))
+    grad_lo = grad_out.new_empty((T, C))
+    grad_H = grad_out.new_empty((T, n, n), dtype=torch.float32)
+    grad_hp = grad_out.new_empty((T, n), dtype=torch.float32)
+    _launch(grad_out, "fmhc_k4_bwd_q8", grad_out.data_ptr(), x_codes.data_ptr(),
+            x_scales.data_ptr(), lo_codes.data_ptr(), lo_scales.data_ptr(), fmt,
+            h_post.data_ptr(), grad_lo.data_ptr(), grad_H.data_ptr(), grad_hp.data_ptr(), T, n, C)
     return grad_lo, grad_H, grad_hp
 
 
@@ -324,15 +333,11 @@ def _fused_rmsnorm_project_backward_q8_cuda(grad_out, x_codes, x_scales, W, proj
     grad_out, W, proj_out = _bf16("grad_out", grad_out), _bf16("W", W), _bf16("proj_out", proj_out)
     grad_out, W, proj_out, x_codes, x_scales = (_aligned(t) for t in (grad_out, W, proj_out, x_codes, x_scales))
     inv_rms = inv_rms.to(torch.float32).contiguous()
-    dev, dt = grad_out.device, grad_out.dtype
-    grad_x = torch.empty((T, n, C), device=dev, dtype=dt)
-    grad_W = torch.empty((32, n * C), device=dev, dtype=dt)
-    with _on_device(grad_out):
-        ws_bytes = int(_native.lib().fmhc_k1_bwd_q8_workspace_size(T, C))
-        ws = torch.empty(max(ws_bytes, 1), device=dev, dtype=torch.uint8)
-        _native.call("fmhc_k1_bwd_q8", grad_out.data_ptr(), x_codes.data_ptr(), x_scales.data_ptr(),
-                     fmt, W.data_ptr(), proj_out.data_ptr(), inv_rms.data_ptr(), grad_x.data_ptr(),
-                     grad_W.data_ptr(), ws.data_ptr(), ws_bytes, T, n, C, _stream(grad_out))
+    grad_x, grad_W = grad_out.new_empty((T, n, C)), grad_out.new_empty((32, n * C))
+    ws, ws_bytes, _keep = _workspace(grad_out, "fmhc_k1_bwd_q8_workspace_size", T, C)
+    _launch(grad_out, "fmhc_k1_bwd_q8", grad_out.data_ptr(), x_codes.data_ptr(),
+            x_scales.data_ptr(), fmt, W.data_ptr(), proj_out.data_ptr(), inv_rms.data_ptr(),
+            grad_x.data_ptr(), grad_W.data_ptr(), ws, ws_bytes, T, n, C)
     return grad_x, grad_W
 
 

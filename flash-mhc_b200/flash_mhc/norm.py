@@ -19,9 +19,9 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import _native
-from .act8 import _DTYPES, _act, _checkpoint, _format, _new_checkpoint, _rows, _same_device, _shape
-from .ops import _lib, _on_device, _stream
+from .act8 import (_DTYPES, _act, _checkpoint, _format, _launch, _new_checkpoint, _rows,
+                   _same_device, _shape, _workspace)
+from .ops import _lib
 
 _lib.define(
     "layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor y, Tensor mean, Tensor rstd)"
@@ -69,16 +69,15 @@ def _forward(op: str, x, weight, bias, eps: float, format=None):
     _same_device(op, x, weight=weight, bias=bias)
     weight, bias, pdt = _params(op, x.shape[-1], weight, bias)
     y = torch.empty_like(x)
-    mean = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
     fmt, codes, scales = -1, None, None
     if format is not None:
         fmt, code_dtype = _format(op, format)
         codes, scales = _new_checkpoint(x, code_dtype)
-    with _on_device(x):
-        _native.call("fmhc_layer_norm_fwd", x.data_ptr(), _DTYPES[x.dtype], _ptr(weight), _ptr(bias),
-                     pdt, eps, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(codes), fmt,
-                     _ptr(scales), _rows(x), x.shape[-1], _stream(x))
+    _launch(x, "fmhc_layer_norm_fwd", x.data_ptr(), _DTYPES[x.dtype], _ptr(weight), _ptr(bias), pdt,
+            eps, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(codes), fmt, _ptr(scales),
+            _rows(x), x.shape[-1])
     return (y, mean, rstd) if format is None else (y, mean, rstd, codes, scales)
 
 
@@ -99,19 +98,16 @@ def _backward(op: str, grad_out, x, codes, scales, mean, rstd, weight, bias):
     C, rows = grad_out.shape[-1], _rows(grad_out)
     weight, bias, pdt = _params(op, C, weight, bias)
     grad_x = torch.empty_like(grad_out)
-    none = lambda: torch.empty(0, device=grad_out.device, dtype=torch.float32)  # noqa: E731
+    none = lambda: grad_out.new_empty((0,), dtype=torch.float32)  # noqa: E731
     grad_w = none() if weight is None else torch.empty_like(weight)
     grad_b = none() if bias is None else torch.empty_like(bias)
-    with _on_device(grad_out):
-        ws, ws_bytes = None, 0
-        if weight is not None or bias is not None:
-            ws_bytes = int(_native.lib().fmhc_layer_norm_bwd_workspace_size(rows, C))
-            ws = torch.empty(max(ws_bytes, 1), device=grad_out.device, dtype=torch.uint8)
-        _native.call("fmhc_layer_norm_bwd", grad_out.data_ptr(), _DTYPES[grad_out.dtype], _ptr(x),
-                     _ptr(codes), fmt, _ptr(scales), mean.data_ptr(), rstd.data_ptr(), _ptr(weight),
-                     pdt, grad_x.data_ptr(), None if weight is None else grad_w.data_ptr(),
-                     None if bias is None else grad_b.data_ptr(), _ptr(ws), ws_bytes, rows, C,
-                     _stream(grad_out))
+    ws, ws_bytes, _keep = None, 0, None
+    if weight is not None or bias is not None:
+        ws, ws_bytes, _keep = _workspace(grad_out, "fmhc_layer_norm_bwd_workspace_size", rows, C)
+    _launch(grad_out, "fmhc_layer_norm_bwd", grad_out.data_ptr(), _DTYPES[grad_out.dtype], _ptr(x),
+            _ptr(codes), fmt, _ptr(scales), mean.data_ptr(), rstd.data_ptr(), _ptr(weight), pdt,
+            grad_x.data_ptr(), None if weight is None else grad_w.data_ptr(),
+            None if bias is None else grad_b.data_ptr(), ws, ws_bytes, rows, C)
     return grad_x, grad_w, grad_b
 
 
