@@ -735,8 +735,8 @@ int fmhc_layer_norm_bwd(const void *grad_y, int x_dtype, const void *x, const vo
       return fail(FMHC_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", w,
                   (long long)workspace_bytes, (long long)need);
   }
-  const bool vec = aligned(grad_y, 16) && aligned(x, 16) && aligned(x_codes, 8) && aligned(weight, 16) &&
-                   aligned(grad_x, 16);
+  const bool vec = aligned(grad_y, 16) && aligned(x, 16) && aligned(x_codes, 8) && aligned(x_scales, 4) &&
+                   aligned(weight, 16) && aligned(grad_x, 16);
   fmhc::launch_ln_bwd(grad_y, x_dtype, x_codes ? x_codes : x, x_codes ? format : -1, x_scales, mean,
                       rstd, weight, param_dtype, grad_x, grad_weight, grad_bias, (float *)workspace,
                       rows, int(C), vec, s);

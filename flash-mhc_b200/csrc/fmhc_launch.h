@@ -102,7 +102,8 @@ void launch_k4_bwd_q8(const void *go, const void *xc, const void *xs, const void
 // layer_norm.cu -- rows of C values of type dtype; w and b (either may be null)
 // of type pdt.  fmt -1: x as it is (codes, scales null); else the forward also
 // writes x in 8 bits and the backward reads codes as its x.  `vec`: every row
-// pointer and w, b 16-byte aligned (codes 8-byte); the width is checked here.
+// pointer and w, b 16-byte aligned (codes 8-byte, scales that are read 4-byte); the
+// width is checked here.
 void launch_ln_fwd(const void *x, int dtype, const void *w, const void *b, int pdt, float eps,
                    void *y, float *mean, float *rstd, void *codes, int fmt, void *scales,
                    int64_t rows, int C, bool vec, cudaStream_t s);

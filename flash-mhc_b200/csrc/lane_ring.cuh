@@ -73,6 +73,10 @@ __device__ __forceinline__ void copy_async_at(uint32_t dst, const void *src) {
   else
     asm volatile("cp.async.ca.shared.global [%0 + %2], [%1], 8;" ::"r"(dst), "l"(src), "n"(OFF) : "memory");
 }
+// Four bytes, or the first `valid` of them and zeros.
+__device__ __forceinline__ void copy_async4(uint32_t dst, const void *src, int valid = 4) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+}
 // Shared-memory loads at an address plus a constant.
 template <int OFF>
 __device__ __forceinline__ uint4 load_shared16(uint32_t a) {
@@ -87,6 +91,16 @@ template <int OFF>
 __device__ __forceinline__ uint2 load_shared8(uint32_t a) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2 + %3];" : "=r"(v.x), "=r"(v.y) : "r"(a), "n"(OFF) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t load_shared_u8(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 load_shared_f32x2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }

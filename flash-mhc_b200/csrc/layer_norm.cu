@@ -291,6 +291,10 @@ template <class E, int FMT> struct Input;
 template <class E> struct Input<E, kNone> { using X = typename Elem<E>::Raw; };
 template <class E> struct Input<E, kInt8> { using X = uint2; };
 template <class E> struct Input<E, kE4m3> { using X = uint2; };
+// mean and rstd, and NV * 2 + 1 words of scale bytes, to a multiple of 16.
+template <int NV, int FMT>
+constexpr int kRowBytes = FMT == kNone ? 16 : (8 + (NV * 2 + 1) * 4 + 15) / 16 * 16;
+
 // xh of a chunk, from x (e unused) or from codes with scale byte e; off is
 // -mean.  The difference comes first and is rounded once (a code times its
 // scale is exact), so that values near the mean keep their relative precision.
@@ -336,8 +340,10 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
   const uint32_t ring_g = shared_addr(dyn) + warp * (S * NV * kChunkG) + lane * int(sizeof(Raw));
   const uint32_t ring_x = shared_addr(dyn) + warps * (S * NV * kChunkG) + warp * (S * NV * kChunkX) +
                           lane * int(sizeof(X));
-  float4 *ws = reinterpret_cast<float4 *>(
-      reinterpret_cast<X *>(reinterpret_cast<Raw *>(dyn) + warps * (S * NV * 32)) + warps * (S * NV * 32));
+  // Per warp and row: mean and rstd, then the words that hold the scale bytes.
+  const uint32_t ring_r = shared_addr(dyn) + warps * (S * NV * (kChunkG + kChunkX)) + warp * (S * kRowBytes<NV, FMT>);
+  float4 *ws = reinterpret_cast<float4 *>(reinterpret_cast<char *>(dyn) + warps * (S * NV * (kChunkG + kChunkX)) +
+                                          warps * (S * kRowBytes<NV, FMT>));
   const int64_t step = int64_t(gridDim.x) * teams;
   int64_t r = int64_t(blockIdx.x) * teams + warp / team;
   pdl_wait();
@@ -349,9 +355,19 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
   const E *x_src = FMT == kNone ? reinterpret_cast<const E *>(x) + r * C + c0 * 8 : nullptr;
   const uint8_t *q_src = FMT == kNone ? nullptr : reinterpret_cast<const uint8_t *>(x) + r * C + c0 * 8;
   E *dst = gx + r * C + c0 * 8;
+  // Scale bytes of the warp's columns: from s_src on, wherever that lies in a word;
+  // the words are copied (the last one up to the tensor's end).
+  const uint8_t *s_src = FMT == kNone ? nullptr : scales + r * nb + wt * NV * 8;
+  const uint8_t *const s_end = FMT == kNone ? nullptr : scales + rows * nb;
   int64_t fetched = r;
   const auto fetch = [&](int stage) {
     if (fetched < rows) {
+      const uint32_t to_r = ring_r + stage * kRowBytes<NV, FMT>;
+      if (lane >= 30) copy_async4(to_r + (lane - 30) * 4, (lane == 30 ? mean : rstd) + fetched);
+      if constexpr (FMT != kNone) {
+        const uint8_t *word = s_src - (reinterpret_cast<uintptr_t>(s_src) & 3) + 4 * lane;
+        if (lane <= NV * 2 && word < s_end) copy_async4(to_r + 8 + lane * 4, word, int(min(s_end - word, int64_t(4))));
+      }
       const uint32_t to_g = ring_g + stage * (NV * kChunkG), to_x = ring_x + stage * (NV * kChunkX);
       unrolled<NV>([&](auto i) {
         if (i * 32 < left) {
@@ -362,6 +378,7 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
       });
     }
     fetched += step;
+    if constexpr (FMT != kNone) s_src += step * nb;
     g_src += hop;
     if constexpr (FMT == kNone) x_src += hop;
     else q_src += hop;
@@ -387,34 +404,22 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int k = 0; k < 4; ++k) dw[i][k] = db[i][k] = both(0.f);
-  // mean, rstd and the scale bytes of a row are loaded one row ahead.
-  float next_m = 0.f, next_rs = 0.f;
-  uint32_t next_e[NV], e[NV];
-  const uint8_t *s_src = FMT == kNone ? nullptr : scales + r * nb + (c0 >> 2);
-  const auto ahead = [&](int64_t row) {
-    if (row < rows) {
-      next_m = __ldg(mean + row);
-      next_rs = __ldg(rstd + row);
-      if constexpr (FMT != kNone) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (i * 32 < left) next_e[i] = __ldg(s_src + i * 8);
-        s_src += step * nb;
-      }
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < NV; ++i) next_e[i] = 0;
-  ahead(r);
+  // Where this lane's scale byte of chunk 0 lies from its row's first word on:
+  // s_src moves with the fetches, so the misalignment is followed separately.
+  uint32_t s_off = FMT == kNone ? 0u : uint32_t(reinterpret_cast<uintptr_t>(scales + r * nb) & 3);
   int par = 0, stage = 0;
   for (; r < rows; r += step, par ^= 1) {
-    const float rs = next_rs;
-    const float2 off = both(-next_m);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) e[i] = next_e[i];
     fetch(stage == 0 ? S - 1 : stage - 1);
-    ahead(r + step);
     copy_wait<S - 1>();
+    __syncwarp();  // mean, rstd and scale bytes were copied by other lanes
+    const uint32_t from_r = ring_r + stage * kRowBytes<NV, FMT>;
+    const float2 stats = load_shared_f32x2(from_r);
+    const float rs = stats.y;
+    const float2 off = both(-stats.x);
+    uint32_t e[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) e[i] = FMT == kNone ? 0u : load_shared_u8(from_r + 8 + s_off + (lane >> 2) + i * 8);
+    s_off = (s_off + uint32_t(step * nb)) & 3u;
     float2 s1 = both(0.f), s2 = both(0.f);
     const uint32_t from_g = ring_g + stage * (NV * kChunkG), from_x = ring_x + stage * (NV * kChunkX);
     unrolled<NV>([&](auto i) {
@@ -744,7 +749,8 @@ void launch_ln_bwd(const void *g, int dtype, const void *x, int fmt, const void 
     FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, FMHC_DISPATCH_NV(p.nv, kMaxNV<E>, {
       auto k = ln_bwd_kernel<E, NV, FMT>;
       const size_t ring = size_t(p.threads) * kStages * NV *
-                          (sizeof(typename Elem<E>::Raw) + sizeof(typename Input<E, FMT>::X));
+                          (sizeof(typename Elem<E>::Raw) + sizeof(typename Input<E, FMT>::X)) +
+                          size_t(p.threads / 32) * kStages * kRowBytes<NV, FMT>;
       // The ring's memory later holds the 64 NV bytes of sums of every thread.
       static_assert(kStages * (sizeof(typename Elem<E>::Raw) + sizeof(typename Input<E, FMT>::X)) >= 64,
                     "sums fit the ring");
