@@ -345,11 +345,13 @@ def _fused_rmsnorm_project_backward_q8_cuda(grad_out, x_codes, x_scales, W, proj
 
 
 def quantize(x: torch.Tensor, format: str = "int8") -> tuple[torch.Tensor, torch.Tensor]:
-    """``x`` in 8 bits: (codes, scales).  CUDA tensors of float32, bfloat16 or float16."""
-    return torch.ops.flash_mhc.act_quantize(x, format)
+    """``x`` in 8 bits: (codes, scales).  CUDA tensors of float32, bfloat16 or float16.
+
+    Takes no part in autograd, whether or not ``x`` requires a gradient."""
+    return torch.ops.flash_mhc.act_quantize(x.detach(), format)
 
 
 def dequantize(codes: torch.Tensor, scales: torch.Tensor,
                dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that (codes, scales) stand for, rounded once to ``dtype``."""
-    return torch.ops.flash_mhc.act_dequantize(codes, scales, dtype)
+    return torch.ops.flash_mhc.act_dequantize(codes.detach(), scales, dtype)

@@ -39,6 +39,7 @@ from itertools import permutations
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 from torch.utils.checkpoint import checkpoint as _checkpoint
 
 from . import ops as _ops  # noqa: F401  (registers torch.ops.flash_mhc.*)
@@ -146,6 +147,7 @@ class _FusedPreMapQ8(torch.autograd.Function):
         return layer_input, H, h_post, xc, xs
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g_li, g_H, g_hpost, _g_xc, _g_xs):
         ops = torch.ops.flash_mhc
         xc, xs, W, proj, inv, h_pre, a_pre, a_post, a_res, bias, perm = ctx.saved_tensors
@@ -179,6 +181,7 @@ class _FusedPostResQ8(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g_out):
         xc, xs, lc, ls, H, hp = ctx.saved_tensors
         g_out = g_out.contiguous()

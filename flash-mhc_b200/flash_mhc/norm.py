@@ -9,8 +9,14 @@
   module (parameters and state_dict of ``torch.nn.LayerNorm``).
 
 The rows are the last dimension; x is float32, bfloat16 or float16, weight and
-bias (either may be missing) any of these, of one type.  ``mean`` and ``rstd``
-are not differentiable outputs.
+bias (either may be missing) any of these, of one type; y has x's type, under
+autocast too.  ``mean`` and ``rstd`` are not differentiable outputs, and the
+gradients have no derivative of their own (asking for one raises).
+
+From an 8-bit input the backward sees x with a rounding error (int8: up to 2^-7
+of the block's largest value, e4m3: 2^-4 of each value), which it divides by the
+row's spread: rows whose mean is much larger than their spread want x kept as it
+is.
 """
 
 from __future__ import annotations
@@ -179,10 +185,28 @@ def _setup_q8(ctx, inputs, output):
     ctx.set_materialize_grads(False)  # no zeros in the size of the codes
 
 
+class _GradsOnce(torch.autograd.Function):
+    """The gradients where a graph of them is asked for: they have no derivative here, and say so.
+
+    ``mark`` requires a gradient, so that the result does, whatever the arguments do
+    (codes never do, although they depend on x)."""
+
+    @staticmethod
+    def forward(ctx, mark, op, *args):
+        return op(*args)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("flash_mhc::layer_norm has no second derivative")
+
+
 def _grads(ctx, gy, op):
     if gy is None:
         return None, None, None
-    gx, gw, gb = op(gy, *ctx.saved_tensors)
+    if torch.is_grad_enabled():  # create_graph=True
+        gx, gw, gb = _GradsOnce.apply(gy.new_empty(0).requires_grad_(), op, gy, *ctx.saved_tensors)
+    else:
+        gx, gw, gb = op(gy, *ctx.saved_tensors)
     need = ctx.needs_input_grad
     return gx if need[0] else None, gw if need[1] else None, gb if need[2] else None
 

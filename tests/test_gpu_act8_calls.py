@@ -1,0 +1,222 @@
+"""Calls of the 8-bit and layer-norm ops at the edges of what they allow: second derivatives,
+offsets past 32 bits, the widest rows, views at odd addresses, captured graphs."""
+
+import pytest
+import torch
+import torch.nn as nn
+
+import flash_mhc  # noqa: F401
+from flash_mhc import act8, norm
+from flash_mhc.block import MHCLiteBlock
+
+pytestmark = pytest.mark.gpu
+
+ops = torch.ops.flash_mhc
+BF = torch.bfloat16
+
+
+def _randn(*shape, dtype=BF):
+    return torch.randn(*shape, device="cuda", dtype=dtype)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_quantising_takes_no_part_in_autograd(fmt):
+    x = _randn(4, 64).requires_grad_()
+    c, s = act8.quantize(x, fmt)
+    assert not c.requires_grad and not s.requires_grad and not act8.dequantize(c, s).requires_grad
+    want = act8.quantize(x.detach(), fmt)
+    assert torch.equal(c.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(s, want[1])
+
+
+@pytest.mark.parametrize("fmt", [None, "int8"])
+def test_second_derivatives_of_the_norm_are_refused(fmt):
+    x, w = _randn(4, 64).requires_grad_(), _randn(64).requires_grad_()
+    y = norm.layer_norm(x, w, None, checkpoint_format=fmt)
+    g = _randn(4, 64)
+    first = torch.autograd.grad(y, (x, w), g, create_graph=True)
+    plain = torch.autograd.grad(norm.layer_norm(x, w, None, checkpoint_format=fmt), (x, w), g)
+    assert all(torch.equal(a, b) for a, b in zip(first, plain))
+    with pytest.raises(RuntimeError, match="second derivative"):
+        first[0].float().pow(2).sum().backward()
+    # alone with a frozen weight and a linear loss, too
+    y = norm.layer_norm(x, None, None, checkpoint_format=fmt)
+    first, = torch.autograd.grad(y, x, g, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        first.float().pow(2).sum().backward()
+
+
+def test_second_derivatives_of_the_block_are_refused():
+    b = MHCLiteBlock(4, 64, nn.Linear(64, 64), checkpoint_format="int8").cuda().to(BF)
+    x = _randn(5, 4, 64).requires_grad_()
+    g, = torch.autograd.grad(b(x).float().pow(2).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.float().pow(2).sum().backward()
+
+
+# ------------------------------------------------------ offsets past 32 bits
+# Every token's or row's result has the same bits wherever it stands, so the last ones of a long
+# tensor are compared with a short call's.
+C = 1024
+T = (1 << 31) // (4 * C) + 37  # 4 T C values: the last ones lie past 2^31
+LAST = 70
+
+
+def test_long_tensors_quantise_and_restore():
+    x = _randn(4 * T, C)
+    c, s = act8.quantize(x)
+    wc, ws = act8.quantize(x[-LAST:])
+    assert torch.equal(c[-LAST:], wc) and torch.equal(s[-LAST:], ws)
+    assert torch.equal(act8.dequantize(c, s)[-LAST:], act8.dequantize(wc, ws))
+
+
+def test_long_tensors_mixings():
+    x, lo = _randn(T, 4, C), _randn(T, C)
+    h, H = torch.rand(T, 4, device="cuda"), torch.rand(T, 4, 4, device="cuda")
+    out, xc, xs = ops.fused_pre_map_q8(x, h, "int8")
+    want = ops.fused_pre_map_q8(x[-LAST:], h[-LAST:], "int8")
+    assert all(torch.equal(a[-LAST:], b) for a, b in zip((out, xc, xs), want))
+    out, lc, ls = ops.fused_post_res_q8(x, lo, H, h, "int8")
+    want = ops.fused_post_res_q8(x[-LAST:], lo[-LAST:], H[-LAST:], h[-LAST:], "int8")
+    assert all(torch.equal(a[-LAST:], b) for a, b in zip((out, lc, ls), want))
+    got = ops.post_res_grad_params_q8(out, xc, xs, lc, ls, h)
+    want = ops.post_res_grad_params_q8(*(t[-LAST:] for t in (out, xc, xs, lc, ls, h)))
+    assert all(torch.equal(a[-LAST:], b) for a, b in zip(got, want))
+    assert torch.equal(ops.pre_map_grad_h_q8(lo, xc, xs)[-LAST:],
+                       ops.pre_map_grad_h_q8(*(t[-LAST:] for t in (lo, xc, xs))))
+
+
+def test_long_tensors_projection_backward():
+    xc = torch.randint(-127, 128, (T, 4, C), device="cuda", dtype=torch.int8)
+    xs = torch.full((T, 4, C // 32), 120, device="cuda", dtype=torch.uint8)
+    W, proj, inv = _randn(32, 4 * C), _randn(T, 32), torch.rand(T, device="cuda") + 0.5
+    go = torch.zeros(T, 32, device="cuda", dtype=BF)
+    go[-LAST:] = _randn(LAST, 32)
+    gx, gW = ops.fused_rmsnorm_project_backward_q8(go, xc, xs, W, proj, inv)
+    wx, wW = ops.fused_rmsnorm_project_backward_q8(*(t[-LAST:] for t in (go, xc, xs)), W, proj[-LAST:], inv[-LAST:])
+    assert torch.equal(gx[-LAST:], wx) and not gx[:-LAST].any()
+    # grad_W: zero but for the last tokens' products, which are added in f32 in two groupings (70
+    # products each: 2 x 70 x 2^-24 of the sum of magnitudes) and rounded to bf16 (2^-8 apart at most)
+    x = act8.dequantize(xc[-LAST:], xs[-LAST:], torch.float32).view(LAST, 4 * C).double()
+    g = (go[-LAST:].float() * inv[-LAST:, None]).to(BF).double()
+    lim = wW.double().abs() * 2**-8 + g.abs().t() @ x.abs() * (140 * 2.0**-24)
+    assert ((gW.double() - wW.double()).abs() <= lim).all()
+
+
+@pytest.mark.parametrize("fmt", [None, "e4m3"])
+def test_long_tensors_norm(fmt):
+    rows = 4 * T
+    x, w, b = _randn(rows, C), _randn(C), _randn(C)
+    fwd = ops.layer_norm(x, w, b, 1e-5) if fmt is None else ops.layer_norm_q8(x, w, b, 1e-5, fmt)
+    want = ops.layer_norm(x[-LAST:], w, b, 1e-5) if fmt is None else ops.layer_norm_q8(x[-LAST:], w, b, 1e-5, fmt)
+    for a, r in zip(fwd, want):
+        assert torch.equal(a[-LAST:].view(torch.uint8), r.view(torch.uint8))
+    g = torch.zeros_like(x)
+    g[-1] = _randn(C)  # one row: the parameters' gradients are its alone
+    kept = (x,) if fmt is None else fwd[3:]
+    bwd = ops.layer_norm_backward if fmt is None else ops.layer_norm_backward_q8
+    got = bwd(g, *kept, fwd[1], fwd[2], w, b)
+    ref = bwd(g[-LAST:], *(t[-LAST:] for t in kept), fwd[1][-LAST:], fwd[2][-LAST:], w, b)
+    assert torch.equal(got[0][-LAST:], ref[0]) and torch.equal(got[1], ref[1]) and torch.equal(got[2], ref[2])
+
+
+# ------------------------------------------------------------- wide rows, views
+
+
+@pytest.mark.parametrize("rows,width", [(3, 16376), (5, 16384), (3, 16392), (2, 16384 * 4)])
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_norm_of_the_widest_rows(rows, width, dtype):
+    """Against 64 bits: y and the gradients within a rounding of the type and f32 sums of `width` values."""
+    x, g, w, b = _randn(rows, width, dtype=dtype), _randn(rows, width, dtype=dtype), _randn(width), _randn(width)
+    y, mean, rstd = ops.layer_norm(x, w, b, 1e-5)
+    X, G, W = x.double(), g.double(), w.double()
+    xh = (X - X.mean(-1, keepdim=True)) * (X.var(-1, unbiased=False, keepdim=True) + 1e-5).rsqrt()
+    # A lane adds width / 1024 values or fewer, then ten levels: at most 100 roundings to 2^-24 in a
+    # sum here, so statistics and sums are right to 1e-5 of their terms' magnitude (about 1 each).
+    step = torch.finfo(dtype).eps / 2
+    lim = lambda want, scale: step * want.abs() + 1e-5 * (1 + scale)  # noqa: E731
+    Y = xh * W + b.double()
+    assert ((y.double() - Y).abs() <= lim(Y, xh.abs() * W.abs())).all()
+    gx, gw, gb = ops.layer_norm_backward(g, x, mean, rstd, w, b)
+    gW = G * W
+    GX = (gW - gW.mean(-1, keepdim=True) - xh * (gW * xh).mean(-1, keepdim=True)) * rstd.double()[:, None]
+    assert ((gx.double() - GX).abs() <= lim(GX, gW.abs() + xh.abs())).all()
+    for got, want, mag in ((gw, (G * xh).sum(0), (G * xh).abs().sum(0)), (gb, G.sum(0), G.abs().sum(0))):
+        assert ((got.double() - want).abs() <= want.abs() * 2**-8 + 1e-5 * (1 + mag)).all()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_checkpoints_at_odd_addresses(fmt):
+    """Codes and scales that are views at every odd offset give the bits of aligned ones, or, where a
+    kernel for any alignment adds in another order, the same sums to f32 rounding."""
+    rows, width = 40, 264
+    x, g, w = _randn(rows, width), _randn(rows, width), _randn(width)
+    y, mean, rstd, c, s = ops.layer_norm_q8(x, w, w, 1e-5, fmt)
+    want = ops.layer_norm_backward_q8(g, c, s, mean, rstd, w, w)
+    for off in (1, 2, 3, 4, 8):
+        move = lambda t: torch.cat([t.view(torch.uint8).flatten().new_zeros(off), t.view(torch.uint8).flatten()])[  # noqa: E731
+            off:].view(t.dtype).view(t.shape)
+        for args in ((move(c), s), (c, move(s)), (move(c), move(s))):
+            assert torch.equal(act8.dequantize(*args), act8.dequantize(c, s))
+            got = ops.layer_norm_backward_q8(g, *args, mean, rstd, w, w)
+            # bf16 results of f32 sums: one step apart at most, near zero 1e-4
+            for a, b in zip(got, want):
+                assert ((a.double() - b.double()).abs() <= b.double().abs() * 2**-7 + 1e-4).all()
+
+
+# ------------------------------------------------------------------- graphs
+
+
+def test_two_graphs_replayed_in_turn():
+    """Two captured training steps of a norm (own workspaces), replayed in turn on new inputs."""
+    shapes = [(300, 512), (70, 1000)]
+    steps = []
+    for rows, width in shapes:
+        m = norm.LayerNorm(width, checkpoint_format="int8", device="cuda", dtype=BF)
+        x, g = _randn(rows, width).requires_grad_(), _randn(rows, width)
+
+        def step(m=m, x=x, g=g):
+            return torch.autograd.grad(m(x), (x, m.weight, m.bias), g)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        steps.append((step, x, g, graph, out))
+    for turn in range(3):
+        for step, x, g, graph, out in steps:
+            with torch.no_grad():
+                x.copy_(_randn(*x.shape))
+                g.copy_(_randn(*g.shape))
+            graph.replay()
+        for step, x, g, graph, out in steps:
+            assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+def test_quantising_in_a_graph():
+    x = _randn(50, 4, 264)
+    act8.dequantize(*act8.quantize(x, "e4m3"))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c, s = act8.quantize(x, "e4m3")
+        r = act8.dequantize(c, s)
+    for _ in range(2):
+        x.copy_(_randn(*x.shape) * 100)
+        graph.replay()
+        assert torch.equal(r, act8.dequantize(*act8.quantize(x, "e4m3")))
+
+
+def test_under_torch_compile():
+    for fmt in (None, "int8"):
+        m = norm.LayerNorm(64, device="cuda", checkpoint_format=fmt)
+        f = torch.compile(lambda v: m(v * 2).sin(), backend="aot_eager", fullgraph=True)  # noqa: B023
+        a, b = (_randn(4, 64, dtype=torch.float32) for _ in range(2))
+        for x in (a, b):
+            xe, xc = x.clone().requires_grad_(), x.clone().requires_grad_()
+            ye, yc = m(xe * 2).sin(), f(xc)
+            ye.sum().backward()
+            yc.sum().backward()
+            assert torch.equal(ye, yc) and torch.equal(xe.grad, xc.grad)
