@@ -36,11 +36,10 @@ using namespace act8;
 namespace {
 
 constexpr int kMaxTeam = 16;          // warps per row
-// Warps per block (one block per SM) and most chunks of eight values per lane.
-#ifndef FMHC_LN_FWD_WARPS
-#define FMHC_LN_FWD_WARPS 24
-#endif
-constexpr int kFwdWarps = FMHC_LN_FWD_WARPS;
+// Warps per block, one block per SM.  Forward (65536 x 2048 / 16384 x 8192 bf16,
+// 16384 x 4096 f16 with e4m3 codes, us): 24 90 / 99 / 65, 16 93 / 113 / 70, 20
+// 92 / 121 / 67, 28 91 / 99 / 73.  Backward: 16, for 128 registers a thread.
+constexpr int kFwdWarps = 24;
 constexpr int kBwdWarps = 16;
 constexpr int kThreads = 256;         // of the kernels for any width
 constexpr int kWarps = kThreads / 32;
@@ -74,6 +73,13 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// Sum of the values of `team` lanes (a power of two), of which every group of
+// that many lanes has a copy.
+__device__ __forceinline__ float group_sum(float v, int team) {
+  for (int o = team >> 1; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
 // Adds a pair over the `team` warps of a row.  `slot` holds one float2 per warp
 // of the block, one array for even and one for odd rows of a team, so one
 // barrier per row is enough: a warp writes a slot again two rows later, after
@@ -84,8 +90,8 @@ __device__ __forceinline__ float2 team_sum(float2 v, float2 *slot, int team, int
   if (team == 1) return v;
   if (lane == 0) slot[warp] = v;
   named_bar_sync(1 + warp / team, team * 32);
-  const float2 o = lane < team ? slot[warp / team * team + lane] : make_float2(0.f, 0.f);
-  return make_float2(warp_sum(o.x), warp_sum(o.y));
+  const float2 o = slot[warp / team * team + (lane & (team - 1))];
+  return make_float2(group_sum(o.x, team), group_sum(o.y, team));
 }
 
 // Pairs of a chunk's eight values.
@@ -172,8 +178,8 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
   const auto count = [&](int i) { return min(max(nchunk - i * NV * 32, 0), NV * 32) * 8; };
   const int c0 = wt * NV * 32 + lane, left = nchunk - c0;
   const int mine = count(wt);
-  // Lane i joins for warp i of the team.
-  const float n_lane = lane < team ? float(count(lane)) : 0.f, inv_n = n_lane > 0.f ? 1.f / n_lane : 0.f;
+  // Lane i joins for warp i of the team, as does every lane `team` on.
+  const float n_lane = float(count(lane & (team - 1))), inv_n = n_lane > 0.f ? 1.f / n_lane : 0.f;
   const float inv_mine = mine ? 1.f / float(mine) : 0.f, inv_C = 1.f / float(C);
   const int64_t step = int64_t(gridDim.x) * teams;
   int64_t r = int64_t(blockIdx.x) * teams + warp / team;
@@ -249,10 +255,10 @@ ln_fwd_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *_
       float2 *slot = slots[par] + first;
       if (lane == 0) slot[wt] = make_float2(s, q);
       named_bar_sync(1 + warp / team, team * 32);
-      const float2 o = lane < team ? slot[lane] : make_float2(0.f, 0.f);
-      mean = __fmul_rn(warp_sum(o.x), inv_C);
+      const float2 o = slot[lane & (team - 1)];
+      mean = __fmul_rn(group_sum(o.x, team), inv_C);
       const float d = n_lane > 0.f ? fmaf(o.x, inv_n, -mean) : 0.f;
-      m2 = warp_sum(fmaf(n_lane * d, d, o.y));
+      m2 = group_sum(fmaf(n_lane * d, d, o.y), team);
     }
     const float rstd = rsqrtf(fmaf(m2, inv_C, eps));
     if (wt == 0 && lane == 0) {
@@ -295,22 +301,22 @@ template <class E> struct Input<E, kE4m3> { using X = uint2; };
 template <int NV, int FMT>
 constexpr int kRowBytes = FMT == kNone ? 16 : (8 + (NV * 2 + 1) * 4 + 15) / 16 * 16;
 
-// xh of a chunk, from x (e unused) or from codes with scale byte e; off is
-// -mean.  The difference comes first and is rounded once (a code times its
-// scale is exact), so that values near the mean keep their relative precision.
+// x - mean of a chunk, from x (e unused) or from codes with scale byte e; off is
+// -mean.  Rounded once (a code times its scale is exact), so that values near
+// the mean keep their relative precision.
 template <class E, int FMT>
-__device__ __forceinline__ void normalised(const typename Input<E, FMT>::X &raw, uint32_t e, float rstd,
-                                           float2 off, float2 (&xh)[4]) {
+__device__ __forceinline__ void centred(const typename Input<E, FMT>::X &raw, uint32_t e, float2 off,
+                                        float2 (&d)[4]) {
   if constexpr (FMT == kNone) {
-    widen2<E>(raw, xh);
+    widen2<E>(raw, d);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) xh[i] = mul2(add2(xh[i], off), both(rstd));
+    for (int i = 0; i < 4; ++i) d[i] = add2(d[i], off);
   } else {
-    decode4x2<FMT>(raw.x, xh[0], xh[1]);
-    decode4x2<FMT>(raw.y, xh[2], xh[3]);
+    decode4x2<FMT>(raw.x, d[0], d[1]);
+    decode4x2<FMT>(raw.y, d[2], d[3]);
     const float2 s = both(scale_value(e));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) xh[i] = mul2(fma2(xh[i], s, off), both(rstd));
+    for (int i = 0; i < 4; ++i) d[i] = fma2(d[i], s, off);
   }
 }
 
@@ -318,11 +324,11 @@ __device__ __forceinline__ void normalised(const typename Input<E, FMT>::X &raw,
 // whose weight does not fit there, from global memory) twice per row; holding
 // them too would pass 128 registers.  For the same reason the second pass reads
 // g and x from the ring again.
-template <class E, int NV, int FMT>
+template <class E, int NV, int FMT, bool W_SHARED>
 __global__ void __launch_bounds__(32 * kBwdWarps, 1)
 ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
               const uint8_t *__restrict__ scales, const float *__restrict__ mean,
-              const float *__restrict__ rstd, const void *__restrict__ w, int pdt, bool w_shared,
+              const float *__restrict__ rstd, const void *__restrict__ w, int pdt,
               E *__restrict__ gx, float *__restrict__ part, int64_t rows, int C, int team) {
   using Raw = typename Elem<E>::Raw;
   using X = typename Input<E, FMT>::X;
@@ -386,13 +392,13 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
   };
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) fetch(s);
-  if (w_shared) {
+  if constexpr (W_SHARED) {
     keep_param(ws, w, pdt, 1.f, nchunk);
     __syncthreads();
   }
   const uint32_t w_lo = shared_addr(ws + c0), w_hi = shared_addr(ws + nchunk + c0);
   const auto weight = [&](auto i, float2 (&f)[4]) {
-    if (w_shared) kept_param<i>(w_lo, w_hi, f);
+    if constexpr (W_SHARED) kept_param<i>(w_lo, w_hi, f);
     else param8x2(w, pdt, c0 + i * 32, 1.f, f);
   };
   const auto load_x = [&](auto i, uint32_t from) -> X {
@@ -424,33 +430,33 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
     const uint32_t from_g = ring_g + stage * (NV * kChunkG), from_x = ring_x + stage * (NV * kChunkX);
     unrolled<NV>([&](auto i) {
       if (i * 32 < left) {
-        float2 fg[4], xh[4], fw[4];
-        normalised<E, FMT>(load_x(i, from_x), e[i], rs, off, xh);
+        float2 fg[4], d[4], fw[4];
+        centred<E, FMT>(load_x(i, from_x), e[i], off, d);
         widen2<E>(load_raw<E, i * kChunkG>(from_g), fg);
         weight(i, fw);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float2 gw = mul2(fg[k], fw[k]);
-          dw[i][k] = fma2(fg[k], xh[k], dw[i][k]);
+          const float2 gw = mul2(fg[k], fw[k]), xh = mul2(d[k], both(rs));
+          dw[i][k] = fma2(fg[k], xh, dw[i][k]);
           db[i][k] = add2(db[i][k], fg[k]);
           s1 = add2(s1, gw);
-          s2 = fma2(gw, xh[k], s2);
+          s2 = fma2(gw, xh, s2);
         }
       }
     });
     const float2 sum = team_sum(make_float2(warp_sum(s1.x + s1.y), warp_sum(s2.x + s2.y)), slots[par],
                                 team, warp, lane);
-    const float2 c1 = both(-sum.x * inv_C), c2 = both(-sum.y * inv_C);
+    const float2 c1 = both(-sum.x * inv_C), c2 = both(-sum.y * inv_C * rs);  // c2 times x - mean
     unrolled<NV>([&](auto i) {
       if (i * 32 < left) {
-        float2 fg[4], xh[4], fw[4];
-        normalised<E, FMT>(load_x(i, from_x), e[i], rs, off, xh);
+        float2 fg[4], d[4], fw[4];
+        centred<E, FMT>(load_x(i, from_x), e[i], off, d);
         widen2<E>(load_raw<E, i * kChunkG>(from_g), fg);
         weight(i, fw);
         float o[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float2 v = mul2(both(rs), fma2(fg[k], fw[k], fma2(xh[k], c2, c1)));
+          const float2 v = mul2(both(rs), fma2(fg[k], fw[k], fma2(d[k], c2, c1)));
           o[2 * k] = v.x;
           o[2 * k + 1] = v.y;
         }
@@ -747,20 +753,26 @@ void launch_ln_bwd(const void *g, int dtype, const void *x, int fmt, const void 
     nv = p.nv;
     len = p.sums();
     FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, FMHC_DISPATCH_NV(p.nv, kMaxNV<E>, {
-      auto k = ln_bwd_kernel<E, NV, FMT>;
       const size_t ring = size_t(p.threads) * kStages * NV *
                           (sizeof(typename Elem<E>::Raw) + sizeof(typename Input<E, FMT>::X)) +
                           size_t(p.threads / 32) * kStages * kRowBytes<NV, FMT>;
       // The ring's memory later holds the 64 NV bytes of sums of every thread.
       static_assert(kStages * (sizeof(typename Elem<E>::Raw) + sizeof(typename Input<E, FMT>::X)) >= 64,
                     "sums fit the ring");
-      // The weight goes beside the ring where it fits.
+      // The weight goes beside the ring where it fits: always but for the widest
+      // rows (from 8512 on) whose x is kept as 16-bit values.
       const size_t with_w = ring + size_t(C) * 4;
-      const bool w_shared = w != nullptr && with_w <= kMaxSmem;
-      const size_t smem = w_shared ? with_w : ring;
+      auto k = ln_bwd_kernel<E, NV, FMT, true>;
+      size_t smem = with_w;
+      if constexpr (FMT == kNone && sizeof(E) == 2 && NV == kMaxNV<E>) {
+        if (with_w > kMaxSmem) {
+          k = ln_bwd_kernel<E, NV, FMT, false>;
+          smem = ring;
+        }
+      }
       allow_smem(reinterpret_cast<const void *>(k), smem);
       launch(k, dim3(parts), dim3(p.threads), smem, s, (const E *)g, x, (const uint8_t *)scales, mean,
-             rstd, w, pdt, w_shared, (E *)gx, part, rows, C, p.team);
+             rstd, w, pdt, (E *)gx, part, rows, C, p.team);
     })));
   } else {
     FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, {
