@@ -31,7 +31,8 @@
 // 3 stages instead of 3, 2, 4: 166.  Not faster: codes loaded into registers
 // (241), converter and epilogue in one warp with x kept in registers (171), the
 // same with D1 a unit ahead and grad_x in tiles of its own (193), codes of two
-// chunks at a time (175), a slot loaded half a tile ahead (172).
+// chunks at a time (175), a slot loaded half a tile ahead (172), the epilogue's
+// two halves on alternate units (178: a stage is held longer).
 // Every wait is bounded (sm100_ptx.cuh).
 #pragma once
 
