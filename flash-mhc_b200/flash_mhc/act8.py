@@ -125,8 +125,12 @@ def _launch(t: torch.Tensor, name: str, *args) -> None:
 
 def _workspace(t: torch.Tensor, size_fn: str, *args):
     """(pointer, bytes, tensor) of the scratch that ``size_fn`` asks for on ``t``'s device."""
-    with _on_device(t):
-        n = int(getattr(_native.lib(), size_fn)(*args))
+    size = getattr(_native.lib(), size_fn)
+    if t.device.index == torch._C._cuda_getDevice():
+        n = size(*args)
+    else:
+        with _on_device(t):
+            n = size(*args)
     ws = t.new_empty((max(n, 1),), dtype=torch.uint8)
     return ws.data_ptr(), n, ws
 
