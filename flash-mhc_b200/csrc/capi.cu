@@ -625,8 +625,7 @@ int fmhc_k4_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scal
 int64_t fmhc_k1_bwd_q8_workspace_size(int64_t T, int64_t C) {
   if (T <= 0 || C <= 0 || C > (int64_t(1) << 26)) return 0;
   if (fmhc::k1_tc_bwd_q8_shape(T, 4 * C)) return fmhc::k1_tc_bwd_workspace_bytes(T, 4 * C);
-  // Other widths: x restored to bf16, then the workspace of fmhc_k1_bwd.
-  return ((T * 4 * C * 2 + 255) & ~int64_t(255)) + fmhc_k1_bwd_workspace_size(T, 4 * C, 32);
+  return fmhc::k1_bwd_q8_any_workspace_bytes(T, int(4 * C));
 }
 
 int fmhc_k1_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scales, int format,
@@ -651,19 +650,17 @@ int fmhc_k1_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scal
   if (workspace_bytes < need)
     return fail(FMHC_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", w,
                 (long long)workspace_bytes, (long long)need);
+  FMHC_REQUIRE_ALIGN16(w, grad_out); FMHC_REQUIRE_ALIGN16(w, x_codes); FMHC_REQUIRE_ALIGN16(w, W);
+  FMHC_REQUIRE_ALIGN16(w, proj); FMHC_REQUIRE_ALIGN16(w, grad_x); FMHC_REQUIRE_ALIGN2(w, x_scales);
   if (fmhc::k1_tc_bwd_q8_shape(T, nC)) {
-    FMHC_REQUIRE_ALIGN16(w, grad_out); FMHC_REQUIRE_ALIGN16(w, x_codes); FMHC_REQUIRE_ALIGN16(w, W);
-    FMHC_REQUIRE_ALIGN16(w, proj); FMHC_REQUIRE_ALIGN16(w, grad_x); FMHC_REQUIRE_ALIGN2(w, x_scales);
     if (int e = fmhc::launch_k1_tc_bwd_q8(grad_out, x_codes, x_scales, format, W, proj, inv_rms,
                                           grad_x, grad_W, workspace, T, int(nC), s))
       return fail(e, "%s: %s", w, fmhc::k1_tc_error());
-    return check_launch(w);
+  } else {
+    fmhc::launch_k1_bwd_q8_any(grad_out, x_codes, x_scales, format, W, proj, inv_rms, grad_x,
+                               grad_W, (float *)workspace, T, int(nC), s);
   }
-  const int64_t x_bytes = (T * nC * 2 + 255) & ~int64_t(255);
-  fmhc::launch_act_dequantize(x_codes, format, x_scales, workspace, FMHC_DTYPE_BF16, 4 * T, int(C),
-                              C % 8 == 0 && aligned(x_codes, 8), s);
-  return fmhc_k1_bwd(grad_out, workspace, W, proj, inv_rms, grad_x, grad_W,
-                     (char *)workspace + x_bytes, workspace_bytes - x_bytes, T, nC, 32, stream);
+  return check_launch(w);
 }
 
 // ------------------------------------------------------------------ layer norm
