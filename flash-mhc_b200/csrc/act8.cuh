@@ -132,6 +132,40 @@ __device__ __forceinline__ float decode1(uint8_t c) {
   return f[0];
 }
 
+// Scale byte -> the factor that widen4 takes: 2^(e - 127) as two bf16 or as f32.
+template <int FMT>
+__device__ __forceinline__ uint32_t widen_factor(uint32_t e) {
+  const uint32_t f = __float_as_uint(scale_value(e));
+  return FMT == kInt8 ? __byte_perm(f, 0, 0x3232) : f;
+}
+
+// Four codes -> four bf16 values (exact: at most 7 significant bits).
+template <int FMT>
+__device__ __forceinline__ uint2 widen4(uint32_t w, uint32_t factor) {
+  if constexpr (FMT == kInt8) {
+    // 0x4300 | code is, as bf16, 128 + (code & 127) once bit 7 is cleared, and
+    // 128 or 256 (for a negative code) once bits 0-6 are: the difference is the
+    // code.  Two codes per instruction, exact in bf16.
+    uint32_t o[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t p = __byte_perm(w, 0x43434343u, i ? 0x7372 : 0x7170);
+      const uint32_t hi = p & 0xff7fff7fu, lo = p & 0xff80ff80u;
+      const __nv_bfloat162 v = __hmul2(__hsub2(reinterpret_cast<const __nv_bfloat162 &>(hi),
+                                               reinterpret_cast<const __nv_bfloat162 &>(lo)),
+                                       reinterpret_cast<const __nv_bfloat162 &>(factor));
+      o[i] = reinterpret_cast<const uint32_t &>(v);
+    }
+    return make_uint2(o[0], o[1]);
+  } else {
+    float f[4];
+    decode4<FMT>(w, f);
+    const float2 s = both(__uint_as_float(factor));
+    const float2 a = mul2(make_float2(f[0], f[1]), s), b = mul2(make_float2(f[2], f[3]), s);
+    return make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(b.x, b.y));
+  }
+}
+
 // Eight codes loaded as one access, and widened to scaled f32 values.
 __device__ __forceinline__ uint2 ld_codes8(const uint8_t *p) {
   return __ldcs(reinterpret_cast<const uint2 *>(p));

@@ -651,7 +651,8 @@ int fmhc_k1_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scal
     return fail(FMHC_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", w,
                 (long long)workspace_bytes, (long long)need);
   FMHC_REQUIRE_ALIGN16(w, grad_out); FMHC_REQUIRE_ALIGN16(w, x_codes); FMHC_REQUIRE_ALIGN16(w, W);
-  FMHC_REQUIRE_ALIGN16(w, proj); FMHC_REQUIRE_ALIGN16(w, grad_x); FMHC_REQUIRE_ALIGN2(w, x_scales);
+  FMHC_REQUIRE_ALIGN16(w, proj); FMHC_REQUIRE_ALIGN16(w, grad_x);
+  if (!aligned(x_scales, 4)) return fail(FMHC_ERR_ALIGNMENT, "%s: x_scales must be 4-byte aligned", w);
   if (fmhc::k1_tc_bwd_q8_shape(T, nC)) {
     if (int e = fmhc::launch_k1_tc_bwd_q8(grad_out, x_codes, x_scales, format, W, proj, inv_rms,
                                           grad_x, grad_W, workspace, T, int(nC), s))

@@ -90,40 +90,6 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, site));
 }
 
-// Scale byte -> the factor that widen4 takes: 2^(e - 127) as two bf16 or as f32.
-template <int FMT>
-__device__ __forceinline__ uint32_t widen_factor(uint32_t e) {
-  const uint32_t f = __float_as_uint(act8::scale_value(e));
-  return FMT == act8::kInt8 ? __byte_perm(f, 0, 0x3232) : f;
-}
-
-// Four codes -> four bf16 values (exact: at most 7 significant bits).
-template <int FMT>
-__device__ __forceinline__ uint2 widen4(uint32_t w, uint32_t factor) {
-  if constexpr (FMT == act8::kInt8) {
-    // 0x4300 | code is, as bf16, 128 + (code & 127) once bit 7 is cleared, and
-    // 128 or 256 (for a negative code) once bits 0-6 are: the difference is the
-    // code.  Two codes per instruction, exact in bf16.
-    uint32_t o[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t p = __byte_perm(w, 0x43434343u, i ? 0x7372 : 0x7170);
-      const uint32_t hi = p & 0xff7fff7fu, lo = p & 0xff80ff80u;
-      const __nv_bfloat162 v = __hmul2(__hsub2(reinterpret_cast<const __nv_bfloat162 &>(hi),
-                                               reinterpret_cast<const __nv_bfloat162 &>(lo)),
-                                       reinterpret_cast<const __nv_bfloat162 &>(factor));
-      o[i] = reinterpret_cast<const uint32_t &>(v);
-    }
-    return make_uint2(o[0], o[1]);
-  } else {
-    float f[4];
-    act8::decode4<FMT>(w, f);
-    const float2 s = both(__uint_as_float(factor));
-    const float2 a = mul2(make_float2(f[0], f[1]), s), b = mul2(make_float2(f[2], f[3]), s);
-    return make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(b.x, b.y));
-  }
-}
-
 template <int FMT>
 __global__ void __launch_bounds__(kQ8Threads, 1)
 k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
@@ -449,14 +415,14 @@ k1_bwd_q8_tc_kernel(const __grid_constant__ CUtensorMap tmap_codes,
       uint4 v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4 *>(src + (((4 * h + i) ^ (r & 7)) << 4));
-      const uint32_t f0 = widen_factor<FMT>(sw & 0xffu), f1 = widen_factor<FMT>(sw >> 8);
+      const uint32_t f0 = act8::widen_factor<FMT>(sw & 0xffu), f1 = act8::widen_factor<FMT>(sw >> 8);
       if (!mbar_wait_warp(smem_u32(&sm.empty[stage]), phase ^ 1, abort, kSiteQConvX)) break;
       uint8_t *row = sm.x[stage] + h * kBwdXBox + r * 128;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t f = i < 2 ? f0 : f1;
-        const uint2 a0 = widen4<FMT>(v[i].x, f), a1 = widen4<FMT>(v[i].y, f);
-        const uint2 b0 = widen4<FMT>(v[i].z, f), b1 = widen4<FMT>(v[i].w, f);
+        const uint2 a0 = act8::widen4<FMT>(v[i].x, f), a1 = act8::widen4<FMT>(v[i].y, f);
+        const uint2 b0 = act8::widen4<FMT>(v[i].z, f), b1 = act8::widen4<FMT>(v[i].w, f);
         *reinterpret_cast<uint4 *>(row + (((2 * i) ^ (r & 7)) << 4)) = make_uint4(a0.x, a0.y, a1.x, a1.y);
         *reinterpret_cast<uint4 *>(row + (((2 * i + 1) ^ (r & 7)) << 4)) = make_uint4(b0.x, b0.y, b1.x, b1.y);
       }

@@ -366,7 +366,7 @@ FMHC_API int fmhc_k4_bwd_q8(const void *grad_out, const void *x_codes, const voi
                             int64_t T, int64_t n, int64_t C, void *stream);
 /* fmhc_k1_bwd from a checkpoint of x (T, n, C), D = 32: grad_x (T, n, C) and
  * grad_W (32, nC).  grad_out, x_codes, W, proj and grad_x are 16-byte and
- * x_scales 2-byte aligned (FMHC_ERR_ALIGNMENT otherwise).  `workspace` as
+ * x_scales 4-byte aligned (FMHC_ERR_ALIGNMENT otherwise).  `workspace` as
  * fmhc_k1_bwd's, of at least fmhc_k1_bwd_q8_workspace_size(T, C) bytes. */
 FMHC_API int64_t fmhc_k1_bwd_q8_workspace_size(int64_t T, int64_t C);
 FMHC_API int fmhc_k1_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scales,
