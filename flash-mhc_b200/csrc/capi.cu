@@ -622,9 +622,17 @@ int fmhc_k4_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scal
   return check_launch(w);
 }
 
+// Which kernel: the tcgen05 one for the widths it takes, but for little work, where
+// its set-up and its second launch cost more than they gain (us, tcgen05 / any
+// width: T = 32, C = 4096 14.2 / 6.4; T = 1024, C = 256 7.9 / 6.9; T = 256, C =
+// 1024 8.9 / 8.6; T = 512, C = 1024 9.6 / 11.1; T = 128, C = 4096 13.8 / 17.6).
+static bool k1_bwd_q8_on_tcgen05(int64_t T, int64_t nC) {
+  return fmhc::k1_tc_bwd_q8_shape(T, nC) && T > 32 && T * nC > (int64_t(1) << 20);
+}
+
 int64_t fmhc_k1_bwd_q8_workspace_size(int64_t T, int64_t C) {
   if (T <= 0 || C <= 0 || C > (int64_t(1) << 26)) return 0;
-  if (fmhc::k1_tc_bwd_q8_shape(T, 4 * C)) return fmhc::k1_tc_bwd_workspace_bytes(T, 4 * C);
+  if (k1_bwd_q8_on_tcgen05(T, 4 * C)) return fmhc::k1_tc_bwd_workspace_bytes(T, 4 * C);
   return fmhc::k1_bwd_q8_any_workspace_bytes(T, int(4 * C));
 }
 
@@ -653,7 +661,7 @@ int fmhc_k1_bwd_q8(const void *grad_out, const void *x_codes, const void *x_scal
   FMHC_REQUIRE_ALIGN16(w, grad_out); FMHC_REQUIRE_ALIGN16(w, x_codes); FMHC_REQUIRE_ALIGN16(w, W);
   FMHC_REQUIRE_ALIGN16(w, proj); FMHC_REQUIRE_ALIGN16(w, grad_x);
   if (!aligned(x_scales, 4)) return fail(FMHC_ERR_ALIGNMENT, "%s: x_scales must be 4-byte aligned", w);
-  if (fmhc::k1_tc_bwd_q8_shape(T, nC)) {
+  if (k1_bwd_q8_on_tcgen05(T, nC)) {
     if (int e = fmhc::launch_k1_tc_bwd_q8(grad_out, x_codes, x_scales, format, W, proj, inv_rms,
                                           grad_x, grad_W, workspace, T, int(nC), s))
       return fail(e, "%s: %s", w, fmhc::k1_tc_error());

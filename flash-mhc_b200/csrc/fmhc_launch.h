@@ -98,7 +98,7 @@ void launch_k3_bwd_q8(const void *go, const void *codes, const void *scales, int
 void launch_k4_bwd_q8(const void *go, const void *xc, const void *xs, const void *lc,
                       const void *ls, int fmt, const float *hp, void *glo, float *gH, float *ghp,
                       int64_t T, int C, int vec, cudaStream_t s);
-// C % 32 != 0 (nC = 4 C); the workspace holds partials of grad_W.
+// Any C (nC = 4 C); the workspace holds partials of grad_W.
 int64_t k1_bwd_q8_any_workspace_bytes(int64_t T, int nC);
 void launch_k1_bwd_q8_any(const void *go, const void *codes, const void *scales, int fmt,
                           const void *W, const void *proj, const float *inv_rms, void *gx,

@@ -122,6 +122,28 @@ def test_long_tensors_norm(fmt):
     assert torch.equal(got[0][-LAST:], ref[0]) and torch.equal(got[1], ref[1]) and torch.equal(got[2], ref[2])
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("tokens,width", [(1, 1), (5, 3), (31, 32), (32, 64), (33, 8192), (40, 8192), (129, 4096),
+                                          (1000, 260), (70, 62), (2100, 128), (257, 1023), (9000, 36)])
+def test_projection_backward_at_the_kernels_borders(tokens, width, fmt):
+    """Both kernels of fused_rmsnorm_project_backward_q8 around the sizes where one takes over."""
+    n = 4 * width
+    x, W = _randn(tokens, 4, width), _randn(32, n) * 0.05
+    go, proj, inv = _randn(tokens, 32), _randn(tokens, 32), torch.rand(tokens, device="cuda") + 0.5
+    xc, xs = act8.quantize(x, fmt)
+    gx, gW = ops.fused_rmsnorm_project_backward_q8(go, xc, xs, W, proj, inv)
+    x8 = act8.dequantize(xc, xs, torch.float32).view(tokens, n).double()
+    r, g, p, w = inv.double()[:, None], go.double(), proj.double(), W.double()
+    s = (g * p).sum(1, keepdim=True) * r * r / n
+    want = r * (g @ w) - s * x8
+    # one bf16 rounding, and f32 sums of 32 products with a few more steps
+    mag = r * (g.abs() @ w.abs()) + (g * p).abs().sum(1, keepdim=True) * r * r / n * x8.abs()
+    assert ((gx.view(tokens, n).double() - want).abs() <= want.abs() * 2**-8 + mag * 40 * 2.0**-23 + 1e-30).all()
+    gos = (go.float() * inv[:, None]).to(BF).double()
+    want = gos.t() @ x8
+    assert ((gW.double() - want).abs() <= want.abs() * 2**-8 + (gos.abs().t() @ x8.abs()) * ((tokens + 8) * 2.0**-23) + 1e-30).all()
+
+
 # ------------------------------------------------------------- wide rows, views
 
 
