@@ -97,7 +97,28 @@ dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__
   }
 }
 
-// Any C and any alignment: one warp per block, one value per lane.
+// Any C and any alignment: a warp takes kAnyUnroll neighbouring blocks at a time,
+// one value of each per lane.
+constexpr int kAnyUnroll = 8;
+struct Places {  // this lane's values: where, and whether they exist
+  int64_t at[kAnyUnroll];
+  bool in[kAnyUnroll];
+  __device__ __forceinline__ Places(int64_t b, int64_t blocks, int C, int nb, int lane) {
+    int64_t row = b / nb;
+    int k = int(b - row * nb);
+#pragma unroll
+    for (int u = 0; u < kAnyUnroll; ++u) {
+      const int c = k * kBlock + lane;
+      at[u] = row * C + c;
+      in[u] = b + u < blocks && c < C;
+      if (++k == nb) {
+        k = 0;
+        ++row;
+      }
+    }
+  }
+};
+
 template <class E, int FMT>
 __global__ void __launch_bounds__(kThreads)
 quantize_any_kernel(const E *__restrict__ x, uint8_t *__restrict__ codes,
@@ -106,14 +127,22 @@ quantize_any_kernel(const E *__restrict__ x, uint8_t *__restrict__ codes,
   const int lane = threadIdx.x & 31;
   const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
   const int64_t nwarps = (int64_t(gridDim.x) * kThreads) >> 5;
-  for (int64_t b = warp; b < blocks; b += nwarps) {
-    const int64_t row = b / nb;
-    const int c = int(b - row * nb) * kBlock + lane;
-    const float v = c < C ? Elem<E>::widen1(x[row * C + c]) : 0.f;
-    const uint32_t e = scale_byte<FMT>(
-        __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
-    if (c < C) codes[row * C + c] = encode1<FMT>(v, e);
-    if (lane == 0) scales[b] = uint8_t(e);
+  for (int64_t b = warp * kAnyUnroll; b < blocks; b += nwarps * kAnyUnroll) {
+    const Places p(b, blocks, C, nb, lane);
+    E raw[kAnyUnroll];
+#pragma unroll
+    for (int u = 0; u < kAnyUnroll; ++u)
+      if (p.in[u]) raw[u] = x[p.at[u]];
+    uint32_t mine = 0;  // lane u's: the scale byte of block u
+#pragma unroll
+    for (int u = 0; u < kAnyUnroll; ++u) {
+      const float v = p.in[u] ? Elem<E>::widen1(raw[u]) : 0.f;
+      const uint32_t e = scale_byte<FMT>(
+          __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
+      if (p.in[u]) codes[p.at[u]] = encode1<FMT>(v, e);
+      if (lane == u) mine = e;
+    }
+    if (lane < kAnyUnroll && b + lane < blocks) scales[b + lane] = uint8_t(mine);
   }
 }
 
@@ -125,12 +154,19 @@ dequantize_any_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restri
   const int lane = threadIdx.x & 31;
   const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
   const int64_t nwarps = (int64_t(gridDim.x) * kThreads) >> 5;
-  for (int64_t b = warp; b < blocks; b += nwarps) {
-    const int64_t row = b / nb;
-    const int c = int(b - row * nb) * kBlock + lane;
-    if (c < C)
-      x[row * C + c] = Elem<E>::narrow1(
-          Elem<E>::fit(decode1<FMT>(codes[row * C + c]) * scale_value(scales[b])));
+  for (int64_t b = warp * kAnyUnroll; b < blocks; b += nwarps * kAnyUnroll) {
+    const Places p(b, blocks, C, nb, lane);
+    uint8_t raw[kAnyUnroll], e[kAnyUnroll];
+#pragma unroll
+    for (int u = 0; u < kAnyUnroll; ++u)
+      if (p.in[u]) {
+        raw[u] = codes[p.at[u]];
+        e[u] = scales[b + u];
+      }
+#pragma unroll
+    for (int u = 0; u < kAnyUnroll; ++u)
+      if (p.in[u])
+        x[p.at[u]] = Elem<E>::narrow1(Elem<E>::fit(decode1<FMT>(raw[u]) * scale_value(e[u])));
   }
 }
 
@@ -145,7 +181,7 @@ void quantize(const void *x, void *codes, void *scales, int64_t rows, int C, boo
            (uint8_t *)codes, (uint8_t *)scales, chunks, C, 4 * nb);
   } else {
     auto k = quantize_any_kernel<E, FMT>;
-    launch(k, dim3(grid_for(k, rows * nb, kThreads)), dim3(kThreads), 0, s, (const E *)x,
+    launch(k, dim3(grid_for(k, (rows * nb + kAnyUnroll - 1) / kAnyUnroll, kThreads)), dim3(kThreads), 0, s, (const E *)x,
            (uint8_t *)codes, (uint8_t *)scales, rows * nb, C, nb);
   }
 }
@@ -161,7 +197,7 @@ void dequantize(const void *codes, const void *scales, void *x, int64_t rows, in
            (const uint8_t *)scales, (E *)x, chunks, C, 4 * nb);
   } else {
     auto k = dequantize_any_kernel<E, FMT>;
-    launch(k, dim3(grid_for(k, rows * nb, kThreads)), dim3(kThreads), 0, s, (const uint8_t *)codes,
+    launch(k, dim3(grid_for(k, (rows * nb + kAnyUnroll - 1) / kAnyUnroll, kThreads)), dim3(kThreads), 0, s, (const uint8_t *)codes,
            (const uint8_t *)scales, (E *)x, rows * nb, C, nb);
   }
 }

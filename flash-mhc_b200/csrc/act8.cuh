@@ -127,9 +127,13 @@ __device__ __forceinline__ void decode4x2(uint32_t w, float2 &a, float2 &b) {
 }
 template <int FMT>
 __device__ __forceinline__ float decode1(uint8_t c) {
-  float f[4];
-  decode4<FMT>(uint32_t(c), f);
-  return f[0];
+  if constexpr (FMT == kInt8) {
+    return __uint_as_float(0x4b000000u | (c ^ 0x80u)) - 8388736.f;  // as in decode4
+  } else {
+    float f[4];
+    decode4<FMT>(uint32_t(c), f);
+    return f[0];
+  }
 }
 
 // Scale byte -> the factor that widen4 takes: 2^(e - 127) as two bf16 or as f32.
@@ -308,7 +312,13 @@ __device__ __forceinline__ uint2 encode8(const float (&f)[8], uint32_t e) {
 }
 template <int FMT>
 __device__ __forceinline__ uint8_t encode1(float f, uint32_t e) {
-  return uint8_t(encode4<FMT, true>(f, 0.f, 0.f, 0.f, e));
+  if constexpr (FMT == kInt8) {  // encode4 of one value
+    const float v = f * __uint_as_float((254u - min(e, kTopScale<FMT>)) << 23);
+    const float c = fminf(fmaxf(v, -Format<FMT>::kMax), Format<FMT>::kMax);
+    return e == 255u ? 0 : uint8_t(__float_as_uint(c + 12582912.f));
+  } else {
+    return uint8_t(encode4<FMT, true>(f, 0.f, 0.f, 0.f, e));
+  }
 }
 
 }  // namespace act8

@@ -540,7 +540,9 @@ ln_param_grad_kernel(const float *__restrict__ part, void *__restrict__ gw, void
 }
 
 // ---------------------------------------------- any width and any alignment
-// One block per row; the row is read again for each step (from L1 or L2).
+// One block per row, which is read again for each step (from L1 or L2); forward, the
+// first kKept values of each thread stay in registers.
+constexpr int kKept = 4;
 __device__ float2 block_sum(float2 v, float2 *sh) {
   v.x = warp_sum(v.x);
   v.y = warp_sum(v.y);
@@ -567,22 +569,35 @@ ln_fwd_any_kernel(const E *__restrict__ x, const void *__restrict__ w, const voi
   const int nb = (C + kBlock - 1) / kBlock, lane = threadIdx.x & 31;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const E *xr = x + r * C;
+    float kept[kKept];
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) {
+      const int c = i * kThreads + threadIdx.x;
+      kept[i] = c < C ? Elem<E>::widen1(xr[c]) : 0.f;
+    }
+    // f(column, value) for this thread's columns.
+    const auto each = [&](auto f) {
+#pragma unroll
+      for (int i = 0; i < kKept; ++i)
+        if (i * kThreads + threadIdx.x < C) f(i * kThreads + int(threadIdx.x), kept[i]);
+      for (int c = kKept * kThreads + threadIdx.x; c < C; c += kThreads) f(c, Elem<E>::widen1(xr[c]));
+    };
     float2 v = make_float2(0.f, 0.f);
-    for (int c = threadIdx.x; c < C; c += kThreads) v.x += Elem<E>::widen1(xr[c]);
+    each([&](int, float f) { v.x += f; });
     const float mean = block_sum(v, sh).x / float(C);
     v = make_float2(0.f, 0.f);
-    for (int c = threadIdx.x; c < C; c += kThreads) {
-      const float d = Elem<E>::widen1(xr[c]) - mean;
+    each([&](int, float f) {
+      const float d = f - mean;
       v.x = fmaf(d, d, v.x);
-    }
+    });
     const float rstd = rsqrtf(block_sum(v, sh).x / float(C) + eps);
     if (threadIdx.x == 0) {
       mean_out[r] = mean;
       rstd_out[r] = rstd;
     }
-    for (int c = threadIdx.x; c < C; c += kThreads)
-      y[r * C + c] = Elem<E>::narrow1(fmaf((Elem<E>::widen1(xr[c]) - mean) * rstd,
-                                           param1(w, pdt, c, 1.f), param1(b, pdt, c, 0.f)));
+    each([&](int c, float f) {
+      y[r * C + c] = Elem<E>::narrow1(fmaf((f - mean) * rstd, param1(w, pdt, c, 1.f), param1(b, pdt, c, 0.f)));
+    });
     if constexpr (FMT != kNone) {
       for (int k = threadIdx.x >> 5; k < nb; k += kWarps) {  // a warp per block of 32
         const int c = k * kBlock + lane;
@@ -635,6 +650,92 @@ ln_bwd_any_kernel(const E *__restrict__ g, const void *__restrict__ x,
   }
 }
 
+// Any width up to 32 NV, a warp per row and the row in registers, 32 values apart
+// in a lane: value i of the lanes is block i of 32.
+template <class E, int FMT, int NV>
+__global__ void __launch_bounds__(kThreads)
+ln_fwd_warp_kernel(const E *__restrict__ x, const void *__restrict__ w, const void *__restrict__ b,
+                   int pdt, float eps, E *__restrict__ y, float *__restrict__ mean_out,
+                   float *__restrict__ rstd_out, uint8_t *__restrict__ codes,
+                   uint8_t *__restrict__ scales, int64_t rows, int C) {
+  pdl_wait();
+  const int nb = (C + kBlock - 1) / kBlock, lane = threadIdx.x & 31;
+  const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
+  const int64_t nwarps = (int64_t(gridDim.x) * kThreads) >> 5;
+  for (int64_t r = warp; r < rows; r += nwarps) {
+    const E *xr = x + r * C + lane;
+    float f[NV], s = 0.f, q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) f[i] = i * 32 + lane < C ? Elem<E>::widen1(xr[i * 32]) : 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) s += f[i];
+    const float mean = warp_sum(s) / float(C);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float d = i * 32 + lane < C ? f[i] - mean : 0.f;
+      q = fmaf(d, d, q);
+    }
+    const float rstd = rsqrtf(warp_sum(q) / float(C) + eps);
+    if (lane == 0) {
+      mean_out[r] = mean;
+      rstd_out[r] = rstd;
+    }
+    uint32_t mine = 0;  // lane i's: the scale byte of block i
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = i * 32 + lane;
+      if (c < C)
+        y[r * C + c] = Elem<E>::narrow1(fmaf((f[i] - mean) * rstd, param1(w, pdt, c, 1.f), param1(b, pdt, c, 0.f)));
+      if constexpr (FMT != kNone) {
+        if (i * 32 < C) {
+          const uint32_t e = scale_byte<FMT>(
+              __reduce_max_sync(0xffffffffu, __float_as_uint(f[i]) & 0x7fffffffu));
+          if (c < C) codes[r * C + c] = encode1<FMT>(f[i], e);
+          if (lane == i) mine = e;
+        }
+      }
+    }
+    if constexpr (FMT != kNone) {
+      if (lane < nb) scales[r * nb + lane] = uint8_t(mine);
+    }
+  }
+}
+
+template <class E, int FMT, int NV>
+__global__ void __launch_bounds__(kThreads)
+ln_bwd_warp_kernel(const E *__restrict__ g, const void *__restrict__ x,
+                   const uint8_t *__restrict__ scales, const float *__restrict__ mean,
+                   const float *__restrict__ rstd, const void *__restrict__ w, int pdt,
+                   E *__restrict__ gx, int64_t rows, int C) {
+  pdl_wait();
+  const int nb = (C + kBlock - 1) / kBlock, lane = threadIdx.x & 31;
+  const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
+  const int64_t nwarps = (int64_t(gridDim.x) * kThreads) >> 5;
+  for (int64_t r = warp; r < rows; r += nwarps) {
+    const float m = mean[r], rs = rstd[r];
+    float gw[NV], xh[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = i * 32 + lane;
+      gw[i] = c < C ? Elem<E>::widen1(g[r * C + c]) : 0.f;
+      xh[i] = c < C ? input1<E, FMT>(x, scales, r, c, C, nb) : m;
+    }
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = i * 32 + lane;
+      if (c < C) gw[i] *= param1(w, pdt, c, 1.f);
+      xh[i] = (xh[i] - m) * rs;
+      s1 += gw[i];
+      s2 = fmaf(gw[i], xh[i], s2);
+    }
+    const float c1 = warp_sum(s1) / float(C), c2 = warp_sum(s2) / float(C);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (i * 32 + lane < C) gx[r * C + i * 32 + lane] = Elem<E>::narrow1(rs * (gw[i] - fmaf(xh[i], c2, c1)));
+  }
+}
+
 // Partials of grad_w and grad_b: block (cols of 32, slice of rows); the gradients
 // themselves if there is one slice.
 template <class E, int FMT>
@@ -651,6 +752,7 @@ ln_param_part_any_kernel(const E *__restrict__ g, const void *__restrict__ x,
   const int64_t r0 = rows * blockIdx.y / gridDim.y, r1 = rows * (blockIdx.y + 1) / gridDim.y;
   float a = 0.f, d = 0.f;
   if (c < C) {
+#pragma unroll 4
     for (int64_t r = r0 + warp; r < r1; r += 8) {
       const float fg = Elem<E>::widen1(g[r * C + c]);
       a = fmaf(fg, (input1<E, FMT>(x, scales, r, c, C, nb) - mean[r]) * rstd[r], a);
@@ -705,6 +807,15 @@ int blocks_for(int64_t rows, const Shape &p) {
     else FMHC_DISPATCH_FMT(FMT_RT, __VA_ARGS__);                                \
   } while (0)
 
+// Rows of widths that the ring kernels do not take go one to a warp if there are
+// many of them and they are narrow, else one to a block (us, warp / block:
+// forward 512 x 129 3.1 / 2.5, 2048 x 129 3.3 / 5.4, 65536 x 129 27 / 131, 65536 x
+// 1023 223 / 201; backward 65536 x 1023 327 / 456, 4096 x 1023 27 / 27).
+constexpr int64_t kManyRows = 1024;
+constexpr int kFwdRowInWarp = 512, kBwdRowInWarp = 1024;
+#define FMHC_WARP_KERNEL(KERNEL, C)                                          \
+  ((C) <= 128 ? KERNEL<E, FMT, 4> : (C) <= 256 ? KERNEL<E, FMT, 8> : KERNEL<E, FMT, 16>)
+
 // Slices of 32 rows or more; up to 128 rows are one, which needs no kernel to add
 // partials (backward of f32 rows of 1023, one slice / slices of 32, us: 37 rows
 // 5.4 / 6.8, 128 rows 6.4 / 7.0, 256 rows 7.9 / 7.2).
@@ -733,7 +844,9 @@ void launch_ln_fwd(const void *x, int dtype, const void *w, const void *b, int p
   } else {
     FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, {
       auto k = ln_fwd_any_kernel<E, FMT>;
-      launch(k, dim3(grid_for(k, rows * kWarps, kThreads)), dim3(kThreads), 0, s, (const E *)x, w, b,
+      const bool in_warp = rows >= kManyRows && C <= kFwdRowInWarp;
+      if (in_warp) k = FMHC_WARP_KERNEL(ln_fwd_warp_kernel, C);
+      launch(k, dim3(grid_for(k, in_warp ? rows : rows * kWarps, kThreads)), dim3(kThreads), 0, s, (const E *)x, w, b,
              pdt, eps, (E *)y, mean, rstd, (uint8_t *)codes, (uint8_t *)scales, rows, C);
     }));
   }
@@ -787,7 +900,9 @@ void launch_ln_bwd(const void *g, int dtype, const void *x, int fmt, const void 
   } else {
     FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_FMT_OR_NONE(fmt, {
       auto k = ln_bwd_any_kernel<E, FMT>;
-      launch(k, dim3(grid_for(k, rows * kWarps, kThreads)), dim3(kThreads), 0, s, (const E *)g, x,
+      const bool in_warp = rows >= kManyRows && C <= kBwdRowInWarp;
+      if (in_warp) k = C <= 512 ? FMHC_WARP_KERNEL(ln_bwd_warp_kernel, C) : ln_bwd_warp_kernel<E, FMT, 32>;
+      launch(k, dim3(grid_for(k, in_warp ? rows : rows * kWarps, kThreads)), dim3(kThreads), 0, s, (const E *)g, x,
              (const uint8_t *)scales, mean, rstd, w, pdt, (E *)gx, rows, C);
       if (part != nullptr) {
         parts = any_slices(rows, C);

@@ -169,6 +169,46 @@ def test_norm_of_the_widest_rows(rows, width, dtype):
         assert ((got.double() - want).abs() <= want.abs() * 2**-8 + 1e-5 * (1 + mag)).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,width", [(1023, 77), (1024, 1), (1024, 20), (1100, 129), (1500, 255), (1024, 257), (2000, 511),
+                                        (1024, 513), (1030, 1023)])
+def test_norm_of_many_rows_of_odd_width(rows, width, dtype):
+    """Forward, 8-bit copy and backward from x and from codes where a warp takes a row, and beside it."""
+    x, g, w, b = _randn(rows, width, dtype=dtype), _randn(rows, width, dtype=dtype), _randn(width), _randn(width)
+    y, mean, rstd = ops.layer_norm(x, w, b, 1e-5)
+    X, G, W = x.double(), g.double(), w.double()
+    m64 = X.mean(-1, keepdim=True)
+    r64 = ((X - m64).square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+    step = torch.finfo(dtype).eps / 2
+    xh = (X - m64) * r64
+    # f32 sums of at most 32 values a lane and five levels: 100 roundings to 2^-24 of their terms are 6e-6
+    # of them; a row's spread may be small beside its values, which |x - mean|'s relative error follows
+    err = 1e-5 * (1 + r64 * X.abs().amax(-1, keepdim=True))
+    lim = lambda want, scale: step * want.abs() + err * (1 + scale)  # noqa: E731
+    Y = xh * W + b.double()
+    assert ((y.double() - Y).abs() <= lim(Y, xh.abs() * W.abs())).all()
+    for fmt in (None, "int8", "e4m3"):
+        if fmt is None:
+            read, got = X, ops.layer_norm_backward(g, x, mean, rstd, w, b)
+        else:
+            yq, mq, rq, c, s = ops.layer_norm_q8(x, w, b, 1e-5, fmt)
+            wc, wsc = act8.quantize(x, fmt)
+            assert torch.equal(yq, y) and torch.equal(mq, mean) and torch.equal(rq, rstd)
+            assert torch.equal(c.view(torch.uint8), wc.view(torch.uint8)) and torch.equal(s, wsc)
+            read, got = act8.dequantize(c, s, torch.float32).double(), ops.layer_norm_backward_q8(g, c, s, mean, rstd, w, b)
+        h = (read - mean.double()[:, None]) * rstd.double()[:, None]
+        gW = G * W
+        GX = (gW - gW.mean(-1, keepdim=True) - h * (gW * h).mean(-1, keepdim=True)) * rstd.double()[:, None]
+        mag = rstd.double()[:, None] * (gW.abs() + gW.abs().mean(-1, keepdim=True) + h.abs() * (gW * h).abs().mean(-1, keepdim=True))
+        # From codes of one column, rstd^2 = 1e5 times x's rounding passes the largest f16: a value from 65520 on
+        # (half a step above 65504) rounds to infinity, so where the f32 result can lie there, infinity is right.
+        inf = got[0].double() == torch.inf * GX.sign()
+        over = inf & (GX.abs() + 1e-5 * mag >= 65520) & (dtype == torch.float16)
+        assert (((got[0].double() - GX).abs() <= step * GX.abs() + 1e-5 * mag + 1e-7) | over).all()
+        for a, want, scale in ((got[1], (G * h).sum(0), (G * h).abs().sum(0)), (got[2], G.sum(0), G.abs().sum(0))):
+            assert ((a.double() - want).abs() <= want.abs() * 2**-8 + 2e-5 * scale + 1e-7).all()
+
+
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_checkpoints_at_odd_addresses(fmt):
     """Codes and scales that are views at every odd offset give the bits of aligned ones, or, where a
