@@ -104,17 +104,17 @@ struct Places {  // this lane's values: where, and whether they exist
   int64_t at[kAnyUnroll];
   bool in[kAnyUnroll];
   __device__ __forceinline__ Places(int64_t b, int64_t blocks, int C, int nb, int lane) {
-    int64_t row = b / nb;
+    const int64_t row = b / nb;
     int k = int(b - row * nb);
+    const int last = C - (nb - 1) * kBlock;  // values of a row's last block
+    int64_t i = row * C + k * kBlock + lane;
 #pragma unroll
     for (int u = 0; u < kAnyUnroll; ++u) {
-      const int c = k * kBlock + lane;
-      at[u] = row * C + c;
-      in[u] = b + u < blocks && c < C;
-      if (++k == nb) {
-        k = 0;
-        ++row;
-      }
+      const bool end = k + 1 == nb;
+      at[u] = i;
+      in[u] = b + u < blocks && (!end || lane < last);
+      i += end ? last : kBlock;
+      k = end ? 0 : k + 1;
     }
   }
 };
