@@ -65,18 +65,20 @@ def _format(op: str, name: str):
 
 
 def _scales_shape(shape) -> tuple:
-    return (*shape[:-1], -(-shape[-1] // BLOCK))
+    *rows, C = shape
+    return (*rows, -(-C // BLOCK))
 
 
 def _same_device(op: str, first: torch.Tensor, **others) -> None:
     """The kernels take raw pointers: every tensor has to live on ``first``'s device."""
+    index = first.get_device()  # -1 on the CPU
     for name, t in others.items():
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"flash_mhc::{op}: {name} is on {t.device}, expected {first.device}")
 
 
 def _shape(op: str, name: str, t: torch.Tensor, want: tuple) -> None:
-    if tuple(t.shape) != tuple(want):
+    if t.shape != want:
         raise ValueError(f"flash_mhc::{op}: {name} must be {tuple(want)} (got {tuple(t.shape)})")
 
 
@@ -95,17 +97,22 @@ def _rows(t: torch.Tensor) -> int:
 
 def _checkpoint(op: str, name: str, codes: torch.Tensor, scales: torch.Tensor):
     """(codes, scales, FMHC_ACT8_*) of a checkpoint, checked against each other."""
-    if codes.dtype not in _CODE_FORMATS:
+    fmt = _CODE_FORMATS.get(codes.dtype)
+    if fmt is None:
         raise ValueError(f"flash_mhc::{op}: {name} codes must be int8 or float8_e4m3fn (got {codes.dtype})")
-    if codes.dim() < 1 or codes.shape[-1] < 1:
-        raise ValueError(f"flash_mhc::{op}: {name} codes need a last dimension of at least 1 (got {tuple(codes.shape)})")
+    shape = codes.shape
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"flash_mhc::{op}: {name} codes need a last dimension of at least 1 (got {tuple(shape)})")
     if scales.dtype != torch.uint8:
         raise ValueError(f"flash_mhc::{op}: {name} scales must be uint8 (got {scales.dtype})")
-    _shape(op, f"{name} scales", scales, _scales_shape(codes.shape))
-    return codes.contiguous(), scales.contiguous(), _CODE_FORMATS[codes.dtype]
+    if scales.shape != _scales_shape(shape):
+        _shape(op, f"{name} scales", scales, _scales_shape(shape))
+    return codes.contiguous(), scales.contiguous(), fmt
 
 
 def _new_checkpoint(x: torch.Tensor, code_dtype: torch.dtype):
+    if x.is_contiguous():
+        return torch.empty_like(x, dtype=code_dtype), x.new_empty(_scales_shape(x.shape), dtype=torch.uint8)
     return (torch.empty_like(x, dtype=code_dtype, memory_format=torch.contiguous_format),
             x.new_empty(_scales_shape(x.shape), dtype=torch.uint8))
 
@@ -315,8 +322,8 @@ def _post_res_grad_params_q8_cuda(grad_out, x_codes, x_scales, lo_codes, lo_scal
                          f"(got {x_codes.dtype} and {lo_codes.dtype})")
     grad_out, h_post = _bf16("grad_out", grad_out), _coef(h_post)
     grad_lo = grad_out.new_empty((T, C))
-    grad_H = grad_out.new_empty((T, n, n), dtype=torch.float32)
-    grad_hp = grad_out.new_empty((T, n), dtype=torch.float32)
+    grad_H = h_post.new_empty((T, n, n))  # h_post is f32 by now
+    grad_hp = torch.empty_like(h_post)
     _launch(grad_out, "fmhc_k4_bwd_q8", grad_out.data_ptr(), x_codes.data_ptr(),
             x_scales.data_ptr(), lo_codes.data_ptr(), lo_scales.data_ptr(), fmt,
             h_post.data_ptr(), grad_lo.data_ptr(), grad_H.data_ptr(), grad_hp.data_ptr(), T, n, C)
