@@ -172,6 +172,31 @@ k4_fwd_q8_kernel(const bf16 *__restrict__ x, const bf16 *__restrict__ lo,
 }
 
 // --------------------------------------------------------- backward rings
+// warp_reduce_scatter with its choices between values.  There, `upper ? v[k] :
+// v[k + half]` chooses between addresses and puts v into local memory, which cost
+// K4's backward 26 of 189 us here; the bf16 kernel is short of registers and
+// faster with it (305 against 328 us).
+template <int N>
+__device__ __forceinline__ void reduce_scatter(float (&v)[N], int lane) {
+  int live = N;
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) {
+    if (live > 1) {
+      const int half = live >> 1;
+      const bool upper = (lane & off) != 0;
+#pragma unroll
+      for (int k = 0; k < half; ++k) {
+        const float a = v[k], b = v[k + half];
+        const float send = upper ? a : b, keep = upper ? b : a;
+        v[k] = keep + __shfl_xor_sync(0xffffffffu, send, off);
+      }
+      live = half;
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
+    }
+  }
+}
+
 // Eight codes, scaled.
 template <int FMT>
 __device__ __forceinline__ void restore8(uint2 q, uint32_t e, float2 (&f)[4]) {
@@ -254,7 +279,7 @@ k3_bwd_q8_kernel(const bf16 *__restrict__ go, const uint8_t *__restrict__ codes,
         v[j] = acc[j].x + acc[j].y;
         acc[j] = both(0.f);
       }
-      warp_reduce_scatter<4>(v, lane);
+      reduce_scatter<4>(v, lane);
       if ((lane & 7) == 0) __stcs(gh + now.t * 4 + scatter_index<4>(lane), v[0]);
     }
     now = next;
@@ -369,8 +394,8 @@ k4_bwd_q8_kernel(const bf16 *__restrict__ go, const uint8_t *__restrict__ xc,
           accH[i][j] = both(0.f);
         }
       }
-      warp_reduce_scatter<16>(v, lane);
-      warp_reduce_scatter<4>(w, lane);
+      reduce_scatter<16>(v, lane);
+      reduce_scatter<4>(w, lane);
       if ((lane & 1) == 0) __stcs(gH + now.t * 16 + scatter_index<16>(lane), v[0]);
       if ((lane & 7) == 0) __stcs(ghp + now.t * 4 + scatter_index<4>(lane), w[0]);
     }
@@ -400,7 +425,7 @@ k3_bwd_q8_any_kernel(const bf16 *__restrict__ go, const uint8_t *__restrict__ co
         acc[j] = fmaf(decode1<FMT>(codes[(t * 4 + j) * C + c]) * scale_value(scales[(t * 4 + j) * nb + c / kBlock]),
                       g, acc[j]);
     }
-    warp_reduce_scatter<4>(acc, lane);
+    reduce_scatter<4>(acc, lane);
     if ((lane & 7) == 0) gh[t * 4 + scatter_index<4>(lane)] = acc[0];
   }
 }
@@ -455,8 +480,8 @@ k4_bwd_q8_any_kernel(const bf16 *__restrict__ go, const uint8_t *__restrict__ xc
         for (int i = 0; i < 4; ++i) accH[i * 4 + j] = fmaf(g[i], v, accH[i * 4 + j]);
       }
     }
-    warp_reduce_scatter<16>(accH, lane);
-    warp_reduce_scatter<4>(accP, lane);
+    reduce_scatter<16>(accH, lane);
+    reduce_scatter<4>(accP, lane);
     if ((lane & 1) == 0) gH[t * 16 + scatter_index<16>(lane)] = accH[0];
     if ((lane & 7) == 0) ghp[t * 4 + scatter_index<4>(lane)] = accP[0];
   }

@@ -196,10 +196,8 @@ __device__ __forceinline__ void warp_reduce_scatter(float (&v)[N], int lane) {
       const bool upper = (lane & off) != 0;
 #pragma unroll
       for (int k = 0; k < half; ++k) {
-        // Values first: a choice between two elements would choose between their
-        // addresses, which puts v into local memory.
-        const float a = v[k], b = v[k + half];
-        const float send = upper ? a : b, keep = upper ? b : a;
+        float send = upper ? v[k] : v[k + half];
+        float keep = upper ? v[k + half] : v[k];
         v[k] = keep + __shfl_xor_sync(0xffffffffu, send, off);
       }
       live = half;
