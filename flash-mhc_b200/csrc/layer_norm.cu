@@ -22,6 +22,13 @@
 // 16 warps per SM, too few to cover HBM's latency with loads into registers
 // (a first version ran at a third of the copy rate), so the next rows are
 // prefetched into a shared-memory ring (lane_ring.cuh).
+//
+// Measured, us (floor of the bytes at the copy rate): 65536 x 2048 bf16 forward
+// 87-90 (82), backward 128-134 (123); 131072 x 1024 97-100 (82), 144 (123); with
+// int8 codes 131072 x 1024 forward 113-124 (103), backward 131 (103); e4m3 codes,
+// f16, 16384 x 4096 65 (52), 81 (52).  Memory bounds the plain ones; those with
+// codes are bound by instructions (23 per value forward, 25 backward), and a
+// backward ends with 8 us of joining the parameters' partials.
 #include "act8.cuh"
 #include "fmhc_launch.h"
 #include "grid.cuh"
