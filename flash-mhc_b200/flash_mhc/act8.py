@@ -342,8 +342,8 @@ def _fused_rmsnorm_project_backward_q8_cuda(grad_out, x_codes, x_scales, W, proj
                  inv_rms=inv_rms)
     x_codes, x_scales, fmt = _checkpoint(op, "x", x_codes, x_scales)
     grad_out, W, proj_out = _bf16("grad_out", grad_out), _bf16("W", W), _bf16("proj_out", proj_out)
-    grad_out, W, proj_out, x_codes, x_scales = (_aligned(t) for t in (grad_out, W, proj_out, x_codes, x_scales))
-    inv_rms = inv_rms.to(torch.float32).contiguous()
+    grad_out, W, proj_out = _aligned(grad_out), _aligned(W), _aligned(proj_out)
+    x_codes, x_scales, inv_rms = _aligned(x_codes), _aligned(x_scales), _coef(inv_rms)
     grad_x, grad_W = grad_out.new_empty((T, n, C)), grad_out.new_empty((32, n * C))
     ws, ws_bytes, _keep = _workspace(grad_out, "fmhc_k1_bwd_q8_workspace_size", T, C)
     _launch(grad_out, "fmhc_k1_bwd_q8", grad_out.data_ptr(), x_codes.data_ptr(),

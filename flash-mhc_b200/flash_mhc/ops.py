@@ -230,7 +230,9 @@ def _bf16(name: str, t: torch.Tensor) -> torch.Tensor:
 
 def _coef(t: torch.Tensor) -> torch.Tensor:
     """Small f32 coefficient tensors: contiguous, float32, 16-byte aligned."""
-    t = t.to(torch.float32).contiguous()
+    if t.dtype != torch.float32:
+        t = t.to(torch.float32)
+    t = t.contiguous()
     if t.data_ptr() % 16:
         t = t.clone()
     return t
