@@ -392,7 +392,9 @@ FMHC_API int fmhc_layer_norm_fwd(const void *x, int x_dtype, const void *weight,
 /* Backward, with xh = (x - mean) rstd and gw = grad_y weight:
  *   grad_x      = rstd (gw - <gw> - xh <gw xh>)                  (x_dtype)
  *   grad_weight = sum over rows of grad_y xh, grad_bias = of grad_y  (param_dtype)
- * from x, or from its checkpoint (x_codes, x_scales; x NULL).  grad_weight and
+ * from x, or from its checkpoint (x_codes, x_scales; x NULL).  A checkpoint's
+ * rounding of x is divided by the row's spread: rows whose mean is much larger
+ * than their spread want x itself.  grad_weight and
  * grad_bias may be NULL; sums are f32 in a fixed order (bitwise reproducible).
  * rows == 0 writes zero parameter gradients.  `workspace` (256-byte aligned, at
  * least fmhc_layer_norm_bwd_workspace_size(rows, C) bytes; may be NULL when
