@@ -24,6 +24,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from .act8 import (_DTYPES, _act, _checkpoint, _format, _launch, _new_checkpoint, _rows,
                    _same_device, _shape, _workspace)
@@ -226,7 +227,8 @@ def _register_autograd(name: str, cuda_impl, backward: str, kept) -> None:
             return (None, *(g if n else None for g, n in zip(grads, need)), *ctx.rest)
 
     def kernel(keyset, *args):
-        if torch._C.is_grad_enabled() and torch._C._any_requires_grad(*args):
+        # (Inside forward-mode differentiation, too: the function refuses dual tensors.)
+        if (torch._C.is_grad_enabled() and torch._C._any_requires_grad(*args)) or forward_ad._current_level >= 0:
             return LayerNormFunction.apply(keyset, *args)
         return run(keyset, args)
 

@@ -1,9 +1,12 @@
 """Calls of the 8-bit and layer-norm ops at the edges of what they allow: second derivatives,
 offsets past 32 bits, the widest rows, views at odd addresses, captured graphs."""
 
+import threading
+
 import pytest
 import torch
 import torch.nn as nn
+import torch.utils.checkpoint
 
 import flash_mhc  # noqa: F401
 from flash_mhc import act8, norm
@@ -51,6 +54,54 @@ def test_second_derivatives_of_the_block_are_refused():
     g, = torch.autograd.grad(b(x).float().pow(2).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.float().pow(2).sum().backward()
+
+
+@pytest.mark.parametrize("fmt", [None, "int8"])
+def test_forward_mode_derivatives_are_refused(fmt):
+    x = _randn(4, 64, dtype=torch.float32)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+            norm.layer_norm(dual, None, None, checkpoint_format=fmt)
+        assert torch.equal(norm.layer_norm(x), norm.layer_norm(x.clone()))
+
+
+def test_threads_streams_and_torchs_own_checkpointing():
+    """Two threads train at once on streams of their own; the block under torch's recomputation and with its
+    saved tensors on the host: all with the bits of a plain step."""
+    def make(seed):
+        torch.manual_seed(seed)
+        layer = nn.Sequential(norm.LayerNorm(264, checkpoint_format="int8"), nn.Linear(264, 264))
+        m = MHCLiteBlock(4, 264, layer, checkpoint_format="int8").cuda().to(BF)
+        return m, _randn(700, 4, 264), _randn(700, 4, 264)
+
+    def step(m, x, g, call=lambda m, x: m(x)):
+        x = x.detach().requires_grad_()
+        return torch.autograd.grad(call(m, x), [x, *m.parameters()], g)
+
+    cases = [make(1), make(2)]
+    want = [step(*c) for c in cases]
+    same = lambda got, ref: all(torch.equal(a, b) for a, b in zip(got, ref))  # noqa: E731
+    torch.cuda.synchronize()
+    good = [0, 0]
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                good[i] += same(step(*cases[i]), want[i])
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert good == [20, 20]
+    recompute = lambda m, x: torch.utils.checkpoint.checkpoint(m, x, use_reentrant=False)  # noqa: E731
+    assert torch.equal(step(*cases[0], recompute)[0], want[0][0])
+    with torch.autograd.graph.save_on_cpu():
+        assert same(step(*cases[0]), want[0])
 
 
 # ------------------------------------------------------ offsets past 32 bits
