@@ -14,44 +14,71 @@ constexpr int kThreads = 256;
 // Chunks of eight values in flight per thread (262144 x 1024 bf16 int8 / 262144 x
 // 2048 e4m3, us: quantise 8 128 / 251, 4 128 / 277, 2 134 / 273; restore 2 140 /
 // 269, 4 141 / 282, 16 140 / 278).
-constexpr int kUnroll = 8, kRestoreUnroll = 2;
+constexpr int kRestoreUnroll = 2;
+// Quantising, rows with a shorter last block keep too many places for more than two
+// (262144 x 1000 / x 2040 int8, us: 2 143 / 280, 4 170 / 339, 8 190 / 388).
+template <bool FLAT> constexpr int kUnroll = FLAT ? 8 : 2;
 
 // Rows of C values (C % 8 == 0, 16-byte aligned rows) are seen as 4 * nb
 // chunks of eight, nb = ceil(C / 32) blocks; chunks past C are empty.  Chunk i
 // belongs to block i / 4 of the whole tensor, so four neighbouring lanes find
 // their block's maximum with two shuffles.  FLAT (C % 32 == 0): no empty
 // chunks, and the chunk's place is 8 i without a division.
+//
+// Places of this thread's N chunks from chunk i on, kThreads apart: one division,
+// then additions (262144 x 1000 int8: 143 us; with a division per chunk 154-160).
+template <int N, bool FLAT>
+struct ChunkPlaces {
+  int64_t at[N];
+  bool in[N];
+  __device__ __forceinline__ ChunkPlaces(int64_t i, int64_t chunks, int C, int nb4) {
+    if constexpr (FLAT) {
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        in[u] = i + u * kThreads < chunks;
+        at[u] = (i + u * kThreads) * 8;
+      }
+    } else {
+      int64_t row = i / nb4;
+      int k = int(i - row * nb4);
+      const int rows = kThreads / nb4, rest = kThreads - rows * nb4;
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        in[u] = i + u * kThreads < chunks && k * 8 < C;
+        at[u] = row * C + k * 8;
+        k += rest;
+        row += rows;
+        if (k >= nb4) {
+          k -= nb4;
+          ++row;
+        }
+      }
+    }
+  }
+};
+
 template <class E, int FMT, bool FLAT>
 __global__ void __launch_bounds__(kThreads)
 quantize_kernel(const E *__restrict__ x, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
                 int64_t chunks, int C, int nb4) {
+  constexpr int U = kUnroll<FLAT>;
   pdl_wait();
-  const int64_t step = int64_t(gridDim.x) * kThreads * kUnroll;
-  for (int64_t i0 = int64_t(blockIdx.x) * kThreads * kUnroll; i0 < chunks; i0 += step) {
-    typename Elem<E>::Raw raw[kUnroll];
-    int64_t at[kUnroll];
-    bool in[kUnroll];
+  const int64_t step = int64_t(gridDim.x) * kThreads * U;
+  for (int64_t i0 = int64_t(blockIdx.x) * kThreads * U; i0 < chunks; i0 += step) {
+    typename Elem<E>::Raw raw[U];
+    const ChunkPlaces<U, FLAT> p(i0 + threadIdx.x, chunks, C, nb4);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t i = i0 + u * kThreads + threadIdx.x;
-      in[u] = i < chunks;
-      at[u] = i * 8;
-      if constexpr (!FLAT) {
-        const int64_t row = i / nb4;
-        const int c = int(i - row * nb4) * 8;
-        in[u] = in[u] && c < C;
-        at[u] = row * C + c;
-      }
+    for (int u = 0; u < U; ++u) {
       raw[u] = {};
-      if (in[u]) raw[u] = ld8(x + at[u]);
+      if (p.in[u]) raw[u] = ld8(x + p.at[u]);
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int64_t i = i0 + u * kThreads + threadIdx.x;
       float f[8];
       Elem<E>::widen(raw[u], f);
       const uint32_t e = scale_byte<FMT>(amax_block(amax8_raw<E>(raw[u])));
-      if (in[u]) __stcs(reinterpret_cast<uint2 *>(codes + at[u]), encode8<FMT>(f, e));
+      if (p.in[u]) __stcs(reinterpret_cast<uint2 *>(codes + p.at[u]), encode8<FMT>(f, e));
       if ((threadIdx.x & 3) == 0 && i < chunks) __stcs(scales + (i >> 2), uint8_t(e));
     }
   }
@@ -66,32 +93,22 @@ dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__
   for (int64_t i0 = int64_t(blockIdx.x) * kThreads * kRestoreUnroll; i0 < chunks; i0 += step) {
     uint2 raw[kRestoreUnroll];
     uint32_t e[kRestoreUnroll];
-    int64_t at[kRestoreUnroll];
-    bool in[kRestoreUnroll];
+    const ChunkPlaces<kRestoreUnroll, FLAT> p(i0 + threadIdx.x, chunks, C, nb4);
 #pragma unroll
     for (int u = 0; u < kRestoreUnroll; ++u) {
-      const int64_t i = i0 + u * kThreads + threadIdx.x;
-      in[u] = i < chunks;
-      at[u] = i * 8;
-      if constexpr (!FLAT) {
-        const int64_t row = i / nb4;
-        const int c = int(i - row * nb4) * 8;
-        in[u] = in[u] && c < C;
-        at[u] = row * C + c;
-      }
-      if (in[u]) {
-        raw[u] = ld_codes8(codes + at[u]);
-        e[u] = __ldg(scales + (i >> 2));
+      if (p.in[u]) {
+        raw[u] = ld_codes8(codes + p.at[u]);
+        e[u] = __ldg(scales + ((i0 + u * kThreads + threadIdx.x) >> 2));
       }
     }
 #pragma unroll
     for (int u = 0; u < kRestoreUnroll; ++u) {
-      if (in[u]) {
+      if (p.in[u]) {
         float f[8];
         restore<FMT>(raw[u], scale_value(e[u]), f);
 #pragma unroll
         for (int k = 0; k < 8; ++k) f[k] = Elem<E>::fit(f[k]);
-        st8(x + at[u], f);
+        st8(x + p.at[u], f);
       }
     }
   }
@@ -175,7 +192,8 @@ void quantize(const void *x, void *codes, void *scales, int64_t rows, int C, boo
               cudaStream_t s) {
   const int nb = (C + kBlock - 1) / kBlock;
   if (vec) {
-    const int64_t chunks = rows * nb * 4, warps = (chunks + 32 * kUnroll - 1) / (32 * kUnroll);
+    const int per_warp = 32 * (C % kBlock ? kUnroll<false> : kUnroll<true>);
+    const int64_t chunks = rows * nb * 4, warps = (chunks + per_warp - 1) / per_warp;
     auto k = C % kBlock ? quantize_kernel<E, FMT, false> : quantize_kernel<E, FMT, true>;
     launch(k, dim3(grid_for(k, warps, kThreads)), dim3(kThreads), 0, s, (const E *)x,
            (uint8_t *)codes, (uint8_t *)scales, chunks, C, 4 * nb);
