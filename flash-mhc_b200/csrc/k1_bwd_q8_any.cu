@@ -1,7 +1,7 @@
 // K1 backward from an 8-bit checkpoint of x for little work, and for the widths
-// that the tcgen05 kernel (k1_tc_bwd_q8.cuh) does not take, C % 32 != 0: blocks of
-// 32 then do not line up with its tiles, and rows of 4 C codes need not be what
-// the TMA wants.
+// that the tcgen05 kernel (k1_tc_bwd_q8.cuh) does not take: C % 32 != 0, where
+// blocks of 32 do not line up with its tiles and rows of 4 C codes need not be what
+// the TMA wants, and widths without a work split (k1_bwd_plan.h).
 //
 //   s       = (go . proj) inv^2 / nC
 //   grad_x  = bf16( inv (go W) - s x8 )

@@ -957,64 +957,9 @@ int launch_k1_tc_fwd(const void *x, const void *W, void *out, float *inv_rms, in
 }
 
 // ---------------------------------------------------------------- K1 backward
-namespace k1tc {
-namespace {
-
-struct BwdPlan {
-  int ntt, nkc, G, ngroups, grid, base, rem;
-  int64_t part_bytes;
-};
-
-int64_t round256(int64_t b) { return (b + 255) & ~int64_t(255); }
-
-// Work split of the backward kernel (see k1_tc_bwd.cuh): the nkc k-chunks form
-// nkc / G groups, the grid's CTAs are spread over the groups as evenly as
-// possible (the first `rem` groups get base + 1 CTAs, the rest base), and CTA
-// i of a group of ng takes the token tiles i, i + ng, ...  G (a divisor of
-// nkc, at most 8) minimises an estimate of the kernel time fitted to
-// measurements at nC = 4096 (T = 8192 and 65536, G = 2, 4, 8):
-//   1.56 us per unit of the busiest CTA (64 KiB of HBM traffic)
-// + 0.28 us per token tile of the busiest CTA (slot load and tile prep)
-// + the grad_W partials, G x 16 KiB per CTA written and read back, at 6 TB/s.
-// Large T favours G = 8 (fewest tile switches); small T, where the partials
-// weigh more, favours smaller G.
-BwdPlan bwd_plan(int64_t T, int64_t nC) {
-  BwdPlan p{};
-  p.ntt = int((T + kBwdBT - 1) / kBwdBT);
-  p.nkc = int(nC / kBwdBK);
-  const int sms = device_sms();
-  double best_cost = -1.0;
-  for (int G = kBwdMaxG; G >= 1; G >>= 1) {
-    if (p.nkc % G) continue;
-    const int ngroups = p.nkc / G;
-    int64_t grid = int64_t(ngroups) * p.ntt;
-    if (grid > sms) grid = sms;
-    if (grid < ngroups) continue;  // every group needs a CTA
-    const int base = int(grid / ngroups);
-    const int64_t tiles = (p.ntt + base - 1) / base;
-    const double part_us = double(grid) * G * kND * kBwdBK * 4 * 2 / 6.0e6;
-    const double cost = 1.56 * double(G * tiles) + 0.28 * double(tiles) + part_us;
-    if (best_cost < 0 || cost < best_cost) {
-      best_cost = cost;
-      p.G = G;
-      p.ngroups = ngroups;
-      p.grid = int(grid);
-      p.base = base;
-      p.rem = int(grid % ngroups);
-    }
-  }
-  p.part_bytes = round256(int64_t(p.grid) * p.G * kND * kBwdBK * 4);
-  return p;
-}
-
-}  // namespace
-}  // namespace k1tc
-
 bool k1_tc_bwd_supported(const void *go, const void *x, const void *W, const void *proj,
                          const void *gx, int64_t T, int64_t nC, int64_t D) {
-  if (D != k1tc::kND || nC % k1tc::kBwdBK != 0 || T < 1 || T > (int64_t(1) << 31)) return false;
-  // Each group of at most 8 k-chunks needs its own CTA.
-  if (nC / k1tc::kBwdBK > int64_t(k1tc::kBwdMaxG) * k1tc::device_sms()) return false;
+  if (D != k1tc::kND || !k1tc::bwd_has_plan(T, nC, k1tc::device_sms())) return false;
   const uintptr_t m = reinterpret_cast<uintptr_t>(go) | reinterpret_cast<uintptr_t>(x) |
                       reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(proj) |
                       reinterpret_cast<uintptr_t>(gx);
@@ -1023,17 +968,15 @@ bool k1_tc_bwd_supported(const void *go, const void *x, const void *W, const voi
 }
 
 int64_t k1_tc_bwd_workspace_bytes(int64_t T, int64_t nC) {
-  if (T < 1 || nC < k1tc::kBwdBK || nC % k1tc::kBwdBK) return 0;
-  if (nC / k1tc::kBwdBK > int64_t(k1tc::kBwdMaxG) * k1tc::device_sms()) return 0;
-  const k1tc::BwdPlan p = k1tc::bwd_plan(T, nC);
-  return p.part_bytes;
+  const int sms = k1tc::device_sms();
+  return k1tc::bwd_has_plan(T, nC, sms) ? k1tc::bwd_plan(T, nC, sms).part_bytes : 0;
 }
 
 int launch_k1_tc_bwd(const void *go, const void *x, const void *W, const void *proj,
                      const float *inv_rms, void *gx, void *gW, void *ws, int64_t ws_bytes,
                      int64_t T, int nC, cudaStream_t s) {
   using namespace k1tc;
-  const BwdPlan p = bwd_plan(T, nC);
+  const BwdPlan p = bwd_plan(T, nC, device_sms());
   const bool with_dw = gW != nullptr;
   float *part = nullptr;
   if (with_dw) {
@@ -1080,16 +1023,15 @@ int launch_k1_tc_bwd(const void *go, const void *x, const void *W, const void *p
 }
 
 bool k1_tc_bwd_q8_shape(int64_t T, int64_t nC) {
-  return nC % k1tc::kBwdBK == 0 && T >= 1 && T <= (int64_t(1) << 31) &&
-         nC / k1tc::kBwdBK <= int64_t(k1tc::kBwdMaxG) * k1tc::device_sms() &&
-         k1tc::device_is_sm100() && k1tc::encode_fn() != nullptr;
+  return k1tc::bwd_has_plan(T, nC, k1tc::device_sms()) && k1tc::device_is_sm100() &&
+         k1tc::encode_fn() != nullptr;
 }
 
 int launch_k1_tc_bwd_q8(const void *go, const void *codes, const void *scales, int fmt,
                         const void *W, const void *proj, const float *inv_rms, void *gx, void *gW,
                         void *ws, int64_t T, int nC, cudaStream_t s) {
   using namespace k1tc;
-  const BwdPlan p = bwd_plan(T, nC);
+  const BwdPlan p = bwd_plan(T, nC, device_sms());
   CUtensorMap mq, mgx, mgo, mproj, mw;
   // The codes as pairs of bytes: rows of nC / 2, boxes of 64 (128 columns).
   bool ok = make_map(&mq, codes, uint64_t(nC) / 2, uint64_t(T), uint64_t(nC), 64, kBwdBT,

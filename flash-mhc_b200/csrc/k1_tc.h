@@ -29,7 +29,8 @@ int launch_k1_fwd_rows_cluster(const void *x, const void *W, void *out, float *i
                                float *h_pre = nullptr, float *h_post = nullptr, float *H = nullptr,
                                void *pre_out = nullptr);
 
-// Backward (grad_x, and grad_W when gW != nullptr) on the tensor cores.
+// Backward (grad_x, and grad_W when gW != nullptr) on the tensor cores, for widths
+// that have a work split (k1_bwd_plan.h).
 bool k1_tc_bwd_supported(const void *go, const void *x, const void *W, const void *proj,
                          const void *gx, int64_t T, int64_t nC, int64_t D);
 // Caller workspace for the grad_W variant on the current device (0 if unsupported shape).

@@ -43,6 +43,8 @@
 // runs the same kernel without the grad_W MMAs and needs no workspace.
 #pragma once
 
+#include "k1_bwd_plan.h"
+
 namespace fmhc {
 namespace k1tc {
 
@@ -54,18 +56,12 @@ namespace k1tc {
 #ifndef FMHC_K1B_STORES_IN_FLIGHT
 #define FMHC_K1B_STORES_IN_FLIGHT 2
 #endif
-constexpr int kBwdBT = 128;                       // tokens per unit (MMA M of grad_x)
-constexpr int kBwdBK = 128;                       // k per unit (MMA N of grad_x, M of grad_W)
+static_assert(kBwdD == kND, "projection width");
 constexpr int kBwdStages = FMHC_K1B_STAGES;
 constexpr int kBwdInflight = FMHC_K1B_STORES_IN_FLIGHT;
 static_assert(kBwdInflight >= 1 && kBwdInflight <= 3 && kBwdInflight < kBwdStages,
               "stores in flight");
 constexpr int kBwdSlots = 2;                      // token-tile slots (go, proj, gos, (s, inv))
-#ifndef FMHC_K1B_MAX_G  // largest group of k-chunks (TMEM holds at most 8 x 32 grad_W columns)
-#define FMHC_K1B_MAX_G 8
-#endif
-constexpr int kBwdMaxG = FMHC_K1B_MAX_G;
-static_assert(kBwdMaxG == 1 || kBwdMaxG == 2 || kBwdMaxG == 4 || kBwdMaxG == 8, "group size");
 constexpr int kBwdXBytes = kBwdBT * kBwdBK * 2;   // 32 KiB (two 16 KiB boxes)
 constexpr int kBwdXBox = kBwdBT * 64 * 2;         // 16 KiB
 constexpr int kBwdWBytes = kND * kBwdBK * 2;      // 8 KiB  (two 4 KiB boxes)
