@@ -5,7 +5,8 @@
 // iterations are in flight while the current one is computed, and the kernel's
 // registers hold accumulators only.  A lane waits for its own copies and reads
 // its own slots, so no barrier is involved; it refills a slot only after it has
-// used what it read from it.
+// used what it read from it.  A slot that other lanes read as well (the row slots of
+// the layer norm's backward) needs a warp barrier before its refill and after the wait.
 #pragma once
 
 #include <cuda_runtime.h>

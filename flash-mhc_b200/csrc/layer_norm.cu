@@ -353,7 +353,9 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
   const uint32_t ring_g = shared_addr(dyn) + warp * (S * NV * kChunkG) + lane * int(sizeof(Raw));
   const uint32_t ring_x = shared_addr(dyn) + warps * (S * NV * kChunkG) + warp * (S * NV * kChunkX) +
                           lane * int(sizeof(X));
-  // Per warp and row: mean and rstd, then the words that hold the scale bytes.
+  // Per warp and row: mean and rstd, then the words that hold the scale bytes.  Unlike
+  // the slots of g and x, a few lanes copy these for the whole warp, so a warp
+  // barrier stands on both sides of a refill.
   const uint32_t ring_r = shared_addr(dyn) + warps * (S * NV * (kChunkG + kChunkX)) + warp * (S * kRowBytes<NV, FMT>);
   float4 *ws = reinterpret_cast<float4 *>(reinterpret_cast<char *>(dyn) + warps * (S * NV * (kChunkG + kChunkX)) +
                                           warps * (S * kRowBytes<NV, FMT>));
@@ -422,6 +424,7 @@ ln_bwd_kernel(const E *__restrict__ g, const void *__restrict__ x,
   uint32_t s_off = FMT == kNone ? 0u : uint32_t(reinterpret_cast<uintptr_t>(scales + r * nb) & 3);
   int par = 0, stage = 0;
   for (; r < rows; r += step, par ^= 1) {
+    __syncwarp();  // every lane has read the row slot that other lanes now refill
     fetch(stage == 0 ? S - 1 : stage - 1);
     copy_wait<S - 1>();
     __syncwarp();  // mean, rstd and scale bytes were copied by other lanes
