@@ -26,7 +26,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .ops import _bf16, _coef, _k2_typed_args, _lib, _n4, _on_device
+from .ops import _bf16, _coef, _dense_like, _k2_typed_args, _lib, _n4, _on_device
 
 BLOCK = 32  # values per scale
 # format name -> (FMHC_ACT8_*, dtype of the codes)
@@ -176,7 +176,7 @@ def _fused_pre_map_q8_fake(x_streams, h_pre, format):
 
 @torch.library.register_fake("flash_mhc::fused_post_res_q8")
 def _fused_post_res_q8_fake(x_streams, layer_output, H_merged, h_post, format):
-    return (torch.empty_like(x_streams),
+    return (_dense_like(x_streams),
             *_new_checkpoint(layer_output, _format("fused_post_res_q8", format)[1]))
 
 
@@ -205,7 +205,7 @@ def _post_res_grad_params_q8_fake(grad_out, x_codes, x_scales, lo_codes, lo_scal
 @torch.library.register_fake("flash_mhc::fused_rmsnorm_project_backward_q8")
 def _fused_rmsnorm_project_backward_q8_fake(grad_out, x_codes, x_scales, W, proj_out, inv_rms):
     return (torch.empty(x_codes.shape, device=x_codes.device, dtype=grad_out.dtype),
-            torch.empty_like(W, dtype=grad_out.dtype))
+            _dense_like(W, grad_out.dtype))
 
 
 # --------------------------------------------------------------------- CUDA

@@ -114,6 +114,11 @@ def _autotune_enabled() -> bool:
 # ---------------------------------------------------------------------------
 
 
+def _dense_like(t: torch.Tensor, dtype=None) -> torch.Tensor:
+    """What the CUDA implementations return in ``t``'s shape: contiguous, in whatever order ``t`` is."""
+    return t.new_empty(t.shape, dtype=dtype)
+
+
 @torch.library.register_fake("flash_mhc::fused_rmsnorm_project")
 def _fused_rmsnorm_project_fake(x_flat: torch.Tensor, W: torch.Tensor):
     T = x_flat.shape[0]
@@ -125,12 +130,12 @@ def _fused_rmsnorm_project_fake(x_flat: torch.Tensor, W: torch.Tensor):
 
 @torch.library.register_fake("flash_mhc::fused_rmsnorm_project_bwd_dx")
 def _fused_rmsnorm_project_bwd_dx_fake(grad_out, x_flat, W, proj_out, inv_rms):
-    return torch.empty_like(x_flat)
+    return _dense_like(x_flat)
 
 
 @torch.library.register_fake("flash_mhc::fused_rmsnorm_project_backward")
 def _fused_rmsnorm_project_backward_fake(grad_out, x_flat, W, proj_out, inv_rms):
-    return torch.empty_like(x_flat), torch.empty_like(W, dtype=x_flat.dtype)
+    return _dense_like(x_flat), _dense_like(W, x_flat.dtype)
 
 
 @torch.library.register_fake("flash_mhc::mhc_coeffs")
@@ -153,24 +158,24 @@ def _mhc_pre_forward_fake(x_streams, W, alpha_pre, alpha_post, alpha_res, bias, 
 @torch.library.register_fake("flash_mhc::mhc_coeffs_backward")
 def _mhc_coeffs_backward_fake(grad_h_pre, grad_h_post, grad_H_merged, proj, alpha_pre,
                               alpha_post, alpha_res, bias, perm):
-    return torch.empty_like(proj), torch.empty((35,), device=proj.device, dtype=torch.float32)
+    return _dense_like(proj), torch.empty((35,), device=proj.device, dtype=torch.float32)
 
 
 @torch.library.register_fake("flash_mhc::mhc_coeffs_backward_split")
 def _mhc_coeffs_backward_split_fake(grad_h_pre, grad_h_post, grad_H_merged, proj, alpha_pre,
                                     alpha_post, alpha_res, bias, perm):
-    return (torch.empty_like(proj), torch.empty_like(alpha_pre), torch.empty_like(alpha_post),
-            torch.empty_like(alpha_res), torch.empty_like(bias))
+    return (_dense_like(proj), _dense_like(alpha_pre), _dense_like(alpha_post),
+            _dense_like(alpha_res), _dense_like(bias))
 
 
 @torch.library.register_fake("flash_mhc::pre_map_grad_h")
 def _pre_map_grad_h_fake(grad_out, x_streams, h_pre):
-    return torch.empty_like(h_pre, dtype=torch.float32)
+    return _dense_like(h_pre, torch.float32)
 
 
 @torch.library.register_fake("flash_mhc::mhc_grad_x_combine")
 def _mhc_grad_x_combine_fake(gx1, grad_layer_input, h_pre, gx4):
-    return torch.empty_like(gx1)
+    return _dense_like(gx1)
 
 
 @torch.library.register_fake("flash_mhc::post_res_grad_params")
@@ -183,7 +188,7 @@ def _post_res_grad_params_fake(grad_out, x_streams, layer_output, H_merged, h_po
 
 @torch.library.register_fake("flash_mhc::mhc_grad_x_combine_post")
 def _mhc_grad_x_combine_post_fake(gx1, grad_layer_input, h_pre, grad_out, H_merged):
-    return torch.empty_like(gx1)
+    return _dense_like(gx1)
 
 
 @torch.library.register_fake("flash_mhc::fused_pre_map")
@@ -194,22 +199,22 @@ def _fused_pre_map_fake(x_streams: torch.Tensor, h_pre: torch.Tensor):
 
 @torch.library.register_fake("flash_mhc::fused_pre_map_backward")
 def _fused_pre_map_backward_fake(grad_out, x_streams, h_pre):
-    grad_x = torch.empty_like(x_streams)
-    grad_h_pre = torch.empty_like(h_pre, dtype=torch.float32)
+    grad_x = _dense_like(x_streams)
+    grad_h_pre = _dense_like(h_pre, torch.float32)
     return grad_x, grad_h_pre
 
 
 @torch.library.register_fake("flash_mhc::fused_post_res")
 def _fused_post_res_fake(x_streams, layer_output, H_merged, h_post):
-    return torch.empty_like(x_streams)
+    return _dense_like(x_streams)
 
 
 @torch.library.register_fake("flash_mhc::fused_post_res_backward")
 def _fused_post_res_backward_fake(grad_out, x_streams, layer_output, H_merged, h_post):
-    grad_x = torch.empty_like(x_streams)
-    grad_layer_output = torch.empty_like(layer_output)
-    grad_H_merged = torch.empty_like(H_merged, dtype=torch.float32)
-    grad_h_post = torch.empty_like(h_post, dtype=torch.float32)
+    grad_x = _dense_like(x_streams)
+    grad_layer_output = _dense_like(layer_output)
+    grad_H_merged = _dense_like(H_merged, torch.float32)
+    grad_h_post = _dense_like(h_post, torch.float32)
     return grad_x, grad_layer_output, grad_H_merged, grad_h_post
 
 
