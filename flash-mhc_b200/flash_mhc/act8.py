@@ -16,14 +16,16 @@ infinity or a NaN is restored as NaN.
   ``fused_rmsnorm_project_backward_q8``: their backwards, reading codes where
   the ops they are named after read bf16.
 
-``MHCLiteBlock(..., checkpoint_format="int8")`` trains through these.  None of
-the ops here registers an autograd formula of its own (quantising has no useful
-derivative); the block's autograd functions do.
+``MHCLiteBlock(..., checkpoint_format="int8")`` trains through these: its autograd
+functions call them.  On their own they have no derivative (quantising has no
+useful one): codes, scales and what is restored from them take no part in
+autograd, and a backward through any other result raises.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .ops import _bf16, _coef, _dense_like, _k2_typed_args, _lib, _n4, _on_device
@@ -350,6 +352,84 @@ def _fused_rmsnorm_project_backward_q8_cuda(grad_out, x_codes, x_scales, W, proj
             x_scales.data_ptr(), fmt, W.data_ptr(), proj_out.data_ptr(), inv_rms.data_ptr(),
             grad_x.data_ptr(), grad_W.data_ptr(), ws, ws_bytes, T, n, C)
     return grad_x, grad_W
+
+
+# ------------------------------------------------------------------ autograd
+
+
+def _register_autograd(name: str, cuda_impl, make_function) -> None:
+    """The autograd kernel of op ``name``: ``make_function(run)``'s function where a call
+    records a graph (or stands inside forward-mode differentiation: the function
+    refuses dual tensors), else ``run``, which takes the call on below autograd.
+
+    It calls the CUDA implementation itself where nothing else stands between (no
+    tracing, no functional or fake tensors): a second way through the dispatcher
+    costs 4 us of a call's 23.  Whether that is so goes by the call's dispatch keys
+    and is looked up by their bits (1.5 us less than working it out each time)."""
+    op = getattr(torch.ops.flash_mhc, name).default
+    below, cuda = torch._C._after_ADInplaceOrView_keyset, torch._C.DispatchKey.CUDA
+    grad_enabled, any_requires_grad = torch._C.is_grad_enabled, torch._C._any_requires_grad
+    direct: dict[int, bool] = {}
+
+    def run(keyset, args):
+        bits = keyset.raw_repr()
+        if bits not in direct:
+            direct[bits] = (keyset & below).highestPriorityTypeId() == cuda
+        if direct[bits]:
+            return cuda_impl(*args)
+        with torch._C._AutoDispatchBelowAutograd():
+            return op.redispatch(keyset & torch._C._after_autograd_keyset, *args)
+
+    apply = make_function(run).apply
+
+    def kernel(keyset, *args):
+        if (grad_enabled() and any_requires_grad(*args)) or forward_ad._current_level >= 0:
+            return apply(keyset, *args)
+        if direct.get(keyset.raw_repr()):
+            return cuda_impl(*args)
+        return run(keyset, args)
+
+    _lib.impl(name, kernel, "Autograd", with_keyset=True)
+
+
+# Outside autograd: results never require a gradient.
+for _name in ("act_quantize", "act_dequantize"):
+    _lib.impl(_name, torch.library.fallthrough_kernel, "Autograd")
+
+
+def _register_no_derivative(name: str, cuda_impl) -> None:
+    """Op ``name``: a backward through its results raises, but for codes and scales,
+    which are outside autograd."""
+
+    def make_function(run):
+        class NoDerivative(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, keyset, *args):
+                out = run(keyset, args)
+                outs = out if isinstance(out, tuple) else (out,)
+                ctx.mark_non_differentiable(*(t for t in outs if t.dtype not in _DTYPES))
+                ctx.set_materialize_grads(False)
+                return out
+
+            @staticmethod
+            def backward(ctx, *_):
+                raise RuntimeError(f"flash_mhc::{name} has no derivative (MHCLiteBlock(checkpoint_format=...) "
+                                   "differentiates through its own functions)")
+
+        return NoDerivative
+
+    _register_autograd(name, cuda_impl, make_function)
+
+
+for _name, _impl in (
+    ("fused_pre_map_q8", _fused_pre_map_q8_cuda),
+    ("fused_post_res_q8", _fused_post_res_q8_cuda),
+    ("mhc_pre_forward_q8", _mhc_pre_forward_q8_cuda),
+    ("pre_map_grad_h_q8", _pre_map_grad_h_q8_cuda),
+    ("post_res_grad_params_q8", _post_res_grad_params_q8_cuda),
+    ("fused_rmsnorm_project_backward_q8", _fused_rmsnorm_project_backward_q8_cuda),
+):
+    _register_no_derivative(_name, _impl)
 
 
 # ---------------------------------------------------------------- public names

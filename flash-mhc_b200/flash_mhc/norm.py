@@ -24,10 +24,9 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd import forward_ad
 
-from .act8 import (_DTYPES, _act, _checkpoint, _format, _launch, _new_checkpoint, _rows,
-                   _same_device, _shape, _workspace)
+from .act8 import (_DTYPES, _act, _checkpoint, _format, _launch, _new_checkpoint, _register_autograd,
+                   _rows, _same_device, _shape, _workspace)
 from .ops import _lib
 
 _lib.define(
@@ -187,56 +186,40 @@ class _GradsOnce(torch.autograd.Function):
         raise RuntimeError("flash_mhc::layer_norm has no second derivative")
 
 
-def _register_autograd(name: str, cuda_impl, backward: str, kept) -> None:
-    """The autograd kernel of op ``name``: ``kept`` picks what the backward reads in x's place.
-
-    It does what torch.library.register_autograd's does, but calls the CUDA
-    implementation itself where nothing else stands between (no tracing, no
-    functional or fake tensors): a second way through the dispatcher costs 4 us of a
-    call's 23."""
-    op = getattr(torch.ops.flash_mhc, name).default
+def _register_norm(name: str, cuda_impl, backward: str, kept) -> None:
+    """Op ``name``: ``kept`` picks what the backward reads in x's place."""
     backward_op = getattr(torch.ops.flash_mhc, backward)
-    below, cuda = torch._C._after_ADInplaceOrView_keyset, torch._C.DispatchKey.CUDA
 
-    def run(keyset, args):
-        if (keyset & below).highestPriorityTypeId() == cuda:
-            return cuda_impl(*args)
-        with torch._C._AutoDispatchBelowAutograd():
-            return op.redispatch(keyset & torch._C._after_autograd_keyset, *args)
+    def make_function(run):
+        class LayerNormFunction(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, keyset, *args):
+                out = run(keyset, args)
+                ctx.save_for_backward(*kept(args[0], out), out[1], out[2], args[1], args[2])
+                ctx.mark_non_differentiable(*out[1:])
+                ctx.set_materialize_grads(False)  # no zeros in the size of the codes
+                ctx.rest = (None,) * (len(args) - 3)
+                return out
 
-    class LayerNormFunction(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, keyset, *args):
-            out = run(keyset, args)
-            ctx.save_for_backward(*kept(args[0], out), out[1], out[2], args[1], args[2])
-            ctx.mark_non_differentiable(*out[1:])
-            ctx.set_materialize_grads(False)  # no zeros in the size of the codes
-            ctx.rest = (None,) * (len(args) - 3)
-            return out
+            @staticmethod
+            def backward(ctx, gy, *_):
+                if gy is None:
+                    return (None, None, None, None, *ctx.rest)
+                if torch.is_grad_enabled():  # create_graph=True
+                    mark = gy.new_empty(0).requires_grad_()
+                    grads = _GradsOnce.apply(mark, backward_op, gy, *ctx.saved_tensors)
+                else:
+                    grads = backward_op(gy, *ctx.saved_tensors)
+                need = ctx.needs_input_grad[1:]
+                return (None, *(g if n else None for g, n in zip(grads, need)), *ctx.rest)
 
-        @staticmethod
-        def backward(ctx, gy, *_):
-            if gy is None:
-                return (None, None, None, None, *ctx.rest)
-            if torch.is_grad_enabled():  # create_graph=True
-                mark = gy.new_empty(0).requires_grad_()
-                grads = _GradsOnce.apply(mark, backward_op, gy, *ctx.saved_tensors)
-            else:
-                grads = backward_op(gy, *ctx.saved_tensors)
-            need = ctx.needs_input_grad[1:]
-            return (None, *(g if n else None for g, n in zip(grads, need)), *ctx.rest)
+        return LayerNormFunction
 
-    def kernel(keyset, *args):
-        # (Inside forward-mode differentiation, too: the function refuses dual tensors.)
-        if (torch._C.is_grad_enabled() and torch._C._any_requires_grad(*args)) or forward_ad._current_level >= 0:
-            return LayerNormFunction.apply(keyset, *args)
-        return run(keyset, args)
-
-    _lib.impl(name, kernel, "Autograd", with_keyset=True)
+    _register_autograd(name, cuda_impl, make_function)
 
 
-_register_autograd("layer_norm", _layer_norm_cuda, "layer_norm_backward", lambda x, out: (x,))
-_register_autograd("layer_norm_q8", _layer_norm_q8_cuda, "layer_norm_backward_q8", lambda x, out: out[3:])
+_register_norm("layer_norm", _layer_norm_cuda, "layer_norm_backward", lambda x, out: (x,))
+_register_norm("layer_norm_q8", _layer_norm_q8_cuda, "layer_norm_backward_q8", lambda x, out: out[3:])
 
 
 # ---------------------------------------------------------------- public names
