@@ -343,10 +343,16 @@ class MHCLiteBlock(nn.Module):
         # No torch checkpointing here: the fused autograd functions already keep
         # only the small per-token tensors their backward kernels read.
         slot = _StreamGrad()
-        if self.checkpoint_format is not None:
+        fmt = self.checkpoint_format if torch.is_grad_enabled() else None
+        if fmt is not None and (x_streams.requires_grad or any(p.requires_grad for p in self.parameters())):
             return self._forward_fused_q8(x_streams, slot, **kwargs)
         layer_input, H_merged, h_post = self._mhc_pre_map_triton(x_streams, slot)
         layer_output = self.layer(layer_input, **kwargs)
+        if fmt is not None and layer_output.requires_grad:
+            # Only through a tensor that the layer was handed in kwargs or holds itself: no
+            # graph so far, and what K4's backward reads is quantised now.
+            xc, xs = torch.ops.flash_mhc.act_quantize(x_streams, fmt)
+            return _FusedPostResQ8.apply(x_streams, layer_output, H_merged, h_post, xc, xs, slot, fmt)
         return self._mhc_post_res_triton(x_streams, layer_output, H_merged, h_post, slot)
 
     def _forward_fused_q8(self, x_streams: torch.Tensor, slot, **kwargs) -> torch.Tensor:
