@@ -13,10 +13,11 @@ bias (either may be missing) any of these, of one type; y has x's type, under
 autocast too.  ``mean`` and ``rstd`` are not differentiable outputs, and the
 gradients have no derivative of their own (asking for one raises).
 
-From an 8-bit input the backward sees x with a rounding error (int8: up to 2^-7
-of the block's largest value, e4m3: 2^-4 of each value), which it divides by the
-row's spread: rows whose mean is much larger than their spread want x kept as it
-is.
+From an 8-bit input the backward sees x with a rounding error, which it divides by
+the row's spread: rows whose mean is much larger than their spread want x kept as
+it is.  The error is, with e the scale byte and a the largest value of a block of
+32, at most 2^(e - 128), which is below a / 127, for int8, and at most 2^-4 of each
+value or 2^(e - 137), which is below a / 2^17, whichever is larger, for e4m3.
 """
 
 from __future__ import annotations
