@@ -207,6 +207,8 @@ class MHCLiteBlock(nn.Module):
     forward(x_streams (T, n, C), **kwargs) -> (T, n, C); kwargs go to the layer.
     """
 
+    checkpoint_format = None  # of blocks that were pickled whole before there was the argument
+
     def __init__(
         self,
         n_streams: int,

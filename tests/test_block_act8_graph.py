@@ -123,3 +123,13 @@ def test_compiled(fmt, monkeypatch):
         assert torch.equal(res[0][0], want) and torch.equal(res[1][0], want)
         assert torch.equal(res[0][1], res[1][1]) and all(map(torch.equal, res[0][2], res[1][2]))
     assert any("q8" in n for n in launched) == (fmt is not None)
+
+
+def test_a_block_pickled_before_the_argument_existed():
+    """A whole module that was saved without the attribute runs as one without a format."""
+    with FakeTensorMode():
+        blk = block("int8")
+        del blk.__dict__["checkpoint_format"]
+        with Ops() as seen:
+            out = blk(torch.zeros(T, 4, C, dtype=BF, device="cuda", requires_grad=True))
+    assert out.requires_grad and seen.names == ["mhc_pre_forward", "fused_post_res"]
