@@ -4,7 +4,10 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <mutex>
+#include <new>
+#include <vector>
 
 namespace fmhc {
 
@@ -52,9 +55,9 @@ inline int sm_count() {
 
 constexpr size_t kMaxSmem = 232448 - 1024;  // dynamic shared memory beside a little static
 
-// Dynamic shared memory beyond the default needs an attribute of the kernel, set
-// once per device to the most it will ask for (and again only where this
-// table's 128 places do not suffice).
+// Dynamic shared memory beyond the default needs an attribute of the kernel.  Per
+// kernel and device it only ever grows: another thread may be between setting it
+// and its launch.
 inline void allow_smem(const void *kernel, size_t bytes) {
   struct Entry {
     const void *k;
@@ -62,18 +65,22 @@ inline void allow_smem(const void *kernel, size_t bytes) {
     size_t bytes;
   };
   static std::mutex mu;
-  static Entry set[128];
-  static int used = 0;
+  static std::vector<Entry> set;
   if (bytes <= 40 * 1024) return;  // beside the static arrays, below the default 48 KiB
   int dev = 0;
   cudaGetDevice(&dev);
   std::lock_guard<std::mutex> lock(mu);
-  int at = 0;
-  while (at < used && !(set[at].k == kernel && set[at].dev == dev)) ++at;
-  if (at < used && set[at].bytes >= bytes) return;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) != cudaSuccess) return;
-  if (at == used && used < 128) ++used;
-  if (at < used) set[at] = Entry{kernel, dev, bytes};
+  auto at = std::find_if(set.begin(), set.end(), [&](const Entry &e) { return e.k == kernel && e.dev == dev; });
+  if (at == set.end()) {
+    try {
+      at = set.insert(at, Entry{kernel, dev, 0});
+    } catch (const std::bad_alloc &) {
+      return;  // no exception crosses the C ABI; the launch reports its limit
+    }
+  }
+  if (at->bytes >= bytes) return;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) == cudaSuccess)
+    at->bytes = bytes;
 }
 
 }  // namespace fmhc
