@@ -346,7 +346,7 @@ class MHCLiteBlock(nn.Module):
         # only the small per-token tensors their backward kernels read.
         slot = _StreamGrad()
         fmt = self.checkpoint_format if torch.is_grad_enabled() else None
-        if fmt is not None and (x_streams.requires_grad or any(p.requires_grad for p in self.parameters())):
+        if fmt is not None and self._records_graph(x_streams):
             return self._forward_fused_q8(x_streams, slot, **kwargs)
         layer_input, H_merged, h_post = self._mhc_pre_map_triton(x_streams, slot)
         layer_output = self.layer(layer_input, **kwargs)
@@ -356,6 +356,12 @@ class MHCLiteBlock(nn.Module):
             xc, xs = torch.ops.flash_mhc.act_quantize(x_streams, fmt)
             return _FusedPostResQ8.apply(x_streams, layer_output, H_merged, h_post, xc, xs, slot, fmt)
         return self._mhc_post_res_triton(x_streams, layer_output, H_merged, h_post, slot)
+
+    def _records_graph(self, x_streams: torch.Tensor) -> bool:
+        """Whether a gradient is wanted of x, of the mixing's tensors (parameters, or what
+        stands in their place) or of a parameter of the layer."""
+        mixing = (x_streams, self.W_all.weight, self.W_all.bias, self.alpha_pre, self.alpha_post, self.alpha_res)
+        return any(t.requires_grad for t in mixing) or any(p.requires_grad for p in self.layer.parameters())
 
     def _forward_fused_q8(self, x_streams: torch.Tensor, slot, **kwargs) -> torch.Tensor:
         fmt = self.checkpoint_format

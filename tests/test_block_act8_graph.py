@@ -72,6 +72,12 @@ def check_which_ops_run(fmt, make):
         out, names = forward(blk, x)
         assert out.requires_grad and q8(names) == ["mhc_pre_forward_q8", "fused_post_res_q8"]
         wants.requires_grad_(False)
+    # A tensor in a parameter's place, as sharding wrappers put there.
+    w = torch.zeros_like(blk.W_all.weight).requires_grad_()
+    del blk.W_all.weight
+    blk.W_all.weight = w * 2
+    out, names = forward(blk, x)
+    assert out.requires_grad and q8(names) == ["mhc_pre_forward_q8", "fused_post_res_q8"]
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
