@@ -749,4 +749,148 @@ int fmhc_layer_norm_bwd(const void *grad_y, int x_dtype, const void *x, const vo
   return check_launch(w);
 }
 
+// ------------------------------------------------------- root-mean-square norm
+static int check_rms(const char *w, const void *x, int x_dtype, const void *residual,
+                     const void *weight, int param_dtype, float eps, const void *total) {
+  FMHC_REQUIRE_DTYPE(w, x_dtype);
+  FMHC_REQUIRE_DTYPE(w, param_dtype);
+  if (!(eps >= 0.f)) return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: eps must be >= 0", w);
+  if ((residual == nullptr) != (total == nullptr))
+    return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: residual and total go together", w);
+  for (const void *p : {x, residual, total}) FMHC_REQUIRE_ALIGN_TO(w, p, dtype_size(x_dtype));
+  FMHC_REQUIRE_ALIGN_TO(w, weight, dtype_size(param_dtype));
+  return FMHC_OK;
+}
+
+int fmhc_rms_norm_fwd(const void *x, int x_dtype, const void *residual, const void *weight,
+                      int param_dtype, float eps, void *y, void *total, float *rstd, int64_t rows,
+                      int64_t C, void *stream) {
+  const char *w = "fmhc_rms_norm_fwd";
+  if (int e = check_rows(w, rows, C)) return e;
+  if (int e = check_rms(w, x, x_dtype, residual, weight, param_dtype, eps, total)) return e;
+  if (rows == 0) return ok();
+  FMHC_REQUIRE_PTR(w, x); FMHC_REQUIRE_PTR(w, y); FMHC_REQUIRE_PTR(w, rstd);
+  FMHC_REQUIRE_ALIGN_TO(w, y, dtype_size(x_dtype)); FMHC_REQUIRE_ALIGN_TO(w, rstd, 4);
+  fmhc::launch_rms_fwd(x, x_dtype, residual, weight, param_dtype, eps, y, total, rstd, nullptr, 0,
+                       nullptr, rows, int(C), (cudaStream_t)stream);
+  return check_launch(w);
+}
+
+// Rows of codes: a stride of at least C bytes.
+static int check_codes(const char *w, const char *name, int64_t stride, int64_t C) {
+  if (stride < C)
+    return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: rows of %s must be at least %lld bytes apart (got %lld)", w, name,
+                (long long)C, (long long)stride);
+  return FMHC_OK;
+}
+
+int fmhc_rms_norm_fwd_int8(const void *x, int x_dtype, const void *residual, const void *weight,
+                           int param_dtype, float eps, void *codes, int64_t codes_stride,
+                           float *scales, void *total, int64_t rows, int64_t C, void *stream) {
+  const char *w = "fmhc_rms_norm_fwd_int8";
+  if (int e = check_rows(w, rows, C)) return e;
+  if (int e = check_rms(w, x, x_dtype, residual, weight, param_dtype, eps, total)) return e;
+  if (int e = check_codes(w, "codes", codes_stride, C)) return e;
+  if (rows == 0) return ok();
+  FMHC_REQUIRE_PTR(w, x); FMHC_REQUIRE_PTR(w, codes); FMHC_REQUIRE_PTR(w, scales);
+  FMHC_REQUIRE_ALIGN_TO(w, scales, 4);
+  fmhc::launch_rms_fwd(x, x_dtype, residual, weight, param_dtype, eps, nullptr, total, nullptr, codes,
+                       codes_stride, scales, rows, int(C), (cudaStream_t)stream);
+  return check_launch(w);
+}
+
+int64_t fmhc_rms_norm_bwd_workspace_size(int64_t rows, int64_t C) {
+  if (rows <= 0 || C <= 0 || C > (int64_t(1) << 28)) return 0;
+  return fmhc::rms_bwd_workspace_bytes(rows, int(C));
+}
+
+int fmhc_rms_norm_bwd(const void *grad_y, int x_dtype, const void *grad_total, const void *x,
+                      const float *rstd, const void *weight, int param_dtype, void *grad_x,
+                      void *grad_weight, void *workspace, int64_t workspace_bytes, int64_t rows,
+                      int64_t C, void *stream) {
+  const char *w = "fmhc_rms_norm_bwd";
+  if (int e = check_rows(w, rows, C)) return e;
+  FMHC_REQUIRE_DTYPE(w, x_dtype);
+  FMHC_REQUIRE_DTYPE(w, param_dtype);
+  FMHC_REQUIRE_ALIGN_TO(w, grad_weight, dtype_size(param_dtype));
+  cudaStream_t s = (cudaStream_t)stream;
+  if (rows == 0) {
+    // No rows: the weight's gradient is exactly zero.
+    if (grad_weight != nullptr &&
+        cudaMemsetAsync(grad_weight, 0, size_t(C) * dtype_size(param_dtype), s) != cudaSuccess)
+      return fail(FMHC_ERR_CUDA, "%s: cudaMemsetAsync failed", w);
+    return ok();
+  }
+  FMHC_REQUIRE_PTR(w, grad_y); FMHC_REQUIRE_PTR(w, x); FMHC_REQUIRE_PTR(w, rstd);
+  FMHC_REQUIRE_PTR(w, grad_x);
+  for (const void *p : {grad_y, grad_total, x, (const void *)grad_x})
+    FMHC_REQUIRE_ALIGN_TO(w, p, dtype_size(x_dtype));
+  FMHC_REQUIRE_ALIGN_TO(w, weight, dtype_size(param_dtype)); FMHC_REQUIRE_ALIGN_TO(w, rstd, 4);
+  if (grad_weight != nullptr) {
+    FMHC_REQUIRE_PTR(w, workspace);
+    if (!aligned(workspace, 256)) return fail(FMHC_ERR_ALIGNMENT, "%s: workspace must be 256-byte aligned", w);
+    const int64_t need = fmhc_rms_norm_bwd_workspace_size(rows, C);
+    if (workspace_bytes < need)
+      return fail(FMHC_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", w,
+                  (long long)workspace_bytes, (long long)need);
+  }
+  fmhc::launch_rms_bwd(grad_y, x_dtype, grad_total, x, rstd, weight, param_dtype, grad_x, grad_weight,
+                       (float *)workspace, rows, int(C), s);
+  return check_launch(w);
+}
+
+// ------------------------------------------------- rows and linear layers in int8
+int fmhc_row_quantize(const void *x, int x_dtype, void *codes, int64_t codes_stride, float *scales,
+                      int64_t rows, int64_t C, void *stream) {
+  const char *w = "fmhc_row_quantize";
+  if (int e = check_rows(w, rows, C)) return e;
+  FMHC_REQUIRE_DTYPE(w, x_dtype);
+  if (int e = check_codes(w, "codes", codes_stride, C)) return e;
+  if (rows == 0) return ok();
+  FMHC_REQUIRE_PTR(w, x); FMHC_REQUIRE_PTR(w, codes); FMHC_REQUIRE_PTR(w, scales);
+  FMHC_REQUIRE_ALIGN_TO(w, x, dtype_size(x_dtype)); FMHC_REQUIRE_ALIGN_TO(w, scales, 4);
+  fmhc::launch_row_quantize(x, x_dtype, codes, codes_stride, scales, rows, int(C), (cudaStream_t)stream);
+  return check_launch(w);
+}
+
+int fmhc_row_dequantize(const void *codes, int64_t codes_stride, const float *scales, void *x,
+                        int x_dtype, int64_t rows, int64_t C, void *stream) {
+  const char *w = "fmhc_row_dequantize";
+  if (int e = check_rows(w, rows, C)) return e;
+  FMHC_REQUIRE_DTYPE(w, x_dtype);
+  if (int e = check_codes(w, "codes", codes_stride, C)) return e;
+  if (rows == 0) return ok();
+  FMHC_REQUIRE_PTR(w, codes); FMHC_REQUIRE_PTR(w, scales); FMHC_REQUIRE_PTR(w, x);
+  FMHC_REQUIRE_ALIGN_TO(w, x, dtype_size(x_dtype)); FMHC_REQUIRE_ALIGN_TO(w, scales, 4);
+  fmhc::launch_row_dequantize(codes, codes_stride, scales, x, x_dtype, rows, int(C), (cudaStream_t)stream);
+  return check_launch(w);
+}
+
+int fmhc_int8_linear(const void *codes, int64_t codes_stride, const float *scales,
+                     const void *weight_codes, int64_t weight_stride, const float *weight_scales,
+                     const void *bias, int bias_dtype, void *y, int y_dtype, int64_t T, int64_t N,
+                     int64_t K, void *stream) {
+  const char *w = "fmhc_int8_linear";
+  for (int64_t n : {T, N})
+    if (n < 0 || n >= (int64_t(1) << 31))
+      return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: T and N must be in [0, 2^31) (got %lld)", w, (long long)n);
+  if (K < 1 || K >= (int64_t(1) << 17))
+    return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: K must be in [1, 2^17) (got %lld)", w, (long long)K);
+  FMHC_REQUIRE_DTYPE(w, bias_dtype);
+  FMHC_REQUIRE_DTYPE(w, y_dtype);
+  if (int e = check_codes(w, "codes", codes_stride, K)) return e;
+  if (int e = check_codes(w, "weight_codes", weight_stride, K)) return e;
+  if (codes_stride % 16 || weight_stride % 16)
+    return fail(FMHC_ERR_ALIGNMENT, "%s: rows of codes must be a multiple of 16 bytes apart", w);
+  if (T == 0 || N == 0) return ok();
+  FMHC_REQUIRE_PTR(w, codes); FMHC_REQUIRE_PTR(w, scales); FMHC_REQUIRE_PTR(w, weight_codes);
+  FMHC_REQUIRE_PTR(w, weight_scales); FMHC_REQUIRE_PTR(w, y);
+  FMHC_REQUIRE_ALIGN16(w, codes); FMHC_REQUIRE_ALIGN16(w, weight_codes);
+  FMHC_REQUIRE_ALIGN_TO(w, scales, 4); FMHC_REQUIRE_ALIGN_TO(w, weight_scales, 4);
+  FMHC_REQUIRE_ALIGN_TO(w, bias, dtype_size(bias_dtype)); FMHC_REQUIRE_ALIGN_TO(w, y, dtype_size(y_dtype));
+  fmhc::launch_int8_linear(codes, codes_stride, scales, weight_codes, weight_stride, weight_scales, bias,
+                           bias_dtype, y, y_dtype, T, N, int(K), (cudaStream_t)stream);
+  return check_launch(w);
+}
+
 }  // extern "C"

@@ -117,4 +117,28 @@ void launch_ln_bwd(const void *g, int dtype, const void *x, int fmt, const void 
                    const float *mean, const float *rstd, const void *w, int pdt, void *gx, void *gw,
                    void *gb, float *ws, int64_t rows, int C, bool vec, cudaStream_t s);
 
+// rms_norm.cu -- rows of C values of type dtype; res, w, gt may be null (total is
+// written where res is given).  codes null: y and rstd; else the output as rows of
+// `stride` bytes of codes and f32 scales (rows8.cuh).
+void launch_rms_fwd(const void *x, int dtype, const void *res, const void *w, int pdt, float eps,
+                    void *y, void *total, float *rstd, void *codes, int64_t stride, float *scales,
+                    int64_t rows, int C, cudaStream_t s);
+int64_t rms_bwd_workspace_bytes(int64_t rows, int C);
+void launch_rms_bwd(const void *g, int dtype, const void *gt, const void *x, const float *rstd,
+                    const void *w, int pdt, void *gx, void *gw, float *ws, int64_t rows, int C,
+                    cudaStream_t s);
+
+// rows8.cu -- rows of C values of type dtype to and from codes (rows of `stride`
+// bytes) and f32 scales.
+void launch_row_quantize(const void *x, int dtype, void *codes, int64_t stride, float *scales,
+                         int64_t rows, int C, cudaStream_t s);
+void launch_row_dequantize(const void *codes, int64_t stride, const float *scales, void *x, int dtype,
+                           int64_t rows, int C, cudaStream_t s);
+
+// int8_linear.cu -- y (T, N) of type ydt from codes xc (T, K) and wc (N, K) in rows
+// of xstride and wstride bytes; b may be null.
+void launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const void *wc, int64_t wstride,
+                        const float *ws, const void *b, int bdt, void *y, int ydt, int64_t T, int64_t N,
+                        int K, cudaStream_t s);
+
 }  // namespace fmhc

@@ -62,6 +62,14 @@ _SIGNATURES = {
     "fmhc_layer_norm_bwd_workspace_size": [_i64, _i64],
     "fmhc_layer_norm_bwd": [_vp, _int, _vp, _vp, _int, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp,
                             _i64, _i64, _i64, _vp],
+    "fmhc_rms_norm_fwd": [_vp, _int, _vp, _vp, _int, ctypes.c_float, _vp, _vp, _vp, _i64, _i64, _vp],
+    "fmhc_rms_norm_fwd_int8": [_vp, _int, _vp, _vp, _int, ctypes.c_float, _vp, _i64, _vp, _vp, _i64,
+                               _i64, _vp],
+    "fmhc_rms_norm_bwd_workspace_size": [_i64, _i64],
+    "fmhc_rms_norm_bwd": [_vp, _int, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _i64, _i64, _i64, _vp],
+    "fmhc_row_quantize": [_vp, _int, _vp, _i64, _vp, _i64, _i64, _vp],
+    "fmhc_row_dequantize": [_vp, _i64, _vp, _vp, _int, _i64, _i64, _vp],
+    "fmhc_int8_linear": [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _int, _vp, _int, _i64, _i64, _i64, _vp],
 }
 _RESTYPES = {
     "fmhc_last_error": ctypes.c_char_p,
@@ -70,6 +78,7 @@ _RESTYPES = {
     "fmhc_k2_bwd_workspace_size": _i64,
     "fmhc_k1_bwd_q8_workspace_size": _i64,
     "fmhc_layer_norm_bwd_workspace_size": _i64,
+    "fmhc_rms_norm_bwd_workspace_size": _i64,
 }
 
 STATUS = {

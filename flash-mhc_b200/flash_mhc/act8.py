@@ -397,9 +397,10 @@ for _name in ("act_quantize", "act_dequantize"):
     _lib.impl(_name, torch.library.fallthrough_kernel, "Autograd")
 
 
-def _register_no_derivative(name: str, cuda_impl) -> None:
-    """Op ``name``: a backward through its results raises, but for codes and scales,
-    which are outside autograd."""
+def _register_no_derivative(name: str, cuda_impl, why: str = "MHCLiteBlock(checkpoint_format=...) "
+                            "differentiates through its own functions") -> None:
+    """Op ``name``: a backward through its results raises, but for codes and scales in
+    whole numbers, which are outside autograd."""
 
     def make_function(run):
         class NoDerivative(torch.autograd.Function):
@@ -413,8 +414,7 @@ def _register_no_derivative(name: str, cuda_impl) -> None:
 
             @staticmethod
             def backward(ctx, *_):
-                raise RuntimeError(f"flash_mhc::{name} has no derivative (MHCLiteBlock(checkpoint_format=...) "
-                                   "differentiates through its own functions)")
+                raise RuntimeError(f"flash_mhc::{name} has no derivative ({why})")
 
         return NoDerivative
 

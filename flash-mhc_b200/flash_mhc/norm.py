@@ -1,4 +1,4 @@
-"""Layer norm for the layers that an mHC-lite block wraps: forward, backward, and an 8-bit input checkpoint.
+"""Norms for the layers that an mHC-lite block wraps: layer norm, with an 8-bit input checkpoint, and root-mean-square norm.
 
 * ops ``layer_norm`` / ``layer_norm_backward``: y, mean and rstd; the gradients
   of x, weight and bias in one pass over x and the output's gradient.
@@ -18,6 +18,16 @@ the row's spread: rows whose mean is much larger than their spread want x kept a
 it is.  The error is, with e the scale byte and a the largest value of a block of
 32, at most 2^(e - 128), which is below a / 127, for int8, and at most 2^-4 of each
 value or 2^(e - 137), which is below a / 2^17, whichever is larger, for e4m3.
+
+Root-mean-square norm (y = x / sqrt(mean(x^2) + eps) * weight):
+
+* ops ``rms_norm`` and ``add_rms_norm``: y and rstd; with a residual, of
+  total = x + residual rounded to x's type, which is returned too.
+* op ``rms_norm_backward``: the gradients of what is normalised, to which the
+  gradient of total is added, and of weight, in one pass.
+* :func:`rms_norm`, :func:`add_rms_norm` and :class:`RMSNorm` (parameters and
+  state_dict of ``torch.nn.RMSNorm``).  Types, ``rstd`` and second derivatives
+  are as for layer norm; its output in 8 bits is in ``flash_mhc.int8``.
 """
 
 from __future__ import annotations
@@ -42,6 +52,14 @@ _lib.define(
 )
 _lib.define(
     "layer_norm_backward_q8(Tensor grad_out, Tensor codes, Tensor scales, Tensor mean, Tensor rstd, Tensor? weight, Tensor? bias) -> (Tensor grad_x, Tensor grad_weight, Tensor grad_bias)"
+)
+_lib.define("rms_norm(Tensor x, Tensor? weight, float eps) -> (Tensor y, Tensor rstd)")
+_lib.define(
+    "add_rms_norm(Tensor x, Tensor residual, Tensor? weight, float eps) -> (Tensor y, Tensor total, Tensor rstd)"
+)
+# x: what was normalised (add_rms_norm's total).  grad_weight is empty where the weight is missing.
+_lib.define(
+    "rms_norm_backward(Tensor grad_out, Tensor? grad_total, Tensor x, Tensor rstd, Tensor? weight) -> (Tensor grad_x, Tensor grad_weight)"
 )
 
 
@@ -118,6 +136,57 @@ def _backward(op: str, grad_out, x, codes, scales, mean, rstd, weight, bias):
     return grad_x, grad_w, grad_b
 
 
+def _residual(op: str, x, residual):
+    """``residual`` beside ``x`` (already checked): of its shape and type, contiguous."""
+    _shape(op, "residual", residual, x.shape)
+    if residual.dtype != x.dtype:
+        raise ValueError(f"flash_mhc::{op}: x and residual must have one type (got {x.dtype} and {residual.dtype})")
+    return residual.contiguous()
+
+
+def _rms_forward(op: str, x, residual, weight, eps: float):
+    x = _act(op, "x", x)
+    _same_device(op, x, residual=residual, weight=weight)
+    weight, _, pdt = _params(op, x.shape[-1], weight, None)
+    total = None
+    if residual is not None:
+        residual, total = _residual(op, x, residual), torch.empty_like(x)
+    y, rstd = torch.empty_like(x), x.new_empty(x.shape[:-1], dtype=torch.float32)
+    _launch(x, "fmhc_rms_norm_fwd", x.data_ptr(), _DTYPES[x.dtype], _ptr(residual), _ptr(weight), pdt,
+            eps, y.data_ptr(), _ptr(total), rstd.data_ptr(), _rows(x), x.shape[-1])
+    return (y, rstd) if total is None else (y, total, rstd)
+
+
+def _rms_backward(op: str, grad_out, grad_total, x, rstd, weight):
+    grad_out = _act(op, "grad_out", grad_out)
+    _same_device(op, grad_out, grad_total=grad_total, x=x, rstd=rstd, weight=weight)
+    for name, t in (("x", x), ("grad_total", grad_total)):
+        if t is not None:
+            _shape(op, name, t, grad_out.shape)
+            if t.dtype != grad_out.dtype:
+                raise ValueError(f"flash_mhc::{op}: grad_out and {name} must have one type "
+                                 f"(got {grad_out.dtype} and {t.dtype})")
+    x = x.contiguous()
+    grad_total = None if grad_total is None else grad_total.contiguous()
+    _shape(op, "rstd", rstd, grad_out.shape[:-1])
+    if rstd.dtype != torch.float32:
+        raise ValueError(f"flash_mhc::{op}: rstd must be float32 (got {rstd.dtype})")
+    rstd = rstd.contiguous()
+    C, rows = grad_out.shape[-1], _rows(grad_out)
+    weight, _, pdt = _params(op, C, weight, None)
+    grad_x = torch.empty_like(grad_out)
+    ws, ws_bytes, _keep = None, 0, None
+    if weight is None:
+        grad_w = grad_out.new_empty((0,), dtype=torch.float32)
+    else:
+        grad_w = torch.empty_like(weight)
+        ws, ws_bytes, _keep = _workspace(grad_out, "fmhc_rms_norm_bwd_workspace_size", rows, C)
+    _launch(grad_out, "fmhc_rms_norm_bwd", grad_out.data_ptr(), _DTYPES[grad_out.dtype], _ptr(grad_total),
+            x.data_ptr(), rstd.data_ptr(), _ptr(weight), pdt, grad_x.data_ptr(),
+            None if weight is None else grad_w.data_ptr(), ws, ws_bytes, rows, C)
+    return grad_x, grad_w
+
+
 # -------------------------------------------------------------------- fakes
 
 
@@ -146,6 +215,25 @@ def _layer_norm_backward_q8_fake(grad_out, codes, scales, mean, rstd, weight, bi
     return _layer_norm_backward_fake(grad_out, codes, mean, rstd, weight, bias)
 
 
+@torch.library.register_fake("flash_mhc::rms_norm")
+def _rms_norm_fake(x, weight, eps):
+    return (torch.empty(x.shape, device=x.device, dtype=x.dtype),
+            torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32))
+
+
+@torch.library.register_fake("flash_mhc::add_rms_norm")
+def _add_rms_norm_fake(x, residual, weight, eps):
+    y, rstd = _rms_norm_fake(x, weight, eps)
+    return y, torch.empty_like(y), rstd
+
+
+@torch.library.register_fake("flash_mhc::rms_norm_backward")
+def _rms_norm_backward_fake(grad_out, grad_total, x, rstd, weight):
+    return (torch.empty(grad_out.shape, device=grad_out.device, dtype=grad_out.dtype),
+            torch.empty(0, device=grad_out.device, dtype=torch.float32) if weight is None
+            else torch.empty(weight.shape, device=weight.device, dtype=weight.dtype))
+
+
 # --------------------------------------------------------------------- CUDA
 
 
@@ -169,6 +257,21 @@ def _layer_norm_backward_q8_cuda(grad_out, codes, scales, mean, rstd, weight, bi
     return _backward("layer_norm_backward_q8", grad_out, None, codes, scales, mean, rstd, weight, bias)
 
 
+@torch.library.impl(_lib, "rms_norm", "CUDA")
+def _rms_norm_cuda(x, weight, eps):
+    return _rms_forward("rms_norm", x, None, weight, eps)
+
+
+@torch.library.impl(_lib, "add_rms_norm", "CUDA")
+def _add_rms_norm_cuda(x, residual, weight, eps):
+    return _rms_forward("add_rms_norm", x, residual, weight, eps)
+
+
+@torch.library.impl(_lib, "rms_norm_backward", "CUDA")
+def _rms_norm_backward_cuda(grad_out, grad_total, x, rstd, weight):
+    return _rms_backward("rms_norm_backward", grad_out, grad_total, x, rstd, weight)
+
+
 # ------------------------------------------------------------------ autograd
 
 
@@ -179,12 +282,20 @@ class _GradsOnce(torch.autograd.Function):
     (codes never do, although they depend on x)."""
 
     @staticmethod
-    def forward(ctx, mark, op, *args):
+    def forward(ctx, mark, name, op, *args):
+        ctx.name = name
         return op(*args)
 
     @staticmethod
     def backward(ctx, *_):
-        raise RuntimeError("flash_mhc::layer_norm has no second derivative")
+        raise RuntimeError(f"flash_mhc::{ctx.name} has no second derivative")
+
+
+def _grads(name: str, op, gy, *args):
+    """The gradients that ``op`` gives, by way of _GradsOnce under create_graph=True."""
+    if torch.is_grad_enabled():
+        return _GradsOnce.apply(gy.new_empty(0).requires_grad_(), name, op, gy, *args)
+    return op(gy, *args)
 
 
 def _register_norm(name: str, cuda_impl, backward: str, kept) -> None:
@@ -206,11 +317,7 @@ def _register_norm(name: str, cuda_impl, backward: str, kept) -> None:
             def backward(ctx, gy, *_):
                 if gy is None:
                     return (None, None, None, None, *ctx.rest)
-                if torch.is_grad_enabled():  # create_graph=True
-                    mark = gy.new_empty(0).requires_grad_()
-                    grads = _GradsOnce.apply(mark, backward_op, gy, *ctx.saved_tensors)
-                else:
-                    grads = backward_op(gy, *ctx.saved_tensors)
+                grads = _grads("layer_norm", backward_op, gy, *ctx.saved_tensors)
                 need = ctx.needs_input_grad[1:]
                 return (None, *(g if n else None for g, n in zip(grads, need)), *ctx.rest)
 
@@ -221,6 +328,41 @@ def _register_norm(name: str, cuda_impl, backward: str, kept) -> None:
 
 _register_norm("layer_norm", _layer_norm_cuda, "layer_norm_backward", lambda x, out: (x,))
 _register_norm("layer_norm_q8", _layer_norm_q8_cuda, "layer_norm_backward_q8", lambda x, out: out[3:])
+
+
+def _register_rms_norm(name: str, cuda_impl, add: bool) -> None:
+    """Op ``name``: keeps what it normalised, which is x, or with ``add`` its output total."""
+    backward_op = torch.ops.flash_mhc.rms_norm_backward
+
+    def make_function(run):
+        class RMSNormFunction(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, keyset, *args):
+                out = run(keyset, args)
+                ctx.save_for_backward(out[1] if add else args[0], out[-1], args[-2])
+                ctx.mark_non_differentiable(out[-1])
+                ctx.set_materialize_grads(False)
+                return out
+
+            @staticmethod
+            def backward(ctx, gy, *rest):
+                gt = rest[0] if add else None
+                if gy is None:  # nothing through the norm
+                    gx, gw = gt, None
+                else:
+                    x, rstd, weight = ctx.saved_tensors
+                    gx, gw = _grads(name, backward_op, gy, gt, x, rstd, weight)
+                need = ctx.needs_input_grad[1:]
+                grads = (gx, gx, gw) if add else (gx, gw)
+                return (None, *(g if n else None for g, n in zip(grads, need)), None)
+
+        return RMSNormFunction
+
+    _register_autograd(name, cuda_impl, make_function)
+
+
+_register_rms_norm("rms_norm", _rms_norm_cuda, add=False)
+_register_rms_norm("add_rms_norm", _add_rms_norm_cuda, add=True)
 
 
 # ---------------------------------------------------------------- public names
@@ -271,3 +413,51 @@ class LayerNorm(nn.Module):
         if x.is_cuda and x.dtype in _DTYPES:
             return layer_norm(x, self.weight, self.bias, self.eps, self.checkpoint_format)
         return F.layer_norm(x, (self.hidden_size,), self.weight, self.bias, self.eps)
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6) -> torch.Tensor:
+    """Root-mean-square norm over the last dimension of a CUDA tensor, differentiable in x and weight."""
+    return torch.ops.flash_mhc.rms_norm(x, weight, eps)[0]
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None,
+                 eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """(rms_norm(total), total) with total = x + residual rounded to x's type, in one pass.
+
+    Differentiable in x, residual and weight; x and residual have one shape and type.
+    """
+    return torch.ops.flash_mhc.add_rms_norm(x, residual, weight, eps)[:2]
+
+
+class RMSNorm(nn.Module):
+    """``torch.nn.RMSNorm`` over the last dimension, with the same parameter and state_dict.
+
+    ``forward(x)`` gives y, ``forward(x, residual)`` (y, total) with
+    total = x + residual.  CUDA inputs of float32, bfloat16 or float16 take the
+    fused kernels, every other input torch's.
+    """
+
+    def __init__(self, hidden_size: int, eps: float = 1e-6, elementwise_affine: bool = True, device=None,
+                 dtype=None) -> None:
+        super().__init__()
+        self.hidden_size = hidden_size
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(hidden_size, device=device, dtype=dtype)) if elementwise_affine else None
+
+    def extra_repr(self) -> str:
+        return f"{self.hidden_size}, eps={self.eps}"
+
+    def _check(self, x: torch.Tensor) -> bool:
+        """Whether the fused kernels take ``x``."""
+        if x.shape[-1:] != (self.hidden_size,):
+            raise ValueError(f"RMSNorm: expected a last dimension of {self.hidden_size} (got {tuple(x.shape)})")
+        return x.is_cuda and x.dtype in _DTYPES
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        if self._check(x):
+            if residual is None:
+                return rms_norm(x, self.weight, self.eps)
+            return add_rms_norm(x, residual, self.weight, self.eps)
+        total = x if residual is None else x + residual
+        y = F.rms_norm(total, (self.hidden_size,), self.weight, self.eps)
+        return y if residual is None else (y, total)

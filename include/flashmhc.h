@@ -408,6 +408,61 @@ FMHC_API int fmhc_layer_norm_bwd(const void *grad_y, int x_dtype, const void *x,
                                  void *grad_bias, void *workspace, int64_t workspace_bytes,
                                  int64_t rows, int64_t C, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Root-mean-square norm over the last dimension of v (rows, C), where v is x, or
+ * with a residual x + residual rounded to x's type, which is written to total
+ * (residual and total go together; no output may overlap an input):
+ *   rstd = 1 / sqrt(<v^2> + eps)   (f32, (rows,)),   y = v rstd weight   (x_dtype)
+ * weight (C,) of param_dtype, or NULL (1).
+ * No counterpart in the reference (its users take torch's).
+ */
+FMHC_API int fmhc_rms_norm_fwd(const void *x, int x_dtype, const void *residual,
+                               const void *weight, int param_dtype, float eps, void *y,
+                               void *total, float *rstd, int64_t rows, int64_t C, void *stream);
+/* Backward, with x the normalised v, xh = v rstd and gw = grad_y weight:
+ *   grad_x      = rstd (gw - xh <gw xh>) + grad_total      (x_dtype)
+ *   grad_weight = sum over rows of grad_y xh                (param_dtype)
+ * grad_total and grad_weight may be NULL; sums are f32 in a fixed order.  With a
+ * residual grad_x is the gradient of x and of the residual.  rows == 0 writes a
+ * zero grad_weight.  `workspace` (256-byte aligned, at least
+ * fmhc_rms_norm_bwd_workspace_size(rows, C) bytes; may be NULL when grad_weight is)
+ * holds partial sums. */
+FMHC_API int64_t fmhc_rms_norm_bwd_workspace_size(int64_t rows, int64_t C);
+FMHC_API int fmhc_rms_norm_bwd(const void *grad_y, int x_dtype, const void *grad_total,
+                               const void *x, const float *rstd, const void *weight,
+                               int param_dtype, void *grad_x, void *grad_weight,
+                               void *workspace, int64_t workspace_bytes, int64_t rows,
+                               int64_t C, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Rows in 8 bits, for linear layers: one int8 code per value and one f32 scale per
+ * row.  With a the row's largest magnitude, at least 2^-100: scale = a / 127, code =
+ * v (127 / a) rounded to nearest even, value = code scale.  A row with an infinity
+ * or a NaN has codes 0 and the scale NaN.  Rows of codes are codes_stride bytes
+ * apart; fmhc_int8_linear takes them at multiples of 16.  The bytes between a row's
+ * end and the next row's start are neither read nor written.
+ */
+FMHC_API int fmhc_row_quantize(const void *x, int x_dtype, void *codes, int64_t codes_stride,
+                               float *scales, int64_t rows, int64_t C, void *stream);
+/* codes, scales -> x, rounded once to x_dtype. */
+FMHC_API int fmhc_row_dequantize(const void *codes, int64_t codes_stride, const float *scales,
+                                 void *x, int x_dtype, int64_t rows, int64_t C, void *stream);
+/* fmhc_rms_norm_fwd with y as a row of codes and a scale, not rounded in between. */
+FMHC_API int fmhc_rms_norm_fwd_int8(const void *x, int x_dtype, const void *residual,
+                                    const void *weight, int param_dtype, float eps, void *codes,
+                                    int64_t codes_stride, float *scales, void *total,
+                                    int64_t rows, int64_t C, void *stream);
+/* Linear layer: y[t,n] = (scales[t] weight_scales[n]) sum_k codes[t,k] weight_codes[n,k]
+ * + bias[n], rounded once to y_dtype.  The sum is exact (K < 2^17); the two scales
+ * are multiplied first, in f32.  codes (T, K) and weight_codes (N, K) are 16-byte
+ * aligned with strides that are multiples of 16; bias (N,) of bias_dtype, or NULL;
+ * y (T, N) is dense. */
+FMHC_API int fmhc_int8_linear(const void *codes, int64_t codes_stride, const float *scales,
+                              const void *weight_codes, int64_t weight_stride,
+                              const float *weight_scales, const void *bias, int bias_dtype,
+                              void *y, int y_dtype, int64_t T, int64_t N, int64_t K,
+                              void *stream);
+
 #ifdef __cplusplus
 }
 #endif
