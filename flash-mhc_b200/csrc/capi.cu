@@ -77,8 +77,10 @@ int fmhc_check_device_error(int *code) {
   if (cudaDeviceSynchronize() != cudaSuccess)
     return fail(FMHC_ERR_CUDA, "fmhc_check_device_error: %s", cudaGetErrorString(cudaGetLastError()));
   unsigned v = 0;
-  if (fmhc::read_device_error(&v)) return fail(FMHC_ERR_CUDA, "fmhc_check_device_error: symbol copy failed");
-  *code = int(v);
+  unsigned v8 = 0;
+  if (fmhc::read_device_error(&v) || fmhc::read_int8_linear_error(&v8))
+    return fail(FMHC_ERR_CUDA, "fmhc_check_device_error: symbol copy failed");
+  *code = int(v != 0 ? v : v8);
   return ok();
 }
 
@@ -888,8 +890,10 @@ int fmhc_int8_linear(const void *codes, int64_t codes_stride, const float *scale
   FMHC_REQUIRE_ALIGN16(w, codes); FMHC_REQUIRE_ALIGN16(w, weight_codes);
   FMHC_REQUIRE_ALIGN_TO(w, scales, 4); FMHC_REQUIRE_ALIGN_TO(w, weight_scales, 4);
   FMHC_REQUIRE_ALIGN_TO(w, bias, dtype_size(bias_dtype)); FMHC_REQUIRE_ALIGN_TO(w, y, dtype_size(y_dtype));
-  fmhc::launch_int8_linear(codes, codes_stride, scales, weight_codes, weight_stride, weight_scales, bias,
-                           bias_dtype, y, y_dtype, T, N, int(K), (cudaStream_t)stream);
+  if (int e = fmhc::launch_int8_linear(codes, codes_stride, scales, weight_codes, weight_stride,
+                                       weight_scales, bias, bias_dtype, y, y_dtype, T, N, int(K),
+                                       (cudaStream_t)stream))
+    return e;
   return check_launch(w);
 }
 

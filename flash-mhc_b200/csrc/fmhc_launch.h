@@ -136,9 +136,12 @@ void launch_row_dequantize(const void *codes, int64_t stride, const float *scale
                            int64_t rows, int C, cudaStream_t s);
 
 // int8_linear.cu -- y (T, N) of type ydt from codes xc (T, K) and wc (N, K) in rows
-// of xstride and wstride bytes; b may be null.
-void launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const void *wc, int64_t wstride,
-                        const float *ws, const void *b, int bdt, void *y, int ydt, int64_t T, int64_t N,
-                        int K, cudaStream_t s);
+// of xstride and wstride bytes (multiples of 16, as xc and wc are); b may be null.
+// Returns 0 or an fmhc_status code with the error's text set.
+int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const void *wc, int64_t wstride,
+                       const float *ws, const void *b, int bdt, void *y, int ydt, int64_t T, int64_t N,
+                       int K, cudaStream_t s);
+// Reads and clears this file's device error word.
+int read_int8_linear_error(unsigned *code);
 
 }  // namespace fmhc

@@ -1,18 +1,55 @@
-// Linear layer from 8-bit rows (rows8.cuh):
+// Linear layer from 8-bit rows (rows8.cuh) on the 5th-generation tensor cores:
 //
 //   y[t, n] = (xs[t] ws[n]) sum_k xc[t, k] wc[n, k] + b[n],  rounded once
 //
 // The sum of products is a whole number and exact (K < 2^17 keeps it within 32
-// bits); the product of the two scales is taken first, in f32.
+// bits, whatever the order); the product of the two scales is taken first, in f32.
+//
+// The weight is the MMA's A operand (M = output columns n) and the activations
+// are B (N = rows t), so that a thread of the epilogue holds one output column of
+// many rows: its weight scale and bias stay in registers, a row's scale is one
+// shared-memory word for the warp, a warp's stores of a row are contiguous for any
+// N and any alignment of y, and few rows of activations make a narrow tile instead
+// of an empty one.  TMA fills K's and the tiles' ends with zeros.
+//
+// Two kernels: pairs of CTAs that keep 256 x 256 tiles in TMEM (many tiles), and
+// clusters that split K of one 128 x tn tile each (few).  Every mbarrier wait is
+// bounded (sm100_ptx.cuh); outputs that a kernel gave up on are NaN.
+#include <cuda.h>
+#include <stdint.h>
+
+#include <algorithm>
+
 #include "act8.cuh"
 #include "fmhc_launch.h"
+#include "grid.cuh"
 #include "rows8.cuh"
+#include "sm100_ptx.cuh"
+#include "tma_map.h"
 
 namespace fmhc {
 
 using namespace act8;
+using namespace sm100;
 
 namespace {
+
+constexpr int kBK = 128;                // bytes of K per stage: one swizzle row
+constexpr int kBM = 128;                // output columns per CTA
+constexpr int kATile = kBM * kBK;       // 16 KiB
+constexpr int kThreads = 192;           // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+constexpr int kEpiThreads = 128;
+constexpr int kMaxTn = 256;
+
+struct Args {
+  const float *xs, *ws;
+  const void *bias;
+  int bias_dtype;
+  int64_t T, N;
+  int K;
+  int tn;   // rows t per tile
+  int tiles_n, tiles_t;
+};
 
 __device__ __forceinline__ float bias1(const void *b, int dtype, int64_t n) {
   if (b == nullptr) return 0.f;
@@ -21,50 +58,452 @@ __device__ __forceinline__ float bias1(const void *b, int dtype, int64_t n) {
   return __half2float(reinterpret_cast<const __half *>(b)[n]);
 }
 
-// A 32 x 32 tile of y per block of 256 threads; 64 columns of K at a time.
+// MMAs of one stage that hold something of K: 32 bytes each.
+__device__ __forceinline__ int mmas_of(int kb, int K) { return min((K - kb * kBK + 31) >> 5, 4); }
+
+// 32 rows of a column: `rows` of them are stored, from y on.
 template <class E>
-__global__ void __launch_bounds__(256)
-int8_linear_tile_kernel(const int8_t *__restrict__ xc, int64_t xstride, const float *__restrict__ xs,
-                        const int8_t *__restrict__ wc, int64_t wstride, const float *__restrict__ ws,
-                        const void *__restrict__ b, int bdt, E *__restrict__ y, int64_t T, int64_t N, int K) {
-  __shared__ int xt[32][17], wt[32][17];
-  pdl_wait();
-  const int64_t n0 = int64_t(blockIdx.x) * 32;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  for (int64_t t0 = int64_t(blockIdx.y) * 32; t0 < T; t0 += int64_t(gridDim.y) * 32) {
-    int acc[4] = {0, 0, 0, 0};
-    for (int k0 = 0; k0 < K; k0 += 64) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < 32 * 64; i += 256) {
-        const int r = i >> 6, k = i & 63;
-        reinterpret_cast<int8_t *>(&xt[r][0])[k] = t0 + r < T && k0 + k < K ? xc[(t0 + r) * xstride + k0 + k] : int8_t(0);
-        reinterpret_cast<int8_t *>(&wt[r][0])[k] = n0 + r < N && k0 + k < K ? wc[(n0 + r) * wstride + k0 + k] : int8_t(0);
-      }
-      __syncthreads();
+__device__ __forceinline__ void store_rows(const int (&v)[32], int rows, const float *xs, float ws, float b,
+                                           E *y, int64_t N, bool in) {
+  E o[32];
 #pragma unroll
-      for (int k = 0; k < 16; ++k)
+  for (int j = 0; j < 32; j += 4) {
+    const float4 x = *reinterpret_cast<const float4 *>(xs + j);
+    o[j] = Elem<E>::narrow1(fmaf(__int2float_rn(v[j]), x.x * ws, b));
+    o[j + 1] = Elem<E>::narrow1(fmaf(__int2float_rn(v[j + 1]), x.y * ws, b));
+    o[j + 2] = Elem<E>::narrow1(fmaf(__int2float_rn(v[j + 2]), x.z * ws, b));
+    o[j + 3] = Elem<E>::narrow1(fmaf(__int2float_rn(v[j + 3]), x.w * ws, b));
+  }
+  // No branch between the rows of a whole chunk: one per row made each wait for
+  // the latency of its own arithmetic (tiles of 256 x 256 took 20 us each).
+  if (rows >= 32) {
+    if (in) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = __dp4a(xt[ty * 4 + i][k], wt[tx][k], acc[i]);
+      for (int j = 0; j < 32; ++j, y += N) *y = o[j];
     }
-    if (n0 + tx < N)
-      for (int i = 0; i < 4; ++i) {
-        const int64_t t = t0 + ty * 4 + i;
-        if (t < T) y[t * N + n0 + tx] = Elem<E>::narrow1(fmaf(float(acc[i]), xs[t] * ws[n0 + tx], bias1(b, bdt, n0 + tx)));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j, y += N)
+      if (in && j < rows) *y = o[j];
+  }
+}
+// One column of a tile: rows t0 .. t0 + rows - 1, from this warp's lanes of TMEM.
+template <class E>
+__device__ __forceinline__ void store_column(uint32_t tmem, int rows, const float *xs, float ws, float b,
+                                             E *y, int64_t N, bool in) {
+  for (int c = 0; c < rows; c += 32) {
+    uint32_t v[32];
+    tmem_ld_32x32b_x32(tmem + uint32_t(c), v);
+    tmem_wait_ld();
+    store_rows(reinterpret_cast<const int (&)[32]>(v), rows - c, xs + c, ws, b, y + c * N, N, in);
+  }
+}
+template <class E>
+__device__ __forceinline__ void store_nan(int rows, E *y, int64_t N, bool in) {
+  for (int j = 0; j < rows; ++j, y += N)
+    if (in) *y = Elem<E>::narrow1(__uint_as_float(0x7fc00000u));
+}
+
+// ------------------------------------------------------------- pairs of CTAs
+constexpr int kPairStages = 6;
+struct alignas(1024) PairSmem {
+  uint8_t a[kPairStages][kATile];
+  uint8_t b[kPairStages][kATile];  // half of the tile's rows t: at most 128
+  alignas(16) float xs[2][kMaxTn];
+  uint64_t full[kPairStages], empty[kPairStages];
+  uint64_t tfull[2], tempty[2], mma_done;
+  uint32_t tmem_base;
+  int abort;
+};
+
+enum : unsigned { kSitePairEmpty = 0x201, kSitePairFull = 0x202, kSitePairTempty = 0x203,
+                  kSitePairTfull = 0x204, kSitePairDrain = 0x205 };
+
+// Tile `id` -> (column tile, row tile): groups of eight column tiles, all row tiles
+// of a group before the next, so that what runs at one time shares its operands
+// in L2.
+constexpr int kGroup = 8;
+__device__ __forceinline__ void tile_of(int64_t id, int tiles_n, int tiles_t, int *n, int *t) {
+  const int64_t per = int64_t(kGroup) * tiles_t;
+  const int g = int(id / per);
+  const int first = g * kGroup, size = min(tiles_n - first, kGroup);
+  const int64_t r = id - g * per;
+  *n = first + int(r % size);
+  *t = int(r / size);
+}
+
+// Persistent: pair p takes tiles p, p + pairs, ...  Barriers: `full` is the
+// leader's and counts the bytes of both CTAs' copies; a commit arrives on `empty`
+// and `tfull` of both; the epilogue warps of both arrive on the leader's `tempty`.
+template <class E>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                        E *__restrict__ y, const Args A) {
+  extern __shared__ uint8_t smem_raw[];
+  PairSmem &sm = *reinterpret_cast<PairSmem *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int *abort = &sm.abort;
+  const uint32_t rank = cluster_ctarank();
+  const int64_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int64_t tiles = int64_t(A.tiles_n) * A.tiles_t;
+  const int nk = (A.K + kBK - 1) / kBK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(smem_u32(&sm.full[s]), 1);
+      mbar_init(smem_u32(&sm.empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&sm.tfull[b]), 1);
+      mbar_init(smem_u32(&sm.tempty[b]), 8);
+    }
+    mbar_init(smem_u32(&sm.mma_done), 1);
+    sm.abort = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tmap_w);
+    prefetch_tmap(&tmap_x);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(&sm.tmem_base), 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  cluster_sync_all();  // both CTAs' barriers exist
+  const uint32_t tmem = sm.tmem_base;
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      const int half = A.tn / 2;
+      const uint32_t bytes = 2u * (kATile + uint32_t(half) * kBK);
+      bool ok = true;
+      for (int64_t id = pair; id < tiles && ok; id += pairs) {
+        int tile_n, tile_t;
+        tile_of(id, A.tiles_n, A.tiles_t, &tile_n, &tile_t);
+        const int32_t n0 = tile_n * 2 * kBM + int32_t(rank) * kBM;
+        const int32_t t0 = tile_t * A.tn + int32_t(rank) * half;
+        for (int kb = 0; kb < nk; ++kb) {
+          if (!mbar_wait_cluster(smem_u32(&sm.empty[stage]), phase ^ 1, abort, kSitePairEmpty)) { ok = false; break; }
+          const uint32_t full = smem_u32(&sm.full[stage]);
+          if (rank == 0) mbar_arrive_expect_tx(full, bytes);
+          const uint32_t lead = mapa_shared(full, 0);
+          tma_load_2d_pair(smem_u32(sm.a[stage]), &tmap_w, lead, kb * kBK, n0);
+          tma_load_2d_pair(smem_u32(sm.b[stage]), &tmap_x, lead, kb * kBK, t0);
+          ++issued;
+          if (++stage == kPairStages) { stage = 0; phase ^= 1; }
+        }
       }
+      // The leader's barriers see the last copies of both CTAs land; the other CTA
+      // leaves after it (cluster barrier below).
+      if (rank == 0) {
+        const int n = issued < kPairStages ? issued : kPairStages;
+        int s = stage;
+        uint32_t ph = phase;
+        for (int i = 0; i < n; ++i) {
+          if (--s < 0) { s = kPairStages - 1; ph ^= 1; }
+          mbar_wait(smem_u32(&sm.full[s]), ph, abort, kSitePairDrain, true);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = idesc_i8_s32(2 * kBM, A.tn);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int64_t id = pair; id < tiles && ok; id += pairs) {
+        if (!mbar_wait_cluster(smem_u32(&sm.tempty[acc]), acc_phase ^ 1, abort, kSitePairTempty)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + uint32_t(acc * 256);
+        for (int kb = 0; kb < nk; ++kb) {
+          if (!mbar_wait_cluster(smem_u32(&sm.full[stage]), phase, abort, kSitePairFull)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t ad = smem_desc(smem_u32(sm.a[stage]), 16, 1024, 2);
+          const uint64_t bd = smem_desc(smem_u32(sm.b[stage]), 16, 1024, 2);
+          const int m = mmas_of(kb, A.K);
+          for (int k = 0; k < m; ++k)  // 32 bytes of K on: 2 in the descriptors' units
+            mma_i8_ss_pair(d, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0);
+          mma_commit_pair(smem_u32(&sm.empty[stage]));
+          if (++stage == kPairStages) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        mma_commit_pair(smem_u32(&sm.tfull[acc]));
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      }
+      // All MMAs issued by this thread complete before TMEM is freed.
+      mma_commit_pair(smem_u32(&sm.mma_done));
+      mbar_wait(smem_u32(&sm.mma_done), 0, abort, kSitePairDrain, true);
+    }
+  } else {
+    const int q = warp & 3, me = int(threadIdx.x) - 64;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int64_t id = pair; id < tiles; id += pairs) {
+      int tile_n, tile_t;
+      tile_of(id, A.tiles_n, A.tiles_t, &tile_n, &tile_t);
+      const int64_t n = int64_t(tile_n) * 2 * kBM + rank * kBM + q * 32 + lane;
+      const int64_t t0 = int64_t(tile_t) * A.tn;
+      const int rows = int(min(A.T - t0, int64_t(A.tn)));
+      const bool in = n < A.N;
+      // This buffer was last read two tiles ago, before the barrier of the tile between.
+      for (int i = me; i < rows; i += kEpiThreads) sm.xs[acc][i] = A.xs[t0 + i];
+      const float ws = in ? A.ws[n] : 0.f;
+      const float b = in ? bias1(A.bias, A.bias_dtype, n) : 0.f;
+      named_bar_sync(1, kEpiThreads);
+      E *to = y + t0 * A.N + n;
+      ok = ok && mbar_wait_cluster(smem_u32(&sm.tfull[acc]), acc_phase, abort, kSitePairTfull);
+      ok = __all_sync(0xffffffffu, ok);  // the loads below take whole warps
+      if (!ok) {
+        store_nan(rows, to, A.N, in);
+        continue;
+      }
+      tc_fence_after();
+      store_column(tmem + (uint32_t(q * 32) << 16) + uint32_t(acc * 256), rows, sm.xs[acc], ws, b, to, A.N, in);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&sm.tempty[acc]), 0));
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // nothing arrives at the other CTA any more
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 
+// ------------------------------------------------------- clusters that split K
+// A cluster of S CTAs takes one tile of 128 columns and tn rows; CTA r runs the
+// stages [r nk / S, (r + 1) nk / S).  The partial sums go to each CTA's own shared
+// memory (the stages', which its MMAs have finished with), and after a cluster
+// barrier CTA r adds those of rows r, r + S, ... over the cluster.
+struct SplitTail {
+  uint64_t full[16], empty[16];
+  uint64_t tfull;
+  alignas(16) float xs[kMaxTn];
+  uint32_t tmem_base;
+  int abort;
+};
+
+enum : unsigned { kSiteSplitEmpty = 0x211, kSiteSplitFull = 0x212, kSiteSplitTfull = 0x214,
+                  kSiteSplitDrain = 0x215 };
+
+template <class E>
+__global__ void __launch_bounds__(kThreads)
+int8_linear_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                         E *__restrict__ y, const Args A, int S, int stages, int tmem_cols) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *const base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stage_bytes = kATile + A.tn * kBK;
+  SplitTail &sm = *reinterpret_cast<SplitTail *>(base + stages * stage_bytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int *abort = &sm.abort;
+  const uint32_t rank = S > 1 ? cluster_ctarank() : 0u;
+  const int64_t id = blockIdx.x / unsigned(S);
+  const int tile_n = int(id % A.tiles_n), tile_t = int(id / A.tiles_n);
+  const int nk = (A.K + kBK - 1) / kBK;
+  const int kb0 = int(rank) * nk / S, kb1 = (int(rank) + 1) * nk / S;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(smem_u32(&sm.full[s]), 1);
+      mbar_init(smem_u32(&sm.empty[s]), 1);
+    }
+    mbar_init(smem_u32(&sm.tfull), 1);
+    sm.abort = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tmap_w);
+    prefetch_tmap(&tmap_x);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&sm.tmem_base), uint32_t(tmem_cols));
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  pdl_wait();
+
+  const int q = warp & 3;
+  const int64_t n = int64_t(tile_n) * kBM + q * 32 + lane;
+  const int64_t t0 = int64_t(tile_t) * A.tn;
+  const int rows = int(min(A.T - t0, int64_t(A.tn)));
+  const bool in = n < A.N;
+  int *const part = reinterpret_cast<int *>(base);  // [rows][128]
+  bool ok = true;
+  float ws = 0.f, b = 0.f;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(smem_u32(&sm.empty[stage]), phase ^ 1, abort, kSiteSplitEmpty)) break;
+        const uint32_t full = smem_u32(&sm.full[stage]);
+        mbar_arrive_expect_tx(full, uint32_t(stage_bytes));
+        const uint32_t a = smem_u32(base) + uint32_t(stage * stage_bytes);
+        tma_load_2d(a, &tmap_w, full, kb * kBK, tile_n * kBM);
+        tma_load_2d(a + kATile, &tmap_x, full, kb * kBK, int32_t(t0));
+        ++issued;
+        if (++stage == stages) { stage = 0; phase ^= 1; }
+      }
+      const int left = issued < stages ? issued : stages;
+      for (int i = 0; i < left; ++i) {
+        if (--stage < 0) { stage = stages - 1; phase ^= 1; }
+        mbar_wait(smem_u32(&sm.full[stage]), phase, abort, kSiteSplitDrain, true);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = idesc_i8_s32(kBM, A.tn);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(smem_u32(&sm.full[stage]), phase, abort, kSiteSplitFull)) break;
+        tc_fence_after();
+        const uint32_t a = smem_u32(base) + uint32_t(stage * stage_bytes);
+        const uint64_t ad = smem_desc(a, 16, 1024, 2), bd = smem_desc(a + kATile, 16, 1024, 2);
+        const int m = mmas_of(kb, A.K);
+        for (int k = 0; k < m; ++k) mma_i8_ss(tmem, ad + 2 * k, bd + 2 * k, idesc, kb > kb0 || k > 0);
+        mma_commit(smem_u32(&sm.empty[stage]));
+        if (++stage == stages) { stage = 0; phase ^= 1; }
+      }
+      // Also after a wait that gave up: everything issued is done before TMEM is freed.
+      mma_commit(smem_u32(&sm.tfull));
+      mbar_wait(smem_u32(&sm.tfull), 0, abort, kSiteSplitDrain, true);
+    }
+  } else {
+    const int me = int(threadIdx.x) - 64;
+    for (int i = me; i < rows; i += kEpiThreads) sm.xs[i] = A.xs[t0 + i];
+    ws = in ? A.ws[n] : 0.f;
+    b = in ? bias1(A.bias, A.bias_dtype, n) : 0.f;
+    named_bar_sync(1, kEpiThreads);
+    ok = mbar_wait(smem_u32(&sm.tfull), 0, abort, kSiteSplitTfull) && *abort == 0;
+    ok = __all_sync(0xffffffffu, ok);  // the loads below take whole warps
+    tc_fence_after();
+    if (S == 1) {
+      E *to = y + t0 * A.N + n;
+      if (ok) store_column(tmem + (uint32_t(q * 32) << 16), rows, sm.xs, ws, b, to, A.N, in);
+      else store_nan(rows, to, A.N, in);
+    } else if (ok) {
+      for (int c = 0; c < rows; c += 32) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tmem + (uint32_t(q * 32) << 16) + uint32_t(c), v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (c + j < rows) part[(c + j) * kBM + q * 32 + lane] = int(v[j]);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  if (S > 1) {
+    cluster_sync_all();  // the cluster's partial sums are written
+    if (warp >= 2) {
+      for (int s = 0; s < S; ++s) ok = ok && ld_cluster_s32(mapa_shared(smem_u32(&sm.abort), uint32_t(s))) == 0;
+      const uint32_t own = smem_u32(part) + uint32_t(q * 32 + lane) * 4u;
+      for (int r = int(rank); r < rows; r += S) {
+        int v = 0;
+        for (int s = 0; s < S; ++s) v += ld_cluster_s32(mapa_shared(own + uint32_t(r) * kBM * 4u, uint32_t(s)));
+        const float f = ok ? fmaf(__int2float_rn(v), sm.xs[r] * ws, b) : __uint_as_float(0x7fc00000u);
+        if (in) y[(t0 + r) * A.N + n] = Elem<E>::narrow1(f);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();  // no CTA leaves while another reads its shared memory
+  } else {
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, uint32_t(tmem_cols));
+  }
+}
+
+// ------------------------------------------------------------------ launchers
+bool make_map(CUtensorMap *m, const void *base, int K, int64_t rows, int64_t stride, int box_rows) {
+  const auto fn = encode_fn();
+  if (fn == nullptr) return false;
+  cuuint64_t dims[2] = {cuuint64_t(K), cuuint64_t(rows)};
+  cuuint64_t strides[1] = {cuuint64_t(stride)};
+  cuuint32_t box[2] = {kBK, cuuint32_t(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
 }  // namespace
 
-void launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const void *wc, int64_t wstride,
-                        const float *ws, const void *b, int bdt, void *y, int ydt, int64_t T, int64_t N,
-                        int K, cudaStream_t s) {
+int read_int8_linear_error(unsigned *code) {
+  unsigned v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, sm100::g_device_error, sizeof(v)) != cudaSuccess) return 5;
+  if (v && cudaMemcpyToSymbol(sm100::g_device_error, &zero, sizeof(zero)) != cudaSuccess) return 5;
+  *code = v;
+  return 0;
+}
+
+int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const void *wc, int64_t wstride,
+                       const float *ws, const void *b, int bdt, void *y, int ydt, int64_t T, int64_t N,
+                       int K, cudaStream_t s) {
+  const int sms = sm_count();
+  const int nk = int(ceil_div(K, kBK));
+  Args a{};
+  a.xs = xs; a.ws = ws; a.bias = b; a.bias_dtype = bdt;
+  a.T = T; a.N = N; a.K = K;
+  CUtensorMap mw, mx;
+  const int64_t pair_t = ceil_div(T, kMaxTn);
+  if (ceil_div(N, 2 * kBM) * pair_t * 2 >= sms * 3 / 4 && T > 128) {
+    a.tiles_t = int(pair_t);
+    a.tn = int(ceil_div(ceil_div(T, pair_t), 32) * 32);
+    a.tiles_n = int(ceil_div(N, 2 * kBM));
+    if (!make_map(&mw, wc, K, N, wstride, kBM) || !make_map(&mx, xc, K, T, xstride, a.tn / 2))
+      return set_last_error(5, "fmhc_int8_linear: cuTensorMapEncodeTiled failed");
+    const int64_t pairs = std::min<int64_t>(int64_t(a.tiles_n) * a.tiles_t, sms / 2);
+    const size_t smem = sizeof(PairSmem) + 1024;
+    FMHC_DISPATCH_ELEM(ydt, {
+      auto k = int8_linear_pair_kernel<E>;
+      allow_smem(reinterpret_cast<const void *>(k), smem);
+      launch(k, dim3(unsigned(pairs * 2)), dim3(kThreads), smem, s, mw, mx, (E *)y, a);
+    });
+    return 0;
+  }
+  a.tiles_t = int(ceil_div(T, 128));
+  a.tn = int(ceil_div(ceil_div(T, a.tiles_t), 16) * 16);
+  a.tiles_n = int(ceil_div(N, kBM));
+  if (!make_map(&mw, wc, K, N, wstride, kBM) || !make_map(&mx, xc, K, T, xstride, a.tn))
+    return set_last_error(5, "fmhc_int8_linear: cuTensorMapEncodeTiled failed");
+  const int64_t tiles = int64_t(a.tiles_n) * a.tiles_t;
+  if (tiles > (int64_t(1) << 27))
+    return set_last_error(2, "fmhc_int8_linear: T and N give more than 2^27 tiles");
+  int S = 1;
+  while (S < 8 && tiles * S * 2 <= sms && nk >= S * 4) S *= 2;
+  int cols = 32;
+  while (cols < a.tn) cols *= 2;
+  const int stage_bytes = kATile + a.tn * kBK;
+  const int stages = std::min(int((tiles * S > sms ? 100 : 200) * 1024 / stage_bytes), 12);
+  const size_t smem = size_t(stages) * stage_bytes + sizeof(SplitTail) + 1024;
   FMHC_DISPATCH_ELEM(ydt, {
-    const int64_t rows = (T + 31) / 32;
-    launch(int8_linear_tile_kernel<E>, dim3(unsigned((N + 31) / 32), unsigned(rows < 65535 ? rows : 65535)),
-           dim3(256), 0, s, (const int8_t *)xc, xstride, xs, (const int8_t *)wc, wstride, ws, b, bdt,
-           (E *)y, T, N, K);
+    auto k = int8_linear_split_kernel<E>;
+    allow_smem(reinterpret_cast<const void *>(k), smem);
+    if (S > 1)
+      launch_cluster(k, dim3(unsigned(tiles * S)), dim3(kThreads), smem, s, unsigned(S), mw, mx, (E *)y, a, S, stages, cols);
+    else
+      launch(k, dim3(unsigned(tiles)), dim3(kThreads), smem, s, mw, mx, (E *)y, a, S, stages, cols);
   });
+  return 0;
 }
 
 }  // namespace fmhc

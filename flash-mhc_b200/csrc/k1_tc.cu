@@ -35,6 +35,7 @@
 #include "k1_tc.h"
 #include "k2_token.cuh"
 #include "sm100_ptx.cuh"
+#include "tma_map.h"
 
 namespace fmhc {
 namespace k1tc {
@@ -755,21 +756,6 @@ namespace {
 
 thread_local char g_msg[256] = "";
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  }
-  return fn;
-}
-
 // 2-D bf16 tensor map: inner dimension `inner` (contiguous), `outer` rows of
 // `row_bytes` stride, box inner x outer_box, 128-byte swizzle, zero fill.
 bool make_map(CUtensorMap *m, const void *base, uint64_t inner, uint64_t outer,
@@ -881,7 +867,7 @@ bool k1_tc_fwd_supported(const void *x, const void *W, const void *out, const fl
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(W)) & 15) return false;
   if ((reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(inv_rms) & 3))
     return false;
-  return k1tc::device_is_sm100() && k1tc::encode_fn() != nullptr;
+  return k1tc::device_is_sm100() && encode_fn() != nullptr;
 }
 
 int launch_k1_tc_fwd(const void *x, const void *W, void *out, float *inv_rms, int64_t T, int nC,
@@ -964,7 +950,7 @@ bool k1_tc_bwd_supported(const void *go, const void *x, const void *W, const voi
                       reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(proj) |
                       reinterpret_cast<uintptr_t>(gx);
   if (m & 15) return false;
-  return k1tc::device_is_sm100() && k1tc::encode_fn() != nullptr;
+  return k1tc::device_is_sm100() && encode_fn() != nullptr;
 }
 
 int64_t k1_tc_bwd_workspace_bytes(int64_t T, int64_t nC) {
@@ -1024,7 +1010,7 @@ int launch_k1_tc_bwd(const void *go, const void *x, const void *W, const void *p
 
 bool k1_tc_bwd_q8_shape(int64_t T, int64_t nC) {
   return k1tc::bwd_has_plan(T, nC, k1tc::device_sms()) && k1tc::device_is_sm100() &&
-         k1tc::encode_fn() != nullptr;
+         encode_fn() != nullptr;
 }
 
 int launch_k1_tc_bwd_q8(const void *go, const void *codes, const void *scales, int fmt,
