@@ -58,9 +58,6 @@ __device__ __forceinline__ float bias1(const void *b, int dtype, int64_t n) {
   return __half2float(reinterpret_cast<const __half *>(b)[n]);
 }
 
-// MMAs of one stage that hold something of K: 32 bytes each.
-__device__ __forceinline__ int mmas_of(int kb, int K) { return min((K - kb * kBK + 31) >> 5, 4); }
-
 // 32 rows of a column: `rows` of them are stored, from y on.
 template <class E>
 __device__ __forceinline__ void store_rows(const int (&v)[32], int rows, const float *xs, float ws, float b,
@@ -175,7 +172,7 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid
   pdl_wait();
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int stage = 0, issued = 0;
       uint32_t phase = 0;
       const int half = A.tn / 2;
@@ -210,8 +207,9 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0 && elect_one()) {
       const uint32_t idesc = idesc_i8_s32(2 * kBM, A.tn);
+      const uint64_t ad0 = smem_desc(smem_u32(sm.a[0]), 16, 1024, 2), bd0 = smem_desc(smem_u32(sm.b[0]), 16, 1024, 2);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
@@ -222,10 +220,9 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid
         for (int kb = 0; kb < nk; ++kb) {
           if (!mbar_wait_cluster(smem_u32(&sm.full[stage]), phase, abort, kSitePairFull)) { ok = false; break; }
           tc_fence_after();
-          const uint64_t ad = smem_desc(smem_u32(sm.a[stage]), 16, 1024, 2);
-          const uint64_t bd = smem_desc(smem_u32(sm.b[stage]), 16, 1024, 2);
-          const int m = mmas_of(kb, A.K);
-          for (int k = 0; k < m; ++k)  // 32 bytes of K on: 2 in the descriptors' units
+          const uint64_t ad = ad0 + uint64_t(stage * (kATile / 16)), bd = bd0 + uint64_t(stage * (kATile / 16));
+#pragma unroll
+          for (int k = 0; k < kBK / 32; ++k)  // 32 bytes of K on: 2 in the descriptors' units
             mma_i8_ss_pair(d, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0);
           mma_commit_pair(smem_u32(&sm.empty[stage]));
           if (++stage == kPairStages) { stage = 0; phase ^= 1; }
@@ -296,10 +293,59 @@ struct SplitTail {
 enum : unsigned { kSiteSplitEmpty = 0x211, kSiteSplitFull = 0x212, kSiteSplitTfull = 0x214,
                   kSiteSplitDrain = 0x215 };
 
-template <class E>
+// Rows r = rank + S i of a tile, a warp per row and four columns from n0 + 4 lane per
+// lane: the S partial sums of four rows are in flight at a time (one row after the
+// other waited for the other CTAs' memory each time: 128 x 4096 x 4096 18.7 us).
+template <class E, int S>
+__device__ __forceinline__ void add_partials(const SplitTail &sm, const int *part, int rank, int warp, int lane,
+                                             int rows, int64_t n0, const Args &A, E *y) {
+  constexpr int kRows = 4;
+  bool ok = true;
+  uint32_t from[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    ok = ok && ld_cluster_s32(mapa_shared(smem_u32(&sm.abort), uint32_t(s))) == 0;
+    from[s] = mapa_shared(smem_u32(part) + uint32_t(lane) * 16u, uint32_t(s));
+  }
+  const int64_t n = n0 + 4 * lane;
+  float ws[4], b[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    ws[k] = n + k < A.N ? A.ws[n + k] : 0.f;
+    b[k] = n + k < A.N ? bias1(A.bias, A.bias_dtype, n + k) : 0.f;
+  }
+  for (int r0 = rank + S * warp; r0 < rows; r0 += S * 4 * kRows) {
+    int4 v[kRows][S];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (r0 + i * S * 4 < rows) v[i][s] = ld_cluster_s32x4(from[s] + uint32_t(r0 + i * S * 4) * kBM * 4u);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int r = r0 + i * S * 4;
+      if (r >= rows) break;
+      int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        sum[0] += v[i][s].x;
+        sum[1] += v[i][s].y;
+        sum[2] += v[i][s].z;
+        sum[3] += v[i][s].w;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = ok ? fmaf(__int2float_rn(sum[k]), sm.xs[r] * ws[k], b[k]) : __uint_as_float(0x7fc00000u);
+        if (n + k < A.N) y[r * A.N + n + k] = Elem<E>::narrow1(f);
+      }
+    }
+  }
+}
+
+template <class E, int S>
 __global__ void __launch_bounds__(kThreads)
 int8_linear_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
-                         E *__restrict__ y, const Args A, int S, int stages, int tmem_cols) {
+                         E *__restrict__ y, const Args A, int stages, int tmem_cols) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *const base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int stage_bytes = kATile + A.tn * kBK;
@@ -343,7 +389,7 @@ int8_linear_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
   float ws = 0.f, b = 0.f;
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int stage = 0, issued = 0;
       uint32_t phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
@@ -363,17 +409,17 @@ int8_linear_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t idesc = idesc_i8_s32(kBM, A.tn);
+      const uint64_t ad0 = smem_desc(smem_u32(base), 16, 1024, 2);
       int stage = 0;
       uint32_t phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!mbar_wait(smem_u32(&sm.full[stage]), phase, abort, kSiteSplitFull)) break;
         tc_fence_after();
-        const uint32_t a = smem_u32(base) + uint32_t(stage * stage_bytes);
-        const uint64_t ad = smem_desc(a, 16, 1024, 2), bd = smem_desc(a + kATile, 16, 1024, 2);
-        const int m = mmas_of(kb, A.K);
-        for (int k = 0; k < m; ++k) mma_i8_ss(tmem, ad + 2 * k, bd + 2 * k, idesc, kb > kb0 || k > 0);
+        const uint64_t ad = ad0 + uint64_t((stage * stage_bytes) >> 4), bd = ad + kATile / 16;
+#pragma unroll
+        for (int k = 0; k < kBK / 32; ++k) mma_i8_ss(tmem, ad + 2 * k, bd + 2 * k, idesc, kb > kb0 || k > 0);
         mma_commit(smem_u32(&sm.empty[stage]));
         if (++stage == stages) { stage = 0; phase ^= 1; }
       }
@@ -409,16 +455,7 @@ int8_linear_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
   __syncwarp();
   if (S > 1) {
     cluster_sync_all();  // the cluster's partial sums are written
-    if (warp >= 2) {
-      for (int s = 0; s < S; ++s) ok = ok && ld_cluster_s32(mapa_shared(smem_u32(&sm.abort), uint32_t(s))) == 0;
-      const uint32_t own = smem_u32(part) + uint32_t(q * 32 + lane) * 4u;
-      for (int r = int(rank); r < rows; r += S) {
-        int v = 0;
-        for (int s = 0; s < S; ++s) v += ld_cluster_s32(mapa_shared(own + uint32_t(r) * kBM * 4u, uint32_t(s)));
-        const float f = ok ? fmaf(__int2float_rn(v), sm.xs[r] * ws, b) : __uint_as_float(0x7fc00000u);
-        if (in) y[(t0 + r) * A.N + n] = Elem<E>::narrow1(f);
-      }
-    }
+    if (warp >= 2) add_partials<E, S>(sm, part, int(rank), warp - 2, lane, rows, int64_t(tile_n) * kBM, A, y + t0 * A.N);
     __syncwarp();
     cluster_sync_all();  // no CTA leaves while another reads its shared memory
   } else {
@@ -496,12 +533,10 @@ int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const v
   const int stages = std::min(int((tiles * S > sms ? 100 : 200) * 1024 / stage_bytes), 12);
   const size_t smem = size_t(stages) * stage_bytes + sizeof(SplitTail) + 1024;
   FMHC_DISPATCH_ELEM(ydt, {
-    auto k = int8_linear_split_kernel<E>;
+    auto k = S == 1 ? int8_linear_split_kernel<E, 1> : S == 2 ? int8_linear_split_kernel<E, 2>
+           : S == 4 ? int8_linear_split_kernel<E, 4> : int8_linear_split_kernel<E, 8>;
     allow_smem(reinterpret_cast<const void *>(k), smem);
-    if (S > 1)
-      launch_cluster(k, dim3(unsigned(tiles * S)), dim3(kThreads), smem, s, unsigned(S), mw, mx, (E *)y, a, S, stages, cols);
-    else
-      launch(k, dim3(unsigned(tiles)), dim3(kThreads), smem, s, mw, mx, (E *)y, a, S, stages, cols);
+    launch_cluster(k, dim3(unsigned(tiles * S)), dim3(kThreads), smem, s, unsigned(S), mw, mx, (E *)y, a, stages, cols);
   });
   return 0;
 }
