@@ -39,6 +39,7 @@ constexpr int kBM = 128;                // output columns per CTA
 constexpr int kATile = kBM * kBK;       // 16 KiB
 constexpr int kThreads = 192;           // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
 constexpr int kEpiThreads = 128;
+constexpr int kPairEpiThreads = 256;    // of a pair's CTA: warps 2-9
 constexpr int kMaxTn = 256;
 
 struct Args {
@@ -58,7 +59,16 @@ __device__ __forceinline__ float bias1(const void *b, int dtype, int64_t n) {
   return __half2float(reinterpret_cast<const __half *>(b)[n]);
 }
 
-// 32 rows of a column: `rows` of them are stored, from y on.
+__device__ __forceinline__ void narrow4(const float (&f)[4], float *o) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) o[k] = f[k];
+}
+// 32 rows of a column: `rows` of them are stored, from y (row 0, this column) on.
+// No branch stands between the rows of a whole chunk: one per row made each wait for
+// the latency of its own arithmetic (tiles of 256 x 256 took 20 us each).  Two columns
+// of a row per store, swapped between lanes, were slower (65536 x 1024 x 1024: 63.4
+// against 67.6 us), and so was converting the sums by ordinary arithmetic (83 against
+// 72 at the time).
 template <class E>
 __device__ __forceinline__ void store_rows(const int (&v)[32], int rows, const float *xs, float ws, float b,
                                            E *y, int64_t N, bool in) {
@@ -71,8 +81,6 @@ __device__ __forceinline__ void store_rows(const int (&v)[32], int rows, const f
     o[j + 2] = Elem<E>::narrow1(fmaf(__int2float_rn(v[j + 2]), x.z * ws, b));
     o[j + 3] = Elem<E>::narrow1(fmaf(__int2float_rn(v[j + 3]), x.w * ws, b));
   }
-  // No branch between the rows of a whole chunk: one per row made each wait for
-  // the latency of its own arithmetic (tiles of 256 x 256 took 20 us each).
   if (rows >= 32) {
     if (in) {
 #pragma unroll
@@ -84,15 +92,22 @@ __device__ __forceinline__ void store_rows(const int (&v)[32], int rows, const f
       if (in && j < rows) *y = o[j];
   }
 }
-// One column of a tile: rows t0 .. t0 + rows - 1, from this warp's lanes of TMEM.
+// One column of a tile: `rows` rows from this warp's lanes of TMEM.  The next chunk is
+// on its way from TMEM while one is stored.
 template <class E>
 __device__ __forceinline__ void store_column(uint32_t tmem, int rows, const float *xs, float ws, float b,
                                              E *y, int64_t N, bool in) {
-  for (int c = 0; c < rows; c += 32) {
-    uint32_t v[32];
-    tmem_ld_32x32b_x32(tmem + uint32_t(c), v);
+  uint32_t v[2][32];
+  if (rows > 0) tmem_ld_32x32b_x32(tmem, v[0]);
+  for (int c = 0; c < rows; c += 64) {
     tmem_wait_ld();
-    store_rows(reinterpret_cast<const int (&)[32]>(v), rows - c, xs + c, ws, b, y + c * N, N, in);
+    if (c + 32 < rows) tmem_ld_32x32b_x32(tmem + uint32_t(c + 32), v[1]);
+    store_rows(reinterpret_cast<const int (&)[32]>(v[0]), rows - c, xs + c, ws, b, y, N, in);
+    if (c + 32 >= rows) break;
+    tmem_wait_ld();
+    if (c + 64 < rows) tmem_ld_32x32b_x32(tmem + uint32_t(c + 64), v[0]);
+    store_rows(reinterpret_cast<const int (&)[32]>(v[1]), rows - c - 32, xs + c + 32, ws, b, y + 32 * N, N, in);
+    y += 64 * N;
   }
 }
 template <class E>
@@ -133,7 +148,7 @@ __device__ __forceinline__ void tile_of(int64_t id, int tiles_n, int tiles_t, in
 // leader's and counts the bytes of both CTAs' copies; a commit arrives on `empty`
 // and `tfull` of both; the epilogue warps of both arrive on the leader's `tempty`.
 template <class E>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + kPairEpiThreads, 1)
 int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                         E *__restrict__ y, const Args A) {
   extern __shared__ uint8_t smem_raw[];
@@ -152,7 +167,7 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&sm.tfull[b]), 1);
-      mbar_init(smem_u32(&sm.tempty[b]), 8);
+      mbar_init(smem_u32(&sm.tempty[b]), 16);
     }
     mbar_init(smem_u32(&sm.mma_done), 1);
     sm.abort = 0;
@@ -236,34 +251,47 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid
       mbar_wait(smem_u32(&sm.mma_done), 0, abort, kSitePairDrain, true);
     }
   } else {
-    const int q = warp & 3, me = int(threadIdx.x) - 64;
+    // Warp w of eight: the lanes of quarter w % 4 and half of the rows.  What a tile
+    // needs from global memory is loaded while the one before is stored.
+    const int q = warp & 3, me = int(threadIdx.x) - 64, half = A.tn / 2, h0 = warp < 6 ? 0 : half;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (int64_t id = pair; id < tiles; id += pairs) {
+    int64_t n = 0, t0 = 0;
+    int rows = 0;
+    float ws = 0.f, b = 0.f, x = 0.f;
+    const auto next = [&](int64_t id) {
+      if (id >= tiles) return;
       int tile_n, tile_t;
       tile_of(id, A.tiles_n, A.tiles_t, &tile_n, &tile_t);
-      const int64_t n = int64_t(tile_n) * 2 * kBM + rank * kBM + q * 32 + lane;
-      const int64_t t0 = int64_t(tile_t) * A.tn;
-      const int rows = int(min(A.T - t0, int64_t(A.tn)));
-      const bool in = n < A.N;
+      n = int64_t(tile_n) * 2 * kBM + rank * kBM + q * 32 + lane;
+      t0 = int64_t(tile_t) * A.tn;
+      rows = int(min(A.T - t0, int64_t(A.tn)));
+      ws = n < A.N ? A.ws[n] : 0.f;
+      b = n < A.N ? bias1(A.bias, A.bias_dtype, n) : 0.f;
+      x = me < rows ? A.xs[t0 + me] : 0.f;
+    };
+    next(pair);
+    for (int64_t id = pair; id < tiles; id += pairs) {
       // This buffer was last read two tiles ago, before the barrier of the tile between.
-      for (int i = me; i < rows; i += kEpiThreads) sm.xs[acc][i] = A.xs[t0 + i];
-      const float ws = in ? A.ws[n] : 0.f;
-      const float b = in ? bias1(A.bias, A.bias_dtype, n) : 0.f;
-      named_bar_sync(1, kEpiThreads);
-      E *to = y + t0 * A.N + n;
+      sm.xs[acc][me] = x;
+      named_bar_sync(1, kPairEpiThreads);
+      const float w0 = ws, b0 = b;
+      const bool in = n < A.N;
+      const int mine = min(rows - h0, half);
+      E *const to = y + (t0 + h0) * A.N + n;
+      next(id + pairs);
       ok = ok && mbar_wait_cluster(smem_u32(&sm.tfull[acc]), acc_phase, abort, kSitePairTfull);
       ok = __all_sync(0xffffffffu, ok);  // the loads below take whole warps
       if (!ok) {
-        store_nan(rows, to, A.N, in);
+        store_nan(mine, to, A.N, in);
         continue;
       }
       tc_fence_after();
-      store_column(tmem + (uint32_t(q * 32) << 16) + uint32_t(acc * 256), rows, sm.xs[acc], ws, b, to, A.N, in);
+      store_column(tmem + (uint32_t(q * 32) << 16) + uint32_t(acc * 256 + h0), mine, sm.xs[acc] + h0, w0, b0, to, A.N, in);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&sm.tempty[acc]), 0));
+      if (lane == 0) mbar_arrive_cta_remote(mapa_shared(smem_u32(&sm.tempty[acc]), 0));
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
   }
@@ -513,7 +541,7 @@ int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const v
     FMHC_DISPATCH_ELEM(ydt, {
       auto k = int8_linear_pair_kernel<E>;
       allow_smem(reinterpret_cast<const void *>(k), smem);
-      launch(k, dim3(unsigned(pairs * 2)), dim3(kThreads), smem, s, mw, mx, (E *)y, a);
+      launch(k, dim3(unsigned(pairs * 2)), dim3(64 + kPairEpiThreads), smem, s, mw, mx, (E *)y, a);
     });
     return 0;
   }

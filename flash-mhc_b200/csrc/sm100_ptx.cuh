@@ -109,6 +109,11 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t remote_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote_bar)
                : "memory");
 }
+// The same for a thread that only hands on TMEM it has read: its global stores need
+// not be visible first (waiting for them cost a tenth of the 8-bit linear layer).
+__device__ __forceinline__ void mbar_arrive_cta_remote(uint32_t remote_bar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(remote_bar) : "memory");
+}
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
