@@ -266,14 +266,17 @@ __device__ __forceinline__ typename Elem<E>::Raw ld8(const E *p) {
   }
 }
 template <class E>
-__device__ __forceinline__ void st8(E *p, const float (&f)[8]) {
+__device__ __forceinline__ void st_raw(E *p, const typename Elem<E>::Raw &r) {
   if constexpr (sizeof(E) == 2) {
-    __stcs(reinterpret_cast<uint4 *>(p), Elem<E>::narrow(f));
+    __stcs(reinterpret_cast<uint4 *>(p), r);
   } else {
-    const typename Elem<E>::Raw r = Elem<E>::narrow(f);
     __stcs(reinterpret_cast<uint4 *>(p), r.a);
     __stcs(reinterpret_cast<uint4 *>(p) + 1, r.b);
   }
+}
+template <class E>
+__device__ __forceinline__ void st8(E *p, const float (&f)[8]) {
+  st_raw<E>(p, Elem<E>::narrow(f));
 }
 
 // Largest magnitude among eight raw values, as f32 bits.  Magnitudes of a

@@ -773,8 +773,10 @@ int fmhc_rms_norm_fwd(const void *x, int x_dtype, const void *residual, const vo
   if (rows == 0) return ok();
   FMHC_REQUIRE_PTR(w, x); FMHC_REQUIRE_PTR(w, y); FMHC_REQUIRE_PTR(w, rstd);
   FMHC_REQUIRE_ALIGN_TO(w, y, dtype_size(x_dtype)); FMHC_REQUIRE_ALIGN_TO(w, rstd, 4);
+  const bool vec = aligned(x, 16) && aligned(residual, 16) && aligned(weight, 16) && aligned(y, 16) &&
+                   aligned(total, 16);
   fmhc::launch_rms_fwd(x, x_dtype, residual, weight, param_dtype, eps, y, total, rstd, nullptr, 0,
-                       nullptr, rows, int(C), (cudaStream_t)stream);
+                       nullptr, rows, int(C), vec, (cudaStream_t)stream);
   return check_launch(w);
 }
 
@@ -796,8 +798,10 @@ int fmhc_rms_norm_fwd_int8(const void *x, int x_dtype, const void *residual, con
   if (rows == 0) return ok();
   FMHC_REQUIRE_PTR(w, x); FMHC_REQUIRE_PTR(w, codes); FMHC_REQUIRE_PTR(w, scales);
   FMHC_REQUIRE_ALIGN_TO(w, scales, 4);
+  const bool vec = aligned(x, 16) && aligned(residual, 16) && aligned(weight, 16) && aligned(total, 16) &&
+                   aligned(codes, 8) && codes_stride % 8 == 0;
   fmhc::launch_rms_fwd(x, x_dtype, residual, weight, param_dtype, eps, nullptr, total, nullptr, codes,
-                       codes_stride, scales, rows, int(C), (cudaStream_t)stream);
+                       codes_stride, scales, rows, int(C), vec, (cudaStream_t)stream);
   return check_launch(w);
 }
 
@@ -836,8 +840,10 @@ int fmhc_rms_norm_bwd(const void *grad_y, int x_dtype, const void *grad_total, c
       return fail(FMHC_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", w,
                   (long long)workspace_bytes, (long long)need);
   }
+  const bool vec = aligned(grad_y, 16) && aligned(grad_total, 16) && aligned(x, 16) && aligned(weight, 16) &&
+                   aligned(grad_x, 16);
   fmhc::launch_rms_bwd(grad_y, x_dtype, grad_total, x, rstd, weight, param_dtype, grad_x, grad_weight,
-                       (float *)workspace, rows, int(C), s);
+                       (float *)workspace, rows, int(C), vec, s);
   return check_launch(w);
 }
 

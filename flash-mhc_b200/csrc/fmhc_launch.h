@@ -119,14 +119,15 @@ void launch_ln_bwd(const void *g, int dtype, const void *x, int fmt, const void 
 
 // rms_norm.cu -- rows of C values of type dtype; res, w, gt may be null (total is
 // written where res is given).  codes null: y and rstd; else the output as rows of
-// `stride` bytes of codes and f32 scales (rows8.cuh).
+// `stride` bytes of codes and f32 scales (rows8.cuh).  `vec`: every row pointer and w
+// 16-byte aligned, codes and their stride multiples of 8; the width is checked here.
 void launch_rms_fwd(const void *x, int dtype, const void *res, const void *w, int pdt, float eps,
                     void *y, void *total, float *rstd, void *codes, int64_t stride, float *scales,
-                    int64_t rows, int C, cudaStream_t s);
+                    int64_t rows, int C, bool vec, cudaStream_t s);
 int64_t rms_bwd_workspace_bytes(int64_t rows, int C);
 void launch_rms_bwd(const void *g, int dtype, const void *gt, const void *x, const float *rstd,
                     const void *w, int pdt, void *gx, void *gw, float *ws, int64_t rows, int C,
-                    cudaStream_t s);
+                    bool vec, cudaStream_t s);
 
 // rows8.cu -- rows of C values of type dtype to and from codes (rows of `stride`
 // bytes) and f32 scales.

@@ -59,10 +59,6 @@ __device__ __forceinline__ float bias1(const void *b, int dtype, int64_t n) {
   return __half2float(reinterpret_cast<const __half *>(b)[n]);
 }
 
-__device__ __forceinline__ void narrow4(const float (&f)[4], float *o) {
-#pragma unroll
-  for (int k = 0; k < 4; ++k) o[k] = f[k];
-}
 // 32 rows of a column: `rows` of them are stored, from y (row 0, this column) on.
 // No branch stands between the rows of a whole chunk: one per row made each wait for
 // the latency of its own arithmetic (tiles of 256 x 256 took 20 us each).  Two columns

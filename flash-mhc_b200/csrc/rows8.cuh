@@ -45,6 +45,10 @@ __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d, fl
 __device__ __forceinline__ int8_t code1(float v, float inv) {
   return inv == 0.f ? int8_t(0) : int8_t(code_bits(v, inv) & 0xffu);
 }
+// Eight codes to an 8-byte aligned place.
+__device__ __forceinline__ void store_codes8(int8_t *p, const float (&f)[8], float inv) {
+  __stcs(reinterpret_cast<uint2 *>(p), make_uint2(code4(f[0], f[1], f[2], f[3], inv), code4(f[4], f[5], f[6], f[7], inv)));
+}
 
 }  // namespace rows8
 }  // namespace fmhc
