@@ -130,11 +130,12 @@ void launch_rms_bwd(const void *g, int dtype, const void *gt, const void *x, con
                     bool vec, cudaStream_t s);
 
 // rows8.cu -- rows of C values of type dtype to and from codes (rows of `stride`
-// bytes) and f32 scales.
+// bytes) and f32 scales.  `vec`: C % 8 == 0, x 16-byte aligned, codes and their stride
+// multiples of 8.
 void launch_row_quantize(const void *x, int dtype, void *codes, int64_t stride, float *scales,
-                         int64_t rows, int C, cudaStream_t s);
+                         int64_t rows, int C, bool vec, cudaStream_t s);
 void launch_row_dequantize(const void *codes, int64_t stride, const float *scales, void *x, int dtype,
-                           int64_t rows, int C, cudaStream_t s);
+                           int64_t rows, int C, bool vec, cudaStream_t s);
 
 // int8_linear.cu -- y (T, N) of type ydt from codes xc (T, K) and wc (N, K) in rows
 // of xstride and wstride bytes (multiples of 16, as xc and wc are); b may be null.

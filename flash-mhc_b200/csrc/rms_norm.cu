@@ -32,21 +32,6 @@ constexpr int kMaxParts = 1024;
 template <class E> constexpr int kMaxNV = sizeof(E) == 2 ? 4 : 2;
 template <class E, int NV, bool THIRD> constexpr int kStagesOf = THIRD && NV == kMaxNV<E> ? 2 : 3;
 
-// One value or the largest of one per warp, over the `team` warps of a row; slots
-// and barriers as in norm_rows' team_sum.
-__device__ __forceinline__ float team_sum1(float v, float *slot, int team, int warp, int lane) {
-  if (team == 1) return v;
-  if (lane == 0) slot[warp] = v;
-  named_bar_sync(1 + warp / team, team * 32);
-  return group_sum(slot[warp / team * team + (lane & (team - 1))], team);
-}
-__device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t *slot, int team, int warp, int lane) {
-  if (team == 1) return v;
-  if (lane == 0) slot[warp] = v;
-  named_bar_sync(1 + warp / team, team * 32);
-  return __reduce_max_sync(0xffffffffu, slot[warp / team * team + (lane & (team - 1))]);
-}
-
 // -------------------------------------------------------------------- forward
 // A team of 1..16 warps holds a row, NV chunks of eight values per lane, so that
 // everything is read once; the next rows are prefetched into a shared-memory ring

@@ -1,17 +1,109 @@
 // Rows put into 8 bits and restored (format: rows8.cuh).
-#include "act8.cuh"
 #include "fmhc_launch.h"
-#include "grid.cuh"
+#include "norm_rows.cuh"
 #include "rows8.cuh"
 
 namespace fmhc {
 
 using namespace act8;
+using namespace norm_rows;
 
 namespace {
 
+constexpr int kQuantWarps = 24;  // per block, one block per SM
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kStages = 3;
+template <class E> constexpr int kMaxNV = sizeof(E) == 2 ? 4 : 2;
+
+// A team of warps holds a row, as in the norms (rms_norm.cu), and the next rows are
+// prefetched into a shared-memory ring: x is read once.
+template <class E, int NV>
+__global__ void __launch_bounds__(32 * kQuantWarps, 1)
+row_quantize_kernel(const E *__restrict__ x, int8_t *__restrict__ codes, int64_t stride,
+                    float *__restrict__ scales, int64_t rows, int C, int team) {
+  using Raw = typename Elem<E>::Raw;
+  constexpr int S = kStages, kChunk = 32 * int(sizeof(Raw)), kStage = NV * kChunk;
+  extern __shared__ uint4 dyn[];
+  __shared__ uint32_t slots[2][kQuantWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int teams = (blockDim.x >> 5) / team, wt = warp % team;
+  const uint32_t ring = shared_addr(dyn) + warp * (S * kStage) + lane * int(sizeof(Raw));
+  const int c0 = wt * NV * 32 + lane, left = C / 8 - c0;
+  const int64_t step = int64_t(gridDim.x) * teams;
+  int64_t r = int64_t(blockIdx.x) * teams + warp / team;
+  pdl_wait();
+  const int64_t hop = step * C;
+  const E *src = x + r * C + c0 * 8;
+  int8_t *dst = codes + r * stride + c0 * 8;
+  int64_t fetched = r;
+  const auto fetch = [&](int stage) {
+    if (fetched < rows)
+      unrolled<NV>([&](auto i) {
+        if (i * 32 < left) copy_raw<E, i * kChunk>(ring + stage * kStage, src + i * 256);
+      });
+    fetched += step;
+    src += hop;
+    copy_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch(s);
+  int par = 0, stage = 0;
+  for (; r < rows; r += step, par ^= 1) {
+    fetch(stage == 0 ? S - 1 : stage - 1);
+    copy_wait<S - 1>();
+    Raw v[NV];
+    uint32_t m = 0;
+    unrolled<NV>([&](auto i) {
+      if (i * 32 < left) {
+        v[i] = load_raw<E, i * kChunk>(ring + stage * kStage);
+        m = max(m, amax8_raw<E>(v[i]));
+      }
+    });
+    if (++stage == S) stage = 0;
+    m = team_max(__reduce_max_sync(0xffffffffu, m), slots[par], team, warp, lane);
+    const rows8::RowScale q = rows8::row_scale(m);
+    if (wt == 0 && lane == 0) scales[r] = q.scale;
+    unrolled<NV>([&](auto i) {
+      if (i * 32 < left) {
+        float f[8];
+        Elem<E>::widen(v[i], f);
+        rows8::store_codes8(dst + i * 256, f, q.inv);
+      }
+    });
+    dst += step * stride;
+  }
+}
+
+// Restoring: a group of lanes (a power of two, up to 32) takes up to four chunks of
+// eight codes per lane of one row, so that narrow rows share a warp and wide ones
+// spread over several.
+constexpr int kRestoreChunks = 4;
+template <class E>
+__global__ void __launch_bounds__(kThreads)
+row_dequantize_kernel(const int8_t *__restrict__ codes, int64_t stride, const float *__restrict__ scales,
+                      E *__restrict__ x, int64_t rows, int C, int group, int64_t units, int segments) {
+  pdl_wait();
+  const int lane = threadIdx.x & (group - 1);
+  const int64_t hop = (int64_t(gridDim.x) * kThreads) / group;
+  for (int64_t u = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / group; u < units; u += hop) {
+    const int64_t r = units <= 0xffffffffll ? int64_t(uint32_t(u) / uint32_t(segments)) : u / segments;
+    const int c0 = int(u - r * segments) * (kRestoreChunks * group) + lane;
+    const uint2 *from = reinterpret_cast<const uint2 *>(codes + r * stride) + c0;
+    const float s = __ldg(scales + r);
+    uint2 v[kRestoreChunks];
+#pragma unroll
+    for (int i = 0; i < kRestoreChunks; ++i)
+      if ((c0 + i * group) * 8 < C) v[i] = __ldcs(from + i * group);
+#pragma unroll
+    for (int i = 0; i < kRestoreChunks; ++i)
+      if ((c0 + i * group) * 8 < C) {
+        float f[8];
+        restore<kInt8>(v[i], s, f);
+        st8(x + r * C + int64_t(c0 + i * group) * 8, f);
+      }
+  }
+}
 
 template <class E>
 __global__ void __launch_bounds__(kThreads)
@@ -50,8 +142,17 @@ row_dequantize_any_kernel(const int8_t *__restrict__ codes, int64_t stride, cons
 }  // namespace
 
 void launch_row_quantize(const void *x, int dtype, void *codes, int64_t stride, float *scales,
-                         int64_t rows, int C, cudaStream_t s) {
+                         int64_t rows, int C, bool vec, cudaStream_t s) {
   FMHC_DISPATCH_ELEM(dtype, {
+    Shape p;
+    if (vec && register_shape(rows, C, kMaxNV<E>, kQuantWarps, &p)) {
+      auto k = p.nv == 1 ? row_quantize_kernel<E, 1> : p.nv == 2 ? row_quantize_kernel<E, 2> : row_quantize_kernel<E, kMaxNV<E>>;
+      const size_t smem = size_t(p.threads) * kStages * p.nv * sizeof(typename Elem<E>::Raw);
+      allow_smem(reinterpret_cast<const void *>(k), smem);
+      launch(k, dim3(blocks_for(rows, p)), dim3(p.threads), smem, s, (const E *)x, (int8_t *)codes, stride, scales,
+             rows, C, p.team);
+      return;
+    }
     auto k = row_quantize_any_kernel<E>;
     launch(k, dim3(grid_for(k, rows * kWarps, kThreads)), dim3(kThreads), 0, s, (const E *)x,
            (int8_t *)codes, stride, scales, rows, C);
@@ -59,8 +160,18 @@ void launch_row_quantize(const void *x, int dtype, void *codes, int64_t stride, 
 }
 
 void launch_row_dequantize(const void *codes, int64_t stride, const float *scales, void *x, int dtype,
-                           int64_t rows, int C, cudaStream_t s) {
+                           int64_t rows, int C, bool vec, cudaStream_t s) {
   FMHC_DISPATCH_ELEM(dtype, {
+    if (vec) {
+      int group = 1;
+      while (group < 32 && group * 8 < C) group *= 2;
+      const int segments = (C + 8 * kRestoreChunks * group - 1) / (8 * kRestoreChunks * group);
+      const int64_t units = rows * segments;
+      auto k = row_dequantize_kernel<E>;
+      launch(k, dim3(grid_for(k, (units * group + 31) / 32, kThreads)), dim3(kThreads), 0, s, (const int8_t *)codes,
+             stride, scales, (E *)x, rows, C, group, units, segments);
+      return;
+    }
     auto k = row_dequantize_any_kernel<E>;
     launch(k, dim3(grid_for(k, rows * kWarps, kThreads)), dim3(kThreads), 0, s, (const int8_t *)codes,
            stride, scales, (E *)x, rows, C);
