@@ -857,7 +857,7 @@ int fmhc_row_quantize(const void *x, int x_dtype, void *codes, int64_t codes_str
   if (rows == 0) return ok();
   FMHC_REQUIRE_PTR(w, x); FMHC_REQUIRE_PTR(w, codes); FMHC_REQUIRE_PTR(w, scales);
   FMHC_REQUIRE_ALIGN_TO(w, x, dtype_size(x_dtype)); FMHC_REQUIRE_ALIGN_TO(w, scales, 4);
-  const bool vec = C % 8 == 0 && aligned(x, 16) && aligned(codes, 8) && codes_stride % 8 == 0;
+  const bool vec = aligned(x, 16) && aligned(codes, 8) && codes_stride % 8 == 0;
   fmhc::launch_row_quantize(x, x_dtype, codes, codes_stride, scales, rows, int(C), vec, (cudaStream_t)stream);
   return check_launch(w);
 }
@@ -871,7 +871,7 @@ int fmhc_row_dequantize(const void *codes, int64_t codes_stride, const float *sc
   if (rows == 0) return ok();
   FMHC_REQUIRE_PTR(w, codes); FMHC_REQUIRE_PTR(w, scales); FMHC_REQUIRE_PTR(w, x);
   FMHC_REQUIRE_ALIGN_TO(w, x, dtype_size(x_dtype)); FMHC_REQUIRE_ALIGN_TO(w, scales, 4);
-  const bool vec = C % 8 == 0 && aligned(x, 16) && aligned(codes, 8) && codes_stride % 8 == 0;
+  const bool vec = aligned(x, 16) && aligned(codes, 8) && codes_stride % 8 == 0;
   fmhc::launch_row_dequantize(codes, codes_stride, scales, x, x_dtype, rows, int(C), vec, (cudaStream_t)stream);
   return check_launch(w);
 }

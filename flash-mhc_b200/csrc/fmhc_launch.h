@@ -130,8 +130,8 @@ void launch_rms_bwd(const void *g, int dtype, const void *gt, const void *x, con
                     bool vec, cudaStream_t s);
 
 // rows8.cu -- rows of C values of type dtype to and from codes (rows of `stride`
-// bytes) and f32 scales.  `vec`: C % 8 == 0, x 16-byte aligned, codes and their stride
-// multiples of 8.
+// bytes) and f32 scales.  `vec`: x 16-byte aligned, codes and their stride multiples
+// of 8.
 void launch_row_quantize(const void *x, int dtype, void *codes, int64_t stride, float *scales,
                          int64_t rows, int C, bool vec, cudaStream_t s);
 void launch_row_dequantize(const void *codes, int64_t stride, const float *scales, void *x, int dtype,

@@ -12,6 +12,7 @@
 #include "fmhc_launch.h"
 #include "norm_rows.cuh"
 #include "rows8.cuh"
+#include "rows_general.h"
 
 namespace fmhc {
 
@@ -440,6 +441,10 @@ int any_slices(int64_t rows, int C) {
   return int(std::min<int64_t>(std::max<int64_t>(n, 1), kMaxParts));
 }
 
+// Rows that the kernels for any width take: not of whole chunks, or so narrow that
+// several share a warp.
+bool general_width(int C) { return C % 8 != 0 || C <= 128; }
+
 // Rows over teams for the kernels above: chunks up to half the most with a third
 // array where that covers the width, else up to the most.
 template <class E>
@@ -511,7 +516,11 @@ void launch_rms_fwd(const void *x, int dtype, const void *res, const void *w, in
   FMHC_DISPATCH_ELEM(dtype, {
     auto fast = res != nullptr ? codes != nullptr ? launch_fwd<E, true, true> : launch_fwd<E, true, false>
                                : codes != nullptr ? launch_fwd<E, false, true> : launch_fwd<E, false, false>;
-    if (vec && fast(x, res, w, pdt, eps, y, total, rstd, codes, stride, scales, rows, C, s)) return;
+    if (vec && general_width(C)) {
+      if (launch_general_fwd(x, dtype, res, w, pdt, eps, y, total, rstd, codes, stride, scales, true, rows, C, s)) return;
+    } else if (vec && fast(x, res, w, pdt, eps, y, total, rstd, codes, stride, scales, rows, C, s)) {
+      return;
+    }
     auto k = codes != nullptr ? rms_fwd_any_kernel<E, true> : rms_fwd_any_kernel<E, false>;
     launch(k, dim3(grid_for(k, rows * kWarps, kThreads)), dim3(kThreads), 0, s, (const E *)x,
            (const E *)res, w, pdt, eps, (E *)y, (E *)total, rstd, (int8_t *)codes, stride, scales, rows, C);
@@ -522,7 +531,7 @@ int64_t rms_bwd_workspace_bytes(int64_t rows, int C) {
   if (rows < 1 || C < 1) return 0;
   // The largest of the paths, so that the size depends on neither the type nor
   // the alignment.
-  int64_t n = any_slices(rows, C);
+  int64_t n = std::max(any_slices(rows, C), general_bwd_parts(rows, C));
   Shape p;
   for (bool third : {false, true}) {
     if (shape_for<float>(rows, C, third, kBwdWarps, &p)) n = std::max<int64_t>(n, blocks_for(rows, p));
@@ -536,7 +545,16 @@ void launch_rms_bwd(const void *g, int dtype, const void *gt, const void *x, con
                     bool vec, cudaStream_t s) {
   FMHC_DISPATCH_ELEM(dtype, {
     auto fast = gt != nullptr ? launch_bwd<E, true> : launch_bwd<E, false>;
-    if (vec && fast(g, gt, x, rstd, w, pdt, gx, gw, ws, rows, C, s)) return;
+    if (vec && general_width(C)) {
+      if (launch_general_bwd(g, dtype, gt, x, rstd, w, pdt, gx, gw != nullptr ? ws : nullptr, rows, C, s)) {
+        if (gw != nullptr)
+          launch(rms_weight_grad_kernel, dim3((C + 31) / 32), dim3(32 * kSumWarps), 0, s, (const float *)ws, gw, pdt,
+                 general_bwd_parts(rows, C), C);
+        return;
+      }
+    } else if (vec && fast(g, gt, x, rstd, w, pdt, gx, gw, ws, rows, C, s)) {
+      return;
+    }
     auto k = rms_bwd_any_kernel<E>;
     launch(k, dim3(grid_for(k, rows * kWarps, kThreads)), dim3(kThreads), 0, s, (const E *)g,
            (const E *)gt, (const E *)x, rstd, w, pdt, (E *)gx, rows, C);

@@ -2,6 +2,7 @@
 #include "fmhc_launch.h"
 #include "norm_rows.cuh"
 #include "rows8.cuh"
+#include "rows_general.h"
 
 namespace fmhc {
 
@@ -105,6 +106,57 @@ row_dequantize_kernel(const int8_t *__restrict__ codes, int64_t stride, const fl
   }
 }
 
+// The same for rows of any width: the chunks are the aligned ones of x (see
+// rows_general.cu), whose codes lie in two blocks of eight.
+template <class E>
+__global__ void __launch_bounds__(kThreads)
+row_dequantize_general_kernel(const int8_t *__restrict__ codes, int64_t stride, const float *__restrict__ scales,
+                              E *__restrict__ x, int64_t rows, int C, int group, int64_t units, int segments) {
+  pdl_wait();
+  const int lane = threadIdx.x & (group - 1);
+  const int64_t hop = (int64_t(gridDim.x) * kThreads) / group;
+  for (int64_t u = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / group; u < units; u += hop) {
+    const int64_t r = units <= 0xffffffffll ? int64_t(uint32_t(u) / uint32_t(segments)) : u / segments;
+    const int c0 = int(u - r * segments) * (kRestoreChunks * group) + lane;
+    const int a = int((r * C) & 7), chunks = (a + C + 7) >> 3, blocks = (C + 7) >> 3;
+    const int8_t *row = codes + r * stride;
+    const float s = __ldg(scales + r);
+    uint64_t v[kRestoreChunks];
+#pragma unroll
+    for (int i = 0; i < kRestoreChunks; ++i) {
+      const int j = c0 + i * group;
+      // Whole blocks only: what a row's last one lacks is read value by value below.
+      const auto block = [&](int b) -> uint64_t {
+        if (b < 0 || b >= blocks) return 0;
+        if (b * 8 + 8 <= C) {
+          const uint2 q = *reinterpret_cast<const uint2 *>(row + b * 8);
+          return uint64_t(q.y) << 32 | q.x;
+        }
+        uint64_t q = 0;
+        for (int k = 0; b * 8 + k < C; ++k) q |= uint64_t(uint8_t(row[b * 8 + k])) << (8 * k);
+        return q;
+      };
+      if (j < chunks) v[i] = a == 0 ? block(j) : block(j - 1) >> (64 - 8 * a) | block(j) << (8 * a);
+    }
+#pragma unroll
+    for (int i = 0; i < kRestoreChunks; ++i) {
+      const int j = c0 + i * group, e = 8 * j - a;
+      if (j < chunks) {
+        float f[8];
+        restore<kInt8>(make_uint2(uint32_t(v[i]), uint32_t(v[i] >> 32)), s, f);
+        E *to = x + r * C + e;
+        if (e >= 0 && e + 8 <= C) {
+          st8(to, f);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (e + k >= 0 && e + k < C) to[k] = Elem<E>::narrow1(f[k]);
+        }
+      }
+    }
+  }
+}
+
 template <class E>
 __global__ void __launch_bounds__(kThreads)
 row_quantize_any_kernel(const E *__restrict__ x, int8_t *__restrict__ codes, int64_t stride,
@@ -145,7 +197,11 @@ void launch_row_quantize(const void *x, int dtype, void *codes, int64_t stride, 
                          int64_t rows, int C, bool vec, cudaStream_t s) {
   FMHC_DISPATCH_ELEM(dtype, {
     Shape p;
-    if (vec && register_shape(rows, C, kMaxNV<E>, kQuantWarps, &p)) {
+    if (vec && (C % 8 != 0 || C <= 128)) {
+      if (launch_general_fwd(x, dtype, nullptr, nullptr, 0, 0.f, nullptr, nullptr, nullptr, codes, stride, scales, false,
+                             rows, C, s))
+        return;
+    } else if (vec && register_shape(rows, C, kMaxNV<E>, kQuantWarps, &p)) {
       auto k = p.nv == 1 ? row_quantize_kernel<E, 1> : p.nv == 2 ? row_quantize_kernel<E, 2> : row_quantize_kernel<E, kMaxNV<E>>;
       const size_t smem = size_t(p.threads) * kStages * p.nv * sizeof(typename Elem<E>::Raw);
       allow_smem(reinterpret_cast<const void *>(k), smem);
@@ -163,11 +219,12 @@ void launch_row_dequantize(const void *codes, int64_t stride, const float *scale
                            int64_t rows, int C, bool vec, cudaStream_t s) {
   FMHC_DISPATCH_ELEM(dtype, {
     if (vec) {
+      const int chunks = C % 8 ? (C + 14) / 8 : C / 8;
       int group = 1;
-      while (group < 32 && group * 8 < C) group *= 2;
-      const int segments = (C + 8 * kRestoreChunks * group - 1) / (8 * kRestoreChunks * group);
+      while (group < 32 && group < chunks) group *= 2;
+      const int segments = (chunks + kRestoreChunks * group - 1) / (kRestoreChunks * group);
       const int64_t units = rows * segments;
-      auto k = row_dequantize_kernel<E>;
+      auto k = C % 8 ? row_dequantize_general_kernel<E> : row_dequantize_kernel<E>;
       launch(k, dim3(grid_for(k, (units * group + 31) / 32, kThreads)), dim3(kThreads), 0, s, (const int8_t *)codes,
              stride, scales, (E *)x, rows, C, group, units, segments);
       return;
