@@ -65,19 +65,19 @@ __device__ __forceinline__ float2 team_sum(float2 v, float2 *slot, int team, int
   return make_float2(group_sum(o.x, team), group_sum(o.y, team));
 }
 
-// One value or the largest of one per warp, over the `team` warps of a row; slots
-// and barriers as in team_sum.
+// One value or the largest of one per warp, over the `team` warps of a row, of any
+// number up to 32; slots and barriers as in team_sum.
 __device__ __forceinline__ float team_sum1(float v, float *slot, int team, int warp, int lane) {
   if (team == 1) return v;
   if (lane == 0) slot[warp] = v;
   named_bar_sync(1 + warp / team, team * 32);
-  return group_sum(slot[warp / team * team + (lane & (team - 1))], team);
+  return warp_sum(lane < team ? slot[warp / team * team + lane] : 0.f);
 }
 __device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t *slot, int team, int warp, int lane) {
   if (team == 1) return v;
   if (lane == 0) slot[warp] = v;
   named_bar_sync(1 + warp / team, team * 32);
-  return __reduce_max_sync(0xffffffffu, slot[warp / team * team + (lane & (team - 1))]);
+  return __reduce_max_sync(0xffffffffu, lane < team ? slot[warp / team * team + lane] : 0u);
 }
 
 // Pairs of a chunk's eight values.

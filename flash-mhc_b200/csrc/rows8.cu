@@ -107,7 +107,7 @@ row_dequantize_kernel(const int8_t *__restrict__ codes, int64_t stride, const fl
 }
 
 // The same for rows of any width: the chunks are the aligned ones of x (see
-// rows_general.cu), whose codes lie in two blocks of eight.
+// rows_general.cu), whose codes start anywhere in a word.
 template <class E>
 __global__ void __launch_bounds__(kThreads)
 row_dequantize_general_kernel(const int8_t *__restrict__ codes, int64_t stride, const float *__restrict__ scales,
@@ -118,32 +118,31 @@ row_dequantize_general_kernel(const int8_t *__restrict__ codes, int64_t stride, 
   for (int64_t u = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / group; u < units; u += hop) {
     const int64_t r = units <= 0xffffffffll ? int64_t(uint32_t(u) / uint32_t(segments)) : u / segments;
     const int c0 = int(u - r * segments) * (kRestoreChunks * group) + lane;
-    const int a = int((r * C) & 7), chunks = (a + C + 7) >> 3, blocks = (C + 7) >> 3;
+    const int a = int((r * C) & 7), chunks = (a + C + 7) >> 3;
     const int8_t *row = codes + r * stride;
     const float s = __ldg(scales + r);
-    uint64_t v[kRestoreChunks];
+    uint2 v[kRestoreChunks];
 #pragma unroll
     for (int i = 0; i < kRestoreChunks; ++i) {
-      const int j = c0 + i * group;
-      // Whole blocks only: what a row's last one lacks is read value by value below.
-      const auto block = [&](int b) -> uint64_t {
-        if (b < 0 || b >= blocks) return 0;
-        if (b * 8 + 8 <= C) {
-          const uint2 q = *reinterpret_cast<const uint2 *>(row + b * 8);
-          return uint64_t(q.y) << 32 | q.x;
-        }
-        uint64_t q = 0;
-        for (int k = 0; b * 8 + k < C; ++k) q |= uint64_t(uint8_t(row[b * 8 + k])) << (8 * k);
-        return q;
-      };
-      if (j < chunks) v[i] = a == 0 ? block(j) : block(j - 1) >> (64 - 8 * a) | block(j) << (8 * a);
+      const int j = c0 + i * group, e = 8 * j - a;
+      if (j >= chunks) continue;
+      if (e >= 0 && e + 12 <= C) {  // three words hold its eight codes
+        const uint32_t *q = reinterpret_cast<const uint32_t *>(row + (e & ~3));
+        const uint32_t q0 = __ldg(q), q1 = __ldg(q + 1), q2 = __ldg(q + 2);
+        v[i] = make_uint2(__funnelshift_r(q0, q1, 8 * (e & 3)), __funnelshift_r(q1, q2, 8 * (e & 3)));
+      } else {  // only the row's own bytes
+        v[i] = make_uint2(0u, 0u);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (e + k >= 0 && e + k < C) (k < 4 ? v[i].x : v[i].y) |= uint32_t(uint8_t(row[e + k])) << (8 * (k & 3));
+      }
     }
 #pragma unroll
     for (int i = 0; i < kRestoreChunks; ++i) {
       const int j = c0 + i * group, e = 8 * j - a;
       if (j < chunks) {
         float f[8];
-        restore<kInt8>(make_uint2(uint32_t(v[i]), uint32_t(v[i] >> 32)), s, f);
+        restore<kInt8>(v[i], s, f);
         E *to = x + r * C + e;
         if (e >= 0 && e + 8 <= C) {
           st8(to, f);

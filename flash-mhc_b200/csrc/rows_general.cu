@@ -101,6 +101,11 @@ __device__ __forceinline__ void load_weight(const void *w, int pdt, const Part &
     }
 }
 
+__device__ __forceinline__ void store_bytes(int8_t *to, uint2 v, int n) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (k < n) to[k] = int8_t((k < 4 ? v.x : v.y) >> (8 * (k & 3)));
+}
 // The codes of a row start at a multiple of 8 bytes, its chunks a bytes further: block
 // j of eight codes is the end of chunk j and the beginning of chunk j + 1, which
 // the next lane has.
@@ -108,31 +113,22 @@ template <int NV>
 __device__ __forceinline__ void store_codes(int8_t *row, const uint2 (&q)[NV], const Part &p, bool valid, int lane,
                                             int group, bool first_warp) {
   const int gl = lane & (group - 1), next = (lane & ~(group - 1)) | ((gl + 1) & (group - 1));
+  const bool near = p.a < 4;  // the block starts in the chunk's first word
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const uint2 own = q[i], send = i + 1 < NV && gl == 0 && group == 32 ? q[i + 1 < NV ? i + 1 : i] : own;
-    uint2 after;
-    after.x = __shfl_sync(0xffffffffu, send.x, next);
-    after.y = __shfl_sync(0xffffffffu, send.y, next);
+    const uint32_t x = __shfl_sync(0xffffffffu, send.x, next), y = __shfl_sync(0xffffffffu, send.y, next);
     // Not in this warp: the chunk after the last one of a warp that is not the row's last.
     const bool beyond = p.a != 0 && group == 32 && lane == 31 && i + 1 == NV && i * 32 + 1 < p.left;
     if (valid && i * 32 < p.left) {
       const int block = 8 * (p.c0 + 32 * i);  // first element
-      const uint64_t mine = uint64_t(own.y) << 32 | own.x, theirs = uint64_t(after.y) << 32 | after.x;
-      const uint64_t v = p.a == 0 ? mine : mine >> (8 * p.a) | theirs << (64 - 8 * p.a);
+      const uint32_t w0 = near ? own.x : own.y, w1 = near ? own.y : x, w2 = near ? x : y;
+      const uint2 v = make_uint2(__funnelshift_r(w0, w1, 8 * p.a), __funnelshift_r(w1, w2, 8 * p.a));
       const int n = min(beyond ? 8 - p.a : 8, p.C - block);
-      if (n == 8) {
-        __stcs(reinterpret_cast<uint2 *>(row + block), make_uint2(uint32_t(v), uint32_t(v >> 32)));
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (k < n) row[block + k] = int8_t(v >> (8 * k));
-      }
-      if (i == 0 && lane == 0 && !first_warp) {  // what the warp before has not
-#pragma unroll
-        for (int k = 0; k < 7; ++k)
-          if (k < p.a && p.element(0) + k < p.C) row[p.element(0) + k] = int8_t(mine >> (8 * k));
-      }
+      if (n == 8) __stcs(reinterpret_cast<uint2 *>(row + block), v);
+      else store_bytes(row + block, v, n);
+      // What the warp before has not.
+      if (i == 0 && lane == 0 && !first_warp) store_bytes(row + p.element(0), own, min(p.a, p.C - p.element(0)));
     }
   }
 }
@@ -377,7 +373,7 @@ bool split_for(int64_t rows, int C, int max_warps, Split *p) {
     while (p->group / 2 >= chunks) p->group /= 2;
   } else {
     if (chunks > 32) p->nv = kMaxNV;
-    while (32 * p->nv * p->team < chunks) p->team *= 2;
+    p->team = (chunks + 32 * p->nv - 1) / (32 * p->nv);
   }
   const int sms = sm_count(), per_warp = 32 / p->group;
   const int64_t want = (rows + int64_t(sms) * per_warp - 1) / (int64_t(sms) * per_warp);
