@@ -303,68 +303,22 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid
 
 // ------------------------------------------------------- clusters that split K
 // A cluster of S CTAs takes one tile of 128 columns and tn rows; CTA r runs the
-// stages [r nk / S, (r + 1) nk / S).  The partial sums go to each CTA's own shared
-// memory (the stages', which its MMAs have finished with), and after a cluster
-// barrier CTA r adds those of rows r, r + S, ... over the cluster.
+// stages [r nk / S, (r + 1) nk / S).  Each thread of the epilogue stores its column's
+// partial sums into the shared memory of the CTAs that finish the rows (row t: CTA
+// t mod S), and after a cluster barrier those add them: stores do not wait for an
+// answer, where loading the others' sums after the barrier took 1.5 us for 16 rows and
+// 5 for 128.
 struct SplitTail {
   uint64_t full[16], empty[16];
   uint64_t tfull;
   alignas(16) float xs[kMaxTn];
   uint32_t tmem_base;
   int abort;
+  int bad;  // a CTA of the cluster gave up
 };
 
 enum : unsigned { kSiteSplitEmpty = 0x211, kSiteSplitFull = 0x212, kSiteSplitTfull = 0x214,
                   kSiteSplitDrain = 0x215 };
-
-// Rows r = rank + S i of a tile, a warp per row and four columns from n0 + 4 lane per
-// lane: the S partial sums of four rows are in flight at a time (one row after the
-// other waited for the other CTAs' memory each time: 128 x 4096 x 4096 18.7 us).
-template <class E, int S>
-__device__ __forceinline__ void add_partials(const SplitTail &sm, const int *part, int rank, int warp, int lane,
-                                             int rows, int64_t n0, const Args &A, E *y) {
-  constexpr int kRows = 4;
-  bool ok = true;
-  uint32_t from[S];
-#pragma unroll
-  for (int s = 0; s < S; ++s) {
-    ok = ok && ld_cluster_s32(mapa_shared(smem_u32(&sm.abort), uint32_t(s))) == 0;
-    from[s] = mapa_shared(smem_u32(part) + uint32_t(lane) * 16u, uint32_t(s));
-  }
-  const int64_t n = n0 + 4 * lane;
-  float ws[4], b[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    ws[k] = n + k < A.N ? A.ws[n + k] : 0.f;
-    b[k] = n + k < A.N ? bias1(A.bias, A.bias_dtype, n + k) : 0.f;
-  }
-  for (int r0 = rank + S * warp; r0 < rows; r0 += S * 4 * kRows) {
-    int4 v[kRows][S];
-#pragma unroll
-    for (int i = 0; i < kRows; ++i)
-#pragma unroll
-      for (int s = 0; s < S; ++s)
-        if (r0 + i * S * 4 < rows) v[i][s] = ld_cluster_s32x4(from[s] + uint32_t(r0 + i * S * 4) * kBM * 4u);
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int r = r0 + i * S * 4;
-      if (r >= rows) break;
-      int sum[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        sum[0] += v[i][s].x;
-        sum[1] += v[i][s].y;
-        sum[2] += v[i][s].z;
-        sum[3] += v[i][s].w;
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float f = ok ? fmaf(__int2float_rn(sum[k]), sm.xs[r] * ws[k], b[k]) : __uint_as_float(0x7fc00000u);
-        if (n + k < A.N) y[r * A.N + n + k] = Elem<E>::narrow1(f);
-      }
-    }
-  }
-}
 
 template <class E, int S>
 __global__ void __launch_bounds__(kThreads)
@@ -374,6 +328,7 @@ int8_linear_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
   uint8_t *const base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int stage_bytes = kATile + A.tn * kBK;
   SplitTail &sm = *reinterpret_cast<SplitTail *>(base + stages * stage_bytes);
+  int *const part = reinterpret_cast<int *>(&sm + 1);  // S > 1: [S][tn / S, rounded up][128]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int *abort = &sm.abort;
   const uint32_t rank = S > 1 ? cluster_ctarank() : 0u;
@@ -389,6 +344,7 @@ int8_linear_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
     }
     mbar_init(smem_u32(&sm.tfull), 1);
     sm.abort = 0;
+    sm.bad = 0;
     fence_mbar_init();
     prefetch_tmap(&tmap_w);
     prefetch_tmap(&tmap_x);
@@ -400,6 +356,7 @@ int8_linear_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (S > 1) cluster_sync_all();  // every CTA has started, and its `bad` is 0
   const uint32_t tmem = sm.tmem_base;
   pdl_wait();
 
@@ -408,8 +365,6 @@ int8_linear_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
   const int64_t t0 = int64_t(tile_t) * A.tn;
   const int rows = int(min(A.T - t0, int64_t(A.tn)));
   const bool in = n < A.N;
-  int *const part = reinterpret_cast<int *>(base);  // [rows][128]
-  bool ok = true;
   float ws = 0.f, b = 0.f;
 
   if (warp == 0) {
@@ -457,37 +412,149 @@ int8_linear_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
     ws = in ? A.ws[n] : 0.f;
     b = in ? bias1(A.bias, A.bias_dtype, n) : 0.f;
     named_bar_sync(1, kEpiThreads);
-    ok = mbar_wait(smem_u32(&sm.tfull), 0, abort, kSiteSplitTfull) && *abort == 0;
+    bool ok = mbar_wait(smem_u32(&sm.tfull), 0, abort, kSiteSplitTfull) && *abort == 0;
     ok = __all_sync(0xffffffffu, ok);  // the loads below take whole warps
     tc_fence_after();
-    if (S == 1) {
+    if constexpr (S == 1) {
       E *to = y + t0 * A.N + n;
       if (ok) store_column(tmem + (uint32_t(q * 32) << 16), rows, sm.xs, ws, b, to, A.N, in);
       else store_nan(rows, to, A.N, in);
-    } else if (ok) {
-      for (int c = 0; c < rows; c += 32) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(tmem + (uint32_t(q * 32) << 16) + uint32_t(c), v);
-        tmem_wait_ld();
+    } else {
+      const int each = (A.tn + S - 1) / S;
+      uint32_t to[S];
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (c + j < rows) part[(c + j) * kBM + q * 32 + lane] = int(v[j]);
+      for (int s = 0; s < S; ++s)
+        to[s] = mapa_shared(smem_u32(part + int(rank) * each * kBM + q * 32 + lane), uint32_t(s));
+      if (ok) {
+        for (int c = 0; c < rows; c += 32) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(tmem + (uint32_t(q * 32) << 16) + uint32_t(c), v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j < rows) st_cluster_u32(to[j % S] + uint32_t((c + j) / S * kBM * 4), v[j]);
+        }
+      } else {
+        for (uint32_t s = 0; s < S; ++s) st_cluster_u32(mapa_shared(smem_u32(&sm.bad), s), 1u);
       }
     }
   }
   tc_fence_before();
-  __syncwarp();
-  if (S > 1) {
-    cluster_sync_all();  // the cluster's partial sums are written
-    if (warp >= 2) add_partials<E, S>(sm, part, int(rank), warp - 2, lane, rows, int64_t(tile_n) * kBM, A, y + t0 * A.N);
+  if constexpr (S > 1) {
     __syncwarp();
-    cluster_sync_all();  // no CTA leaves while another reads its shared memory
-  } else {
-    __syncthreads();
+    cluster_sync_all();  // the cluster's partial sums have arrived
+    if (warp >= 2) {
+      const int each = (A.tn + S - 1) / S;
+      const bool ok = *reinterpret_cast<volatile int *>(&sm.bad) == 0;
+      const int *from = part + q * 32 + lane;
+      E *to = y + (t0 + rank) * A.N + n;
+#pragma unroll 4
+      for (int i = 0; int(rank) + i * S < rows; ++i) {
+        int v = 0;
+#pragma unroll
+        for (int s = 0; s < S; ++s) v += from[(s * each + i) * kBM];
+        const float f = ok ? fmaf(__int2float_rn(v), sm.xs[int(rank) + i * S] * ws, b) : __uint_as_float(0x7fc00000u);
+        if (in) to[int64_t(i) * S * A.N] = Elem<E>::narrow1(f);
+      }
+    }
   }
+  __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, uint32_t(tmem_cols));
+  }
+}
+
+// ------------------------------------------------------------ a handful of rows
+// Up to eight rows t read the weight once at the rate of memory, and dot products of
+// four bytes on the CUDA cores keep up with it.  A warp takes kRowCols columns n and
+// every `split`-th stretch of kRowBytes bytes of K per lane-wide load; its lanes' sums
+// are added by the warp, and those of `split` warps in shared memory.
+constexpr int kRowsMost = 8;
+constexpr int kRowWarps = 4, kRowCols = 2, kRowDepth = 4;  // loads in flight: columns x depth
+
+// 16 codes from k on, of which `there` are the row's own; zeros for the others.
+__device__ __forceinline__ uint4 load_codes16(const int8_t *p, int there) {
+  if (there >= 16) return __ldg(reinterpret_cast<const uint4 *>(p));
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
+    if (k < there) w[k >> 2] |= uint32_t(uint8_t(p[k])) << (8 * (k & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <class E, int TT>
+__global__ void __launch_bounds__(32 * kRowWarps)
+int8_linear_rows_kernel(const int8_t *__restrict__ xc, int64_t xstride, const int8_t *__restrict__ wc, int64_t wstride,
+                        E *__restrict__ y, const Args A, int split) {
+  __shared__ int sums[kRowWarps][kRowCols][TT];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t n0 = (int64_t(blockIdx.x) * (kRowWarps / split) + warp / split) * kRowCols;
+  const int T = int(A.T), K = A.K;
+  pdl_wait();
+  const int8_t *w[kRowCols];
+#pragma unroll
+  for (int c = 0; c < kRowCols; ++c) w[c] = wc + min(n0 + c, A.N - 1) * wstride;
+  int acc[kRowCols][TT];
+#pragma unroll
+  for (int c = 0; c < kRowCols; ++c)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[c][t] = 0;
+  const int8_t *x[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) x[t] = xc + min(t, T - 1) * xstride;
+  const auto add = [&](const uint4 &q, const uint4 (&v)[kRowCols], int t) {
+#pragma unroll
+    for (int c = 0; c < kRowCols; ++c) {
+      acc[c][t] = __dp4a(int(q.x), int(v[c].x), acc[c][t]);
+      acc[c][t] = __dp4a(int(q.y), int(v[c].y), acc[c][t]);
+      acc[c][t] = __dp4a(int(q.z), int(v[c].z), acc[c][t]);
+      acc[c][t] = __dp4a(int(q.w), int(v[c].w), acc[c][t]);
+    }
+  };
+  constexpr int kStretch = 512 * kRowDepth;
+  int k0 = (warp % split) * kStretch;
+  for (; k0 + kStretch <= K; k0 += split * kStretch) {  // whole stretches: no branch between the loads
+    const int k = k0 + lane * 16;
+    uint4 v[kRowDepth][kRowCols];
+#pragma unroll
+    for (int d = 0; d < kRowDepth; ++d)
+#pragma unroll
+      for (int c = 0; c < kRowCols; ++c) v[d][c] = __ldg(reinterpret_cast<const uint4 *>(w[c] + k + d * 512));
+#pragma unroll
+    for (int d = 0; d < kRowDepth; ++d) {
+      uint4 q[TT];
+#pragma unroll
+      for (int t = 0; t < TT; ++t) q[t] = __ldg(reinterpret_cast<const uint4 *>(x[t] + k + d * 512));
+#pragma unroll
+      for (int t = 0; t < TT; ++t) add(q[t], v[d], t);
+    }
+  }
+  for (int k = k0 + lane * 16; k < min(K, k0 + kStretch); k += 512) {  // the last, shorter one
+    uint4 v[kRowCols];
+#pragma unroll
+    for (int c = 0; c < kRowCols; ++c) v[c] = load_codes16(w[c] + k, K - k);
+#pragma unroll
+    for (int t = 0; t < TT; ++t) add(load_codes16(x[t] + k, K - k), v, t);
+  }
+#pragma unroll
+  for (int c = 0; c < kRowCols; ++c)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      const int v = __reduce_add_sync(0xffffffffu, acc[c][t]);
+      if (lane == 0) sums[warp][c][t] = v;
+    }
+  __syncthreads();
+  // One value per thread: column c of warp group `g`, row t.
+  constexpr int kOut = kRowCols * TT;
+  for (int i = threadIdx.x; i < kRowWarps / split * kOut; i += blockDim.x) {
+    const int g = i / kOut, t = i / kRowCols % TT, c = i % kRowCols;
+    const int64_t n = (int64_t(blockIdx.x) * (kRowWarps / split) + g) * kRowCols + c;
+    if (t < T && n < A.N) {
+      int v = 0;
+      for (int k = 0; k < split; ++k) v += sums[g * split + k][c][t];
+      y[t * A.N + n] = Elem<E>::narrow1(fmaf(__int2float_rn(v), A.xs[t] * A.ws[n], bias1(A.bias, A.bias_dtype, n)));
+    }
   }
 }
 
@@ -524,6 +591,22 @@ int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const v
   Args a{};
   a.xs = xs; a.ws = ws; a.bias = b; a.bias_dtype = bdt;
   a.T = T; a.N = N; a.K = K;
+  // The kernel for a handful of rows is the faster one while its arithmetic is little
+  // (us, it / tiles of 128 columns: T x N x K 1 x 4096 x 4096 5.3 / 7.7, 2 x 4096 x 4096
+  // 6.9 / 8.0, 4 x 4096 x 4096 9.9 / 8.1, 1 x 16384 x 4096 13.3 / 13.1, 8 x 16384 x 4096
+  // 33 / 13.6).
+  if (T <= kRowsMost && T * N * K <= int64_t(1) << 25) {
+    int split = 1;  // warps that share K: enough blocks for every SM, while there is K for them
+    while (split < kRowWarps && ceil_div(N, kRowCols * (kRowWarps / split)) < 2 * sms && K > split * 512 * kRowDepth) split *= 2;
+    const int64_t blocks = ceil_div(N, int64_t(kRowCols) * (kRowWarps / split));
+    FMHC_DISPATCH_ELEM(ydt, {
+      auto k = T == 1 ? int8_linear_rows_kernel<E, 1> : T == 2 ? int8_linear_rows_kernel<E, 2>
+             : T <= 4 ? int8_linear_rows_kernel<E, 4> : int8_linear_rows_kernel<E, 8>;
+      launch(k, dim3(unsigned(blocks)), dim3(32 * kRowWarps), 0, s, (const int8_t *)xc, xstride, (const int8_t *)wc, wstride,
+             (E *)y, a, split);
+    });
+    return 0;
+  }
   CUtensorMap mw, mx;
   const int64_t pair_t = ceil_div(T, kMaxTn);
   if (ceil_div(N, 2 * kBM) * pair_t * 2 >= sms * 3 / 4 && T > 128) {
@@ -554,8 +637,9 @@ int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const v
   int cols = 32;
   while (cols < a.tn) cols *= 2;
   const int stage_bytes = kATile + a.tn * kBK;
-  const int stages = std::min(int((tiles * S > sms ? 100 : 200) * 1024 / stage_bytes), 12);
-  const size_t smem = size_t(stages) * stage_bytes + sizeof(SplitTail) + 1024;
+  const int part_bytes = S > 1 ? S * ((a.tn + S - 1) / S) * kBM * 4 : 0;
+  const int stages = std::min(((tiles * S > sms ? 100 : 200) * 1024 - part_bytes) / stage_bytes, 12);
+  const size_t smem = size_t(stages) * stage_bytes + sizeof(SplitTail) + part_bytes + 1024;
   FMHC_DISPATCH_ELEM(ydt, {
     auto k = S == 1 ? int8_linear_split_kernel<E, 1> : S == 2 ? int8_linear_split_kernel<E, 2>
            : S == 4 ? int8_linear_split_kernel<E, 4> : int8_linear_split_kernel<E, 8>;

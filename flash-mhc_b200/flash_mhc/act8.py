@@ -24,6 +24,8 @@ autograd, and a backward through any other result raises.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd import forward_ad
 
@@ -134,14 +136,16 @@ def _launch(t: torch.Tensor, name: str, *args) -> None:
 
 def _workspace(t: torch.Tensor, size_fn: str, *args):
     """(pointer, bytes, tensor) of the scratch that ``size_fn`` asks for on ``t``'s device."""
-    size = getattr(_native.lib(), size_fn)
-    if t.device.index == torch._C._cuda_getDevice():
-        n = size(*args)
-    else:
-        with _on_device(t):
-            n = size(*args)
+    n = _workspace_bytes(size_fn, t.device.index, *args)
     ws = t.new_empty((max(n, 1),), dtype=torch.uint8)
     return ws.data_ptr(), n, ws
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(size_fn: str, index: int, *args) -> int:
+    """What ``size_fn`` gives for these sizes on device ``index``: always the same."""
+    with torch.cuda.device(index):
+        return getattr(_native.lib(), size_fn)(*args)
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:

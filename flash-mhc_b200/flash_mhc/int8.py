@@ -50,10 +50,11 @@ _lib.define(
 
 def _new_codes(x: torch.Tensor) -> torch.Tensor:
     """Uninitialised codes in ``x``'s shape, rows at multiples of ALIGN bytes."""
-    *lead, C = x.shape
-    pad = -C % ALIGN
-    codes = x.new_empty((*lead, C + pad), dtype=torch.int8)
-    return codes[..., :C] if pad else codes
+    shape = x.shape
+    pad = -shape[-1] % ALIGN
+    if pad == 0:
+        return x.new_empty(shape, dtype=torch.int8)
+    return x.new_empty((*shape[:-1], shape[-1] + pad), dtype=torch.int8)[..., :shape[-1]]
 
 
 def _new_rows(x: torch.Tensor):
@@ -80,11 +81,17 @@ def _row_codes(op: str, name: str, codes: torch.Tensor, scales_name: str, scales
     """(codes as (rows, C), f32 scales, row stride) of rows in 8 bits, checked."""
     if codes.dtype != torch.int8:
         raise ValueError(f"flash_mhc::{op}: {name} must be int8 (got {codes.dtype})")
-    if codes.dim() < 1 or codes.shape[-1] < 1:
-        raise ValueError(f"flash_mhc::{op}: {name} needs a last dimension of at least 1 (got {tuple(codes.shape)})")
+    shape = codes.shape
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"flash_mhc::{op}: {name} needs a last dimension of at least 1 (got {tuple(shape)})")
     if scales.dtype != torch.float32:
         raise ValueError(f"flash_mhc::{op}: {scales_name} must be float32 (got {scales.dtype})")
-    _shape(op, scales_name, scales, codes.shape[:-1])
+    if scales.shape != shape[:-1]:
+        _shape(op, scales_name, scales, shape[:-1])
+    if len(shape) == 2:  # nearly always laid out
+        stride, one = codes.stride()
+        if one == 1 and stride >= shape[1] and stride % ALIGN == 0 and codes.data_ptr() % ALIGN == 0:
+            return codes, scales.contiguous(), stride
     codes = _laid_out(codes)
     return codes, scales.contiguous(), _stride(codes)
 
@@ -176,14 +183,16 @@ def _int8_linear_cuda(codes, scales, weight_codes, weight_scales, bias, dtype):
     op = "int8_linear"
     _same_device(op, codes, scales=scales, weight_codes=weight_codes, weight_scales=weight_scales, bias=bias)
     y_dtype = _float_dtype(op, dtype)
-    if weight_codes.dim() != 2:
-        raise ValueError(f"flash_mhc::{op}: weight_codes must be (N, K) (got {tuple(weight_codes.shape)})")
-    N, K = weight_codes.shape
+    w_shape = weight_codes.shape
+    if len(w_shape) != 2:
+        raise ValueError(f"flash_mhc::{op}: weight_codes must be (N, K) (got {tuple(w_shape)})")
+    N, K = w_shape
     lead = codes.shape[:-1]
-    _shape(op, "codes", codes, (*lead, K))
+    if codes.shape[-1:] != w_shape[1:]:
+        _shape(op, "codes", codes, (*lead, K))
     codes, scales, stride = _row_codes(op, "codes", codes, "scales", scales)
     weight_codes, weight_scales, w_stride = _row_codes(op, "weight_codes", weight_codes, "weight_scales", weight_scales)
-    _, bias, b_dtype = _params(op, N, None, bias)
+    _, bias, b_dtype = (None, None, 0) if bias is None else _params(op, N, None, bias)
     y = scales.new_empty((*lead, N), dtype=dtype)
     _launch(codes, "fmhc_int8_linear", codes.data_ptr(), stride, scales.data_ptr(), weight_codes.data_ptr(),
             w_stride, weight_scales.data_ptr(), _ptr(bias), b_dtype, y.data_ptr(), y_dtype, codes.shape[0], N, K)
