@@ -609,6 +609,9 @@ int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const v
   }
   CUtensorMap mw, mx;
   const int64_t pair_t = ceil_div(T, kMaxTn);
+  // Pairs of CTAs once they keep three quarters of the SMs busy (us, pairs / tiles of
+  // one CTA: 256 x 4096 x 4096 15.4 / 8.9, 1024 x 2048 x 2048 11.2 / 7.7, 512 x 4096 x
+  // 4096 15.6 / 11.1, 1024 x 4096 x 4096 16.2 / 17.5, 512 x 16384 x 4096 28.5 / 38.1).
   if (ceil_div(N, 2 * kBM) * pair_t * 2 >= sms * 3 / 4 && T > 128) {
     a.tiles_t = int(pair_t);
     a.tn = int(ceil_div(ceil_div(T, pair_t), 32) * 32);
@@ -624,16 +627,26 @@ int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const v
     });
     return 0;
   }
-  a.tiles_t = int(ceil_div(T, 128));
-  a.tn = int(ceil_div(ceil_div(T, a.tiles_t), 16) * 16);
   a.tiles_n = int(ceil_div(N, kBM));
+  // Tiles of up to 128 rows, narrower ones (down to 32, or 64 for a long K) where that
+  // gives more SMs one (us, down to 32 / always 128: 100 x 4096 x 4096 8.1 / 10.0, 256 x
+  // 4096 x 4096 8.9 / 11.0; 64 x 4096 x 16384 16.8 / 15.6).
+  const int least = nk >= 64 ? 64 : 32;
+  int64_t tiles_t = std::max(ceil_div(T, 128), std::min<int64_t>(ceil_div(T, least), sms / a.tiles_n));
+  a.tn = int(ceil_div(ceil_div(T, tiles_t), 16) * 16);
+  a.tiles_t = int(ceil_div(T, a.tn));
   if (!make_map(&mw, wc, K, N, wstride, kBM) || !make_map(&mx, xc, K, T, xstride, a.tn))
     return set_last_error(5, "fmhc_int8_linear: cuTensorMapEncodeTiled failed");
   const int64_t tiles = int64_t(a.tiles_n) * a.tiles_t;
   if (tiles > (int64_t(1) << 27))
     return set_last_error(2, "fmhc_int8_linear: T and N give more than 2^27 tiles");
-  int S = 1;
-  while (S < 8 && tiles * S * 2 <= sms && nk >= S * 4) S *= 2;
+  // K is split where the stages that a CTA is spared (about 0.12 us each) outweigh the
+  // cluster's exchange of partial sums, which grows with the tile (us, 1 / 4 CTAs: 16 x
+  // 1024 x 1024 3.8 / 3.5, 16 x 4096 x 4096 7.9 / 6.9, 64 x 2048 x 2048 5.2 / 5.5, 64 x
+  // 4096 x 16384 23 / 16), up to as many clusters as run at one time (16 of eight CTAs
+  // do not: 16 x 2048 x 2048 7.0, of four 4.1).
+  const int worth = 4 + a.tn / 5;
+  const int S = tiles <= 8 && nk >= 2 * worth ? 8 : tiles <= 32 && nk >= worth ? 4 : tiles <= 64 && nk >= 2 * worth ? 2 : 1;
   int cols = 32;
   while (cols < a.tn) cols *= 2;
   const int stage_bytes = kATile + a.tn * kBK;
