@@ -445,12 +445,30 @@ int any_slices(int64_t rows, int C) {
 // several share a warp.
 bool general_width(int C) { return C % 8 != 0 || C <= 128; }
 
-// Rows over teams for the kernels above: chunks up to half the most with a third
-// array where that covers the width, else up to the most.
+// Rows over teams for the kernels above.  `half`: chunks up to half the most where
+// that covers the width, and else up to the most with 16 warps.
 template <class E>
-bool shape_for(int64_t rows, int C, bool third, int max_warps, Shape *p) {
-  if (third && register_shape(rows, C, kMaxNV<E> / 2, max_warps, p)) return true;
-  return register_shape(rows, C, kMaxNV<E>, third ? 16 : max_warps, p);
+bool shape_for(int64_t rows, int C, bool half, int max_warps, Shape *p) {
+  if (half && register_shape(rows, C, kMaxNV<E> / 2, max_warps, p)) return true;
+  return register_shape(rows, C, kMaxNV<E>, half ? 16 : max_warps, p);
+}
+
+// The forward: half the chunks with a residual, whose ring is twice as large.  16-bit
+// rows of up to four warps with a residual go into 8 bits 20 warps at a time (us, 24 /
+// 20 / 16 warps: 65536 x 2048 167 / 147 / 157, 131072 x 1024 170 / 158 / 150; without
+// codes 183 / 183 / 185; without a residual 81 / 86 / 95).
+template <class E, bool RES, bool CODES>
+bool fwd_shape(int64_t rows, int C, Shape *p) {
+  if (!shape_for<E>(rows, C, RES, kFwdWarps, p)) return false;
+  if (RES && CODES && sizeof(E) == 2 && p->team > 1 && p->team <= 4) shape_for<E>(rows, C, RES, 20, p);
+  return true;
+}
+// The backward: half the chunks for 16-bit rows too (us, half / all: 65536 x 2048 bf16
+// 122 / 144, 131072 x 1024 130 / 144), but not for f32 ones without a third array
+// (65536 x 2048 297 / 255).
+template <class E>
+bool bwd_shape(int64_t rows, int C, bool third, Shape *p) {
+  return shape_for<E>(rows, C, third || sizeof(E) == 2, kBwdWarps, p);
 }
 
 #define FMHC_DISPATCH_NV(NV_RT, ...)                         \
@@ -464,7 +482,7 @@ template <class E, bool RES, bool CODES>
 bool launch_fwd(const void *x, const void *res, const void *w, int pdt, float eps, void *y, void *total,
                 float *rstd, void *codes, int64_t stride, float *scales, int64_t rows, int C, cudaStream_t s) {
   Shape p;
-  if (!shape_for<E>(rows, C, RES, kFwdWarps, &p)) return false;
+  if (!fwd_shape<E, RES, CODES>(rows, C, &p)) return false;
   FMHC_DISPATCH_NV(p.nv, {
     auto k = rms_fwd_kernel<E, NV, RES, CODES>;
     const size_t smem = size_t(p.threads) * kStagesOf<E, NV, RES> * NV * sizeof(typename Elem<E>::Raw) * (RES ? 2 : 1) +
@@ -480,7 +498,7 @@ template <class E, bool THIRD>
 bool launch_bwd(const void *g, const void *gt, const void *x, const float *rstd, const void *w, int pdt, void *gx,
                 void *gw, float *ws, int64_t rows, int C, cudaStream_t s) {
   Shape p;
-  if (!shape_for<E>(rows, C, THIRD, kBwdWarps, &p)) return false;
+  if (!bwd_shape<E>(rows, C, THIRD, &p)) return false;
   float *part = gw != nullptr ? ws : nullptr;
   const int parts = blocks_for(rows, p);
   FMHC_DISPATCH_NV(p.nv, {
@@ -534,8 +552,8 @@ int64_t rms_bwd_workspace_bytes(int64_t rows, int C) {
   int64_t n = std::max(any_slices(rows, C), general_bwd_parts(rows, C));
   Shape p;
   for (bool third : {false, true}) {
-    if (shape_for<float>(rows, C, third, kBwdWarps, &p)) n = std::max<int64_t>(n, blocks_for(rows, p));
-    if (shape_for<__half>(rows, C, third, kBwdWarps, &p)) n = std::max<int64_t>(n, blocks_for(rows, p));
+    if (bwd_shape<float>(rows, C, third, &p)) n = std::max<int64_t>(n, blocks_for(rows, p));
+    if (bwd_shape<__half>(rows, C, third, &p)) n = std::max<int64_t>(n, blocks_for(rows, p));
   }
   return (n * C * 4 + 255) & ~int64_t(255);
 }
