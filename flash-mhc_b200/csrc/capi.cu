@@ -882,8 +882,8 @@ int fmhc_int8_linear(const void *codes, int64_t codes_stride, const float *scale
                      int64_t K, void *stream) {
   const char *w = "fmhc_int8_linear";
   for (int64_t n : {T, N})
-    if (n < 0 || n >= (int64_t(1) << 31))
-      return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: T and N must be in [0, 2^31) (got %lld)", w, (long long)n);
+    if (n < 0 || n >= (int64_t(1) << 31) - 512)  // the last tile's end fits 32 bits too
+      return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: T and N must be in [0, 2^31 - 512) (got %lld)", w, (long long)n);
   if (K < 1 || K >= (int64_t(1) << 17))
     return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: K must be in [1, 2^17) (got %lld)", w, (long long)K);
   FMHC_REQUIRE_DTYPE(w, bias_dtype);

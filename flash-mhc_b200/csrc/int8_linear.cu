@@ -205,16 +205,17 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid
           if (++stage == kPairStages) { stage = 0; phase ^= 1; }
         }
       }
-      // The leader's barriers see the last copies of both CTAs land; the other CTA
-      // leaves after it (cluster barrier below).
-      if (rank == 0) {
-        const int n = issued < kPairStages ? issued : kPairStages;
-        int s = stage;
-        uint32_t ph = phase;
-        for (int i = 0; i < n; ++i) {
-          if (--s < 0) { s = kPairStages - 1; ph ^= 1; }
-          mbar_wait(smem_u32(&sm.full[s]), ph, abort, kSitePairDrain, true);
-        }
+      // Leave when the MMAs have used what was loaded: then the copies have landed, and no
+      // commit arrives here any more.  After a wait that gave up, the leader's barriers
+      // see the last copies of both CTAs land; the other CTA leaves after it (cluster
+      // barrier below).
+      const int n = issued < kPairStages ? issued : kPairStages;
+      int s = stage;
+      uint32_t ph = phase;
+      for (int i = 0; i < n; ++i) {
+        if (--s < 0) { s = kPairStages - 1; ph ^= 1; }
+        ok = ok && mbar_wait_cluster(smem_u32(&sm.empty[s]), ph, abort, kSitePairEmpty);
+        if (!ok && rank == 0) mbar_wait(smem_u32(&sm.full[s]), ph, abort, kSitePairDrain, true);
       }
     }
   } else if (warp == 1) {
@@ -243,7 +244,7 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
       // All MMAs issued by this thread complete before TMEM is freed.
-      mma_commit_pair(smem_u32(&sm.mma_done));
+      mma_commit_pair_here(smem_u32(&sm.mma_done));
       mbar_wait(smem_u32(&sm.mma_done), 0, abort, kSitePairDrain, true);
     }
   } else {

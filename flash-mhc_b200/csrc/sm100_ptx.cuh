@@ -325,6 +325,12 @@ __device__ __forceinline__ void mma_i8_ss_pair(uint32_t d_tmem, uint64_t a_desc,
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// mma_commit for a pair's MMAs: on a barrier of this CTA, or (below) on the barrier at
+// this address in both CTAs.
+__device__ __forceinline__ void mma_commit_pair_here(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+               : "memory");
+}
 // Arrive (once) on the barrier at this address in both CTAs when all previously
 // issued MMAs of this thread are done.
 __device__ __forceinline__ void mma_commit_pair(uint32_t bar) {

@@ -456,7 +456,7 @@ FMHC_API int fmhc_rms_norm_fwd_int8(const void *x, int x_dtype, const void *resi
  * + bias[n], rounded once to y_dtype.  The sum is exact (K < 2^17); the two scales
  * are multiplied first, in f32.  codes (T, K) and weight_codes (N, K) are 16-byte
  * aligned with strides that are multiples of 16; bias (N,) of bias_dtype, or NULL;
- * y (T, N) is dense. */
+ * y (T, N) is dense; T and N are below 2^31 - 512. */
 FMHC_API int fmhc_int8_linear(const void *codes, int64_t codes_stride, const float *scales,
                               const void *weight_codes, int64_t weight_stride,
                               const float *weight_scales, const void *bias, int bias_dtype,

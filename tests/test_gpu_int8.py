@@ -271,6 +271,8 @@ def test_int8_linear_module_on_cuda():
     q = int8.Int8Linear.from_linear(lin, norm.RMSNorm(200, device="cuda"))
     assert q.weight_codes.stride() == (208, 1)
     x, r = torch.randn(30, 200, device="cuda"), torch.randn(30, 200, device="cuda")
+    with pytest.raises(RuntimeError, match="for serving"):
+        q(x.clone().requires_grad_()).sum().backward()
     with torch.no_grad():
         y, total = q(x, r)
         assert torch.equal(total, x + r) and y.dtype == F32 and torch.equal(q(total), y)
@@ -285,5 +287,3 @@ def test_int8_linear_module_on_cuda():
         back = moved.cuda()
         assert back.weight_codes.stride() == (208, 1) and torch.equal(back(x, r)[0], y)
         assert q.half()(x.half(), r.half())[0].dtype == HF
-    with pytest.raises(RuntimeError, match="for serving"):
-        q(x.half().requires_grad_()).sum().backward()
