@@ -65,19 +65,33 @@ __device__ __forceinline__ float2 team_sum(float2 v, float2 *slot, int team, int
   return make_float2(group_sum(o.x, team), group_sum(o.y, team));
 }
 
-// One value or the largest of one per warp, over the `team` warps of a row, of any
-// number up to 32; slots and barriers as in team_sum.
-__device__ __forceinline__ float team_sum1(float v, float *slot, int team, int warp, int lane) {
-  if (team == 1) return v;
-  if (lane == 0) slot[warp] = v;
-  named_bar_sync(1 + warp / team, team * 32);
-  return warp_sum(lane < team ? slot[warp / team * team + lane] : 0.f);
+// The warps of a row, any number up to 32 of them: what joining one value per warp
+// needs, worked out once.  Slots and barriers as in team_sum.
+struct Team {
+  int size, first, bar, lane, span;  // warps; the first of them; barrier; lane; a power of two >= size
+  __device__ __forceinline__ Team(int team, int warp, int lane_) {
+    size = team;
+    first = warp / team * team;
+    bar = 1 + warp / team;
+    lane = lane_;
+    span = 1;
+    while (span < team) span *= 2;
+  }
+  __device__ __forceinline__ int slot() const { return first + min(lane & (span - 1), size - 1); }
+  __device__ __forceinline__ bool mine() const { return (lane & (span - 1)) < size; }
+};
+__device__ __forceinline__ float team_sum1(float v, float *slots, const Team &t, int warp) {
+  if (t.size == 1) return v;
+  if (t.lane == 0) slots[warp] = v;
+  named_bar_sync(t.bar, t.size * 32);
+  const float o = slots[t.slot()];
+  return group_sum(t.mine() ? o : 0.f, t.span);
 }
-__device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t *slot, int team, int warp, int lane) {
-  if (team == 1) return v;
-  if (lane == 0) slot[warp] = v;
-  named_bar_sync(1 + warp / team, team * 32);
-  return __reduce_max_sync(0xffffffffu, lane < team ? slot[warp / team * team + lane] : 0u);
+__device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t *slots, const Team &t, int warp) {
+  if (t.size == 1) return v;
+  if (t.lane == 0) slots[warp] = v;
+  named_bar_sync(t.bar, t.size * 32);
+  return __reduce_max_sync(0xffffffffu, slots[t.slot()]);
 }
 
 // Pairs of a chunk's eight values.

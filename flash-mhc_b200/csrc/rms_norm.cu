@@ -27,12 +27,13 @@ constexpr int kThreads = 256;  // of the kernels for any width
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxParts = 1024;
 
-// Chunks per lane, and rows in flight in the ring: with a third array (the residual,
-// or the gradient of total) half as many chunks, up to which the ring holds three
-// rows; wider rows take twice the chunks and two rows.
+// Most chunks per lane.  With a third array (the residual, or the gradient of total) rows
+// take half as many where that covers their width.
 template <class E> constexpr int kMaxNV = sizeof(E) == 2 ? 4 : 2;
-template <class E, int NV, bool THIRD> constexpr int kStagesOf = THIRD && NV == kMaxNV<E> ? 2 : 3;
-
+// Rows in flight in the ring: the one in use and the next.  A third row made most cases
+// slower (us, two / three: forward with a residual to 8 bits 131072 x 1024 142 / 165,
+// backward with a third array 157 / 175).
+constexpr int kStages = 2;
 // -------------------------------------------------------------------- forward
 // A team of 1..16 warps holds a row, NV chunks of eight values per lane, so that
 // everything is read once; the next rows are prefetched into a shared-memory ring
@@ -45,7 +46,7 @@ rms_fwd_kernel(const E *__restrict__ x, const E *__restrict__ res, const void *_
                int8_t *__restrict__ codes, int64_t stride, float *__restrict__ scales, int64_t rows,
                int C, int team) {
   using Raw = typename Elem<E>::Raw;
-  constexpr int S = kStagesOf<E, NV, RES>;
+  constexpr int S = kStages;
   constexpr int kChunk = 32 * int(sizeof(Raw));  // a warp's chunk in the ring
   constexpr int kStage = NV * kChunk * (RES ? 2 : 1);
   extern __shared__ uint4 dyn[];
@@ -53,6 +54,7 @@ rms_fwd_kernel(const E *__restrict__ x, const E *__restrict__ res, const void *_
   __shared__ uint32_t max_slots[2][kFwdWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int teams = warps / team, wt = warp % team;
+  const Team tm(team, warp, lane);
   const int nchunk = C / 8;
   const uint32_t ring = shared_addr(dyn) + warp * (S * kStage) + lane * int(sizeof(Raw));
   // Warp i of the team holds the NV * 32 chunks from i * NV * 32, those below
@@ -120,7 +122,7 @@ rms_fwd_kernel(const E *__restrict__ x, const E *__restrict__ res, const void *_
       }
     });
     if (++stage == S) stage = 0;
-    const float s = team_sum1(warp_sum(q + q1), sum_slots[par], team, warp, lane);
+    const float s = team_sum1(warp_sum(q + q1), sum_slots[par], tm, warp);
     const float rstd = rsqrtf(fmaf(s, inv_C, eps));
     if constexpr (!CODES) {
       if (wt == 0 && lane == 0) rstd_out[r] = rstd;
@@ -147,7 +149,7 @@ rms_fwd_kernel(const E *__restrict__ x, const E *__restrict__ res, const void *_
           }
         }
       });
-      m = team_max(__reduce_max_sync(0xffffffffu, m), max_slots[par], team, warp, lane);
+      m = team_max(__reduce_max_sync(0xffffffffu, m), max_slots[par], tm, warp);
       const rows8::RowScale sc = rows8::row_scale(m);
       if (wt == 0 && lane == 0) scales[r] = sc.scale;
       unrolled<NV>([&](auto i) {
@@ -166,13 +168,12 @@ rms_fwd_kernel(const E *__restrict__ x, const E *__restrict__ res, const void *_
 // total.  The second pass over a row reads the ring again, and the weight comes from
 // shared memory as f32 (or, for rows whose weight does not fit there, from global
 // memory) twice: holding them would pass 128 registers.
-template <class E, int NV, bool THIRD, bool W_SHARED>
+template <class E, int NV, int S, bool THIRD, bool W_SHARED>
 __global__ void __launch_bounds__(32 * kBwdWarps, 1)
 rms_bwd_kernel(const E *__restrict__ g, const E *__restrict__ gt, const E *__restrict__ x,
                const float *__restrict__ rstd, const void *__restrict__ w, int pdt, E *__restrict__ gx,
                float *__restrict__ part, int64_t rows, int C, int team) {
   using Raw = typename Elem<E>::Raw;
-  constexpr int S = kStagesOf<E, NV, THIRD>;
   constexpr int kChunk = 32 * int(sizeof(Raw));
   constexpr int kStage = NV * kChunk * (THIRD ? 3 : 2);
   constexpr int kRow = 16;  // rstd of the row, per warp and stage
@@ -180,6 +181,7 @@ rms_bwd_kernel(const E *__restrict__ g, const E *__restrict__ gt, const E *__res
   __shared__ float slots[2][kBwdWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int teams = warps / team, wt = warp % team;
+  const Team tm(team, warp, lane);
   const int nchunk = C / 8;
   const uint32_t ring = shared_addr(dyn) + warp * (S * kStage) + lane * int(sizeof(Raw));
   // Copied by one lane for the whole warp, so a warp barrier stands on both sides of a
@@ -253,7 +255,7 @@ rms_bwd_kernel(const E *__restrict__ g, const E *__restrict__ gt, const E *__res
         }
       }
     });
-    const float sum = team_sum1(warp_sum(dot.x + dot.y), slots[par], team, warp, lane);
+    const float sum = team_sum1(warp_sum(dot.x + dot.y), slots[par], tm, warp);
     const float2 c = both(-sum * inv_C * rs);  // times x
     unrolled<NV>([&](auto i) {
       if (i * 32 < left) {
@@ -453,15 +455,14 @@ bool shape_for(int64_t rows, int C, bool half, int max_warps, Shape *p) {
   return register_shape(rows, C, kMaxNV<E>, half ? 16 : max_warps, p);
 }
 
-// The forward: half the chunks with a residual, whose ring is twice as large.  16-bit
-// rows of up to four warps with a residual go into 8 bits 20 warps at a time (us, 24 /
-// 20 / 16 warps: 65536 x 2048 167 / 147 / 157, 131072 x 1024 170 / 158 / 150; without
-// codes 183 / 183 / 185; without a residual 81 / 86 / 95).
+// The forward: 16 warps, but 24 for what is bound by arithmetic: rows that go into 8 bits
+// without a residual or from f32, and f32 rows on their own (us, 16 / 24: 32768 x 4096
+// bf16 84 / 94, with a residual 163 / 184, both and to 8 bits 131072 x 1024 143 / 162;
+// to 8 bits 65536 x 2048 82 / 72, from f32 with a residual 288 / 269, f32 207 / 197).
 template <class E, bool RES, bool CODES>
 bool fwd_shape(int64_t rows, int C, Shape *p) {
-  if (!shape_for<E>(rows, C, RES, kFwdWarps, p)) return false;
-  if (RES && CODES && sizeof(E) == 2 && p->team > 1 && p->team <= 4) shape_for<E>(rows, C, RES, 20, p);
-  return true;
+  constexpr bool kF32 = sizeof(E) == 4;
+  return shape_for<E>(rows, C, RES, (RES ? CODES && kF32 : CODES || kF32) ? kFwdWarps : 16, p);
 }
 // The backward: half the chunks for 16-bit rows too (us, half / all: 65536 x 2048 bf16
 // 122 / 144, 131072 x 1024 130 / 144), but not for f32 ones without a third array
@@ -485,7 +486,7 @@ bool launch_fwd(const void *x, const void *res, const void *w, int pdt, float ep
   if (!fwd_shape<E, RES, CODES>(rows, C, &p)) return false;
   FMHC_DISPATCH_NV(p.nv, {
     auto k = rms_fwd_kernel<E, NV, RES, CODES>;
-    const size_t smem = size_t(p.threads) * kStagesOf<E, NV, RES> * NV * sizeof(typename Elem<E>::Raw) * (RES ? 2 : 1) +
+    const size_t smem = size_t(p.threads) * kStages * NV * sizeof(typename Elem<E>::Raw) * (RES ? 2 : 1) +
                         size_t(C) * 4;
     allow_smem(reinterpret_cast<const void *>(k), smem);
     launch(k, dim3(blocks_for(rows, p)), dim3(p.threads), smem, s, (const E *)x, (const E *)res, w, pdt, eps,
@@ -501,18 +502,20 @@ bool launch_bwd(const void *g, const void *gt, const void *x, const float *rstd,
   if (!bwd_shape<E>(rows, C, THIRD, &p)) return false;
   float *part = gw != nullptr ? ws : nullptr;
   const int parts = blocks_for(rows, p);
+  // Three rows in flight for two arrays of wide rows (us, two / three: 32768 x 4096 134 /
+  // 121, 65536 x 2048 128 / 127, 131072 x 1024 125 / 136).
+  const int stages = !THIRD && p.team >= 8 ? 3 : kStages;
   FMHC_DISPATCH_NV(p.nv, {
-    constexpr int S = kStagesOf<E, NV, THIRD>;
-    const size_t ring = size_t(p.threads) * S * NV * sizeof(typename Elem<E>::Raw) * (THIRD ? 3 : 2) +
-                        size_t(p.threads / 32) * S * 16;
+    const size_t ring = size_t(p.threads) * stages * NV * sizeof(typename Elem<E>::Raw) * (THIRD ? 3 : 2) +
+                        size_t(p.threads / 32) * stages * 16;
     // The ring's memory later holds the 32 NV bytes of sums of every thread.
-    static_assert(S * sizeof(typename Elem<E>::Raw) * 2 >= 32, "sums fit the ring");
+    static_assert(kStages * sizeof(typename Elem<E>::Raw) * 2 >= 32, "sums fit the ring");
     const size_t with_w = ring + size_t(C) * 4;
-    auto k = rms_bwd_kernel<E, NV, THIRD, true>;
+    auto k = stages == 3 ? rms_bwd_kernel<E, NV, 3, THIRD, true> : rms_bwd_kernel<E, NV, kStages, THIRD, true>;
     size_t smem = with_w;
     if constexpr (NV == kMaxNV<E>) {
       if (with_w > kMaxSmem) {
-        k = rms_bwd_kernel<E, NV, THIRD, false>;
+        k = stages == 3 ? rms_bwd_kernel<E, NV, 3, THIRD, false> : rms_bwd_kernel<E, NV, kStages, THIRD, false>;
         smem = ring;
       }
     }

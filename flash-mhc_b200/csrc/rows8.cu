@@ -11,10 +11,13 @@ using namespace norm_rows;
 
 namespace {
 
-constexpr int kQuantWarps = 24;  // per block, one block per SM
+// Warps per block, one block per SM, and rows in flight in the ring (us, 24 warps and
+// three rows / 16 and three / 16 and two: 32768 x 4096 bf16 68 / 63 / 63, 131072 x 1024
+// 68 / 67 / 61, 65536 x 2048 f32 125 / 97 / 102).
+constexpr int kQuantWarps = 16;
+template <class E> constexpr int kStages = sizeof(E) == 4 ? 3 : 2;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kStages = 3;
 template <class E> constexpr int kMaxNV = sizeof(E) == 2 ? 4 : 2;
 
 // A team of warps holds a row, as in the norms (rms_norm.cu), and the next rows are
@@ -24,11 +27,12 @@ __global__ void __launch_bounds__(32 * kQuantWarps, 1)
 row_quantize_kernel(const E *__restrict__ x, int8_t *__restrict__ codes, int64_t stride,
                     float *__restrict__ scales, int64_t rows, int C, int team) {
   using Raw = typename Elem<E>::Raw;
-  constexpr int S = kStages, kChunk = 32 * int(sizeof(Raw)), kStage = NV * kChunk;
+  constexpr int S = kStages<E>, kChunk = 32 * int(sizeof(Raw)), kStage = NV * kChunk;
   extern __shared__ uint4 dyn[];
   __shared__ uint32_t slots[2][kQuantWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int teams = (blockDim.x >> 5) / team, wt = warp % team;
+  const Team tm(team, warp, lane);
   const uint32_t ring = shared_addr(dyn) + warp * (S * kStage) + lane * int(sizeof(Raw));
   const int c0 = wt * NV * 32 + lane, left = C / 8 - c0;
   const int64_t step = int64_t(gridDim.x) * teams;
@@ -62,7 +66,7 @@ row_quantize_kernel(const E *__restrict__ x, int8_t *__restrict__ codes, int64_t
       }
     });
     if (++stage == S) stage = 0;
-    m = team_max(__reduce_max_sync(0xffffffffu, m), slots[par], team, warp, lane);
+    m = team_max(__reduce_max_sync(0xffffffffu, m), slots[par], tm, warp);
     const rows8::RowScale q = rows8::row_scale(m);
     if (wt == 0 && lane == 0) scales[r] = q.scale;
     unrolled<NV>([&](auto i) {
@@ -202,7 +206,7 @@ void launch_row_quantize(const void *x, int dtype, void *codes, int64_t stride, 
         return;
     } else if (vec && register_shape(rows, C, kMaxNV<E>, kQuantWarps, &p)) {
       auto k = p.nv == 1 ? row_quantize_kernel<E, 1> : p.nv == 2 ? row_quantize_kernel<E, 2> : row_quantize_kernel<E, kMaxNV<E>>;
-      const size_t smem = size_t(p.threads) * kStages * p.nv * sizeof(typename Elem<E>::Raw);
+      const size_t smem = size_t(p.threads) * kStages<E> * p.nv * sizeof(typename Elem<E>::Raw);
       allow_smem(reinterpret_cast<const void *>(k), smem);
       launch(k, dim3(blocks_for(rows, p)), dim3(p.threads), smem, s, (const E *)x, (int8_t *)codes, stride, scales,
              rows, C, p.team);

@@ -31,8 +31,7 @@ namespace {
 constexpr int kFwdWarps = 24;  // per block, one block per SM
 constexpr int kBwdWarps = 16;
 constexpr int kMaxNV = 2;      // chunks per lane: the weight's columns take 8 registers each
-// Rows in flight in the ring.
-template <class E, int NV, bool THIRD> constexpr int kStagesOf = THIRD && sizeof(E) == 4 && NV == 2 ? 2 : 3;
+constexpr int kStages = 2;     // rows in flight in the ring
 
 // What a lane holds of its rows.
 struct Part {
@@ -143,13 +142,14 @@ general_fwd_kernel(const E *__restrict__ x, const E *__restrict__ res, const voi
                    int8_t *__restrict__ codes, int64_t stride, float *__restrict__ scales, int64_t rows, int C,
                    int team, int group) {
   using Raw = typename Elem<E>::Raw;
-  constexpr int S = kStagesOf<E, NV, RES>;
+  constexpr int S = kStages;
   constexpr int kChunk = 32 * int(sizeof(Raw)), kStage = NV * kChunk * (RES ? 2 : 1);
   extern __shared__ uint4 dyn[];
   __shared__ float sum_slots[2][kFwdWarps];
   __shared__ uint32_t max_slots[2][kFwdWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int teams = (blockDim.x >> 5) / team, wt = warp % team;
+  const Team tm(team, warp, lane);
   const int per_warp = 32 / group, sub = lane / group;
   const uint32_t ring = shared_addr(dyn) + warp * (S * kStage) + lane * int(sizeof(Raw));
   const int64_t step = int64_t(gridDim.x) * teams * per_warp;
@@ -206,7 +206,7 @@ general_fwd_kernel(const E *__restrict__ x, const E *__restrict__ res, const voi
     });
     if (++stage == S) stage = 0;
     if constexpr (NORM) {
-      q = team_sum1(group_total(q, group), sum_slots[par], team, warp, lane);
+      q = team_sum1(group_total(q, group), sum_slots[par], tm, warp);
       const float rstd = rsqrtf(fmaf(q, inv_C, eps));
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -230,7 +230,7 @@ general_fwd_kernel(const E *__restrict__ x, const E *__restrict__ res, const voi
 #pragma unroll
           for (int k = 0; k < 8; ++k) m = max(m, rows8::magnitude(f[i][k]));
         }
-      m = team_max(group_most(m, group), max_slots[par], team, warp, lane);
+      m = team_max(group_most(m, group), max_slots[par], tm, warp);
       const rows8::RowScale sc = rows8::row_scale(m);
       if (valid && (lane & (group - 1)) == 0 && wt == 0) scales[r] = sc.scale;
       uint2 out[NV];
@@ -250,13 +250,14 @@ general_bwd_kernel(const E *__restrict__ g, const E *__restrict__ gt, const E *_
                    const float *__restrict__ rstd, const void *__restrict__ w, int pdt, E *__restrict__ gx,
                    float *__restrict__ part, int64_t rows, int C, int team, int group) {
   using Raw = typename Elem<E>::Raw;
-  constexpr int S = kStagesOf<E, NV, THIRD>;
+  constexpr int S = kStages;
   constexpr int kChunk = 32 * int(sizeof(Raw)), kStage = NV * kChunk * (THIRD ? 3 : 2);
   constexpr int kRow = 128;  // rstd of up to 32 rows, per warp and stage
   extern __shared__ uint4 dyn[];
   __shared__ float slots[2][kBwdWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int teams = warps / team, wt = warp % team;
+  const Team tm(team, warp, lane);
   const int per_warp = 32 / group, sub = lane / group;
   const uint32_t ring = shared_addr(dyn) + warp * (S * kStage) + lane * int(sizeof(Raw));
   // Copied by one lane of a group for all of it: a warp barrier stands on both sides of
@@ -321,7 +322,7 @@ general_bwd_kernel(const E *__restrict__ g, const E *__restrict__ gt, const E *_
         }
       }
     });
-    const float sum = team_sum1(group_total(dot, group), slots[par], team, warp, lane);
+    const float sum = team_sum1(group_total(dot, group), slots[par], tm, warp);
     const float c = -sum * inv_C * rs;  // times x
     unrolled<NV>([&](auto i) {
       if (valid && i * 32 < p.left) {
@@ -399,7 +400,7 @@ void launch_fwd(const Split &p, const void *x, const void *res, const void *w, i
                 cudaStream_t s) {
   FMHC_DISPATCH_NV(p.nv, {
     auto k = general_fwd_kernel<E, NV, RES, CODES, NORM>;
-    const size_t smem = size_t(p.threads()) * kStagesOf<E, NV, RES> * NV * sizeof(typename Elem<E>::Raw) * (RES ? 2 : 1);
+    const size_t smem = size_t(p.threads()) * kStages * NV * sizeof(typename Elem<E>::Raw) * (RES ? 2 : 1);
     allow_smem(reinterpret_cast<const void *>(k), smem);
     launch(k, dim3(p.grid), dim3(p.threads()), smem, s, (const E *)x, (const E *)res, w, pdt, eps, (E *)y, (E *)total,
            rstd, (int8_t *)codes, stride, scales, rows, C, p.team, p.group);
@@ -434,9 +435,8 @@ bool launch_general_bwd(const void *g, int dtype, const void *gt, const void *x,
   FMHC_DISPATCH_ELEM(dtype, FMHC_DISPATCH_NV(p.nv, {
     const bool third = gt != nullptr;
     auto k = third ? general_bwd_kernel<E, NV, true> : general_bwd_kernel<E, NV, false>;
-    const int S = third ? kStagesOf<E, NV, true> : kStagesOf<E, NV, false>;
-    const size_t smem = size_t(p.threads()) * S * NV * sizeof(typename Elem<E>::Raw) * (third ? 3 : 2) +
-                        size_t(p.threads() / 32) * S * 128;
+    const size_t smem = size_t(p.threads()) * kStages * NV * sizeof(typename Elem<E>::Raw) * (third ? 3 : 2) +
+                        size_t(p.threads() / 32) * kStages * 128;
     allow_smem(reinterpret_cast<const void *>(k), smem);
     launch(k, dim3(p.grid), dim3(p.threads()), smem, s, (const E *)g, (const E *)gt, (const E *)x, rstd, w, pdt,
            (E *)gx, part, rows, C, p.team, p.group);
