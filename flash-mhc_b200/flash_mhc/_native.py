@@ -127,7 +127,7 @@ class FlashMHCError(RuntimeError):
 
 def call(name: str, *args) -> None:
     """Call C-ABI function ``name``; raise FlashMHCError on a non-zero status."""
-    L = lib()
+    L = _lib if _lib is not None else lib()
     st = getattr(L, name)(*args)
     if st != 0:
         msg = L.fmhc_last_error().decode(errors="replace")

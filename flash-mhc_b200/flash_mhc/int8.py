@@ -26,9 +26,9 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
-from .act8 import (_DTYPES, _act, _launch, _register_no_derivative, _rows, _same_device, _shape)
+from .act8 import _DTYPES, _act, _launch, _new_per_row, _register_no_derivative, _same_device, _shape
 from .block import MHCLiteBlock
-from .norm import RMSNorm, _params, _ptr, _residual
+from .norm import RMSNorm, _params, _ptr, _residual, _weight
 from .ops import _lib
 
 ALIGN = 16  # bytes between the starts of rows of codes: a multiple of this
@@ -53,17 +53,18 @@ def _new_codes(x: torch.Tensor) -> torch.Tensor:
     shape = x.shape
     pad = -shape[-1] % ALIGN
     if pad == 0:
-        return x.new_empty(shape, dtype=torch.int8)
+        return torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
     return x.new_empty((*shape[:-1], shape[-1] + pad), dtype=torch.int8)[..., :shape[-1]]
 
 
 def _new_rows(x: torch.Tensor):
-    return _new_codes(x), x.new_empty(x.shape[:-1], dtype=torch.float32)
+    return _new_codes(x), _new_per_row(x)
 
 
 def _stride(codes: torch.Tensor) -> int:
     """Bytes from row to row of a tensor that :func:`_new_codes` or :func:`_laid_out` gave."""
-    return codes.stride(-2) if codes.dim() > 1 and codes.shape[-2] > 1 else codes.shape[-1] + -codes.shape[-1] % ALIGN
+    shape = codes.shape
+    return codes.stride(-2) if len(shape) > 1 and shape[-2] > 1 else shape[-1] + -shape[-1] % ALIGN
 
 
 def _laid_out(codes: torch.Tensor) -> torch.Tensor:
@@ -138,7 +139,7 @@ def _row_quantize_cuda(x):
     x = _act("row_quantize", "x", x)
     codes, scales = _new_rows(x)
     _launch(x, "fmhc_row_quantize", x.data_ptr(), _DTYPES[x.dtype], codes.data_ptr(), _stride(codes),
-            scales.data_ptr(), _rows(x), x.shape[-1])
+            scales.data_ptr(), scales.numel(), x.shape[-1])
     return codes, scales
 
 
@@ -149,7 +150,7 @@ def _row_dequantize_cuda(codes, scales, dtype):
     out_dtype = _float_dtype(op, dtype)
     shape = codes.shape
     codes, scales, stride = _row_codes(op, "codes", codes, "scales", scales)
-    x = scales.new_empty(shape, dtype=dtype)
+    x = scales.new_empty(*shape, dtype=dtype)
     _launch(codes, "fmhc_row_dequantize", codes.data_ptr(), stride, scales.data_ptr(), x.data_ptr(),
             out_dtype, codes.shape[0], codes.shape[1])
     return x
@@ -158,13 +159,13 @@ def _row_dequantize_cuda(codes, scales, dtype):
 def _norm_int8(op: str, x, residual, weight, eps: float):
     x = _act(op, "x", x)
     _same_device(op, x, residual=residual, weight=weight)
-    weight, _, pdt = _params(op, x.shape[-1], weight, None)
+    weight, pdt = _weight(op, x.shape[-1], weight)
     total = None
     if residual is not None:
         residual, total = _residual(op, x, residual), torch.empty_like(x)
     codes, scales = _new_rows(x)
     _launch(x, "fmhc_rms_norm_fwd_int8", x.data_ptr(), _DTYPES[x.dtype], _ptr(residual), _ptr(weight), pdt,
-            eps, codes.data_ptr(), _stride(codes), scales.data_ptr(), _ptr(total), _rows(x), x.shape[-1])
+            eps, codes.data_ptr(), _stride(codes), scales.data_ptr(), _ptr(total), scales.numel(), x.shape[-1])
     return (codes, scales) if total is None else (codes, scales, total)
 
 
@@ -193,7 +194,7 @@ def _int8_linear_cuda(codes, scales, weight_codes, weight_scales, bias, dtype):
     codes, scales, stride = _row_codes(op, "codes", codes, "scales", scales)
     weight_codes, weight_scales, w_stride = _row_codes(op, "weight_codes", weight_codes, "weight_scales", weight_scales)
     _, bias, b_dtype = (None, None, 0) if bias is None else _params(op, N, None, bias)
-    y = scales.new_empty((*lead, N), dtype=dtype)
+    y = scales.new_empty(*lead, N, dtype=dtype)
     _launch(codes, "fmhc_int8_linear", codes.data_ptr(), stride, scales.data_ptr(), weight_codes.data_ptr(),
             w_stride, weight_scales.data_ptr(), _ptr(bias), b_dtype, y.data_ptr(), y_dtype, codes.shape[0], N, K)
     return y

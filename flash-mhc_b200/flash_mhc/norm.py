@@ -36,7 +36,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .act8 import (_DTYPES, _act, _checkpoint, _format, _launch, _new_checkpoint, _register_autograd,
+from .act8 import (_DTYPES, _act, _checkpoint, _format, _launch, _new_checkpoint, _new_per_row, _register_autograd,
                    _rows, _same_device, _shape, _workspace)
 from .ops import _lib
 
@@ -75,6 +75,16 @@ def _params(op: str, C: int, weight, bias):
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"flash_mhc::{op}: weight and bias must have one type (got {weight.dtype} and {bias.dtype})")
     return (None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), dt)
+
+
+def _weight(op: str, C: int, weight):
+    """``weight`` as _params gives it, by a shorter way where nothing is wrong with it."""
+    if weight is None:
+        return None, 0
+    if len(weight.shape) == 1 and weight.shape[0] == C and weight.dtype in _DTYPES:
+        return weight.contiguous(), _DTYPES[weight.dtype]
+    weight, _, dt = _params(op, C, weight, None)
+    return weight, dt
 
 
 def _ptr(t):
@@ -138,7 +148,8 @@ def _backward(op: str, grad_out, x, codes, scales, mean, rstd, weight, bias):
 
 def _residual(op: str, x, residual):
     """``residual`` beside ``x`` (already checked): of its shape and type, contiguous."""
-    _shape(op, "residual", residual, x.shape)
+    if residual.shape != x.shape:
+        _shape(op, "residual", residual, x.shape)
     if residual.dtype != x.dtype:
         raise ValueError(f"flash_mhc::{op}: x and residual must have one type (got {x.dtype} and {residual.dtype})")
     return residual.contiguous()
@@ -147,33 +158,34 @@ def _residual(op: str, x, residual):
 def _rms_forward(op: str, x, residual, weight, eps: float):
     x = _act(op, "x", x)
     _same_device(op, x, residual=residual, weight=weight)
-    weight, _, pdt = _params(op, x.shape[-1], weight, None)
+    C = x.shape[-1]
+    weight, pdt = _weight(op, C, weight)
     total = None
     if residual is not None:
         residual, total = _residual(op, x, residual), torch.empty_like(x)
-    y, rstd = torch.empty_like(x), x.new_empty(x.shape[:-1], dtype=torch.float32)
+    y, rstd = torch.empty_like(x), _new_per_row(x)
     _launch(x, "fmhc_rms_norm_fwd", x.data_ptr(), _DTYPES[x.dtype], _ptr(residual), _ptr(weight), pdt,
-            eps, y.data_ptr(), _ptr(total), rstd.data_ptr(), _rows(x), x.shape[-1])
+            eps, y.data_ptr(), _ptr(total), rstd.data_ptr(), x.numel() // C, C)
     return (y, rstd) if total is None else (y, total, rstd)
 
 
 def _rms_backward(op: str, grad_out, grad_total, x, rstd, weight):
     grad_out = _act(op, "grad_out", grad_out)
     _same_device(op, grad_out, grad_total=grad_total, x=x, rstd=rstd, weight=weight)
+    shape, dtype = grad_out.shape, grad_out.dtype
     for name, t in (("x", x), ("grad_total", grad_total)):
-        if t is not None:
-            _shape(op, name, t, grad_out.shape)
-            if t.dtype != grad_out.dtype:
-                raise ValueError(f"flash_mhc::{op}: grad_out and {name} must have one type "
-                                 f"(got {grad_out.dtype} and {t.dtype})")
+        if t is not None and (t.shape != shape or t.dtype != dtype):
+            _shape(op, name, t, shape)
+            raise ValueError(f"flash_mhc::{op}: grad_out and {name} must have one type (got {dtype} and {t.dtype})")
     x = x.contiguous()
     grad_total = None if grad_total is None else grad_total.contiguous()
-    _shape(op, "rstd", rstd, grad_out.shape[:-1])
+    if rstd.shape != shape[:-1]:
+        _shape(op, "rstd", rstd, shape[:-1])
     if rstd.dtype != torch.float32:
         raise ValueError(f"flash_mhc::{op}: rstd must be float32 (got {rstd.dtype})")
     rstd = rstd.contiguous()
-    C, rows = grad_out.shape[-1], _rows(grad_out)
-    weight, _, pdt = _params(op, C, weight, None)
+    C, rows = shape[-1], grad_out.numel() // shape[-1]
+    weight, pdt = _weight(op, C, weight)
     grad_x = torch.empty_like(grad_out)
     ws, ws_bytes, _keep = None, 0, None
     if weight is None:
@@ -181,7 +193,7 @@ def _rms_backward(op: str, grad_out, grad_total, x, rstd, weight):
     else:
         grad_w = torch.empty_like(weight)
         ws, ws_bytes, _keep = _workspace(grad_out, "fmhc_rms_norm_bwd_workspace_size", rows, C)
-    _launch(grad_out, "fmhc_rms_norm_bwd", grad_out.data_ptr(), _DTYPES[grad_out.dtype], _ptr(grad_total),
+    _launch(grad_out, "fmhc_rms_norm_bwd", grad_out.data_ptr(), _DTYPES[dtype], _ptr(grad_total),
             x.data_ptr(), rstd.data_ptr(), _ptr(weight), pdt, grad_x.data_ptr(),
             None if weight is None else grad_w.data_ptr(), ws, ws_bytes, rows, C)
     return grad_x, grad_w
