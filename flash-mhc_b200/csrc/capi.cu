@@ -876,11 +876,10 @@ int fmhc_row_dequantize(const void *codes, int64_t codes_stride, const float *sc
   return check_launch(w);
 }
 
-int fmhc_int8_linear(const void *codes, int64_t codes_stride, const float *scales,
-                     const void *weight_codes, int64_t weight_stride, const float *weight_scales,
-                     const void *bias, int bias_dtype, void *y, int y_dtype, int64_t T, int64_t N,
-                     int64_t K, void *stream) {
-  const char *w = "fmhc_int8_linear";
+static int int8_linear(const char *w, const void *codes, int64_t codes_stride, const float *scales,
+                       const void *weight_codes, int64_t weight_stride, const float *weight_scales,
+                       const void *bias, int bias_dtype, void *y, int y_dtype, int64_t T, int64_t N,
+                       int64_t K, void *stream, bool lose_copy) {
   for (int64_t n : {T, N})
     if (n < 0 || n >= (int64_t(1) << 31) - 512)  // the last tile's end fits 32 bits too
       return fail(FMHC_ERR_INVALID_ARGUMENT, "%s: T and N must be in [0, 2^31 - 512) (got %lld)", w, (long long)n);
@@ -900,9 +899,26 @@ int fmhc_int8_linear(const void *codes, int64_t codes_stride, const float *scale
   FMHC_REQUIRE_ALIGN_TO(w, bias, dtype_size(bias_dtype)); FMHC_REQUIRE_ALIGN_TO(w, y, dtype_size(y_dtype));
   if (int e = fmhc::launch_int8_linear(codes, codes_stride, scales, weight_codes, weight_stride,
                                        weight_scales, bias, bias_dtype, y, y_dtype, T, N, int(K),
-                                       (cudaStream_t)stream))
+                                       (cudaStream_t)stream, lose_copy))
     return e;
   return check_launch(w);
+}
+
+int fmhc_int8_linear(const void *codes, int64_t codes_stride, const float *scales,
+                     const void *weight_codes, int64_t weight_stride, const float *weight_scales,
+                     const void *bias, int bias_dtype, void *y, int y_dtype, int64_t T, int64_t N,
+                     int64_t K, void *stream) {
+  return int8_linear("fmhc_int8_linear", codes, codes_stride, scales, weight_codes, weight_stride,
+                     weight_scales, bias, bias_dtype, y, y_dtype, T, N, K, stream, false);
+}
+
+int fmhc_debug_int8_linear_lost_copy(const void *codes, int64_t codes_stride, const float *scales,
+                                     const void *weight_codes, int64_t weight_stride,
+                                     const float *weight_scales, void *y, int64_t T, int64_t N,
+                                     int64_t K, void *stream) {
+  return int8_linear("fmhc_debug_int8_linear_lost_copy", codes, codes_stride, scales, weight_codes,
+                     weight_stride, weight_scales, nullptr, FMHC_DTYPE_F32, y, FMHC_DTYPE_BF16, T, N, K,
+                     stream, true);
 }
 
 }  // extern "C"

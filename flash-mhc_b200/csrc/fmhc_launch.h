@@ -139,10 +139,11 @@ void launch_row_dequantize(const void *codes, int64_t stride, const float *scale
 
 // int8_linear.cu -- y (T, N) of type ydt from codes xc (T, K) and wc (N, K) in rows
 // of xstride and wstride bytes (multiples of 16, as xc and wc are); b may be null.
-// Returns 0 or an fmhc_status code with the error's text set.
+// Returns 0 or an fmhc_status code with the error's text set.  lose_copy: test hook,
+// y of bf16 (the kernels' LOSE_COPY).
 int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const void *wc, int64_t wstride,
                        const float *ws, const void *b, int bdt, void *y, int ydt, int64_t T, int64_t N,
-                       int K, cudaStream_t s);
+                       int K, cudaStream_t s, bool lose_copy = false);
 // Reads and clears this file's device error word.
 int read_int8_linear_error(unsigned *code);
 

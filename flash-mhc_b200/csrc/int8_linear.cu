@@ -19,6 +19,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "act8.cuh"
 #include "fmhc_launch.h"
@@ -143,7 +144,9 @@ __device__ __forceinline__ void tile_of(int64_t id, int tiles_n, int tiles_t, in
 // Persistent: pair p takes tiles p, p + pairs, ...  Barriers: `full` is the
 // leader's and counts the bytes of both CTAs' copies; a commit arrives on `empty`
 // and `tfull` of both; the epilogue warps of both arrive on the leader's `tempty`.
-template <class E>
+// LOSE_COPY (test hook only, as in k1_tc.cu): the first CTA arms its first stage's
+// barrier but issues no copy for it, so the waits on that stage can only expire.
+template <class E, bool LOSE_COPY = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + kPairEpiThreads, 1)
 int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                         E *__restrict__ y, const Args A) {
@@ -199,8 +202,10 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid
           const uint32_t full = smem_u32(&sm.full[stage]);
           if (rank == 0) mbar_arrive_expect_tx(full, bytes);
           const uint32_t lead = mapa_shared(full, 0);
-          tma_load_2d_pair(smem_u32(sm.a[stage]), &tmap_w, lead, kb * kBK, n0);
-          tma_load_2d_pair(smem_u32(sm.b[stage]), &tmap_x, lead, kb * kBK, t0);
+          if (!(LOSE_COPY && blockIdx.x == 0 && issued == 0)) {
+            tma_load_2d_pair(smem_u32(sm.a[stage]), &tmap_w, lead, kb * kBK, n0);
+            tma_load_2d_pair(smem_u32(sm.b[stage]), &tmap_x, lead, kb * kBK, t0);
+          }
           ++issued;
           if (++stage == kPairStages) { stage = 0; phase ^= 1; }
         }
@@ -321,7 +326,7 @@ struct SplitTail {
 enum : unsigned { kSiteSplitEmpty = 0x211, kSiteSplitFull = 0x212, kSiteSplitTfull = 0x214,
                   kSiteSplitDrain = 0x215 };
 
-template <class E, int S>
+template <class E, int S, bool LOSE_COPY = false>
 __global__ void __launch_bounds__(kThreads)
 int8_linear_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                          E *__restrict__ y, const Args A, int stages, int tmem_cols) {
@@ -377,8 +382,10 @@ int8_linear_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
         const uint32_t full = smem_u32(&sm.full[stage]);
         mbar_arrive_expect_tx(full, uint32_t(stage_bytes));
         const uint32_t a = smem_u32(base) + uint32_t(stage * stage_bytes);
-        tma_load_2d(a, &tmap_w, full, kb * kBK, tile_n * kBM);
-        tma_load_2d(a + kATile, &tmap_x, full, kb * kBK, int32_t(t0));
+        if (!(LOSE_COPY && blockIdx.x == 0 && issued == 0)) {
+          tma_load_2d(a, &tmap_w, full, kb * kBK, tile_n * kBM);
+          tma_load_2d(a + kATile, &tmap_x, full, kb * kBK, int32_t(t0));
+        }
         ++issued;
         if (++stage == stages) { stage = 0; phase ^= 1; }
       }
@@ -586,7 +593,7 @@ int read_int8_linear_error(unsigned *code) {
 
 int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const void *wc, int64_t wstride,
                        const float *ws, const void *b, int bdt, void *y, int ydt, int64_t T, int64_t N,
-                       int K, cudaStream_t s) {
+                       int K, cudaStream_t s, bool lose_copy) {
   const int sms = sm_count();
   const int nk = int(ceil_div(K, kBK));
   Args a{};
@@ -596,7 +603,7 @@ int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const v
   // (us, it / tiles of 128 columns: T x N x K 1 x 4096 x 4096 5.3 / 7.7, 2 x 4096 x 4096
   // 6.9 / 8.0, 4 x 4096 x 4096 9.9 / 8.1, 1 x 16384 x 4096 13.3 / 13.1, 8 x 16384 x 4096
   // 33 / 13.6).
-  if (T <= kRowsMost && T * N * K <= int64_t(1) << 25) {
+  if (!lose_copy && T <= kRowsMost && T * N * K <= int64_t(1) << 25) {
     int split = 1;  // warps that share K: enough blocks for every SM, while there is K for them
     while (split < kRowWarps && ceil_div(N, kRowCols * (kRowWarps / split)) < 2 * sms && K > split * 512 * kRowDepth) split *= 2;
     const int64_t blocks = ceil_div(N, int64_t(kRowCols) * (kRowWarps / split));
@@ -623,6 +630,9 @@ int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const v
     const size_t smem = sizeof(PairSmem) + 1024;
     FMHC_DISPATCH_ELEM(ydt, {
       auto k = int8_linear_pair_kernel<E>;
+      if constexpr (std::is_same<E, __nv_bfloat16>::value) {
+        if (lose_copy) k = int8_linear_pair_kernel<E, true>;
+      }
       allow_smem(reinterpret_cast<const void *>(k), smem);
       launch(k, dim3(unsigned(pairs * 2)), dim3(64 + kPairEpiThreads), smem, s, mw, mx, (E *)y, a);
     });
@@ -657,6 +667,11 @@ int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const v
   FMHC_DISPATCH_ELEM(ydt, {
     auto k = S == 1 ? int8_linear_split_kernel<E, 1> : S == 2 ? int8_linear_split_kernel<E, 2>
            : S == 4 ? int8_linear_split_kernel<E, 4> : int8_linear_split_kernel<E, 8>;
+    if constexpr (std::is_same<E, __nv_bfloat16>::value) {
+      if (lose_copy)
+        k = S == 1 ? int8_linear_split_kernel<E, 1, true> : S == 2 ? int8_linear_split_kernel<E, 2, true>
+          : S == 4 ? int8_linear_split_kernel<E, 4, true> : int8_linear_split_kernel<E, 8, true>;
+    }
     allow_smem(reinterpret_cast<const void *>(k), smem);
     launch_cluster(k, dim3(unsigned(tiles * S)), dim3(kThreads), smem, s, unsigned(S), mw, mx, (E *)y, a, stages, cols);
   });

@@ -70,6 +70,7 @@ _SIGNATURES = {
     "fmhc_row_quantize": [_vp, _int, _vp, _i64, _vp, _i64, _i64, _vp],
     "fmhc_row_dequantize": [_vp, _i64, _vp, _vp, _int, _i64, _i64, _vp],
     "fmhc_int8_linear": [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _int, _vp, _int, _i64, _i64, _i64, _vp],
+    "fmhc_debug_int8_linear_lost_copy": [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp],
 }
 _RESTYPES = {
     "fmhc_last_error": ctypes.c_char_p,

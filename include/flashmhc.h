@@ -463,6 +463,16 @@ FMHC_API int fmhc_int8_linear(const void *codes, int64_t codes_stride, const flo
                               void *y, int y_dtype, int64_t T, int64_t N, int64_t K,
                               void *stream);
 
+/* Test hook for the failure path of fmhc_int8_linear (not for production use), as
+ * fmhc_debug_k1_fwd_lost_copy: the tensor-core kernel that the sizes choose, in which
+ * the first CTA loses its first copy.  Its waits expire (about 1 s each), it records a
+ * site code in the error word, and the parts of y (bf16) that it gave up on are NaN. */
+FMHC_API int fmhc_debug_int8_linear_lost_copy(const void *codes, int64_t codes_stride,
+                                              const float *scales, const void *weight_codes,
+                                              int64_t weight_stride, const float *weight_scales,
+                                              void *y, int64_t T, int64_t N, int64_t K,
+                                              void *stream);
+
 #ifdef __cplusplus
 }
 #endif
