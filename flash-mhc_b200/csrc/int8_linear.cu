@@ -24,6 +24,7 @@
 #include "act8.cuh"
 #include "fmhc_launch.h"
 #include "grid.cuh"
+#include "lane_ring.cuh"
 #include "rows8.cuh"
 #include "sm100_ptx.cuh"
 #include "tma_map.h"
@@ -64,8 +65,9 @@ __device__ __forceinline__ float bias1(const void *b, int dtype, int64_t n) {
 // No branch stands between the rows of a whole chunk: one per row made each wait for
 // the latency of its own arithmetic (tiles of 256 x 256 took 20 us each).  Two columns
 // of a row per store, swapped between lanes, were slower (65536 x 1024 x 1024: 63.4
-// against 67.6 us), and so was converting the sums by ordinary arithmetic (83 against
-// 72 at the time).
+// against 67.6 us), and so were converting the sums by ordinary arithmetic (83 against
+// 72 at the time) and row addresses from a multiplication or from a base that the warp
+// shares (24973 x 10752 x 48: 224 and 233 against 175).
 template <class E>
 __device__ __forceinline__ void store_rows(const int (&v)[32], int rows, const float *xs, float ws, float b,
                                            E *y, int64_t N, bool in) {
@@ -73,10 +75,13 @@ __device__ __forceinline__ void store_rows(const int (&v)[32], int rows, const f
 #pragma unroll
   for (int j = 0; j < 32; j += 4) {
     const float4 x = *reinterpret_cast<const float4 *>(xs + j);
-    o[j] = Elem<E>::narrow1(fmaf(__int2float_rn(v[j]), x.x * ws, b));
-    o[j + 1] = Elem<E>::narrow1(fmaf(__int2float_rn(v[j + 1]), x.y * ws, b));
-    o[j + 2] = Elem<E>::narrow1(fmaf(__int2float_rn(v[j + 2]), x.z * ws, b));
-    o[j + 3] = Elem<E>::narrow1(fmaf(__int2float_rn(v[j + 3]), x.w * ws, b));
+    const float2 p0 = mul2(make_float2(x.x, x.y), both(ws)), p1 = mul2(make_float2(x.z, x.w), both(ws));
+    const float2 f0 = fma2(make_float2(__int2float_rn(v[j]), __int2float_rn(v[j + 1])), p0, both(b));
+    const float2 f1 = fma2(make_float2(__int2float_rn(v[j + 2]), __int2float_rn(v[j + 3])), p1, both(b));
+    o[j] = Elem<E>::narrow1(f0.x);
+    o[j + 1] = Elem<E>::narrow1(f0.y);
+    o[j + 2] = Elem<E>::narrow1(f1.x);
+    o[j + 3] = Elem<E>::narrow1(f1.y);
   }
   if (rows >= 32) {
     if (in) {
@@ -89,22 +94,16 @@ __device__ __forceinline__ void store_rows(const int (&v)[32], int rows, const f
       if (in && j < rows) *y = o[j];
   }
 }
-// One column of a tile: `rows` rows from this warp's lanes of TMEM.  The next chunk is
-// on its way from TMEM while one is stored.
+// One column of a tile: `rows` rows from this warp's lanes of TMEM.  (Loading the next
+// chunk ahead costs registers and was slower: 24973 x 10752 x 48 166 against 158 us.)
 template <class E>
 __device__ __forceinline__ void store_column(uint32_t tmem, int rows, const float *xs, float ws, float b,
                                              E *y, int64_t N, bool in) {
-  uint32_t v[2][32];
-  if (rows > 0) tmem_ld_32x32b_x32(tmem, v[0]);
-  for (int c = 0; c < rows; c += 64) {
+  for (int c = 0; c < rows; c += 32) {
+    uint32_t v[32];
+    tmem_ld_32x32b_x32(tmem + uint32_t(c), v);
     tmem_wait_ld();
-    if (c + 32 < rows) tmem_ld_32x32b_x32(tmem + uint32_t(c + 32), v[1]);
-    store_rows(reinterpret_cast<const int (&)[32]>(v[0]), rows - c, xs + c, ws, b, y, N, in);
-    if (c + 32 >= rows) break;
-    tmem_wait_ld();
-    if (c + 64 < rows) tmem_ld_32x32b_x32(tmem + uint32_t(c + 64), v[0]);
-    store_rows(reinterpret_cast<const int (&)[32]>(v[1]), rows - c - 32, xs + c + 32, ws, b, y + 32 * N, N, in);
-    y += 64 * N;
+    store_rows(reinterpret_cast<const int (&)[32]>(v), rows - c, xs + c, ws, b, y + c * N, N, in);
   }
 }
 template <class E>

@@ -9,6 +9,13 @@
 //
 // Sums are f32.  The norm is that of the rounded total, which the backward reads
 // too, so forward and gradients belong to the same values.
+//
+// Memory bounds them.  Measured, bf16, us (floor of the bytes at the copy rate): norm
+// 65536 x 2048 93 (83), 16384 x 8192 85 (83); with a residual 131072 x 1024 183 (165),
+// 32768 x 4096 163 (165); to 8 bits 65536 x 2048 72 (62), with a residual 146 (144);
+// backward 65536 x 2048 128 (124), with the gradient of total 131072 x 1024 156 (165,
+// part of grad_x being still in L2).  f32 65536 x 2048: 197 (165), with a residual 365
+// (330), backward 252 (248).
 #include "fmhc_launch.h"
 #include "norm_rows.cuh"
 #include "rows8.cuh"
@@ -301,6 +308,7 @@ rms_bwd_kernel(const E *__restrict__ g, const E *__restrict__ gt, const E *__res
 }
 
 // ---------------------------------------------- any width and any alignment
+// For pointers that are not 16-byte aligned and rows past the other kernels' widths.
 // One block per row, which is read again for each step (from L1 or L2).
 __device__ float block_sum(float v, float *sh) {
   v = warp_sum(v);
@@ -434,7 +442,7 @@ rms_weight_grad_kernel(const float *__restrict__ part, void *__restrict__ gw, in
 }
 
 // Slices of 32 rows or more; up to 128 rows are one, which needs no kernel to add
-// partials.
+// partials (as layer norm's, and measured there).
 int any_slices(int64_t rows, int C) {
   if (rows <= 128) return 1;
   const int64_t cols = (C + 31) / 32;

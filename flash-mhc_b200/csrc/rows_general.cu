@@ -11,8 +11,16 @@
 // the weight's gradient in registers.  Narrow rows take a power-of-two group of lanes
 // each, 32 / group of them in a warp.
 //
-// Measured, us (one block per row before; floor of the bytes at the copy rate), bf16:
-// TABLE
+// Measured, bf16, us: one block per row (rms_norm.cu, rows8.cu) / these (the bytes at the
+// copy rate).
+//                       131072 x 64          131072 x 77          65536 x 1023
+//   norm                20 / 10.5 (5.2)      168 / 19 (6.2)       162 / 72 (41)
+//   backward            33 / 17 (7.7)        196 / 32 (9.3)       430 / 121 (62)
+//   add, norm, 8 bits   35 / 16 (9.0)        256 / 39 (11)        317 / 159 (72)
+//   quantise            21 / 10.5 (3.9)      120 / 25 (4.7)       107 / 97 (31)
+// (64: the kernels for wide rows, a warp per row, in place of a block.)  Instructions
+// bound them (70 % of the issue slots at 1023): masks, the ends' stores value by value,
+// and codes moved between lanes.
 #include "rows_general.h"
 
 #include <numeric>
