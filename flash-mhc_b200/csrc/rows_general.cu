@@ -87,10 +87,6 @@ __device__ __forceinline__ void copy_part(uint32_t dst, const E *src, int64_t th
   }
 }
 
-__device__ __forceinline__ float group_total(float v, int group) {
-  for (int o = group >> 1; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
 __device__ __forceinline__ uint32_t group_most(uint32_t v, int group) {
   for (int o = group >> 1; o >= 1; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
@@ -214,7 +210,7 @@ general_fwd_kernel(const E *__restrict__ x, const E *__restrict__ res, const voi
     });
     if (++stage == S) stage = 0;
     if constexpr (NORM) {
-      q = team_sum1(group_total(q, group), sum_slots[par], tm, warp);
+      q = team_sum1(group_sum(q, group), sum_slots[par], tm, warp);
       const float rstd = rsqrtf(fmaf(q, inv_C, eps));
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -330,7 +326,7 @@ general_bwd_kernel(const E *__restrict__ g, const E *__restrict__ gt, const E *_
         }
       }
     });
-    const float sum = team_sum1(group_total(dot, group), slots[par], tm, warp);
+    const float sum = team_sum1(group_sum(dot, group), slots[par], tm, warp);
     const float c = -sum * inv_C * rs;  // times x
     unrolled<NV>([&](auto i) {
       if (valid && i * 32 < p.left) {

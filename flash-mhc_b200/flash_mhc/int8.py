@@ -303,6 +303,8 @@ class Int8Linear(nn.Module):
         super().__init__()
         if norm is not None and norm.hidden_size != in_features:
             raise ValueError(f"Int8Linear: the norm must be over {in_features} values (got {norm.hidden_size})")
+        if not 0 < in_features < 1 << 17:
+            raise ValueError(f"Int8Linear: in_features must be in [1, 2^17) (got {in_features})")
         _float_dtype("Int8Linear", dtype)
         self.in_features, self.out_features, self.dtype = in_features, out_features, dtype
         like = torch.empty(0, dtype=dtype, device=device)
@@ -348,7 +350,7 @@ class Int8Linear(nn.Module):
             if residual is not None:
                 raise ValueError("Int8Linear: a residual is added in front of the layer's norm, and it has none")
             return (*_quantize(x), None, x.dtype)
-        if norm._check(x):
+        if norm._check(x, residual):
             if residual is None:
                 return (*rms_norm_int8(x, norm.weight, norm.eps), None, x.dtype)
             codes, scales, total = add_rms_norm_int8(x, residual, norm.weight, norm.eps)
@@ -385,8 +387,8 @@ def convert_linears(module: nn.Module) -> nn.Module:
     a linear layer or a ``nn.Sequential`` that gets shorter.  In a ``nn.Sequential``
     an ``RMSNorm`` in front of a linear layer becomes part of it.  An
     ``MHCLiteBlock`` keeps its own projection and has its wrapped layer converted.
-    Subclasses of ``nn.Linear``, layers with hooks and layers of other types than
-    float32, bfloat16 and float16 stay as they are.
+    Subclasses of ``nn.Linear``, layers with hooks, layers of other types than float32,
+    bfloat16 and float16 and layers of 2^17 inputs or more stay as they are.
     """
     return _convert(module, {})
 
@@ -397,7 +399,8 @@ def _has_hooks(m: nn.Module) -> bool:
 
 
 def _convertible(m: nn.Module | None) -> bool:
-    return type(m) is nn.Linear and m.weight.dtype in _DTYPES and not _has_hooks(m)
+    return (type(m) is nn.Linear and m.weight.dtype in _DTYPES and 0 < m.in_features < 1 << 17
+            and not _has_hooks(m))
 
 
 def _convert(module: nn.Module, done: dict[int, nn.Module]) -> nn.Module:

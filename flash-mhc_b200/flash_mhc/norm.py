@@ -459,14 +459,17 @@ class RMSNorm(nn.Module):
     def extra_repr(self) -> str:
         return f"{self.hidden_size}, eps={self.eps}"
 
-    def _check(self, x: torch.Tensor) -> bool:
+    def _check(self, x: torch.Tensor, residual: torch.Tensor | None) -> bool:
         """Whether the fused kernels take ``x``."""
         if x.shape[-1:] != (self.hidden_size,):
             raise ValueError(f"RMSNorm: expected a last dimension of {self.hidden_size} (got {tuple(x.shape)})")
+        if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+            raise ValueError(f"RMSNorm: the residual must be {tuple(x.shape)} and {x.dtype} like x "
+                             f"(got {tuple(residual.shape)} and {residual.dtype})")
         return x.is_cuda and x.dtype in _DTYPES
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
-        if self._check(x):
+        if self._check(x, residual):
             if residual is None:
                 return rms_norm(x, self.weight, self.eps)
             return add_rms_norm(x, residual, self.weight, self.eps)

@@ -287,3 +287,48 @@ def test_int8_linear_module_on_cuda():
         back = moved.cuda()
         assert back.weight_codes.stride() == (208, 1) and torch.equal(back(x, r)[0], y)
         assert q.half()(x.half(), r.half())[0].dtype == HF
+
+
+def test_offsets_past_32_bits():
+    """A weight, activations and an output of more than 2^32 bytes: the far ends against a call on them alone."""
+    g = _gen(9)
+    K = 65536
+    wc = torch.randint(-127, 128, (66000, K), generator=g, device="cuda", dtype=torch.int8)
+    ws = torch.rand(66000, generator=g, device="cuda")
+    xc, xs = wc[-300:].flip(0).contiguous(), ws[-300:].flip(0).contiguous()
+    for T in (1, 20, 300):
+        y = int8.linear(xc[:T], xs[:T], wc, ws)
+        for at in (slice(0, 200), slice(65500, 66000)):
+            assert torch.equal(y[:, at], int8.linear(xc[:T], xs[:T], wc[at], ws[at]))
+    y = int8.linear(wc, ws, xc[:5], xs[:5])
+    assert torch.equal(y[-200:], int8.linear(wc[-200:], ws[-200:], xc[:5], xs[:5]))
+    back = int8.dequantize_rows(wc, ws)
+    assert torch.equal(back[-3:], int8.dequantize_rows(wc[-3:], ws[-3:]))
+    again = int8.quantize_rows(back)
+    assert torch.equal(again[0][-3:], int8.quantize_rows(back[-3:].clone())[0])
+    del back, again, y, wc
+    # an output of 5e9 elements
+    wide = torch.randint(-127, 128, (70001, 32), generator=g, device="cuda", dtype=torch.int8)
+    ones = torch.ones(70001, device="cuda")
+    y = int8.linear(wide, ones, wide, ones)
+    assert torch.equal(y[-100:, -100:], int8.linear(wide[-100:], ones[-100:], wide[-100:], ones[-100:]))
+    assert torch.equal(y[35000:35010, 69990:], int8.linear(wide[35000:35010], ones[:10], wide[69990:], ones[:11]))
+
+
+def test_compiled():
+    """Through torch.compile's tracing (no code generation): the same values, and gradients for the norm."""
+    torch.manual_seed(0)
+    x, r, w = (torch.randn(*s, device="cuda", requires_grad=True) for s in ((40, 200), (40, 200), (200,)))
+    f = lambda x, r, w: norm.add_rms_norm(x, r, w)  # noqa: E731
+    c = torch.compile(f, backend="aot_eager", fullgraph=True)
+    for fn in (f, c):
+        y, total = fn(x, r, w)
+        grads = torch.autograd.grad(y.square().sum() + total.sum(), (x, r, w))
+        if fn is f:
+            want = (y, total, *grads)
+        else:
+            assert all(torch.equal(a, b) for a, b in zip(want, (y, total, *grads)))
+    lin = int8.Int8Linear.from_linear(nn.Linear(200, 90).cuda(), norm.RMSNorm(200, device="cuda"))
+    with torch.no_grad():
+        for a, b in zip(lin(x, r), torch.compile(lin, backend="aot_eager")(x, r)):
+            assert torch.equal(a, b)

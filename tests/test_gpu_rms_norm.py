@@ -328,3 +328,22 @@ def test_refusals():
         dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
         with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
             ops.rms_norm(dual, w, EPS)
+
+
+@pytest.mark.parametrize("C", [2048, 2047])
+def test_offsets_past_32_bits(C):
+    """More than 2^31 values: the last rows against a call on them alone."""
+    rows, last = 1_100_000, 64
+    g = torch.Generator(device="cuda").manual_seed(C)
+    x = torch.empty(rows, C, device="cuda", dtype=BF).normal_(generator=g)
+    w = torch.rand(C, device="cuda", generator=g)
+    y, total, rstd = ops.add_rms_norm(x, x, w, EPS)
+    few = ops.add_rms_norm(x[-last:].clone(), x[-last:].clone(), w, EPS)
+    for a, b in zip((y, total, rstd), few):
+        assert torch.equal(a[-last:], b)
+    gx, gw = ops.rms_norm_backward(y, total, x, rstd, w)
+    few = ops.rms_norm_backward(y[-last:].clone(), total[-last:].clone(), x[-last:].clone(), rstd[-last:].clone(), w)
+    assert torch.equal(gx[-last:], few[0]) and torch.isfinite(gw).all()
+    codes, scales = ops.rms_norm_int8(x, w, EPS)
+    few = ops.rms_norm_int8(x[-last:].clone(), w, EPS)
+    assert torch.equal(codes[-last:], few[0]) and torch.equal(scales[-last:], few[1])

@@ -222,6 +222,12 @@ def test_int8_linear_on_cpu():
         q(x, x)
     with pytest.raises(ValueError, match="norm must be"):
         int8.Int8Linear(8, 8, norm=norm.RMSNorm(9))
+    with pytest.raises(ValueError, match="in_features"):
+        int8.Int8Linear(1 << 17, 1, device="meta")
+    with pytest.raises(ValueError, match="residual must be"):
+        int8.Int8Linear(8, 8, norm=norm.RMSNorm(8))(torch.zeros(3, 8), torch.zeros(8))
+    with pytest.raises(ValueError, match="residual must be"):
+        norm.RMSNorm(8)(torch.zeros(3, 8), torch.zeros(3, 8, dtype=BF))
     n = int8.Int8Linear.from_linear(layer, norm.RMSNorm(40))
     with pytest.raises(ValueError, match="without a norm"):
         n((c, s))
