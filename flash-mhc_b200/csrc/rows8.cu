@@ -1,6 +1,6 @@
 // Rows put into 8 bits and restored (format: rows8.cuh).  Memory bounds both: 32768 x
 // 4096 bf16 63 us and 70 us (the bytes at the copy rate take 62).  Restoring writes twice
-// what it reads; rows that start anywhere in a word restore 65536 x 1023 in 87 us (31),
+// what it reads; rows that start anywhere in a word restore 65536 x 1023 in 70 us (31),
 // bound by instructions.
 #include "fmhc_launch.h"
 #include "norm_rows.cuh"
@@ -83,71 +83,83 @@ row_quantize_kernel(const E *__restrict__ x, int8_t *__restrict__ codes, int64_t
   }
 }
 
-// Restoring: a group of lanes (a power of two, up to 32) takes up to four chunks of
-// eight codes per lane of one row, so that narrow rows share a warp and wide ones
-// spread over several.
-constexpr int kRestoreChunks = 4;
+// Restoring: a group of lanes (a power of two, up to 32) takes `per` chunks of eight
+// codes of one row, up to kRestoreChunks per lane, all of them in flight at a time:
+// narrow rows share a warp and wide ones are cut into equal segments.
+constexpr int kRestoreChunks = 4;  // (of 8: 65536 x 1023 101 us instead of 70)
+struct Restore {
+  int group, segments, per;
+  int64_t units;
+};
+__device__ __forceinline__ int64_t row_of(int64_t u, const Restore &p) {
+  return p.units <= 0xffffffffll ? int64_t(uint32_t(u) / uint32_t(p.segments)) : u / p.segments;
+}
+
 template <class E>
 __global__ void __launch_bounds__(kThreads)
 row_dequantize_kernel(const int8_t *__restrict__ codes, int64_t stride, const float *__restrict__ scales,
-                      E *__restrict__ x, int64_t rows, int C, int group, int64_t units, int segments) {
+                      E *__restrict__ x, int64_t rows, int C, const Restore p) {
   pdl_wait();
-  const int lane = threadIdx.x & (group - 1);
-  const int64_t hop = (int64_t(gridDim.x) * kThreads) / group;
-  for (int64_t u = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / group; u < units; u += hop) {
-    const int64_t r = units <= 0xffffffffll ? int64_t(uint32_t(u) / uint32_t(segments)) : u / segments;
-    const int c0 = int(u - r * segments) * (kRestoreChunks * group) + lane;
-    const uint2 *from = reinterpret_cast<const uint2 *>(codes + r * stride) + c0;
+  const int lane = threadIdx.x & (p.group - 1);
+  const int64_t hop = (int64_t(gridDim.x) * kThreads) / p.group;
+  for (int64_t u = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / p.group; u < p.units; u += hop) {
+    const int64_t r = row_of(u, p);
+    const int c0 = int(u - r * p.segments) * p.per, end = min(c0 + p.per, C / 8);
+    const uint2 *from = reinterpret_cast<const uint2 *>(codes + r * stride);
     const float s = __ldg(scales + r);
     uint2 v[kRestoreChunks];
 #pragma unroll
     for (int i = 0; i < kRestoreChunks; ++i)
-      if ((c0 + i * group) * 8 < C) v[i] = __ldcs(from + i * group);
+      if (c0 + lane + i * p.group < end) v[i] = __ldcs(from + c0 + lane + i * p.group);
 #pragma unroll
-    for (int i = 0; i < kRestoreChunks; ++i)
-      if ((c0 + i * group) * 8 < C) {
+    for (int i = 0; i < kRestoreChunks; ++i) {
+      const int c = c0 + lane + i * p.group;
+      if (c < end) {
         float f[8];
         restore<kInt8>(v[i], s, f);
-        st8(x + r * C + int64_t(c0 + i * group) * 8, f);
+        st8(x + r * C + int64_t(c) * 8, f);
       }
+    }
   }
 }
 
 // The same for rows of any width: the chunks are the aligned ones of x (see
-// rows_general.cu), whose codes start anywhere in a word.
+// rows_general.cu), whose codes start anywhere in a word and lie in up to three.
 template <class E>
 __global__ void __launch_bounds__(kThreads)
 row_dequantize_general_kernel(const int8_t *__restrict__ codes, int64_t stride, const float *__restrict__ scales,
-                              E *__restrict__ x, int64_t rows, int C, int group, int64_t units, int segments) {
+                              E *__restrict__ x, int64_t rows, int C, const Restore p) {
   pdl_wait();
-  const int lane = threadIdx.x & (group - 1);
-  const int64_t hop = (int64_t(gridDim.x) * kThreads) / group;
-  for (int64_t u = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / group; u < units; u += hop) {
-    const int64_t r = units <= 0xffffffffll ? int64_t(uint32_t(u) / uint32_t(segments)) : u / segments;
-    const int c0 = int(u - r * segments) * (kRestoreChunks * group) + lane;
-    const int a = int((r * C) & 7), chunks = (a + C + 7) >> 3;
+  const int lane = threadIdx.x & (p.group - 1);
+  const int64_t hop = (int64_t(gridDim.x) * kThreads) / p.group;
+  for (int64_t u = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / p.group; u < p.units; u += hop) {
+    const int64_t r = row_of(u, p);
+    const int a = int((r * C) & 7), c0 = int(u - r * p.segments) * p.per, end = min(c0 + p.per, (a + C + 7) >> 3);
     const int8_t *row = codes + r * stride;
     const float s = __ldg(scales + r);
+    // Words that hold a code of the row; the last one may end behind the row, which is
+    // beyond the tensor only in its last row.
+    const int words = r + 1 < rows ? C : C & ~3;
+    const auto word = [&](int at) -> uint32_t {
+      if (at >= 0 && at < words) return __ldg(reinterpret_cast<const uint32_t *>(row + at));
+      uint32_t w = 0;
+      if (at >= 0)
+        for (int k = 0; at + k < C; ++k) w |= uint32_t(uint8_t(row[at + k])) << (8 * k);
+      return w;
+    };
     uint2 v[kRestoreChunks];
 #pragma unroll
     for (int i = 0; i < kRestoreChunks; ++i) {
-      const int j = c0 + i * group, e = 8 * j - a;
-      if (j >= chunks) continue;
-      if (e >= 0 && e + 12 <= C) {  // three words hold its eight codes
-        const uint32_t *q = reinterpret_cast<const uint32_t *>(row + (e & ~3));
-        const uint32_t q0 = __ldg(q), q1 = __ldg(q + 1), q2 = __ldg(q + 2);
+      const int c = c0 + lane + i * p.group, e = 8 * c - a;
+      if (c < end) {
+        const uint32_t q0 = word(e & ~3), q1 = word((e & ~3) + 4), q2 = word((e & ~3) + 8);
         v[i] = make_uint2(__funnelshift_r(q0, q1, 8 * (e & 3)), __funnelshift_r(q1, q2, 8 * (e & 3)));
-      } else {  // only the row's own bytes
-        v[i] = make_uint2(0u, 0u);
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (e + k >= 0 && e + k < C) (k < 4 ? v[i].x : v[i].y) |= uint32_t(uint8_t(row[e + k])) << (8 * (k & 3));
       }
     }
 #pragma unroll
     for (int i = 0; i < kRestoreChunks; ++i) {
-      const int j = c0 + i * group, e = 8 * j - a;
-      if (j < chunks) {
+      const int c = c0 + lane + i * p.group, e = 8 * c - a;
+      if (c < end) {
         float f[8];
         restore<kInt8>(v[i], s, f);
         E *to = x + r * C + e;
@@ -225,14 +237,15 @@ void launch_row_dequantize(const void *codes, int64_t stride, const float *scale
                            int64_t rows, int C, bool vec, cudaStream_t s) {
   FMHC_DISPATCH_ELEM(dtype, {
     if (vec) {
-      const int chunks = C % 8 ? (C + 14) / 8 : C / 8;
-      int group = 1;
-      while (group < 32 && group < chunks) group *= 2;
-      const int segments = (chunks + kRestoreChunks * group - 1) / (kRestoreChunks * group);
-      const int64_t units = rows * segments;
+      const int chunks = C % 8 ? (C + 14) / 8 : C / 8;  // of a row, wherever it starts
+      Restore p{1, 0, 0, 0};
+      while (p.group < 32 && p.group < chunks) p.group *= 2;
+      p.segments = (chunks + kRestoreChunks * p.group - 1) / (kRestoreChunks * p.group);
+      p.per = (chunks + p.segments - 1) / p.segments;
+      p.units = rows * p.segments;
       auto k = C % 8 ? row_dequantize_general_kernel<E> : row_dequantize_kernel<E>;
-      launch(k, dim3(grid_for(k, (units * group + 31) / 32, kThreads)), dim3(kThreads), 0, s, (const int8_t *)codes,
-             stride, scales, (E *)x, rows, C, group, units, segments);
+      launch(k, dim3(grid_for(k, (p.units * p.group + 31) / 32, kThreads)), dim3(kThreads), 0, s, (const int8_t *)codes,
+             stride, scales, (E *)x, rows, C, p);
       return;
     }
     auto k = row_dequantize_any_kernel<E>;
