@@ -127,6 +127,15 @@ def test_linear_at_larger_sizes(T, N, K):
     assert _native.check_device_error() == 0
 
 
+# pairs of CTAs: rows that fill a tile badly, one column, odd columns, one byte of K, several tiles per pair
+@pytest.mark.parametrize("T,N,K", [(129, 16001, 200), (300, 14501, 1), (2000, 3999, 1023), (4097, 1025, 17), (70000, 1, 64),
+                                   (20001, 127, 129), (9000, 2305, 2000), (257, 20000, 128), (513, 8191, 640), (33000, 300, 40)])
+def test_linear_in_pairs(T, N, K):
+    for out, bias in ((F32, BF), (HF, None), (BF, F32)):
+        _check_linear(*_operands(T, N, K, bias), out)
+    assert _native.check_device_error() == 0
+
+
 def test_linear_at_the_ends_of_the_range():
     """Every product at its largest: the sum reaches 2.1e9; and codes of -128, which quantising never gives."""
     for T in (1, 5, 40, 300):
