@@ -334,8 +334,9 @@ class Int8Linear(nn.Module):
         super()._apply(fn, recurse)
         if self.weight_scales.dtype != torch.float32:
             self.weight_scales = scales.to(self.weight_scales.device)
-        if not self.weight_codes.is_meta:
-            self.weight_codes = _laid_out(self.weight_codes)
+        codes = self.weight_codes
+        if codes.stride(0) % ALIGN:
+            self.weight_codes = _new_codes(codes).copy_(codes)
         self.dtype = dtype
         return self
 
@@ -388,7 +389,9 @@ def convert_linears(module: nn.Module) -> nn.Module:
     an ``RMSNorm`` in front of a linear layer becomes part of it.  An
     ``MHCLiteBlock`` keeps its own projection and has its wrapped layer converted.
     Subclasses of ``nn.Linear``, layers with hooks, layers of other types than float32,
-    bfloat16 and float16 and layers of 2^17 inputs or more stay as they are.
+    bfloat16 and float16 and layers of 2^17 inputs or more stay as they are.  An
+    :class:`Int8Linear` has no ``weight``: a module that reads its linear layers'
+    weights itself (torch's transformer layers do) cannot be converted.
     """
     return _convert(module, {})
 
@@ -403,10 +406,11 @@ def _convertible(m: nn.Module | None) -> bool:
             and not _has_hooks(m))
 
 
-def _convert(module: nn.Module, done: dict[int, nn.Module]) -> nn.Module:
+def _convert(module: nn.Module, done: dict[int, tuple[nn.Module, nn.Module]]) -> nn.Module:
     if id(module) in done:  # a module that stands in several places stays one
-        return done[id(module)]
-    done[id(module)] = result = module
+        return done[id(module)][1]
+    result = module
+    done[id(module)] = module, result  # the module too, so that its id is not another's
     if _convertible(module):
         result = Int8Linear.from_linear(module)
     elif type(module) is nn.Sequential:
@@ -429,5 +433,5 @@ def _convert(module: nn.Module, done: dict[int, nn.Module]) -> nn.Module:
         for name, child in module._modules.items():
             if child is not None and not (isinstance(module, MHCLiteBlock) and name == "W_all"):
                 module._modules[name] = _convert(child, done)
-    done[id(module)] = result
+    done[id(module)] = module, result
     return result
