@@ -386,7 +386,7 @@ def convert_linears(module: nn.Module) -> nn.Module:
 
     Submodules are replaced in place; the result is ``module`` unless that is itself
     a linear layer or a ``nn.Sequential`` that gets shorter.  In a ``nn.Sequential``
-    an ``RMSNorm`` in front of a linear layer becomes part of it.  An
+    without hooks an ``RMSNorm`` in front of a linear layer becomes part of it.  An
     ``MHCLiteBlock`` keeps its own projection and has its wrapped layer converted.
     Subclasses of ``nn.Linear``, layers with hooks, layers of other types than float32,
     bfloat16 and float16 and layers of 2^17 inputs or more stay as they are.  An
@@ -418,7 +418,7 @@ def _convert(module: nn.Module, done: dict[int, tuple[nn.Module, nn.Module]]) ->
         while i < len(old):
             m, after = old[i], old[i + 1] if i + 1 < len(old) else None
             if (type(m) is RMSNorm and not _has_hooks(m) and _convertible(after)
-                    and m.hidden_size == after.in_features):
+                    and m.hidden_size == after.in_features and not _has_hooks(module)):
                 new.append(Int8Linear.from_linear(after, m))
                 i += 2
             else:
