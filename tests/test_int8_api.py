@@ -289,10 +289,10 @@ def test_convert_linears():
 
 def test_convert_linears_keeps_a_sequentials_hooks():
     seen = []
-    m = nn.Sequential(RMSNorm(8), nn.Linear(8, 8))
+    m = nn.Sequential(norm.RMSNorm(8), nn.Linear(8, 8))
     m.register_forward_hook(lambda *a: seen.append(1))
     c = int8.convert_linears(m)
-    assert c is m and type(c[0]) is RMSNorm and type(c[1]) is int8.Int8Linear and c[1].norm is None
+    assert c is m and type(c[0]) is norm.RMSNorm and type(c[1]) is int8.Int8Linear and c[1].norm is None
     with torch.no_grad():
         c(torch.randn(2, 8))
     assert seen == [1]
