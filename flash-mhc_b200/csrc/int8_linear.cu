@@ -286,6 +286,7 @@ int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid
       ok = __all_sync(0xffffffffu, ok);  // the loads below take whole warps
       if (!ok) {
         store_nan(mine, to, A.N, in);
+        acc ^= 1;  // the scales of the rows still go where the other warps read them
         continue;
       }
       tc_fence_after();
