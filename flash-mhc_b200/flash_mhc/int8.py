@@ -265,8 +265,11 @@ def _quantize_plain(x: torch.Tensor):
     a = v.abs().amax(-1)
     bad = ~torch.isfinite(a)
     a = a.clamp(min=LEAST)
-    q = torch.where(bad.unsqueeze(-1), 0.0, v * (127.0 / a).unsqueeze(-1)).round()
-    return _new_codes(v).copy_(q), torch.where(bad, torch.nan, a / 127.0)
+    # Divided by tensors: torch takes 127 / a from a number by way of 1 / a, which is
+    # rounded twice and sends values between two codes another way than the kernels.
+    most = torch.full_like(a, 127.0)
+    q = torch.where(bad.unsqueeze(-1), 0.0, v * (most / a).unsqueeze(-1)).round()
+    return _new_codes(v).copy_(q), torch.where(bad, torch.nan, a / most)
 
 
 def _quantize(x: torch.Tensor):
