@@ -2,11 +2,16 @@
 
 from __future__ import annotations
 
+import copy
+from collections import OrderedDict
+
 import numpy as np
 import pytest
 import torch
+import torch.nn as nn
+from torch._subclasses.fake_tensor import FakeTensorMode
 
-from flash_mhc import int8
+from flash_mhc import int8, norm
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
