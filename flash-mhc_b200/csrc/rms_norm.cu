@@ -151,7 +151,7 @@ rms_fwd_kernel(const E *__restrict__ x, const E *__restrict__ res, const void *_
           kept_param<i>(w_lo, w_hi, fw);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            f[i][k] *= rstd * fw[k];
+            f[i][k] = f[i][k] * rstd * fw[k];  // as y: rstd w alone may leave f32's range
             m = max(m, rows8::magnitude(f[i][k]));
           }
         }

@@ -40,3 +40,19 @@ def test_codes_are_the_formats_to_the_bit(C, dtype):
     for t in (x, x.cpu()):
         c, s = int8._quantize_plain(t)
         assert torch.equal(c.to(codes.device), codes) and torch.equal(s.to(scales.device), scales)
+
+
+# rows of a warp, of a team of warps, of several rows per warp, of an odd width; past the widths of the other kernels
+@pytest.mark.parametrize("C", [256, 2048, 4096, 64, 1023, 9000])
+@pytest.mark.parametrize("size,weight", [(1e17, 3e-27), (1e-10, 1e36)])
+def test_a_norm_to_8_bits_whose_weight_is_far_from_one(C, size, weight):
+    """rstd w is 3e-44 or 1e39, out of f32's range, where the normalised values and their products with w are not."""
+    x = (torch.randn(40, C, generator=_gen(C), device="cuda") * size).clamp(-4 * size, 4 * size)
+    w = torch.linspace(1, 2, C, device="cuda") * weight
+    y = x.double() / (x.double().square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+    a = y.abs().amax(-1)
+    for codes, scales, *_ in (int8.rms_norm_int8(x, w), int8.add_rms_norm_int8(x, torch.zeros_like(x), w)):
+        # the sum of squares (C u, its mean's 3 u), the square root's 2 u, two products and the division: C + 8 roundings
+        rel = (C + 8) * U
+        assert ((scales.double() - a / 127).abs() <= rel * a / 127).all()
+        assert ((codes.double() - y * (127 / a)[:, None]).abs() <= 0.5 + 2 * 127 * rel).all()
