@@ -1,9 +1,12 @@
 // Linear layer from 8-bit rows (rows8.cuh) on the 5th-generation tensor cores:
 //
-//   y[t, n] = (xs[t] ws[n]) sum_k xc[t, k] wc[n, k] + b[n],  rounded once
+//   y[t, n] = xs[t] (ws[n] sum_k xc[t, k] wc[n, k]) + b[n]
 //
-// The sum of products is a whole number and exact (K < 2^17 keeps it within 32
-// bits, whatever the order); the product of the two scales is taken first, in f32.
+// The sum of products is a whole number and exact (K < 2^17 keeps it within 32 bits,
+// whatever the order).  Rounded to f32: the sum (beyond 2^24), its product with ws, and
+// that times xs plus b, once; then y to its type.  The product of the two scales is not
+// taken: it leaves f32's range where y does not (two scales of 1e-21, or a sum of 0 and
+// scales of 1e20).  A sum times a weight's scale does only from weights of 2^104 on.
 //
 // The weight is the MMA's A operand (M = output columns n) and the activations
 // are B (N = rows t), so that a thread of the epilogue holds one output column of
@@ -61,6 +64,11 @@ __device__ __forceinline__ float bias1(const void *b, int dtype, int64_t n) {
   return __half2float(reinterpret_cast<const __half *>(b)[n]);
 }
 
+// One output, as every kernel here rounds it.
+__device__ __forceinline__ float scaled(int sum, float ws, float xs, float b) {
+  return fmaf(__fmul_rn(__int2float_rn(sum), ws), xs, b);
+}
+
 // 32 rows of a column: `rows` of them are stored, from y (row 0, this column) on.
 // No branch stands between the rows of a whole chunk: one per row made each wait for
 // the latency of its own arithmetic (tiles of 256 x 256 took 20 us each).  Two columns
@@ -75,9 +83,10 @@ __device__ __forceinline__ void store_rows(const int (&v)[32], int rows, const f
 #pragma unroll
   for (int j = 0; j < 32; j += 4) {
     const float4 x = *reinterpret_cast<const float4 *>(xs + j);
-    const float2 p0 = mul2(make_float2(x.x, x.y), both(ws)), p1 = mul2(make_float2(x.z, x.w), both(ws));
-    const float2 f0 = fma2(make_float2(__int2float_rn(v[j]), __int2float_rn(v[j + 1])), p0, both(b));
-    const float2 f1 = fma2(make_float2(__int2float_rn(v[j + 2]), __int2float_rn(v[j + 3])), p1, both(b));
+    const float2 p0 = mul2(make_float2(__int2float_rn(v[j]), __int2float_rn(v[j + 1])), both(ws));
+    const float2 p1 = mul2(make_float2(__int2float_rn(v[j + 2]), __int2float_rn(v[j + 3])), both(ws));
+    const float2 f0 = fma2(p0, make_float2(x.x, x.y), both(b));
+    const float2 f1 = fma2(p1, make_float2(x.z, x.w), both(b));
     o[j] = Elem<E>::narrow1(f0.x);
     o[j + 1] = Elem<E>::narrow1(f0.y);
     o[j + 2] = Elem<E>::narrow1(f1.x);
@@ -461,7 +470,7 @@ int8_linear_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
         int v = 0;
 #pragma unroll
         for (int s = 0; s < S; ++s) v += from[(s * each + i) * kBM];
-        const float f = ok ? fmaf(__int2float_rn(v), sm.xs[int(rank) + i * S] * ws, b) : __uint_as_float(0x7fc00000u);
+        const float f = ok ? scaled(v, ws, sm.xs[int(rank) + i * S], b) : __uint_as_float(0x7fc00000u);
         if (in) to[int64_t(i) * S * A.N] = Elem<E>::narrow1(f);
       }
     }
@@ -561,7 +570,7 @@ int8_linear_rows_kernel(const int8_t *__restrict__ xc, int64_t xstride, const in
     if (t < T && n < A.N) {
       int v = 0;
       for (int k = 0; k < split; ++k) v += sums[g * split + k][c][t];
-      y[t * A.N + n] = Elem<E>::narrow1(fmaf(__int2float_rn(v), A.xs[t] * A.ws[n], bias1(A.bias, A.bias_dtype, n)));
+      y[t * A.N + n] = Elem<E>::narrow1(scaled(v, A.ws[n], A.xs[t], bias1(A.bias, A.bias_dtype, n)));
     }
   }
 }

@@ -246,11 +246,12 @@ def add_rms_norm_int8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Ten
 
 def linear(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.Tensor, weight_scales: torch.Tensor,
            bias: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """scales weight_scales (codes @ weight_codes.T) + bias in ``dtype``: a linear layer of rows in 8 bits.
+    """scales (weight_scales (codes @ weight_codes.T)) + bias in ``dtype``: a linear layer of rows in 8 bits.
 
     ``codes`` is (..., K) and ``weight_codes`` (N, K), K below 2^17; ``bias`` is
-    float32, bfloat16 or float16.  The two scales are multiplied in 32 bits and the
-    result is rounded once.  Codes whose rows do not start at multiples of 16 bytes
+    float32, bfloat16 or float16.  The exact sum of products is rounded to 32 bits,
+    multiplied with the weight's scale and then the row's in 32 bits, and rounded to
+    ``dtype``.  Codes whose rows do not start at multiples of 16 bytes
     are copied first (those that this module makes do).
     """
     return torch.ops.flash_mhc.int8_linear(codes, scales, weight_codes, weight_scales, bias, dtype)
@@ -379,7 +380,7 @@ class Int8Linear(nn.Module):
             y = linear(codes, scales, self.weight_codes, self.weight_scales, self.bias, dtype)
         else:
             products = codes.double() @ self.weight_codes.double().t()  # whole numbers below 2^53
-            y = products.float() * (scales.unsqueeze(-1) * self.weight_scales)
+            y = products.float() * self.weight_scales * scales.unsqueeze(-1)  # as the kernels order them
             y = (y if self.bias is None else y + self.bias.float()).to(dtype)
         return y if total is None else (y, total)
 

@@ -452,9 +452,10 @@ FMHC_API int fmhc_rms_norm_fwd_int8(const void *x, int x_dtype, const void *resi
                                     const void *weight, int param_dtype, float eps, void *codes,
                                     int64_t codes_stride, float *scales, void *total,
                                     int64_t rows, int64_t C, void *stream);
-/* Linear layer: y[t,n] = (scales[t] weight_scales[n]) sum_k codes[t,k] weight_codes[n,k]
- * + bias[n], rounded once to y_dtype.  The sum is exact (K < 2^17); the two scales
- * are multiplied first, in f32.  codes (T, K) and weight_codes (N, K) are 16-byte
+/* Linear layer: y[t,n] = scales[t] (weight_scales[n] sum_k codes[t,k] weight_codes[n,k])
+ * + bias[n].  The sum is exact (K < 2^17); rounded to f32 are the sum (beyond 2^24), its
+ * product with the weight's scale, and that times the row's scale plus the bias, once;
+ * y_dtype's rounding comes last.  codes (T, K) and weight_codes (N, K) are 16-byte
  * aligned with strides that are multiples of 16; bias (N,) of bias_dtype, or NULL;
  * y (T, N) is dense; T and N are below 2^31 - 512. */
 FMHC_API int fmhc_int8_linear(const void *codes, int64_t codes_stride, const float *scales,

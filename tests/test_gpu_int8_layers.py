@@ -56,3 +56,33 @@ def test_a_norm_to_8_bits_whose_weight_is_far_from_one(C, size, weight):
         rel = (C + 8) * U
         assert ((scales.double() - a / 127).abs() <= rel * a / 127).all()
         assert ((codes.double() - y * (127 / a)[:, None]).abs() <= 0.5 + 2 * 127 * rel).all()
+
+
+# the kernel for a handful of rows, one CTA per tile, clusters that split K, pairs of CTAs
+@pytest.mark.parametrize("T,N,K", [(1, 300, 512), (5, 300, 512), (40, 300, 512), (16, 1024, 4096), (1024, 4096, 512)])
+@pytest.mark.parametrize("xs,ws", [(3e-22, 2e-21), (2e-21, 3e-22), (1e34, 1e-30), (2e36, 1e-20), (1e-25, 1e25), (1e-31, 1e29)])
+def test_scales_at_the_ends_of_the_range(T, N, K, xs, ws):
+    """The scales' product leaves f32's range or not: y does not, and neither does the sum times the weight's scale."""
+    g = _gen(T + N)
+    xc, wc = (torch.randint(-127, 128, (n, K), generator=g, device="cuda", dtype=torch.int8) for n in (T, N))
+    sx, sw = (torch.linspace(1, 1.5, n, device="cuda") * s for n, s in ((T, xs), (N, ws)))
+    sums = (xc.double() @ wc.double().t())
+    b = torch.randn(N, generator=g, device="cuda") * float(np.float32(xs * ws * 1e4))
+    for bias in (None, b):
+        y = int8.linear(xc, sx, wc, sw, bias, F32).double()
+        want = sums * sw.double() * sx.double()[:, None]
+        lim = 3 * U * want.abs()
+        if bias is not None:
+            want = want + bias.double()
+            lim = lim + U * want.abs()
+        assert ((y - want).abs() <= lim + 2.0 ** -149).all()  # the least step of f32
+
+
+@pytest.mark.parametrize("T,N,K", [(1, 300, 512), (40, 300, 512), (16, 1024, 4096), (1024, 4096, 512)])
+def test_a_sum_of_zero_is_zero_under_any_scales(T, N, K):
+    """Orthogonal rows of codes, with scales whose product is infinite in f32: y is the bias."""
+    xc, wc = torch.zeros(T, K, dtype=torch.int8, device="cuda"), torch.zeros(N, K, dtype=torch.int8, device="cuda")
+    xc[:, : K // 2], wc[:, K // 2:] = 3, 5
+    b = torch.randn(N, generator=_gen(N), device="cuda")
+    y = int8.linear(xc, torch.full((T,), 1e30, device="cuda"), wc, torch.full((N,), 1e30, device="cuda"), b, F32)
+    assert torch.equal(y, b.expand(T, N))
