@@ -2,6 +2,7 @@
 // 4096 bf16 63 us and 70 us (the bytes at the copy rate take 62).  Restoring writes twice
 // what it reads; rows that start anywhere in a word restore 65536 x 1023 in 70 us (31),
 // bound by instructions.
+#include "code_word.h"
 #include "fmhc_launch.h"
 #include "norm_rows.cuh"
 #include "rows8.cuh"
@@ -137,23 +138,16 @@ row_dequantize_general_kernel(const int8_t *__restrict__ codes, int64_t stride, 
     const int a = int((r * C) & 7), c0 = int(u - r * p.segments) * p.per, end = min(c0 + p.per, (a + C + 7) >> 3);
     const int8_t *row = codes + r * stride;
     const float s = __ldg(scales + r);
-    // Words that hold a code of the row; the last one may end behind the row, which is
-    // beyond the tensor only in its last row.
-    const int words = r + 1 < rows ? C : C & ~3;
-    const auto word = [&](int at) -> uint32_t {
-      if (at >= 0 && at < words) return __ldg(reinterpret_cast<const uint32_t *>(row + at));
-      uint32_t w = 0;
-      if (at >= 0)
-        for (int k = 0; at + k < C; ++k) w |= uint32_t(uint8_t(row[at + k])) << (8 * k);
-      return w;
-    };
+    const auto whole = [&](int at) { return __ldg(reinterpret_cast<const uint32_t *>(row + at)); };
+    const auto single = [&](int at) { return __ldg(row + at); };
     uint2 v[kRestoreChunks];
 #pragma unroll
     for (int i = 0; i < kRestoreChunks; ++i) {
       const int c = c0 + lane + i * p.group, e = 8 * c - a;
       if (c < end) {
-        const uint32_t q0 = word(e & ~3), q1 = word((e & ~3) + 4), q2 = word((e & ~3) + 8);
-        v[i] = make_uint2(__funnelshift_r(q0, q1, 8 * (e & 3)), __funnelshift_r(q1, q2, 8 * (e & 3)));
+        uint32_t q[3];
+        code_words(e & ~3, C, whole, single, q);
+        v[i] = make_uint2(__funnelshift_r(q[0], q[1], 8 * (e & 3)), __funnelshift_r(q[1], q[2], 8 * (e & 3)));
       }
     }
 #pragma unroll
