@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch._subclasses.fake_tensor import FakeTensor
 
 from .act8 import _DTYPES, _act, _launch, _new_per_row, _register_no_derivative, _same_device, _shape
 from .block import MHCLiteBlock
@@ -299,7 +300,9 @@ class Int8Linear(nn.Module):
     ``dtype``).  With a ``norm`` (an :class:`flash_mhc.norm.RMSNorm`) the layer is
     linear(norm(x)), the norm writing 8 bits at once, and ``forward(x, residual)``
     gives (linear(norm(total)), total) with total = x + residual.  On the CPU the
-    same is computed with torch.
+    same is computed with torch.  Rows of codes are laid out again when they are loaded,
+    so that a state dict may hold them packed (a format that wants contiguous tensors
+    takes ``weight_codes.contiguous()``).
     """
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, norm: RMSNorm | None = None,
@@ -338,11 +341,24 @@ class Int8Linear(nn.Module):
         super()._apply(fn, recurse)
         if self.weight_scales.dtype != torch.float32:
             self.weight_scales = scales.to(self.weight_scales.device)
-        codes = self.weight_codes
-        if codes.stride(0) % ALIGN:
-            self.weight_codes = _new_codes(codes).copy_(codes)
+        self._lay_out()
         self.dtype = dtype
         return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        # assign=True puts the tensors of a state dict in place, whose rows may be packed.
+        super()._load_from_state_dict(*args, **kwargs)
+        self._lay_out()
+
+    def _lay_out(self) -> None:
+        codes = self.weight_codes
+        if codes.dtype != torch.int8:
+            return  # nothing that the layer takes: its forward says so
+        if isinstance(codes, FakeTensor):  # has no address
+            if codes.stride(0) % ALIGN:
+                self.weight_codes = _new_codes(codes).copy_(codes)
+            return
+        self.weight_codes = _laid_out(codes)
 
     def _rows_of(self, x, residual):
         """(codes, scales, total or None, type of the result) of the layer's input."""

@@ -27,3 +27,33 @@ def test_codes_without_a_gpu_are_the_formats(dtype):
     assert a.dtype == np.float32
     assert np.array_equal(scales.numpy(), a / np.float32(127))
     assert np.array_equal(codes.numpy(), np.rint(v * (np.float32(127) / a)[:, None]).astype(np.int8))
+
+
+def test_codes_that_are_loaded_are_laid_out():
+    """assign=True puts the state dict's own tensors in place, whose rows may be packed: a forward would copy them every time."""
+    q = int8.Int8Linear.from_linear(nn.Linear(40, 9))
+    x = torch.randn(4, 40)
+    with torch.no_grad():
+        want = q(x)
+    packed = {k: v.contiguous() for k, v in q.state_dict().items()}
+    assert packed["weight_codes"].stride() == (40, 1)
+    far = torch.zeros(9 * 40 + 1, dtype=torch.int8)[1:].view(9, 40).copy_(packed["weight_codes"])
+    for assign in (True, False):
+        for codes in (packed["weight_codes"], packed["weight_codes"].t().contiguous().t(), far, q.weight_codes):
+            m = int8.Int8Linear(40, 9, device="meta" if assign else None, dtype=torch.float32)
+            m.load_state_dict({**packed, "weight_codes": codes}, assign=assign)
+            assert m.weight_codes.stride() == (48, 1) and int8._laid_out(m.weight_codes) is m.weight_codes
+            with torch.no_grad():
+                assert torch.equal(m(x), want)
+    m.load_state_dict(q.state_dict(), assign=True)
+    assert m.weight_codes.data_ptr() == q.weight_codes.data_ptr()  # laid out: as it is
+    whole = nn.Sequential(int8.Int8Linear(40, 9, device="meta"))
+    whole.load_state_dict({"0." + k: v for k, v in packed.items()}, assign=True)
+    assert whole[0].weight_codes.stride() == (48, 1)
+    assert q.state_dict()["weight_codes"].data_ptr() == q.weight_codes.data_ptr()  # references, as torch's are
+    with pytest.raises(RuntimeError, match="size mismatch"):
+        q.load_state_dict({**packed, "weight_codes": packed["weight_codes"][:, :39]}, assign=True)
+    with FakeTensorMode():
+        f = int8.Int8Linear(40, 9)
+        f.load_state_dict(int8.Int8Linear(40, 9).state_dict(), assign=True)
+        assert f.weight_codes.stride() == (48, 1)
