@@ -23,6 +23,8 @@ through the others raises.
 
 from __future__ import annotations
 
+import copy
+
 import torch
 import torch.nn as nn
 from torch._subclasses.fake_tensor import FakeTensor
@@ -329,7 +331,8 @@ class Int8Linear(nn.Module):
         new.weight_codes, new.weight_scales = _quantize(w)
         if layer.bias is not None:
             new.bias = layer.bias.detach().clone()
-        return new.train(layer.training)
+        new.training = layer.training  # the norm keeps its own mode
+        return new
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
@@ -406,14 +409,16 @@ def convert_linears(module: nn.Module) -> nn.Module:
 
     Submodules are replaced in place; the result is ``module`` unless that is itself
     a linear layer or a ``nn.Sequential`` that gets shorter.  In a ``nn.Sequential``
-    without hooks an ``RMSNorm`` in front of a linear layer becomes part of it.  An
+    without hooks an ``RMSNorm`` in front of a linear layer becomes part of it.  The
+    shorter container has the attributes, modes and names of the longer one (but is
+    numbered anew if that was numbered); a layer with its norm has the layer's name.  An
     ``MHCLiteBlock`` keeps its own projection and has its wrapped layer converted.
     Subclasses of ``nn.Linear``, layers with hooks, layers of other types than float32,
     bfloat16 and float16 and layers of 2^17 inputs or more stay as they are.  An
     :class:`Int8Linear` has no ``weight``: a module that reads its linear layers'
     weights itself (torch's transformer layers do) cannot be converted.
     """
-    return _convert(module, {})
+    return _Conversion(module).of(module)
 
 
 def _has_hooks(m: nn.Module) -> bool:
@@ -421,37 +426,58 @@ def _has_hooks(m: nn.Module) -> bool:
                                              "_backward_pre_hooks"))
 
 
-def _convertible(m: nn.Module | None) -> bool:
-    return (type(m) is nn.Linear and m.weight.dtype in _DTYPES and 0 < m.in_features < 1 << 17
-            and not _has_hooks(m))
+def _shortens(m: nn.Module) -> bool:
+    return type(m) is nn.Sequential and not _has_hooks(m)
 
 
-def _convert(module: nn.Module, done: dict[int, tuple[nn.Module, nn.Module]]) -> nn.Module:
-    if id(module) in done:  # a module that stands in several places stays one
-        return done[id(module)][1]
-    result = module
-    done[id(module)] = module, result  # the module too, so that its id is not another's
-    if _convertible(module):
-        result = Int8Linear.from_linear(module)
-    elif type(module) is nn.Sequential:
-        old, new, i = list(module), [], 0
-        while i < len(old):
-            m, after = old[i], old[i + 1] if i + 1 < len(old) else None
-            if (type(m) is RMSNorm and not _has_hooks(m) and _convertible(after)
-                    and m.hidden_size == after.in_features and not _has_hooks(module)):
-                new.append(Int8Linear.from_linear(after, m))
-                i += 2
+class _Conversion:
+    """What is known of a module's parts before and while they are replaced, by their ids.
+
+    ``alive`` keeps the originals, so that no id becomes another's."""
+
+    def __init__(self, root: nn.Module) -> None:
+        self.alive = list(root.modules())
+        self.done: dict[int, nn.Module] = {}
+        self.kept: set[int] = set()  # layers whose weights their parents read
+        for m in self.alive:
+            if isinstance(m, MHCLiteBlock):
+                self.kept.add(id(m.W_all))
+
+    def convertible(self, m: nn.Module) -> bool:
+        return (type(m) is nn.Linear and m.weight.dtype in _DTYPES and 0 < m.in_features < 1 << 17
+                and not _has_hooks(m) and id(m) not in self.kept)
+
+    def takes(self, layer: nn.Module, norm: nn.Module) -> bool:
+        """Whether ``norm``, of a Sequential that may get shorter, becomes part of ``layer`` behind it."""
+        return self.convertible(layer) and norm.hidden_size == layer.in_features
+
+    def of(self, module: nn.Module) -> nn.Module:
+        """What stands in ``module``'s place."""
+        if id(module) not in self.done:
+            self.done[id(module)] = module  # a module that stands in itself
+            self.done[id(module)] = self._of(module)
+        return self.done[id(module)]
+
+    def _of(self, module: nn.Module) -> nn.Module:
+        if self.convertible(module):
+            return Int8Linear.from_linear(module)
+        children = [(name, m) for name, m in module._modules.items() if m is not None]
+        new: dict[str, nn.Module] = {}
+        norm = None
+        for i, (name, m) in enumerate(children):
+            after = children[i + 1][1] if i + 1 < len(children) else None
+            if _shortens(module) and type(m) is RMSNorm and after is not None and self.takes(after, m):
+                norm = m
             else:
-                new.append(_convert(m, done))
-                i += 1
-        if len(new) != len(old):
-            result = nn.Sequential(*new).train(module.training)
-        else:
-            for name, m in zip(module._modules, new):
-                module._modules[name] = m
-    else:
-        for name, child in module._modules.items():
-            if child is not None and not (isinstance(module, MHCLiteBlock) and name == "W_all"):
-                module._modules[name] = _convert(child, done)
-    done[id(module)] = module, result
-    return result
+                new[name] = self.of(m) if norm is None else Int8Linear.from_linear(m, norm)
+                norm = None
+        if len(new) == len(children):
+            module._modules.update(new)
+            return module
+        if [name for name, _ in children] == [str(i) for i in range(len(children))]:
+            new = {str(i): m for i, m in enumerate(new.values())}
+        shorter = nn.Sequential()
+        for name, value in vars(module).items():
+            shorter.__dict__[name] = copy.copy(value) if isinstance(value, (dict, set)) else value
+        shorter._modules = new
+        return shorter

@@ -57,3 +57,30 @@ def test_codes_that_are_loaded_are_laid_out():
         f = int8.Int8Linear(40, 9)
         f.load_state_dict(int8.Int8Linear(40, 9).state_dict(), assign=True)
         assert f.weight_codes.stride() == (48, 1)
+
+
+def _named():
+    m = nn.Sequential(OrderedDict(n=norm.RMSNorm(8), up=nn.Linear(8, 12), drop=nn.Dropout(0.9), down=nn.Linear(12, 8)))
+    m.note = ["kept"]
+    return m
+
+
+def test_a_container_that_gets_shorter_keeps_names_modes_and_attributes():
+    m = _named()
+    m.drop.eval()
+    m.n.eval()
+    whole = nn.Module()
+    whole.ffn = m
+    assert int8.convert_linears(whole) is whole
+    c = whole.ffn
+    assert type(c) is nn.Sequential and list(c._modules) == ["up", "drop", "down"] and c.note == ["kept"]
+    assert c.training and not c.drop.training and c.up.training and c.down.training
+    assert c.up.norm is m.n and not c.up.norm.training and type(c.down) is int8.Int8Linear
+    assert set(c.state_dict()) == {"up.weight_codes", "up.weight_scales", "up.bias", "up.norm.weight",
+                                   "down.weight_codes", "down.weight_scales", "down.bias"}
+    c.register_forward_hook(lambda *a: None)
+    assert list(m._modules) == ["n", "up", "drop", "down"] and not m._forward_hooks  # the longer one is as it was
+    numbered = int8.convert_linears(nn.Sequential(norm.RMSNorm(8), nn.Linear(8, 8), norm.RMSNorm(8), nn.Linear(8, 8)).eval())
+    assert list(numbered._modules) == ["0", "1"] and not any(t.training for t in numbered.modules())
+    numbered.append(nn.GELU())
+    assert list(numbered._modules) == ["0", "1", "2"]
