@@ -414,9 +414,10 @@ def convert_linears(module: nn.Module) -> nn.Module:
     numbered anew if that was numbered); a layer with its norm has the layer's name.  An
     ``MHCLiteBlock`` keeps its own projection and has its wrapped layer converted.
     Subclasses of ``nn.Linear``, layers with hooks, layers of other types than float32,
-    bfloat16 and float16 and layers of 2^17 inputs or more stay as they are.  An
-    :class:`Int8Linear` has no ``weight``: a module that reads its linear layers'
-    weights itself (torch's transformer layers do) cannot be converted.
+    bfloat16 and float16 and layers of 2^17 inputs or more stay as they are, and so do
+    those whose weights ``nn.TransformerEncoderLayer`` reads itself.  An
+    :class:`Int8Linear` has no ``weight``: other modules that read their linear
+    layers' weights themselves cannot be converted.
     """
     return _Conversion(module).of(module)
 
@@ -442,6 +443,8 @@ class _Conversion:
         for m in self.alive:
             if isinstance(m, MHCLiteBlock):
                 self.kept.add(id(m.W_all))
+            elif isinstance(m, nn.TransformerEncoderLayer):
+                self.kept.update((id(m.linear1), id(m.linear2)))
 
     def convertible(self, m: nn.Module) -> bool:
         return (type(m) is nn.Linear and m.weight.dtype in _DTYPES and 0 < m.in_features < 1 << 17

@@ -84,3 +84,23 @@ def test_a_container_that_gets_shorter_keeps_names_modes_and_attributes():
     assert list(numbered._modules) == ["0", "1"] and not any(t.training for t in numbered.modules())
     numbered.append(nn.GELU())
     assert list(numbered._modules) == ["0", "1", "2"]
+
+
+def test_torchs_own_modules_run_converted():
+    """Those that read a linear layer's weight keep it."""
+    torch.manual_seed(0)
+    x = torch.randn(2, 5, 8)
+    enc = lambda: nn.TransformerEncoderLayer(8, 2, 16, batch_first=True)  # noqa: E731
+    for m, args in ((enc(), (x,)), (nn.TransformerEncoder(enc(), 2), (x,)),
+                    (nn.TransformerDecoderLayer(8, 2, 16, batch_first=True), (x, x)),
+                    (nn.Transformer(8, 2, 1, 1, 16, batch_first=True), (x, x)),
+                    (nn.MultiheadAttention(8, 2, batch_first=True), (x, x, x)),
+                    (nn.AdaptiveLogSoftmaxWithLoss(8, 20, [5, 10]), (x.view(10, 8), torch.arange(10)))):
+        for mode in (True, False):
+            with torch.no_grad():
+                int8.convert_linears(copy.deepcopy(m).train(mode))(*args)
+    layer = enc().eval()
+    with torch.no_grad():
+        want = layer(x)
+        assert torch.equal(int8.convert_linears(layer)(x), want)
+    assert type(layer.linear1) is nn.Linear and type(layer.linear2) is nn.Linear
