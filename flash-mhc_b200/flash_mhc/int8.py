@@ -415,8 +415,9 @@ def convert_linears(module: nn.Module) -> nn.Module:
     ``MHCLiteBlock`` keeps its own projection and has its wrapped layer converted.
     Subclasses of ``nn.Linear``, layers with hooks, layers of other types than float32,
     bfloat16 and float16 and layers of 2^17 inputs or more stay as they are, and so do
-    those whose weights ``nn.TransformerEncoderLayer`` reads itself.  An
-    :class:`Int8Linear` has no ``weight``: other modules that read their linear
+    those whose weights ``nn.TransformerEncoderLayer`` reads itself.  A layer that stands
+    in several places stays one; a norm becomes part of it if it precedes it in all of
+    them.  An :class:`Int8Linear` has no ``weight``: other modules that read their linear
     layers' weights themselves cannot be converted.
     """
     return _Conversion(module).of(module)
@@ -440,11 +441,18 @@ class _Conversion:
         self.alive = list(root.modules())
         self.done: dict[int, nn.Module] = {}
         self.kept: set[int] = set()  # layers whose weights their parents read
+        self.before: dict[int, set[int | None]] = {id(root): {None}}  # norms in front of a layer, or none
         for m in self.alive:
             if isinstance(m, MHCLiteBlock):
                 self.kept.add(id(m.W_all))
             elif isinstance(m, nn.TransformerEncoderLayer):
                 self.kept.update((id(m.linear1), id(m.linear2)))
+            last = None
+            for child in m._modules.values():
+                if child is not None:
+                    self.before.setdefault(id(child), set()).add(None if last is None else id(last))
+                    fits = _shortens(m) and type(child) is RMSNorm and not _has_hooks(child)
+                    last = child if fits else None
 
     def convertible(self, m: nn.Module) -> bool:
         return (type(m) is nn.Linear and m.weight.dtype in _DTYPES and 0 < m.in_features < 1 << 17
@@ -452,18 +460,19 @@ class _Conversion:
 
     def takes(self, layer: nn.Module, norm: nn.Module) -> bool:
         """Whether ``norm``, of a Sequential that may get shorter, becomes part of ``layer`` behind it."""
-        return self.convertible(layer) and norm.hidden_size == layer.in_features
+        return (self.before[id(layer)] == {id(norm)} and self.convertible(layer)
+                and norm.hidden_size == layer.in_features)
 
-    def of(self, module: nn.Module) -> nn.Module:
-        """What stands in ``module``'s place."""
+    def of(self, module: nn.Module, norm: RMSNorm | None = None) -> nn.Module:
+        """What stands in ``module``'s place (with ``norm``: in both their places)."""
         if id(module) not in self.done:
             self.done[id(module)] = module  # a module that stands in itself
-            self.done[id(module)] = self._of(module)
+            self.done[id(module)] = self._of(module, norm)
         return self.done[id(module)]
 
-    def _of(self, module: nn.Module) -> nn.Module:
+    def _of(self, module: nn.Module, norm: RMSNorm | None) -> nn.Module:
         if self.convertible(module):
-            return Int8Linear.from_linear(module)
+            return Int8Linear.from_linear(module, norm)
         children = [(name, m) for name, m in module._modules.items() if m is not None]
         new: dict[str, nn.Module] = {}
         norm = None
@@ -472,7 +481,7 @@ class _Conversion:
             if _shortens(module) and type(m) is RMSNorm and after is not None and self.takes(after, m):
                 norm = m
             else:
-                new[name] = self.of(m) if norm is None else Int8Linear.from_linear(m, norm)
+                new[name] = self.of(m, norm)
                 norm = None
         if len(new) == len(children):
             module._modules.update(new)

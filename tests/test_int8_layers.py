@@ -104,3 +104,35 @@ def test_torchs_own_modules_run_converted():
         want = layer(x)
         assert torch.equal(int8.convert_linears(layer)(x), want)
     assert type(layer.linear1) is nn.Linear and type(layer.linear2) is nn.Linear
+
+
+def test_a_layer_in_several_places_stays_one():
+    lin, n1, n2 = nn.Linear(8, 8), norm.RMSNorm(8), norm.RMSNorm(8)
+    with torch.no_grad():
+        n2.weight.fill_(2.0)
+    x = torch.randn(3, 8)
+
+    def converted(*parts):
+        m = nn.Module()
+        m.parts = nn.ModuleList(parts)
+        c = int8.convert_linears(copy.deepcopy(m)).parts
+        with torch.no_grad():
+            for a, b in zip(parts, c):
+                assert (a(x) - b(x)).abs().max() < 0.2 * a(x).abs().max()  # 8 bits: far from another norm's or none
+        return c, [q for q in c.modules() if type(q) is int8.Int8Linear]
+
+    c, q = converted(nn.Sequential(n1, lin), nn.Sequential(n1, lin, nn.GELU()))  # behind one norm everywhere
+    assert len(q) == 1 and q[0].norm is not None and c[0][0] is c[1][0]
+    c, q = converted(nn.Sequential(n1, lin), nn.Sequential(n2, lin))  # behind two
+    assert len(q) == 1 and q[0].norm is None and len(c[0]) == len(c[1]) == 2
+    c, q = converted(nn.Sequential(n1, lin), lin)  # with a norm and without
+    assert len(q) == 1 and q[0].norm is None and c[1] is c[0][1]
+    c, q = converted(lin, nn.Sequential(nn.Identity(), n1, lin))
+    assert len(q) == 1 and q[0].norm is None and c[0] is c[1][2]
+    c, q = converted(nn.Sequential(n1, lin), nn.Sequential(n1, nn.Linear(8, 8)))  # one norm, two layers
+    assert len(q) == 2 and q[0].norm is q[1].norm is not None
+    s = nn.Sequential(n1, lin)
+    c, q = converted(s, s)
+    assert len(q) == 1 and c[0] is c[1] and len(c[0]) == 1
+    alone = int8.convert_linears(lin)
+    assert type(alone) is int8.Int8Linear and alone.norm is None
