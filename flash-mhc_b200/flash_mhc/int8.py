@@ -369,6 +369,8 @@ class Int8Linear(nn.Module):
             if self.norm is not None or residual is not None:
                 raise ValueError("Int8Linear: rows in 8 bits go to a layer without a norm, and without a residual")
             return (*x, None, self.dtype)
+        if not x.is_floating_point():
+            raise ValueError(f"Int8Linear: activations must be floating-point numbers (got {x.dtype})")
         norm = self.norm
         if norm is None:
             if residual is not None:
@@ -396,7 +398,13 @@ class Int8Linear(nn.Module):
                 return _Served.apply(*(out if isinstance(out, tuple) else (out,)), *wanted)
         codes, scales, total, dtype = self._rows_of(x, residual)
         if codes.is_cuda:
-            y = linear(codes, scales, self.weight_codes, self.weight_scales, self.bias, dtype)
+            # A type that the kernel has not is that of a layer that was converted as a
+            # whole, or of its input: from 32 bits, as on the CPU.
+            bias = self.bias
+            if bias is not None and bias.dtype not in _DTYPES:
+                bias = bias.float()
+            y = linear(codes, scales, self.weight_codes, self.weight_scales, bias,
+                       dtype if dtype in _DTYPES else torch.float32).to(dtype)
         else:
             products = codes.double() @ self.weight_codes.double().t()  # whole numbers below 2^53
             y = products.float() * self.weight_scales * scales.unsqueeze(-1)  # as the kernels order them

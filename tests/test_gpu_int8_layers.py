@@ -86,3 +86,21 @@ def test_a_sum_of_zero_is_zero_under_any_scales(T, N, K):
     b = torch.randn(N, generator=_gen(N), device="cuda")
     y = int8.linear(xc, torch.full((T,), 1e30, device="cuda"), wc, torch.full((N,), 1e30, device="cuda"), b, F32)
     assert torch.equal(y, b.expand(T, N))
+
+
+@pytest.mark.parametrize("bias", [True, False])
+def test_float64_as_on_the_cpu(bias):
+    """A layer that was converted as a whole, and float64 activations: from 32 bits, in their type."""
+    torch.manual_seed(0)
+    x = torch.randn(30, 200)
+    q = int8.Int8Linear.from_linear(nn.Linear(200, 90, bias=bias))
+    for m in (q, copy.deepcopy(q).double()):
+        with torch.no_grad():
+            want = m(x.double())
+            c, s = int8._quantize_plain(x)
+            size = (c.double() @ m.weight_codes.double().t()).abs() * s.double()[:, None] * m.weight_scales.double()
+            g = copy.deepcopy(m).cuda()
+            for y in (g(x.double().cuda()), g((c.cuda(), s.cuda()))):
+                # three or four roundings on each side, of the sum's part and of the result
+                assert ((y.double().cpu() - want).abs() <= 8 * U * (size + want.abs())).all()
+            assert g(x.double().cuda()).dtype == want.dtype == torch.float64 and g((c.cuda(), s.cuda())).dtype == m.dtype

@@ -136,3 +136,19 @@ def test_a_layer_in_several_places_stays_one():
     assert len(q) == 1 and c[0] is c[1] and len(c[0]) == 1
     alone = int8.convert_linears(lin)
     assert type(alone) is int8.Int8Linear and alone.norm is None
+
+
+def test_float64_layers_and_activations():
+    torch.manual_seed(0)
+    q = int8.Int8Linear.from_linear(nn.Linear(40, 9), norm.RMSNorm(40))
+    x = torch.randn(4, 40)
+    with torch.no_grad():
+        want = q(x)
+        assert q(x.double()).dtype == torch.float64 and torch.equal(q(x.double()).float(), want)
+        y = q.double()(x.double())
+        assert q.weight_scales.dtype == torch.float32 and y.dtype == torch.float64
+        assert torch.equal(y.float(), want)
+        with pytest.raises(ValueError, match="floating-point"):
+            q(torch.ones(4, 40, dtype=torch.int64))
+        with pytest.raises(ValueError, match="floating-point"):
+            int8.Int8Linear(40, 9)(torch.ones(4, 40, dtype=torch.int8))
