@@ -104,3 +104,19 @@ def test_float64_as_on_the_cpu(bias):
                 # three or four roundings on each side, of the sum's part and of the result
                 assert ((y.double().cpu() - want).abs() <= 8 * U * (size + want.abs())).all()
             assert g(x.double().cuda()).dtype == want.dtype == torch.float64 and g((c.cuda(), s.cuda())).dtype == m.dtype
+
+
+def test_a_lost_copy_costs_a_pair_its_tile_alone():
+    """Pairs of CTAs, one tile each: the first tile (256 rows and columns) is NaN, everything else as without the loss."""
+    T, N, K = 1024, 4096, 2048
+    g = _gen(T)
+    xc, wc = (torch.randint(-127, 128, (n, K), generator=g, device="cuda", dtype=torch.int8) for n in (T, N))
+    xs, ws = torch.rand(T, generator=g, device="cuda"), torch.rand(N, generator=g, device="cuda")
+    want = int8.linear(xc, xs, wc, ws)
+    y = torch.zeros_like(want)
+    _native.call("fmhc_debug_int8_linear_lost_copy", xc.data_ptr(), K, xs.data_ptr(), wc.data_ptr(), K, ws.data_ptr(),
+                 y.data_ptr(), T, N, K, torch.cuda.current_stream().cuda_stream)
+    assert 0x201 <= _native.check_device_error() <= 0x205 and _native.check_device_error() == 0
+    lost = torch.zeros_like(y, dtype=torch.bool)
+    lost[:256, :256] = True
+    assert torch.equal(torch.isnan(y), lost) and torch.equal(y[~lost], want[~lost])
