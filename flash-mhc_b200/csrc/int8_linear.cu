@@ -483,11 +483,11 @@ int8_linear_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
 }
 
 // ------------------------------------------------------------ a handful of rows
-// Up to eight rows t read the weight once at the rate of memory, and dot products of
+// Up to four rows t read the weight once at the rate of memory, and dot products of
 // four bytes on the CUDA cores keep up with it.  A warp takes kRowCols columns n and
 // every `split`-th stretch of kRowBytes bytes of K per lane-wide load; its lanes' sums
 // are added by the warp, and those of `split` warps in shared memory.
-constexpr int kRowsMost = 8;
+constexpr int kRowsMost = 4;
 constexpr int kRowWarps = 4, kRowCols = 2, kRowDepth = 4;  // loads in flight: columns x depth
 
 // 16 codes from k on, of which `there` are the row's own; zeros for the others.
@@ -609,16 +609,19 @@ int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const v
   a.xs = xs; a.ws = ws; a.bias = b; a.bias_dtype = bdt;
   a.T = T; a.N = N; a.K = K;
   // The kernel for a handful of rows is the faster one while its arithmetic is little
-  // (us, it / tiles of 128 columns: T x N x K 1 x 4096 x 4096 5.3 / 7.7, 2 x 4096 x 4096
-  // 6.9 / 8.0, 4 x 4096 x 4096 9.9 / 8.1, 1 x 16384 x 4096 13.3 / 13.1, 8 x 16384 x 4096
-  // 33 / 13.6).
-  if (!lose_copy && T <= kRowsMost && T * N * K <= int64_t(1) << 25) {
+  // (us, it / tiles of 128 columns: T x N x K 1 x 4096 x 4096 5.4 / 6.7, 1 x 8192 x 4096
+  // 7.2 / 8.9, 1 x 16384 x 4096 13.1 / 13.0; 2 x 2048 x 2048 2.3 / 3.8, 4 x 2048 x 2048
+  // 3.1 / 3.9, 4 x 4096 x 1024 3.4 / 3.7, 2 x 2896 x 2896 5.8 / 5.7, 2 x 4096 x 4096
+  // 7.1 / 6.6, 4 x 4096 x 2048 6.0 / 5.2).  For five rows and more the tiles are (an
+  // instance for eight took 8 x 1024 x 1024 in 4.6 us, they 3.4; 5 x 3000 x 2200 11.4 / 5.1;
+  // the only ones it was faster at are as small as 5 x 512 x 512, 2.5 / 2.8).
+  if (!lose_copy && T <= kRowsMost && T * N * K <= int64_t(1) << (T == 1 ? 25 : 24)) {
     int split = 1;  // warps that share K: enough blocks for every SM, while there is K for them
     while (split < kRowWarps && ceil_div(N, kRowCols * (kRowWarps / split)) < 2 * sms && K > split * 512 * kRowDepth) split *= 2;
     const int64_t blocks = ceil_div(N, int64_t(kRowCols) * (kRowWarps / split));
     FMHC_DISPATCH_ELEM(ydt, {
       auto k = T == 1 ? int8_linear_rows_kernel<E, 1> : T == 2 ? int8_linear_rows_kernel<E, 2>
-             : T <= 4 ? int8_linear_rows_kernel<E, 4> : int8_linear_rows_kernel<E, 8>;
+             : int8_linear_rows_kernel<E, kRowsMost>;
       launch(k, dim3(unsigned(blocks)), dim3(32 * kRowWarps), 0, s, (const int8_t *)xc, xstride, (const int8_t *)wc, wstride,
              (E *)y, a, split);
     });
@@ -627,8 +630,8 @@ int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const v
   CUtensorMap mw, mx;
   const int64_t pair_t = ceil_div(T, kMaxTn);
   // Pairs of CTAs once they keep three quarters of the SMs busy (us, pairs / tiles of
-  // one CTA: 256 x 4096 x 4096 15.4 / 8.9, 1024 x 2048 x 2048 11.2 / 7.7, 512 x 4096 x
-  // 4096 15.6 / 11.1, 1024 x 4096 x 4096 16.2 / 17.5, 512 x 16384 x 4096 28.5 / 38.1).
+  // one CTA: 256 x 4096 x 4096 14.9 / 8.7, 1024 x 2048 x 2048 10.9 / 7.8, 512 x 4096 x
+  // 4096 15.4 / 11.0, 1024 x 4096 x 4096 16.0 / 17.0, 512 x 16384 x 4096 26.9 / 36.2).
   if (ceil_div(N, 2 * kBM) * pair_t * 2 >= sms * 3 / 4 && T > 128) {
     a.tiles_t = int(pair_t);
     a.tn = int(ceil_div(ceil_div(T, pair_t), 32) * 32);
@@ -649,8 +652,8 @@ int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const v
   }
   a.tiles_n = int(ceil_div(N, kBM));
   // Tiles of up to 128 rows, narrower ones (down to 32, or 64 for a long K) where that
-  // gives more SMs one (us, down to 32 / always 128: 100 x 4096 x 4096 8.1 / 10.0, 256 x
-  // 4096 x 4096 8.9 / 11.0; 64 x 4096 x 16384 16.8 / 15.6).
+  // gives more SMs one (us, as chosen / always 128: 100 x 4096 x 4096 8.0 / 10.2, 256 x
+  // 4096 x 4096 8.8 / 10.9; 64 x 4096 x 16384 with tiles of 64 / of 32 15.7 / 16.8).
   const int least = nk >= 64 ? 64 : 32;
   int64_t tiles_t = std::max(ceil_div(T, 128), std::min<int64_t>(ceil_div(T, least), sms / a.tiles_n));
   a.tn = int(ceil_div(ceil_div(T, tiles_t), 16) * 16);
@@ -661,10 +664,10 @@ int launch_int8_linear(const void *xc, int64_t xstride, const float *xs, const v
   if (tiles > (int64_t(1) << 27))
     return set_last_error(2, "fmhc_int8_linear: T and N give more than 2^27 tiles");
   // K is split where the stages that a CTA is spared (about 0.12 us each) outweigh the
-  // cluster's exchange of partial sums, which grows with the tile (us, 1 / 4 CTAs: 16 x
-  // 1024 x 1024 3.8 / 3.5, 16 x 4096 x 4096 7.9 / 6.9, 64 x 2048 x 2048 5.2 / 5.5, 64 x
-  // 4096 x 16384 23 / 16), up to as many clusters as run at one time (16 of eight CTAs
-  // do not: 16 x 2048 x 2048 7.0, of four 4.1).
+  // cluster's exchange of partial sums, which grows with the tile (us, 1 / 2 / 4 CTAs: 16 x
+  // 1024 x 1024 3.7 / 4.0 / 3.5, 16 x 4096 x 4096 7.8 / 7.5 / 6.9, 64 x 2048 x 2048 5.3 /
+  // 5.6 / 5.0, 64 x 4096 x 16384 23 / 19 / 16), up to as many clusters as run at one time
+  // (16 of eight CTAs do not: 16 x 2048 x 2048 7.1, of four 4.1).
   const int worth = 4 + a.tn / 5;
   const int S = tiles <= 8 && nk >= 2 * worth ? 8 : tiles <= 32 && nk >= worth ? 4 : tiles <= 64 && nk >= 2 * worth ? 2 : 1;
   int cols = 32;
