@@ -421,19 +421,21 @@ def convert_linears(module: nn.Module) -> nn.Module:
     shorter container has the attributes, modes and names of the longer one (but is
     numbered anew if that was numbered); a layer with its norm has the layer's name.  An
     ``MHCLiteBlock`` keeps its own projection and has its wrapped layer converted.
-    Subclasses of ``nn.Linear``, layers with hooks, layers of other types than float32,
-    bfloat16 and float16 and layers of 2^17 inputs or more stay as they are, and so do
-    those whose weights ``nn.TransformerEncoderLayer`` reads itself.  A layer that stands
-    in several places stays one; a norm becomes part of it if it precedes it in all of
-    them.  An :class:`Int8Linear` has no ``weight``: other modules that read their linear
-    layers' weights themselves cannot be converted.
+    Subclasses of ``nn.Linear``, layers with hooks (or a ``forward`` that was set on
+    them), layers of other types than float32, bfloat16 and float16 and layers of 2^17
+    inputs or more stay as they are, and so do those whose weights
+    ``nn.TransformerEncoderLayer`` reads itself.  A layer that stands in several places
+    stays one; a norm becomes part of it if it precedes it in all of them.  An
+    :class:`Int8Linear` has no ``weight``: other modules that read their linear layers'
+    weights themselves cannot be converted.
     """
     return _Conversion(module).of(module)
 
 
 def _has_hooks(m: nn.Module) -> bool:
-    return any(getattr(m, name) for name in ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks",
-                                             "_backward_pre_hooks"))
+    """Hooks, or a forward that was set on the module itself."""
+    return "forward" in vars(m) or any(getattr(m, name) for name in (
+        "_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks"))
 
 
 def _shortens(m: nn.Module) -> bool:
@@ -498,6 +500,7 @@ class _Conversion:
             new = {str(i): m for i, m in enumerate(new.values())}
         shorter = nn.Sequential()
         for name, value in vars(module).items():
-            shorter.__dict__[name] = copy.copy(value) if isinstance(value, (dict, set)) else value
+            if name != "_compiled_call_impl":  # runs the longer one
+                shorter.__dict__[name] = copy.copy(value) if isinstance(value, (dict, set)) else value
         shorter._modules = new
         return shorter

@@ -152,3 +152,28 @@ def test_float64_layers_and_activations():
             q(torch.ones(4, 40, dtype=torch.int64))
         with pytest.raises(ValueError, match="floating-point"):
             int8.Int8Linear(40, 9)(torch.ones(4, 40, dtype=torch.int8))
+
+
+def test_convert_linears_sees_a_forward_of_the_modules_own():
+    """A forward that was set on a module, as wrappers do, is a hook; a compiled call is the longer container's alone."""
+    seen = []
+
+    def wrapped(m):
+        old = m.forward
+        m.forward = lambda *a: (seen.append(type(m)), old(*a))[1]
+        return m
+
+    x = torch.randn(3, 8)
+    m = nn.Sequential(wrapped(nn.Linear(8, 8)), nn.Linear(8, 8), norm.RMSNorm(8), nn.Linear(8, 8))
+    c = int8.convert_linears(m)
+    assert type(c[0]) is nn.Linear and [type(t) for t in c[1:]] == [int8.Int8Linear] * 2 and c[2].norm is m[2]
+    s = wrapped(nn.Sequential(norm.RMSNorm(8), nn.Linear(8, 8)))
+    q = int8.convert_linears(s)
+    assert q is s and type(q[0]) is norm.RMSNorm and type(q[1]) is int8.Int8Linear
+    with torch.no_grad():
+        c(x), q(x)
+    assert seen == [nn.Linear, nn.Sequential]
+    p = nn.Sequential(norm.RMSNorm(8), nn.Linear(8, 8))
+    p.compile(backend="eager")
+    with torch.no_grad():
+        assert torch.equal(int8.convert_linears(p)(x), int8.convert_linears(copy.deepcopy(nn.Sequential(*p)))(x))
