@@ -1,7 +1,8 @@
 // Rows put into 8 bits and restored (format: rows8.cuh).  Memory bounds both: 32768 x
 // 4096 bf16 63 us and 70 us (the bytes at the copy rate take 62).  Restoring writes twice
-// what it reads; rows that start anywhere in a word restore 65536 x 1023 in 70 us (31),
-// bound by instructions.
+// what it reads (to f32 four times: 65536 x 2048 159 us, 103); rows that start anywhere in
+// a word restore 65536 x 1023 in 63 us (31) and 20000 x 5001 in 76 (46), bound by
+// instructions.
 #include "code_word.h"
 #include "fmhc_launch.h"
 #include "norm_rows.cuh"
@@ -87,7 +88,7 @@ row_quantize_kernel(const E *__restrict__ x, int8_t *__restrict__ codes, int64_t
 // Restoring: a group of lanes (a power of two, up to 32) takes `per` chunks of eight
 // codes of one row, up to kRestoreChunks per lane, all of them in flight at a time:
 // narrow rows share a warp and wide ones are cut into equal segments.
-constexpr int kRestoreChunks = 4;  // (of 8: 65536 x 1023 101 us instead of 70)
+constexpr int kRestoreChunks = 4;  // (of 8: 65536 x 1023 101 us, where 4 then took 70)
 struct Restore {
   int group, segments, per;
   int64_t units;
